@@ -19,13 +19,17 @@
 #include <string>
 
 #include "cvs.h"
+#include "cvs_host.h"
 #include "cvs_kernels.h"
 
-using namespace cvs;
+namespace cvs {
 
 namespace {
-
 thread_local std::string g_err;
+constexpr int kMaxDevices = 64;
+DevInfo g_dev[kMaxDevices];
+std::mutex g_dev_mu;
+}  // namespace
 
 int fail(int code, const char* fmt, ...) {
   char buf[512];
@@ -40,17 +44,6 @@ int fail(int code, const char* fmt, ...) {
 int hip_fail(hipError_t e, const char* what) {
   return fail(CVS_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
-
-struct DevInfo {
-  bool ready = false;
-  bool gfx950 = false;
-  int cus = 0;
-  char arch[64] = {0};
-};
-
-constexpr int kMaxDevices = 64;
-DevInfo g_dev[kMaxDevices];
-std::mutex g_dev_mu;
 
 int dev_info(int device, DevInfo* out) {
   if (device < 0 || device >= kMaxDevices) return fail(CVS_ERR_INVALID, "invalid device index %d", device);
@@ -69,22 +62,11 @@ int dev_info(int device, DevInfo* out) {
   return CVS_OK;
 }
 
-// Switches to `device` for the lifetime of the guard (the reference's CUDAGuard).
-struct DeviceGuard {
-  int prev = -1;
-  bool switched = false;
-  hipError_t err = hipSuccess;
-  explicit DeviceGuard(int device) {
-    err = hipGetDevice(&prev);
-    if (err == hipSuccess && prev != device) {
-      err = hipSetDevice(device);
-      switched = (err == hipSuccess);
-    }
-  }
-  ~DeviceGuard() {
-    if (switched) (void)hipSetDevice(prev);
-  }
-};
+}  // namespace cvs
+
+using namespace cvs;
+
+namespace {
 
 int check_inputs(const void* q, const void* x, int64_t nq, int64_t n, int64_t d) {
   if (d <= 0 || d % 64 != 0) return fail(CVS_ERR_INVALID, "width must be a multiple of 64 (zero-pad it)");

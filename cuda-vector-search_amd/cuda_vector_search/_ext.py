@@ -166,7 +166,41 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.cvs_search_plan.argtypes = [i64, i64, i64, i64, i64, i32, i32, i32, i32, ctypes.POINTER(i64)]
     lib.cvs_search.restype = i32
     lib.cvs_search.argtypes = [vp, i64, i32, vp, vp, i64, i64, i64, i64, i64, i32, vp, i64, vp, vp, i32, vp]
+    _bind_encoder(lib)
     return lib
+
+
+class AttentionArgs(ctypes.Structure):
+    """cvs_attention (include/cvs.h)."""
+
+    _fields_ = [(n, ctypes.c_int64) for n in ("batch", "q_len", "k_len", "heads", "k_heads", "width")] + [
+        (n, ctypes.c_void_p) for n in ("q", "k", "v")] + [
+        (n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride")] + [
+        ("scale", ctypes.c_double), ("type", ctypes.c_int), ("causal", ctypes.c_int)] + [
+        (n, ctypes.c_void_p) for n in ("key_lengths", "query_lengths", "query_start", "bias_table")] + [
+        ("buckets", ctypes.c_int64), ("max_distance", ctypes.c_int64)]
+
+
+def _bind_encoder(lib: ctypes.CDLL) -> None:
+    """Signatures of the text-encoder operators."""
+    i64, i32, vp, f64 = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_double
+    out = ctypes.POINTER(i64)
+    att = ctypes.POINTER(AttentionArgs)
+    for name, args in {
+        "cvs_layer_norm": [vp, vp, vp, i64, i64, i64, f64, i32, vp, vp, vp, i32, vp],
+        "cvs_layer_norm_backward_plan": [i64, i64, i32, i32, out],
+        "cvs_layer_norm_backward": [vp] * 5 + [i64] * 4 + [i32, vp, vp, vp, vp, i64, i32, vp],
+        "cvs_linear_plan": [i64, i64, i64, i32, out],
+        "cvs_linear": [vp] * 4 + [i64] * 5 + [i32, i32, vp, vp, vp, i64, i32, vp],
+        "cvs_linear_backward_plan": [i64, i64, i64, i32, i32, out],
+        "cvs_linear_backward": [vp] * 4 + [i64] * 5 + [i32, i32, vp, vp, vp, vp, i64, i32, vp],
+        "cvs_attention_plan": [att, i32, i32, out],
+        "cvs_attention_forward": [att, vp, vp, vp, i64, i32, vp],
+        "cvs_attention_backward": [att, vp, out, vp, vp, vp, vp, vp, vp, vp, i64, i32, vp],
+    }.items():
+        fn = getattr(lib, name)
+        fn.restype = i32
+        fn.argtypes = args
 
 
 def open_library(path: str | Path | None = None) -> ctypes.CDLL:

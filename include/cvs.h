@@ -259,6 +259,101 @@ int cvs_search(const void* q, int64_t dim, int normalize, const void* x, const v
                int64_t n, int64_t d, int64_t k, int flags, void* workspace, int64_t workspace_bytes, float* out_v,
                void* out_i, int device, void* stream);
 
+/*
+ * Operators of a text encoder (no counterpart in the reference, which searches
+ * embeddings that a caller brings): what turns text into the rows of a corpus, and
+ * what trains it.  The conventions are those above, with these types; results
+ * are rounded once, to the type of the inputs, and every sum is fp32.  None uses
+ * atomics whose order could change a result: the same call gives the same bits.
+ */
+#define CVS_TYPE_F16 0
+#define CVS_TYPE_BF16 1
+#define CVS_TYPE_F32 2 /* layer norm only */
+
+/*
+ * Layer norm of n rows of d elements (rows of x are x_stride elements apart, those of y
+ * d): y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(mean((x - mean)^2) + eps).
+ * weight and bias (may be NULL) are [d], of x's type.  mean and rstd (fp32 [n], both
+ * or neither NULL) receive the statistics the backward pass takes.
+ */
+int cvs_layer_norm(const void* x, const void* weight, const void* bias, int64_t n, int64_t d, int64_t x_stride,
+                   double eps, int type, void* y, float* mean, float* rstd, int device, void* stream);
+
+/*
+ * Gradients of cvs_layer_norm for dy (rows dy_stride elements apart): dx [n, d], dweight
+ * and dbias [d] (either may be NULL).  `workspace` (256-byte aligned) holds at least
+ * what the plan reports.
+ */
+int cvs_layer_norm_backward_plan(int64_t n, int64_t d, int type, int device, int64_t* workspace_bytes);
+int cvs_layer_norm_backward(const void* dy, const void* x, const void* weight, const float* mean, const float* rstd,
+                            int64_t n, int64_t d, int64_t dy_stride, int64_t x_stride, int type, void* dx, void* dweight,
+                            void* dbias, void* workspace, int64_t workspace_bytes, int device, void* stream);
+
+#define CVS_ACT_NONE 0
+#define CVS_ACT_GELU 1 /* z * (1 + erf(z / sqrt 2)) / 2 */
+#define CVS_ACT_RELU 2
+#define CVS_ACT_TANH 3
+
+/*
+ * y[m, n] = act(x w^T + bias) + residual for x [m, k], w [n, k]: bias [n], residual [m, n]
+ * (rows residual_stride elements apart) and pre [m, n] (receives x w^T + bias, which the
+ * backward pass takes) may be NULL.  Types CVS_TYPE_F16 and CVS_TYPE_BF16; k, n and the
+ * strides are multiples of 8, pointers 16-byte aligned.  m may be anything.
+ */
+int cvs_linear_plan(int64_t m, int64_t k, int64_t n, int device, int64_t* workspace_bytes);
+int cvs_linear(const void* x, const void* w, const void* bias, const void* residual, int64_t m, int64_t k, int64_t n,
+               int64_t x_stride, int64_t residual_stride, int act, int type, void* y, void* pre, void* workspace,
+               int64_t workspace_bytes, int device, void* stream);
+
+/*
+ * Gradients of cvs_linear for dy [m, n] (rows dy_stride elements apart): dx [m, k], dw [n, k],
+ * dbias [n], each of which may be NULL.  The residual's gradient is dy itself.  pre is
+ * what the forward call wrote ([m, n]; may be NULL when act is CVS_ACT_NONE).
+ */
+int cvs_linear_backward_plan(int64_t m, int64_t k, int64_t n, int act, int device, int64_t* workspace_bytes);
+int cvs_linear_backward(const void* dy, const void* x, const void* w, const void* pre, int64_t m, int64_t k, int64_t n,
+                        int64_t dy_stride, int64_t x_stride, int act, int type, void* dx, void* dw, void* dbias,
+                        void* workspace, int64_t workspace_bytes, int device, void* stream);
+
+/*
+ * Softmax attention with an optional learned bias by relative position.  Query head h
+ * reads key head h / (heads / k_heads).  Row i of a sequence stands at key position
+ * i + start (query_start[b], or k_len - q_len) and sees key j when j < key_lengths[b]
+ * and, if causal, j <= i + start; rows at or past query_lengths[b] see nothing.  A row
+ * that sees nothing has output 0 and log sum -inf.
+ *   score[i, j] = scale * q_i . k_j + bias_table[bucket(j - i - start)][h]
+ * bucket: distances below exact = per / 2 have one each, the per - exact others
+ * divide exact .. max_distance evenly in the logarithm (the last takes all further ones);
+ * causal: per = buckets, and only the past counts; else per = buckets / 2 for keys at
+ * or before the row, and another per for those after it.
+ * Strides (batch, position, head) in elements, multiples of 8; width a multiple of 8, at
+ * most 128; elements of a head contiguous; pointers 16-byte aligned.  Outputs are contiguous:
+ * out and dq [batch, q_len, heads, width], dk and dv [batch, k_len, k_heads, width],
+ * lse (natural logarithm) [batch, heads, q_len], dbias_table [buckets, heads].
+ */
+#define CVS_ATTENTION_MAX_BUCKETS 128
+#define CVS_ATTENTION_MAX_DISTANCE 256
+typedef struct cvs_attention {
+  int64_t batch, q_len, k_len, heads, k_heads, width;
+  const void *q, *k, *v;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  double scale; /* positive */
+  int type;     /* CVS_TYPE_F16 or CVS_TYPE_BF16 */
+  int causal;
+  const int32_t* key_lengths;   /* [batch] or NULL: k_len */
+  const int32_t* query_lengths; /* [batch] or NULL: q_len */
+  const int32_t* query_start;   /* [batch] or NULL */
+  const void* bias_table;       /* [buckets, heads] or NULL */
+  int64_t buckets, max_distance;
+} cvs_attention;
+
+int cvs_attention_plan(const cvs_attention* p, int backward, int device, int64_t* workspace_bytes);
+int cvs_attention_forward(const cvs_attention* p, void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                          int device, void* stream);
+int cvs_attention_backward(const cvs_attention* p, const void* dout, const int64_t* dout_stride, const void* out,
+                           const float* lse, void* dq, void* dk, void* dv, void* dbias_table, void* workspace,
+                           int64_t workspace_bytes, int device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
