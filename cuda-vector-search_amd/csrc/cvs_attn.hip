@@ -24,13 +24,15 @@ template <class T, int DP, bool BIAS>
 __global__ __launch_bounds__(kBlock, 2) void attn_forward_kernel(AttnArgs a) {
   typedef typename Frag<T>::V V;
   constexpr int KS = DP / 16, DB = DP / 32, TILE = kKeys * DP * 2;
-  __shared__ __attribute__((aligned(128))) unsigned char sk[2][TILE], sv[2][TILE];
+  __shared__ __attribute__((aligned(1024))) unsigned char sk[2][TILE], sv[2][TILE];
   extern __shared__ float tab[];
 
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int heads = a.batch * a.heads;
-  const int bh = blockIdx.x % heads, block = blockIdx.x / heads;
+  int block = blockIdx.x / heads;
+  if (a.causal) block = (a.lq + kAttnRows - 1) / kAttnRows - 1 - block;  // those with most keys first
+  const int bh = blockIdx.x % heads;
   const int b = bh / a.heads, h = bh % a.heads, hk = h / (a.heads / a.k_heads);
   const int nk = key_count(a, b), nq = query_count(a, b), off = query_offset(a, b);
   const int r0 = block * kAttnRows + wave * 32;
@@ -42,13 +44,16 @@ __global__ __launch_bounds__(kBlock, 2) void attn_forward_kernel(AttnArgs a) {
   V qf[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s) qf[s] = global_frag<T>(qrow, s, a.d, i < nq);
-  if (BIAS) load_diag(tab, a, h);
+  if (BIAS) load_bias<T>(tab, a, h);
 
   f32x16 acc[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) acc[d] = zero16();
+  // m: what the row's exponentials are relative to, in units of unscaled scores.  It follows
+  // the maximum only once that is 2^8 past it: rescaling the sums is then rare, and
+  // exponentials up to 2^8 lose nothing.
   float m = -__builtin_inff(), sum = 0.f;
-  const float c = a.scale * kLog2e;
+  const float c = a.scale * kLog2e, slack = 8.f / c;
 
   // this workgroup's keys: a part of those that some row of it sees
   const int last_row = min(block * kAttnRows + kAttnRows, nq) - 1;
@@ -57,58 +62,72 @@ __global__ __launch_bounds__(kBlock, 2) void attn_forward_kernel(AttnArgs a) {
   const int tiles = (end + kKeys - 1) / kKeys;
   const int t0 = (int)((int64_t)tiles * blockIdx.y / a.splits), t1 = (int)((int64_t)tiles * (blockIdx.y + 1) / a.splits);
 
-  TileLoad<DP, kKeys> lk, lv;
-  if (t0 < t1) {
-    lk.load(kbase, 2 * a.ks[1], t0 * kKeys, nk, a.d);
-    lv.load(vbase, 2 * a.vs[1], t0 * kKeys, nk, a.d);
-  }
+  const TileLoad<DP, kKeys> lk(2 * a.ks[1], a.d), lv(2 * a.vs[1], a.d);
+  auto load = [&](int t) {
+    lk.load(kbase, 2 * a.ks[1], t * kKeys, nk, sk[t & 1]);
+    lv.load(vbase, 2 * a.vs[1], t * kKeys, nk, sv[t & 1]);
+  };
+  if (t0 < t1) load(t0);
   for (int t = t0; t < t1; ++t) {
     const int buf = t & 1;
-    lk.store(sk[buf]);
-    lv.store(sv[buf]);
-    __syncthreads();
-    if (t + 1 < t1) {
-      lk.load(kbase, 2 * a.ks[1], (t + 1) * kKeys, nk, a.d);
-      lv.load(vbase, 2 * a.vs[1], (t + 1) * kKeys, nk, a.d);
-    }
+    tile_barrier();
+    if (t + 1 < t1) load(t + 1);
     const int j0 = t * kKeys;
     f32x16 x[2];
+    float shift = 0.f;  // a bias that all of the tile has
+    const int near = j0 - r0 - off;  // position of the tile's first key and the wave's first row
+    if (BIAS) {
+      const int reach = a.max_distance + kReach;
+      if (near - 31 >= a.max_distance || near + kKeys - 1 <= -a.max_distance) {
+        shift = tab[near > 0 ? 2 * reach : 0];
+        x[0] = x[1] = zero16();
+      } else {
+        const float* at = tab + (near - l32 + 8 * g + reach);
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      x[kb] = zero16();
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[kb][e] = at[kb * 32 + elem_row(e, 0)];
+      }
+    } else {
+      x[0] = x[1] = zero16();
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int s = 0; s < KS; ++s) x[kb] = Frag<T>::mfma(row_frag<T, DP>(sk[buf], kb * 32, s), qf[s], x[kb]);
+    if (j0 + kKeys > nk || (a.causal && near + kKeys - 1 > 0)) {
+      const int seen = min(nk - 1, a.causal ? i + off : nk) - j0 - 8 * g;  // last key of the tile that the row sees
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[kb][e] = kb * 32 + elem_row(e, 0) > seen ? -__builtin_inff() : x[kb][e];
     }
-    const bool whole = j0 + kKeys <= nk && (!a.causal || j0 + kKeys - 1 <= r0 + off);
-    float top = m;
+    float top = x[0][0];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, x[kb][e]);
+    top = fmaxf(top, swap_halves(top)) + shift;
+    if (__any(top > m + slack)) {
+      const float next = fmaxf(m, top);
+      const float fade = next == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((m - next) * c);
+      m = next;
+      sum *= fade;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[d][e] *= fade;
+    }
+    const float base = m == -__builtin_inff() ? shift * c : (shift - m) * c;  // (no score yet: all of them -inf, or the bias)
+    float part[2] = {0.f, 0.f};
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int j = j0 + kb * 32 + elem_row(e, g);
-        float v = x[kb][e] * c;
-        if (BIAS) v += tab[min(max(j - i - off, -a.max_distance), a.max_distance) + a.max_distance];
-        if (!whole && (j >= nk || (a.causal && j > i + off))) v = -__builtin_inff();
-        x[kb][e] = v;
-        top = fmaxf(top, v);
+        x[kb][e] = __builtin_amdgcn_exp2f(fmaf(x[kb][e], c, base));
+        part[kb] += x[kb][e];
       }
-    top = fmaxf(top, swap_halves(top));
-    const float base = top == -__builtin_inff() ? 0.f : top;
-    const float fade = __builtin_amdgcn_exp2f(m - base);
-    m = top;
-    float part = 0.f;
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        x[kb][e] = __builtin_amdgcn_exp2f(x[kb][e] - base);
-        part += x[kb][e];
-      }
-    sum = sum * fade + part;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[d][e] *= fade;
+    sum += part[0] + part[1];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -122,6 +141,7 @@ __global__ __launch_bounds__(kBlock, 2) void attn_forward_kernel(AttnArgs a) {
   sum += swap_halves(sum);
   if (i >= a.lq) return;
   if (i >= nq) sum = 0.f, m = -__builtin_inff();
+  m *= c;  // to base-2 logarithms
   const int64_t at = (int64_t)bh * a.lq + i;  // [batch, heads, lq]
   if (a.splits > 1) {
     const int64_t rows = (int64_t)heads * a.lq;
@@ -178,24 +198,10 @@ __global__ __launch_bounds__(kBlock) void attn_join_kernel(AttnArgs a) {
   if (a.lse != nullptr && lane == 0) a.lse[at] = sum == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-template <class T>
-__global__ __launch_bounds__(kBlock) void attn_diag_kernel(AttnArgs a) {
-  const int n = 2 * a.max_distance + 1;
-  const int h = blockIdx.x;
-  for (int t = threadIdx.x; t < n; t += kBlock) {
-    const int rel = t - a.max_distance;
-    const int dist = a.causal ? max(-rel, 0) : abs(rel);
-    int u = 0;
-    while (u + 1 < a.one_way && a.edges[u + 1] <= dist) ++u;
-    const int bucket = !a.causal && rel > 0 ? a.one_way + u : u;
-    a.diag[(int64_t)h * n + t] = (float)((const T*)a.table)[(int64_t)bucket * a.heads + h] * kLog2e;
-  }
-}
-
 template <class T, int DP>
 void launch_width(const AttnArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)((a.lq + kAttnRows - 1) / kAttnRows * (int64_t)a.batch * a.heads), a.splits), block(kBlock);
-  const size_t tab = a.table != nullptr ? (2 * a.max_distance + 1) * sizeof(float) : 0;
+  const size_t tab = (2 * (a.max_distance + kReach) + 1) * sizeof(float);
   if (a.table != nullptr)
     hipLaunchKernelGGL((attn_forward_kernel<T, DP, true>), grid, block, tab, s, a);
   else
@@ -225,14 +231,6 @@ int attn_splits(const AttnArgs& a, int cus) {
   const int64_t wgs = (a.lq + kAttnRows - 1) / kAttnRows * (int64_t)a.batch * a.heads;
   const int64_t tiles = (a.lk + kKeys - 1) / kKeys;
   return (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / std::max<int64_t>(wgs, 1), tiles / 4, (int64_t)64}));
-}
-
-hipError_t launch_attn_diag(const AttnArgs& a, hipStream_t s) {
-  if (a.type == kF16)
-    hipLaunchKernelGGL(attn_diag_kernel<_Float16>, dim3(a.heads), dim3(kBlock), 0, s, a);
-  else
-    hipLaunchKernelGGL(attn_diag_kernel<__bf16>, dim3(a.heads), dim3(kBlock), 0, s, a);
-  return hipGetLastError();
 }
 
 hipError_t launch_attn_forward(const AttnArgs& a, hipStream_t s) {

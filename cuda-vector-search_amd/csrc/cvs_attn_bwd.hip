@@ -4,18 +4,19 @@
 //   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,
 //   dtable[bucket, h] = sum of ds_ij over the pairs whose position falls in the bucket.
 //
-// Two kernels, each with sums that no other workgroup adds to: one walks the queries
-// for 128 keys (dk, dv; the query heads that share a key head one after the other), one
-// the keys for 128 queries (dq, dtable).  That computes the scores and dout . v twice
+// Two kernels, each with sums that no other workgroup adds to: one walks the keys for 128
+// queries (delta, dq, dtable), then one the queries for 128 keys (dk, dv; the query heads
+// that share a key head one after the other).  That computes the scores and dout . v twice
 // (seven products instead of five), and needs neither atomics, whose order would
 // change results, nor a pass that adds up partial dq.  As in the forward kernel, a block
 // of scores is oriented so that, packed to 16 bits, it is an operand of the next
-// product in registers.  Probabilities and ds are rounded to the inputs' type there;
-// everything else is fp32.
+// product in registers, and the products start from what is added to them: scores from
+// the bias, dout . v from -delta.  Probabilities and ds are rounded to the inputs' type for
+// those products; everything else is fp32.
 //
-// dtable: a lane group (half a wave) adds its ds to its own sums by relative
-// position in LDS, where positions beyond the bias's range are registers instead;
-// one position has one lane of the group at a time, so the order of the adds is fixed.
+// Rows that see at most one tile of keys take delta from the probabilities themselves,
+// normalised again: where few keys leave ds small beside its terms, the rounding of
+// out would be most of it.
 #include <algorithm>
 
 #include "cvs_attn_tile.h"
@@ -24,39 +25,218 @@ namespace cvs {
 
 namespace {
 
-constexpr int kTile = 32;  // rows of a streamed tile
 constexpr float kNever = __builtin_inff();
 
-// delta: 8 lanes a row.
-template <class T>
-__global__ __launch_bounds__(kBlock) void attn_delta_kernel(AttnArgs a) {
-  const int64_t row = (int64_t)blockIdx.x * (kBlock / 8) + threadIdx.x / 8;  // of [batch, lq, heads]
-  if (row >= (int64_t)a.batch * a.lq * a.heads) return;
-  const int h = (int)(row % a.heads);
-  const int64_t bi = row / a.heads;
-  const int i = (int)(bi % a.lq);
-  const int64_t b = bi / a.lq;
-  const T* o = (const T*)a.out + row * a.d;
-  const T* g = (const T*)a.dout + b * a.dos[0] + i * a.dos[1] + h * a.dos[2];
-  float s = 0.f;
-  for (int c = threadIdx.x % 8 * 8; c < a.d; c += 64) {
-    const auto x = *reinterpret_cast<const typename Frag<T>::V*>(o + c);
-    const auto y = *reinterpret_cast<const typename Frag<T>::V*>(g + c);
+// Rows of a streamed tile: 64, or 32 of width 128 (two workgroups' tiles fit a CU's LDS).
+template <int DP>
+constexpr int kTile = DP > 64 ? 32 : 64;
+
+// dtable's sums.  A block of ds, laid out by position (row j - i + 31, pitch 36 words: column
+// writes and row reads without bank conflicts; places that no pair of the block has stay
+// zero), is added along the rows, a position a lane, in a fixed order.  (LDS atomics
+// instead took 192 cycles each: 281 us of 32 sequences of up to 512, 12 heads of 64.)
+constexpr int kSkewPitch = 36, kSkew = 64 * kSkewPitch;
+
+__device__ __forceinline__ void add_positions(float* skew, float* sums, const f32x16& ds) {
+  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+  float* to = skew + (8 * g - l32 + 31) * kSkewPitch + l32;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s = fmaf((float)x[j], (float)y[j], s);
-  }
+  for (int e = 0; e < 16; ++e) to[elem_row(e, 0) * kSkewPitch] = ds[e];
+  __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+  const f32x4* from = reinterpret_cast<const f32x4*>(skew + lane * kSkewPitch);
+  f32x4 s = from[0];
 #pragma unroll
-  for (int off = 4; off > 0; off >>= 1) s += __shfl_xor(s, off);
-  if (threadIdx.x % 8 == 0) a.delta[(b * a.heads + h) * a.lq + i] = s;
+  for (int q = 1; q < 8; ++q) s += from[q];
+  sums[lane] += (s[0] + s[1]) + (s[2] + s[3]);
+  __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
 }
 
-// dk and dv of 128 keys: wave w has keys 32 w .. of them as columns.
+// delta, dq of 128 queries (wave w: 32 of them as columns), and their sums for dtable.
 template <class T, int DP, bool BIAS>
-__global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) {
   typedef typename Frag<T>::V V;
-  constexpr int KS = DP / 16, DB = DP / 32, TILE = kTile * DP * 2;
-  __shared__ __attribute__((aligned(128))) unsigned char sq[2][TILE], sg[2][TILE];
-  __shared__ __attribute__((aligned(16))) float slse[2][kTile], sdelta[2][kTile];
+  constexpr int KS = DP / 16, DB = DP / 32, ROWS = kTile<DP>, KB = ROWS / 32, TILE = ROWS * DP * 2;
+  __shared__ __attribute__((aligned(1024))) unsigned char sk[2][TILE], sv[2][TILE];
+  __shared__ __attribute__((aligned(16))) float skew[BIAS ? 4 : 1][BIAS ? kSkew : 4];
+  extern __shared__ float tab[];  // bias by position, then the waves' sums by position
+
+  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int heads = a.batch * a.heads;
+  int block = blockIdx.x / heads;
+  if (a.causal) block = (a.lq + kAttnRows - 1) / kAttnRows - 1 - block;  // those with most keys first
+  const int bh = blockIdx.x % heads;
+  const int b = bh / a.heads, h = bh % a.heads, hk = h / (a.heads / a.k_heads);
+  const int nk = key_count(a, b), nq = query_count(a, b), off = query_offset(a, b);
+  const int r0 = block * kAttnRows + wave * 32;
+  const int i = r0 + l32;
+  const unsigned char* qrow = (const unsigned char*)a.q + 2 * (b * a.qs[0] + i * a.qs[1] + h * a.qs[2]);
+  const unsigned char* grow = (const unsigned char*)a.dout + 2 * (b * a.dos[0] + i * a.dos[1] + h * a.dos[2]);
+  const unsigned char* orow = (const unsigned char*)a.out + 2 * ((((int64_t)b * a.lq + i) * a.heads + h) * a.d);
+  const unsigned char* kbase = (const unsigned char*)a.k + 2 * (b * a.ks[0] + hk * a.ks[2]);
+  const unsigned char* vbase = (const unsigned char*)a.v + 2 * (b * a.vs[0] + hk * a.vs[2]);
+
+  const int last_row = min(block * kAttnRows + kAttnRows, nq) - 1;
+  int end = last_row < block * kAttnRows ? 0 : nk;
+  if (a.causal) end = min(end, max(last_row + off + 1, 0));
+  const int tiles = (end + ROWS - 1) / ROWS;
+  const bool one = nk <= ROWS;  // a row's keys are all in one tile
+  const TileLoad<DP, ROWS> lk(2 * a.ks[1], a.d), lv(2 * a.vs[1], a.d);
+  auto load = [&](int t) {
+    lk.load(kbase, 2 * a.ks[1], t * ROWS, nk, sk[t & 1]);
+    lv.load(vbase, 2 * a.vs[1], t * ROWS, nk, sv[t & 1]);
+  };
+  if (tiles > 0) load(0);
+
+  V qf[KS], gf[KS];
+  float delta = 0.f;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    qf[s] = global_frag<T>(qrow, s, a.d, i < nq);
+    gf[s] = global_frag<T>(grow, s, a.d, i < nq);
+    const V of = global_frag<T>(orow, s, a.d, i < nq);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) delta = fmaf((float)gf[s][j], (float)of[j], delta);
+  }
+  delta = one ? 0.f : delta + swap_halves(delta);
+  const int64_t row_at = (int64_t)bh * a.lq + i;
+  float lse = kNever;
+  if (i < nq) {
+    lse = a.lse[row_at] * kLog2e;
+    if (lse == -__builtin_inff()) lse = kNever;  // a row that sees nothing
+  }
+  const int reach = a.max_distance + kReach, places = 2 * reach + 1;
+  float* sums = tab + places + wave * places + reach;  // by position, this wave's
+  float before = 0.f, after = 0.f;                     // positions all <= -max_distance, all >= max_distance
+  if (BIAS) {
+    load_bias<T>(tab, a, h);
+    for (int t = threadIdx.x; t < 4 * places; t += kBlock) tab[places + t] = 0.f;
+    for (int t = threadIdx.x; t < 4 * kSkew; t += kBlock) skew[t / kSkew][t % kSkew] = 0.f;
+  }
+
+  f32x16 dq[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) dq[d] = zero16();
+  const f32x16 minus_delta = splat16(-delta);
+  const float c = a.scale * kLog2e;
+
+  for (int t = 0; t < tiles; ++t) {
+    const int buf = t & 1;
+    tile_barrier();
+    if (t + 1 < tiles) load(t + 1);
+    f32x16 ds[KB], p[KB];
+    int near[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const int j0 = t * ROWS + kb * 32;
+      near[kb] = j0 - r0 - off;
+      float base = -lse;
+      p[kb] = zero16();
+      if (BIAS) {
+        if (near[kb] - 31 >= a.max_distance || near[kb] + 31 <= -a.max_distance) {
+          base += tab[near[kb] > 0 ? 2 * reach : 0] * c;
+        } else {
+          const float* at = tab + (near[kb] - l32 + 8 * g + reach);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) p[kb][e] = at[elem_row(e, 0)];
+        }
+      }
+      ds[kb] = minus_delta;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        p[kb] = Frag<T>::mfma(row_frag<T, DP>(sk[buf], kb * 32, s), qf[s], p[kb]);
+        ds[kb] = Frag<T>::mfma(row_frag<T, DP>(sv[buf], kb * 32, s), gf[s], ds[kb]);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) p[kb][e] = __builtin_amdgcn_exp2f(fmaf(p[kb][e], c, base));
+      if (j0 + 32 > nk || (a.causal && near[kb] + 31 > 0)) {
+        const int seen = min(nk - 1, a.causal ? i + off : nk) - j0 - 8 * g;  // last key of the block that the row sees
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[kb][e] = elem_row(e, 0) > seen ? 0.f : p[kb][e];
+      }
+    }
+    if (one) {
+      float sp = 0.f, spd = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sp += p[kb][e];
+      sp += swap_halves(sp);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          p[kb][e] = sp == 0.f ? 0.f : p[kb][e] / sp;
+          spd = fmaf(p[kb][e], ds[kb][e], spd);
+        }
+      delta = spd + swap_halves(spd);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) ds[kb][e] -= delta;
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) ds[kb][e] *= p[kb][e];
+      if (BIAS) {
+        if (near[kb] + 31 <= -a.max_distance) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) before += ds[kb][e];
+        } else if (near[kb] - 31 >= a.max_distance) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) after += ds[kb][e];
+        } else {
+          add_positions(skew[wave], sums + near[kb] - 31, ds[kb]);
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const V df = pack8<T>(ds[kb], s);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+          dq[d] = Frag<T>::mfma(col_frag<T, DP>(sk[buf], kb * 32 + 16 * s, d * 32), df, dq[d]);
+      }
+    }
+  }
+  if (i < a.lq) {
+    const int64_t at = (((int64_t)b * a.lq + i) * a.heads + h) * a.d;
+    store_head_row<T, DP>((T*)a.dq + at, dq, a.scale, a.d);
+    if (g == 0) a.delta[row_at] = delta;
+  }
+  if (BIAS) {
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) {
+      before += __shfl_xor(before, s);
+      after += __shfl_xor(after, s);
+    }
+    __syncthreads();
+    if (lane == 0) {  // (the ends hold nothing of blocks in range)
+      sums[-reach] = before;
+      sums[reach] = after;
+    }
+    __syncthreads();
+    // bucket of a direction: distances edges[u] .. edges[u + 1] - 1 (the last: all further ones)
+    const int u = threadIdx.x % a.one_way, side = threadIdx.x / a.one_way;  // side 0: key at or before the query
+    if (threadIdx.x < a.buckets) {
+      float s = 0.f;
+      const int d0 = max((int)a.edges[u], side), d1 = u + 1 < a.one_way ? (int)a.edges[u + 1] : reach + 1;
+      for (int dist = d0; dist < d1; ++dist) {
+        const float* at = tab + places + reach + (side == 1 ? dist : -dist);
+        s += (at[0] + at[places]) + (at[2 * places] + at[3 * places]);
+      }
+      a.part_table[((int64_t)h * a.table_parts + (int64_t)b * (a.table_parts / a.batch) + block) * a.buckets + threadIdx.x] = s;
+    }
+  }
+}
+
+// dk and dv of 128 keys (wave w: 32 of them as columns), over a part of the queries that see them.
+template <class T, int DP, bool BIAS>
+__global__ __launch_bounds__(kBlock, 2) void attn_backward_kv_kernel(AttnArgs a) {
+  typedef typename Frag<T>::V V;
+  constexpr int KS = DP / 16, DB = DP / 32, ROWS = kTile<DP>, QB = ROWS / 32, TILE = ROWS * DP * 2;
+  __shared__ __attribute__((aligned(1024))) unsigned char sq[2][TILE], sg[2][TILE];
+  __shared__ __attribute__((aligned(16))) float slse[2][ROWS], sdelta[2][ROWS];  // -log2 sums, -deltas
   extern __shared__ float tab[];
 
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
@@ -79,225 +259,143 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
 #pragma unroll
   for (int d = 0; d < DB; ++d) dk[d] = dv[d] = zero16();
   const float c = a.scale * kLog2e;
+  const int reach = a.max_distance + kReach;
+  const bool one = nk <= ROWS;  // delta is dout . v's own sum: subtracted as it stands
 
-  // queries that see a key of this workgroup
-  int first = 0;
-  if (a.causal) first = max(block * kAttnRows - off, 0);
-  const int t0 = first / kTile, t1 = block * kAttnRows < nk ? (nq + kTile - 1) / kTile : 0;
-
-  for (int hh = 0; hh < group; ++hh) {
-    const int h = hk * group + hh;
+  // tiles of queries that see a key of this workgroup, those of all heads in a row; this part's
+  const int t0 = (a.causal ? max(block * kAttnRows - off, 0) : 0) / ROWS;
+  const int nt = block * kAttnRows < nk ? max((nq + ROWS - 1) / ROWS - t0, 0) : 0;
+  int f0 = (int)((int64_t)nt * group * blockIdx.y / a.kv_parts);
+  const int f1 = (int)((int64_t)nt * group * (blockIdx.y + 1) / a.kv_parts);
+  const TileLoad<DP, ROWS> lq(2 * a.qs[1], a.d), lg(2 * a.dos[1], a.d);
+  while (f0 < f1) {
+    const int hh = f0 / nt, h = hk * group + hh;
+    const int first = t0 + f0 % nt, last = min(t0 + nt, first + f1 - f0);  // this head's
+    f0 += last - first;
     const unsigned char* qbase = (const unsigned char*)a.q + 2 * (b * a.qs[0] + h * a.qs[2]);
     const unsigned char* gbase = (const unsigned char*)a.dout + 2 * (b * a.dos[0] + h * a.dos[2]);
     const float* lse = a.lse + ((int64_t)b * a.heads + h) * a.lq;
     const float* delta = a.delta + ((int64_t)b * a.heads + h) * a.lq;
     __syncthreads();  // the last head's tiles and bias have been read
-    if (BIAS) load_diag(tab, a, h);
-    TileLoad<DP, kTile> lq, lg;
-    float lrow = 0.f;  // lanes 0 .. 31: log2 sums, 32 .. 63: deltas of the rows
-    auto load_rows = [&](int t) {
-      const int i = t * kTile + (threadIdx.x & 31);
-      if (threadIdx.x < 32) {
-        lrow = i < nq ? lse[i] * kLog2e : kNever;
-        if (lrow == -__builtin_inff()) lrow = kNever;  // a row that sees nothing
-      } else if (threadIdx.x < 64) {
-        lrow = i < nq ? delta[i] : 0.f;
+    if (BIAS) load_bias<T>(tab, a, h);
+    float stat = 0.f;  // threads 0 .. ROWS - 1: -log2 sum of a row, the next ROWS: -delta
+    auto load = [&](int t) {
+      lq.load(qbase, 2 * a.qs[1], t * ROWS, nq, sq[t & 1]);
+      lg.load(gbase, 2 * a.dos[1], t * ROWS, nq, sg[t & 1]);
+      const int i = t * ROWS + threadIdx.x % ROWS;
+      if (threadIdx.x < ROWS) {
+        stat = i < nq ? -lse[i] * kLog2e : -kNever;
+        if (stat == __builtin_inff()) stat = -kNever;  // a row that sees nothing
+      } else if (threadIdx.x < 2 * ROWS) {
+        stat = i < nq ? -delta[i] : 0.f;
       }
     };
-    if (t0 < t1) {
-      lq.load(qbase, 2 * a.qs[1], t0 * kTile, nq, a.d);
-      lg.load(gbase, 2 * a.dos[1], t0 * kTile, nq, a.d);
-      load_rows(t0);
-    }
-    for (int t = t0; t < t1; ++t) {
+    load(first);
+    for (int t = first; t < last; ++t) {
       const int buf = t & 1;
-      lq.store(sq[buf]);
-      lg.store(sg[buf]);
-      if (threadIdx.x < 32)
-        slse[buf][threadIdx.x] = lrow;
-      else if (threadIdx.x < 64)
-        sdelta[buf][threadIdx.x - 32] = lrow;
-      __syncthreads();
-      if (t + 1 < t1) {
-        lq.load(qbase, 2 * a.qs[1], (t + 1) * kTile, nq, a.d);
-        lg.load(gbase, 2 * a.dos[1], (t + 1) * kTile, nq, a.d);
-        load_rows(t + 1);
-      }
-      const int i0 = t * kTile;
-      f32x16 p = zero16(), ds = zero16();
+      if (threadIdx.x < ROWS)
+        slse[buf][threadIdx.x] = stat;
+      else if (threadIdx.x < 2 * ROWS)
+        sdelta[buf][threadIdx.x - ROWS] = stat;
+      tile_barrier();
+      if (t + 1 < last) load(t + 1);
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        p = Frag<T>::mfma(row_frag<T, DP>(sq[buf], 0, s), kf[s], p);
-        ds = Frag<T>::mfma(row_frag<T, DP>(sg[buf], 0, s), vf[s], ds);
-      }
-      const bool whole = !a.causal || j0 + 31 <= i0 + off;
+      for (int qb = 0; qb < QB; ++qb) {
+        const int i0 = t * ROWS + qb * 32;
+        const int near = j0 - i0 - off;
+        f32x16 p = zero16(), ds;
+        float shift = 0.f;
+        if (BIAS) {
+          if (near - 31 >= a.max_distance || near + 31 <= -a.max_distance) {
+            shift = tab[near > 0 ? 2 * reach : 0] * c;
+          } else {
+            const float* at = tab + (near + l32 - 8 * g + reach);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int r = elem_row(e, g), i = i0 + r;
-        float x = p[e] * c;
-        if (BIAS) x += tab[min(max(j - i - off, -a.max_distance), a.max_distance) + a.max_distance];
-        float y = __builtin_amdgcn_exp2f(x - slse[buf][r]);
-        if (!whole && j > i + off) y = 0.f;
-        p[e] = y;
-        ds[e] = y * (ds[e] - sdelta[buf][r]);
-      }
+            for (int e = 0; e < 16; ++e) p[e] = at[-elem_row(e, 0)];
+          }
+        }
+        if (one) {
+          ds = zero16();
+        } else {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const V pf = pack8<T>(p, s), df = pack8<T>(ds, s);
+          for (int e = 0; e < 16; ++e) ds[e] = sdelta[buf][qb * 32 + elem_row(e, g)];
+        }
 #pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          dv[d] = Frag<T>::mfma(col_frag<T, DP>(sg[buf], 16 * s, d * 32), pf, dv[d]);
-          dk[d] = Frag<T>::mfma(col_frag<T, DP>(sq[buf], 16 * s, d * 32), df, dk[d]);
+        for (int s = 0; s < KS; ++s) {
+          p = Frag<T>::mfma(row_frag<T, DP>(sq[buf], qb * 32, s), kf[s], p);
+          ds = Frag<T>::mfma(row_frag<T, DP>(sg[buf], qb * 32, s), vf[s], ds);
+        }
+        if (one) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) ds[e] += sdelta[buf][qb * 32 + elem_row(e, g)];
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float base = slse[buf][qb * 32 + elem_row(e, g)];
+          if (BIAS) base += shift;
+          p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], c, base));
+        }
+        if (a.causal && near + 31 > 0) {
+          const int seen = j - off - i0 - 8 * g;  // first row of the block that sees the key
+#pragma unroll
+          for (int e = 0; e < 16; ++e) p[e] = elem_row(e, 0) < seen ? 0.f : p[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) ds[e] *= p[e];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const V pf = pack8<T>(p, s), df = pack8<T>(ds, s);
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            dv[d] = Frag<T>::mfma(col_frag<T, DP>(sg[buf], qb * 32 + 16 * s, d * 32), pf, dv[d]);
+            dk[d] = Frag<T>::mfma(col_frag<T, DP>(sq[buf], qb * 32 + 16 * s, d * 32), df, dk[d]);
+          }
         }
       }
     }
   }
   if (j >= a.lk) return;
-  const bool in = j < nk;
-  if (!in) {
+  if (j >= nk) {
 #pragma unroll
     for (int d = 0; d < DB; ++d) dk[d] = dv[d] = zero16();
   }
   const int64_t at = (((int64_t)b * a.lk + j) * a.k_heads + hk) * a.d;
+  if (a.kv_parts > 1) {
+    const int64_t all = (int64_t)a.batch * a.lk * a.k_heads * a.d;
+    float* to = a.part_kv + 2 * blockIdx.y * all + at;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int col = d * 32 + 16 * (q >> 1) + 8 * g + 4 * (q & 1);
+        if (col < a.d) {
+          *reinterpret_cast<f32x4*>(to + col) = f32x4{dk[d][4 * q], dk[d][4 * q + 1], dk[d][4 * q + 2], dk[d][4 * q + 3]};
+          *reinterpret_cast<f32x4*>(to + all + col) = f32x4{dv[d][4 * q], dv[d][4 * q + 1], dv[d][4 * q + 2], dv[d][4 * q + 3]};
+        }
+      }
+    return;
+  }
   store_head_row<T, DP>((T*)a.dk + at, dk, a.scale, a.d);
   store_head_row<T, DP>((T*)a.dv + at, dv, 1.f, a.d);
 }
 
-// dq of 128 queries (wave w: 32 of them as columns) and their sums for dtable.
-template <class T, int DP, bool BIAS>
-__global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_q_kernel(AttnArgs a) {
-  typedef typename Frag<T>::V V;
-  constexpr int KS = DP / 16, DB = DP / 32, TILE = kTile * DP * 2;
-  __shared__ __attribute__((aligned(128))) unsigned char sk[2][TILE], sv[2][TILE];
-  extern __shared__ float tab[];  // bias by position, then 8 lane groups' sums by position
-
-  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int heads = a.batch * a.heads;
-  const int bh = blockIdx.x % heads, block = blockIdx.x / heads;
-  const int b = bh / a.heads, h = bh % a.heads, hk = h / (a.heads / a.k_heads);
-  const int nk = key_count(a, b), nq = query_count(a, b), off = query_offset(a, b);
-  const int r0 = block * kAttnRows + wave * 32;
-  const int i = r0 + l32;
-  const unsigned char* qrow = (const unsigned char*)a.q + 2 * (b * a.qs[0] + i * a.qs[1] + h * a.qs[2]);
-  const unsigned char* grow = (const unsigned char*)a.dout + 2 * (b * a.dos[0] + i * a.dos[1] + h * a.dos[2]);
-  const unsigned char* kbase = (const unsigned char*)a.k + 2 * (b * a.ks[0] + hk * a.ks[2]);
-  const unsigned char* vbase = (const unsigned char*)a.v + 2 * (b * a.vs[0] + hk * a.vs[2]);
-  V qf[KS], gf[KS];
-#pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    qf[s] = global_frag<T>(qrow, s, a.d, i < nq);
-    gf[s] = global_frag<T>(grow, s, a.d, i < nq);
+// Adds the parts of dk (blockIdx.y 0) or dv in order: 8 values a thread.
+template <class T>
+__global__ __launch_bounds__(kBlock) void attn_join_kv_kernel(AttnArgs a) {
+  const int64_t all = (int64_t)a.batch * a.lk * a.k_heads * a.d;
+  const int64_t at = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * 8;
+  if (at >= all) return;
+  f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+  for (int p = 0; p < a.kv_parts; ++p) {
+    const f32x4* from = reinterpret_cast<const f32x4*>(a.part_kv + (2 * p + blockIdx.y) * all + at);
+    lo += from[0];
+    hi += from[1];
   }
-  float lse = kNever, delta = 0.f;
-  if (i < nq) {
-    const int64_t at = (int64_t)bh * a.lq + i;
-    lse = a.lse[at] * kLog2e;
-    if (lse == -__builtin_inff()) lse = kNever;
-    delta = a.delta[at];
-  }
-  // sums by position j - i - off = -reach .. reach; a tile with a position of the
-  // bias's range reaches at most 62 beyond it
-  const int reach = a.max_distance + 64, places = 2 * reach + 1;
-  float* sums = tab + 2 * a.max_distance + 1;
-  if (BIAS) {
-    load_diag(tab, a, h);
-    for (int t = threadIdx.x; t < 8 * places; t += kBlock) sums[t] = 0.f;
-  }
-  float* mine = sums + (wave * 2 + g) * places + reach;
-  float before = 0.f, after = 0.f;  // positions all <= -max_distance, all >= max_distance
-
-  f32x16 dq[DB];
+  const float scale = blockIdx.y == 0 ? a.scale : 1.f;
+  typename Frag<T>::V v;
 #pragma unroll
-  for (int d = 0; d < DB; ++d) dq[d] = zero16();
-  const float c = a.scale * kLog2e;
-  const int last_row = min(block * kAttnRows + kAttnRows, nq) - 1;
-  int end = last_row < block * kAttnRows ? 0 : nk;
-  if (a.causal) end = min(end, max(last_row + off + 1, 0));
-  const int tiles = (end + kTile - 1) / kTile;
-
-  TileLoad<DP, kTile> lk, lv;
-  if (tiles > 0) {
-    lk.load(kbase, 2 * a.ks[1], 0, nk, a.d);
-    lv.load(vbase, 2 * a.vs[1], 0, nk, a.d);
-  }
-  for (int t = 0; t < tiles; ++t) {
-    const int buf = t & 1;
-    lk.store(sk[buf]);
-    lv.store(sv[buf]);
-    __syncthreads();
-    if (t + 1 < tiles) {
-      lk.load(kbase, 2 * a.ks[1], (t + 1) * kTile, nk, a.d);
-      lv.load(vbase, 2 * a.vs[1], (t + 1) * kTile, nk, a.d);
-    }
-    const int j0 = t * kTile;
-    f32x16 p = zero16(), ds = zero16();
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      p = Frag<T>::mfma(row_frag<T, DP>(sk[buf], 0, s), qf[s], p);
-      ds = Frag<T>::mfma(row_frag<T, DP>(sv[buf], 0, s), gf[s], ds);
-    }
-    const bool whole = j0 + kTile <= nk && (!a.causal || j0 + kTile - 1 <= r0 + off);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int j = j0 + elem_row(e, g);
-      float x = p[e] * c;
-      if (BIAS) x += tab[min(max(j - i - off, -a.max_distance), a.max_distance) + a.max_distance];
-      float y = __builtin_amdgcn_exp2f(x - lse);
-      if (!whole && (j >= nk || (a.causal && j > i + off))) y = 0.f;
-      ds[e] = y * (ds[e] - delta);
-    }
-    if (BIAS) {
-      const int lo = j0 - (r0 + 31) - off, hi = j0 + 31 - r0 - off;  // this wave's positions
-      if (hi <= -a.max_distance) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) before += ds[e];
-      } else if (lo >= a.max_distance) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) after += ds[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          __hip_atomic_fetch_add(mine + (j0 + elem_row(e, g) - i - off), ds[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-      }
-    }
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const V df = pack8<T>(ds, s);
-#pragma unroll
-      for (int d = 0; d < DB; ++d) dq[d] = Frag<T>::mfma(col_frag<T, DP>(sk[buf], 16 * s, d * 32), df, dq[d]);
-    }
-  }
-  if (i < a.lq) {
-    const int64_t at = (((int64_t)b * a.lq + i) * a.heads + h) * a.d;
-    store_head_row<T, DP>((T*)a.dq + at, dq, a.scale, a.d);
-  }
-  if (BIAS) {
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) {
-      before += __shfl_xor(before, s);
-      after += __shfl_xor(after, s);
-    }
-    __syncthreads();
-    if (l32 == 0) {  // (the group's ends hold nothing of tiles in range)
-      mine[-reach] += before;
-      mine[reach] += after;
-    }
-    __syncthreads();
-    // bucket of a direction: distances edges[u] .. edges[u + 1] - 1 (the last: all further ones)
-    const int u = threadIdx.x % a.one_way, side = threadIdx.x / a.one_way;  // side 0: key at or before the query
-    if (threadIdx.x < a.buckets) {
-      float s = 0.f;
-      const int d1 = u + 1 < a.one_way ? a.edges[u + 1] : reach + 1;
-      for (int dist = a.edges[u]; dist < d1; ++dist) {
-        if (side == 1 && dist == 0) continue;
-        const float* at = sums + reach + (side == 1 ? dist : -dist);
-#pragma unroll
-        for (int w = 0; w < 8; ++w) s += at[w * places];
-      }
-      a.part_table[((int64_t)h * a.table_parts + (int64_t)b * (a.table_parts / a.batch) + block) * a.buckets + threadIdx.x] = s;
-    }
-  }
+  for (int e = 0; e < 4; ++e) v[e] = (T)(lo[e] * scale), v[4 + e] = (T)(hi[e] * scale);
+  *reinterpret_cast<typename Frag<T>::V*>((T*)(blockIdx.y == 0 ? a.dk : a.dv) + at) = v;
 }
 
 // dtable[bucket, h]: the workgroups' sums in order; 64 lanes a (bucket, head).
@@ -315,14 +413,17 @@ __global__ __launch_bounds__(64) void attn_table_kernel(AttnArgs a) {
 template <class T, int DP, bool BIAS>
 hipError_t launch_width(const AttnArgs& a, hipStream_t s) {
   const int64_t qblocks = (a.lq + kAttnRows - 1) / kAttnRows, kblocks = (a.lk + kAttnRows - 1) / kAttnRows;
-  const size_t tab = BIAS ? (2 * a.max_distance + 1) * sizeof(float) : 0;
-  const size_t sums = BIAS ? 8 * (2 * (a.max_distance + 64) + 1) * sizeof(float) : 0;
-  if (kblocks > 0)
-    hipLaunchKernelGGL((attn_backward_kv_kernel<T, DP, BIAS>), dim3((unsigned)(kblocks * a.batch * a.k_heads)), dim3(kBlock),
-                       tab, s, a);
+  const size_t tab = BIAS ? (2 * (a.max_distance + kReach) + 1) * sizeof(float) : 0;
   if (qblocks > 0)
     hipLaunchKernelGGL((attn_backward_q_kernel<T, DP, BIAS>), dim3((unsigned)(qblocks * a.batch * a.heads)), dim3(kBlock),
-                       tab + sums, s, a);
+                       5 * tab, s, a);
+  if (kblocks > 0)
+    hipLaunchKernelGGL((attn_backward_kv_kernel<T, DP, BIAS>), dim3((unsigned)(kblocks * a.batch * a.k_heads), a.kv_parts),
+                       dim3(kBlock), tab, s, a);
+  if (a.kv_parts > 1) {
+    const int64_t threads = (int64_t)a.batch * a.lk * a.k_heads * a.d / 8;
+    hipLaunchKernelGGL(attn_join_kv_kernel<T>, dim3((unsigned)((threads + kBlock - 1) / kBlock), 2), dim3(kBlock), 0, s, a);
+  }
   return hipGetLastError();
 }
 
@@ -335,20 +436,22 @@ hipError_t launch_bias(const AttnArgs& a, hipStream_t s) {
 
 template <class T>
 hipError_t backward(const AttnArgs& a, hipStream_t s) {
-  const int64_t rows = (int64_t)a.batch * a.lq * a.heads;
-  if (rows > 0)
-    hipLaunchKernelGGL(attn_delta_kernel<T>, dim3((unsigned)((rows + kBlock / 8 - 1) / (kBlock / 8))), dim3(kBlock), 0,
-                       s, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
   if (a.table == nullptr) return launch_bias<T, false>(a, s);
-  e = launch_bias<T, true>(a, s);
+  const hipError_t e = launch_bias<T, true>(a, s);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(attn_table_kernel<T>, dim3(a.buckets * a.heads), dim3(64), 0, s, a);
   return hipGetLastError();
 }
 
 }  // namespace
+
+// Parts of the queries for dk and dv: enough workgroups for four rounds' balance where keys
+// are few or causal rows make their work unequal, of at least 8 tiles each.
+int attn_kv_parts(const AttnArgs& a, int cus) {
+  const int64_t wgs = (a.lk + kAttnRows - 1) / kAttnRows * (int64_t)a.batch * a.k_heads;
+  const int64_t tiles = (a.lq + 63) / 64 * (int64_t)(a.heads / a.k_heads);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({4 * cus / wgs, tiles / 8, (int64_t)16}));
+}
 
 hipError_t launch_attn_backward(const AttnArgs& a, hipStream_t s) {
   return a.type == kF16 ? backward<_Float16>(a, s) : backward<__bf16>(a, s);

@@ -12,49 +12,55 @@ namespace cvs {
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
-template <int DP>
-__device__ __forceinline__ int tile_offset(int row, int piece) {  // bytes
-  if constexpr (DP == 32) {
-    const int line = row >> 1;
-    return line * 128 + ((((row & 1) * 4 + piece) ^ (((line & 1) << 1) | ((line >> 1) & 1))) << 4);
-  } else {
-    return row * (2 * DP) + ((piece ^ piece_swizzle(row)) << 4);
-  }
-}
-
-// Rows first .. first + ROWS - 1 of a head (zeros past `rows` and past the width `d`),
-// in registers on their way to LDS.
+// Loads of tiles of ROWS rows of a head straight into LDS, by the four waves of a workgroup:
+// a lane's place in each 1 KiB load is the same in every tile.  Rows from `rows` on and
+// columns from `d` on become zeros.
 template <int DP, int ROWS>
 struct TileLoad {
-  static constexpr int kPieces = ROWS * DP / 8;                        // 16-byte pieces of the tile
-  static constexpr int N = (kPieces + kBlock - 1) / kBlock;
-  u32x4 v[N];
+  static constexpr int N = ROWS * DP * 2 / 4096;
+  static_assert(N * 4096 == ROWS * DP * 2, "whole loads");
+  uint32_t at[N];
+  int row[N];
 
-  __device__ __forceinline__ void load(const unsigned char* base, int64_t stride_bytes, int first, int rows, int d) {
+  __device__ __forceinline__ TileLoad(int64_t stride_bytes, int d) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int t = threadIdx.x + i * kBlock;
-      const int r = t / (DP / 8), p = t % (DP / 8);
-      v[i] = u32x4{0, 0, 0, 0};
-      if ((kPieces % kBlock == 0 || t < kPieces) && first + r < rows && p * 8 < d)
-        v[i] = *reinterpret_cast<const u32x4*>(base + (first + r) * stride_bytes + p * 16);
+      const int line = (wave + 4 * i) * 8 + (lane >> 3), slot = lane & 7;
+      int piece;
+      if constexpr (DP == 32) {
+        const int x = slot ^ pair_swizzle(line);
+        row[i] = 2 * line + (x >> 2), piece = x & 3;
+      } else if constexpr (DP == 64) {
+        row[i] = line, piece = slot ^ piece_swizzle(line);
+      } else {
+        row[i] = line >> 1, piece = ((line & 1) * 8 + slot) ^ piece_swizzle(line >> 1);
+      }
+      at[i] = piece * 8 < d ? (uint32_t)(row[i] * (int)stride_bytes + piece * 16) : kOutside;
     }
   }
-  __device__ __forceinline__ void store(unsigned char* lds) const {
+  // Rows first .. first + ROWS - 1 of the head at `base` (its row 0) to the tile at `lds`.
+  __device__ __forceinline__ void load(const unsigned char* base, int64_t stride_bytes, int first, int rows,
+                                       const unsigned char* lds) const {
+    const uint32_t to = lds_address(lds) + (threadIdx.x >> 6) * 1024;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int t = threadIdx.x + i * kBlock;
-      if (kPieces % kBlock == 0 || t < kPieces)
-        *reinterpret_cast<u32x4*>(lds + tile_offset<DP>(t / (DP / 8), t % (DP / 8))) = v[i];
-    }
+    for (int i = 0; i < N; ++i)
+      load_lds(first + row[i] < rows ? at[i] : kOutside, base + first * stride_bytes, to + i * 4096);
   }
 };
+
+// This wave's loads into LDS have landed and its LDS operations are done; then every wave's.
+__device__ __forceinline__ void tile_barrier() {
+  wait_vmcnt_lgkm0<0>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 // A operand: rows r0 .. r0 + 31 in tile_row order, columns 16 ks .. 16 ks + 15.
 template <class T, int DP>
 __device__ __forceinline__ typename Frag<T>::V row_frag(const unsigned char* lds, int r0, int ks) {
   const int lane = threadIdx.x & 63;
-  return *reinterpret_cast<const typename Frag<T>::V*>(lds + tile_offset<DP>(r0 + tile_row(lane & 31), 2 * ks + (lane >> 5)));
+  return *reinterpret_cast<const typename Frag<T>::V*>(lds + row_offset<DP>(r0 + tile_row(lane & 31), 2 * ks + (lane >> 5)));
 }
 
 // A operand of the transposed tile: its rows are columns c0 .. c0 + 31 (in tile_row
@@ -66,7 +72,7 @@ __device__ __forceinline__ typename Frag<T>::V col_frag(const unsigned char* lds
   const int col = c0 + 16 * (p & 1) + 4 * c;
   const int row = r0 + 8 * (p >> 1) + (s >> 2);
   const unsigned char* at = lds + (col & 4) * 2;
-  return join_tr<T>(read_tr(at + tile_offset<DP>(row, col >> 3)), read_tr(at + tile_offset<DP>(row + 4, col >> 3)));
+  return join_tr<T>(read_tr(at + row_offset<DP>(row, col >> 3)), read_tr(at + row_offset<DP>(row + 4, col >> 3)));
 }
 
 // B operand: column = row `row` of a head in memory (zeros when !in or past d), depth 16 ks + 8 (lane / 32) + 0 .. 7.
@@ -78,12 +84,13 @@ __device__ __forceinline__ typename Frag<T>::V global_frag(const unsigned char* 
   return __builtin_bit_cast(typename Frag<T>::V, v);
 }
 
-__device__ __forceinline__ f32x16 zero16() {
+__device__ __forceinline__ f32x16 splat16(float v) {
   f32x16 z;
 #pragma unroll
-  for (int e = 0; e < 16; ++e) z[e] = 0.f;
+  for (int e = 0; e < 16; ++e) z[e] = v;
   return z;
 }
+__device__ __forceinline__ f32x16 zero16() { return splat16(0.f); }
 
 // Columns 8 s' .. of a transposed accumulator (row = column of the head) to 16 bytes of the output row.
 template <class T, int DP>
@@ -103,10 +110,22 @@ __device__ __forceinline__ void store_head_row(T* row, const f32x16* acc, float 
     }
 }
 
-// The head's bias by relative position in LDS: tab[rel + max_distance].
-__device__ __forceinline__ void load_diag(float* tab, const AttnArgs& a, int head) {
-  const int n = 2 * a.max_distance + 1;
-  for (int t = threadIdx.x; t < n; t += kBlock) tab[t] = a.diag[(int64_t)head * n + t];
+// A head's learned bias by relative position, in LDS, in units of unscaled scores (so that it
+// is what a block of scores starts from): tab[rel + reach], reach = max_distance + kReach.  A
+// block of 32 queries and up to 64 keys that has a position nearer than max_distance has
+// none further than max_distance + kReach; other blocks have one bias throughout.
+constexpr int kReach = 96;
+
+template <class T>
+__device__ __forceinline__ void load_bias(float* tab, const AttnArgs& a, int head) {
+  const int reach = a.max_distance + kReach;
+  const float unit = 1.f / a.scale;
+  for (int t = threadIdx.x; t <= 2 * reach; t += kBlock) {
+    const int rel = t - reach;
+    int u = a.bucket_of[min(abs(rel), a.max_distance)];
+    if (rel > 0) u = a.causal ? 0 : u + a.one_way;
+    tab[t] = (float)((const T*)a.table)[(int64_t)u * a.heads + head] * unit;
+  }
 }
 
 __device__ __forceinline__ int key_count(const AttnArgs& a, int b) {

@@ -60,11 +60,11 @@ struct GemmArgs {
   int splits;
 };
 struct GemmPlan {
-  int tm, tn;   // tile
+  int tile;     // rows and columns of a workgroup's tile
   int splits;   // parts of the reduction
   int64_t ws_bytes;
 };
-GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, bool m_strided, bool n_strided, int cus);
+GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int cus);
 hipError_t launch_gemm(const GemmArgs& a, const GemmPlan& p, hipStream_t s);
 
 // dz = dy act'(pre) ([m, n], when act is not none and dz not null) and the column
@@ -84,8 +84,10 @@ struct ActGradArgs {
 int act_grad_parts(int64_t m, int64_t n, int cus);
 hipError_t launch_act_grad(const ActGradArgs& a, hipStream_t s);
 
-// Column sums of fp32 partial rows: out[j] = sum_p partial[p * stride + j], j < n.
-hipError_t launch_column_sums(const float* partial, int parts, int64_t stride, int n, int type, void* out, hipStream_t s);
+// Column sums of fp32 partial rows, sum_p partial[p * stride + j]: the first n1 columns to
+// out, the n2 after them to out2.
+hipError_t launch_column_sums(const float* partial, int parts, int64_t stride, int n1, int n2, int type, void* out, void* out2,
+                              hipStream_t s);
 
 // ---- attention -----------------------------------------------------------------
 constexpr int kMaxBuckets = 128;
@@ -104,9 +106,9 @@ struct AttnArgs {
   // learned bias by relative position
   const void* table;              // [buckets, heads] or null
   int buckets, max_distance;
-  float* diag;                    // [heads, 2 max_distance + 1] bias * log2 e by key - query position
-  int one_way;                    // buckets of one direction
-  int edges[kMaxBuckets];         // smallest distance of each of them
+  int one_way;                          // buckets of one direction
+  unsigned char bucket_of[kMaxDistance + 1];   // a direction's bucket by distance (the last: all further ones)
+  unsigned short edges[kMaxBuckets + 1];       // smallest distance of each, then one past max_distance
   // forward
   void* out;                      // [batch, lq, heads, d]
   float* lse;                     // [batch, heads, lq] or null
@@ -120,9 +122,11 @@ struct AttnArgs {
   void *dq, *dk, *dv, *dtable;
   float* part_table;              // [heads, batch * query blocks, buckets]
   int table_parts;
+  int kv_parts;                   // parts of the queries that dk and dv are summed over
+  float* part_kv;                 // [kv_parts, 2, batch, lk, k_heads, d] when kv_parts > 1
 };
 constexpr int kAttnRows = 128;    // query (or key) rows of a workgroup
-hipError_t launch_attn_diag(const AttnArgs& a, hipStream_t s);
+int attn_kv_parts(const AttnArgs& a, int cus);
 int attn_splits(const AttnArgs& a, int cus);
 hipError_t launch_attn_forward(const AttnArgs& a, hipStream_t s);
 hipError_t launch_attn_backward(const AttnArgs& a, hipStream_t s);

@@ -79,8 +79,8 @@ struct LinearBackwardPlan {
 
 LinearBackwardPlan plan_linear_backward(int64_t m, int64_t k, int64_t n, int act, int cus) {
   LinearBackwardPlan p;
-  p.dx = plan_gemm(m, k, n, false, true, cus);
-  p.dw = plan_gemm(n, k, m, true, true, cus);
+  p.dx = plan_gemm(m, k, n, cus);
+  p.dw = plan_gemm(n, k, m, cus);
   p.parts = act_grad_parts(m, n, cus);
   int64_t at = 0;
   p.dz = at, at += act == CVS_ACT_NONE ? 0 : up256(m * n * 2);
@@ -122,6 +122,7 @@ int check_heads(const void* p, const int64_t* stride, const char* what) {
   if (!aligned16(p)) return fail(CVS_ERR_INVALID, "%s must be 16-byte aligned", what);
   for (int i = 0; i < 3; ++i)
     if (stride[i] < 0 || stride[i] % 8 != 0) return fail(CVS_ERR_INVALID, "%s: strides must be multiples of 8", what);
+  if (stride[1] > (1 << 23)) return fail(CVS_ERR_INVALID, "%s: a position's stride must be at most 2^23", what);
   return CVS_OK;
 }
 
@@ -141,30 +142,36 @@ AttnArgs attn_args(const cvs_attention* p) {
   if (a.table != nullptr) {
     a.one_way = a.causal ? a.buckets : a.buckets / 2;
     const int exact = a.one_way / 2, wide = a.one_way - exact;
-    for (int u = 0; u <= exact; ++u) a.edges[u] = u;
+    for (int u = 0; u <= exact; ++u) a.edges[u] = (unsigned short)u;
     // (the powers that are whole numbers may come out a hair above them)
     for (int t = 1; t < wide; ++t)
-      a.edges[exact + t] = (int)std::ceil(exact * std::pow((double)a.max_distance / exact, (double)t / wide) - 1e-9);
+      a.edges[exact + t] = (unsigned short)std::ceil(exact * std::pow((double)a.max_distance / exact, (double)t / wide) - 1e-9);
+    a.edges[a.one_way] = (unsigned short)(a.max_distance + 1);
+    for (int dist = 0, u = 0; dist <= a.max_distance; ++dist) {
+      while (u + 1 < a.one_way && a.edges[u + 1] <= dist) ++u;
+      a.bucket_of[dist] = (unsigned char)u;
+    }
   }
   return a;
 }
 
 struct AttnPlan {
-  int splits = 1, table_parts = 0;
-  int64_t diag = 0, part_out = 0, part_ml = 0, delta = 0, part_table = 0, bytes = 0;
+  int splits = 1, table_parts = 0, kv_parts = 1;
+  int64_t part_kv = 0, part_out = 0, part_ml = 0, delta = 0, part_table = 0, bytes = 0;
 };
 
 AttnPlan plan_attention(const AttnArgs& a, bool backward, int cus) {
   AttnPlan p;
   int64_t at = 0;
   const int64_t rows = (int64_t)a.batch * a.heads * a.lq;
-  if (a.table != nullptr) p.diag = at, at += up256((int64_t)a.heads * (2 * a.max_distance + 1) * 4);
   if (backward) {
     p.delta = at, at += up256(rows * 4);
     if (a.table != nullptr) {
       p.table_parts = a.batch * ((a.lq + kAttnRows - 1) / kAttnRows);
       p.part_table = at, at += up256((int64_t)a.heads * p.table_parts * a.buckets * 4);
     }
+    p.kv_parts = rows == 0 || a.lk == 0 ? 1 : attn_kv_parts(a, cus);
+    if (p.kv_parts > 1) p.part_kv = at, at += up256((int64_t)p.kv_parts * 2 * a.batch * a.lk * a.k_heads * a.d * 4);
   } else {
     p.splits = rows == 0 ? 1 : attn_splits(a, cus);
     if (p.splits > 1) {
@@ -232,7 +239,7 @@ int cvs_linear_plan(int64_t m, int64_t k, int64_t n, int device, int64_t* worksp
   DevInfo di;
   int rc = dev_info(device, &di);
   if (rc == CVS_OK) rc = check_linear(m, k, n);
-  if (rc == CVS_OK) *workspace_bytes = m == 0 ? 0 : plan_gemm(m, n, k, false, false, di.cus).ws_bytes;
+  if (rc == CVS_OK) *workspace_bytes = m == 0 ? 0 : plan_gemm(m, n, k, di.cus).ws_bytes;
   return rc;
 }
 
@@ -250,7 +257,7 @@ int cvs_linear(const void* x, const void* w, const void* bias, const void* resid
   if (rc != CVS_OK) return rc;
   if (!aligned16(w) || !aligned16(bias) || !aligned16(y) || !aligned16(pre))
     return fail(CVS_ERR_INVALID, "linear: pointers must be 16-byte aligned");
-  const GemmPlan p = plan_gemm(m, n, k, false, false, di.cus);
+  const GemmPlan p = plan_gemm(m, n, k, di.cus);
   rc = check_workspace(workspace, workspace_bytes, p.ws_bytes);
   if (rc != CVS_OK) return rc;
   DeviceGuard guard(device);
@@ -356,12 +363,9 @@ int cvs_attention_forward(const cvs_attention* p, void* out, float* lse, void* w
   unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
   a.out = out, a.lse = lse;
   a.splits = plan.splits;
-  a.diag = reinterpret_cast<float*>(ws + plan.diag);
   a.part_out = reinterpret_cast<float*>(ws + plan.part_out);
   a.part_ml = reinterpret_cast<float*>(ws + plan.part_ml);
-  hipError_t e = a.table != nullptr ? launch_attn_diag(a, s) : hipSuccess;
-  if (e == hipSuccess) e = launch_attn_forward(a, s);
-  return done(e, "attention launch");
+  return done(launch_attn_forward(a, s), "attention launch");
 }
 
 int cvs_attention_backward(const cvs_attention* p, const void* dout, const int64_t* dout_stride, const void* out,
@@ -394,13 +398,12 @@ int cvs_attention_backward(const cvs_attention* p, const void* dout, const int64
   a.out = const_cast<void*>(out), a.lse = const_cast<float*>(lse), a.dout = dout;
   for (int i = 0; i < 3; ++i) a.dos[i] = dout_stride[i];
   a.dq = dq, a.dk = dk, a.dv = dv, a.dtable = dbias_table;
-  a.diag = reinterpret_cast<float*>(ws + plan.diag);
   a.delta = reinterpret_cast<float*>(ws + plan.delta);
   a.part_table = reinterpret_cast<float*>(ws + plan.part_table);
   a.table_parts = plan.table_parts;
-  hipError_t e = a.table != nullptr ? launch_attn_diag(a, s) : hipSuccess;
-  if (e == hipSuccess) e = launch_attn_backward(a, s);
-  return done(e, "attention backward launch");
+  a.kv_parts = plan.kv_parts;
+  a.part_kv = reinterpret_cast<float*>(ws + plan.part_kv);
+  return done(launch_attn_backward(a, s), "attention backward launch");
 }
 
 }  // extern "C"

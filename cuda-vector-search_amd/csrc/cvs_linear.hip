@@ -19,43 +19,68 @@ namespace cvs {
 namespace {
 
 constexpr int kDepth = 64;                    // reduction steps of a stage
-constexpr uint32_t kOutside = 0x80000000u;    // a byte offset past every buffer
-
-typedef int i32x4s __attribute__((ext_vector_type(4)));
-
-// 16 bytes a lane from base + voff into LDS at lds + 16 * lane; zeros where voff >= kOutside.
-__device__ __forceinline__ void load_lds(uint32_t voff, const unsigned char* base, uint32_t lds) {
-  const uint64_t b = (uint64_t)(uintptr_t)base;
-  const i32x4s rsrc = {__builtin_amdgcn_readfirstlane((int)(uint32_t)b),
-                       __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32) & 0xffff), (int)kOutside, 0x00020000};
-  const uint32_t m = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds);
-  uint32_t saved;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %1\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %2, %3, 0 offen lds\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(saved)
-      : "s"(m), "v"(voff), "s"(rsrc)
-      : "memory");
+// The normal distribution's Phi(-t), t >= 0, is exp(-t^2 / 2) times a smooth function, here
+// a polynomial in q = 1 / (1 + 0.3 t) fitted for least relative error: within 2.2e-6 of
+// Phi for t <= 6, 6e-5 to 14, where Phi is below 1e-44.  (The error function of the
+// math library costs some 40 instructions; with it the epilogue of 16384 x 2048, k = 768,
+// took three times as long as the products.)  *g receives exp(-t^2 / 2).
+__device__ __forceinline__ float phi(float z, float* g) {
+  const float t = fabsf(z);
+  const float q = __builtin_amdgcn_rcpf(fmaf(0.3f, t, 1.f));
+  *g = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+  float r = -0.0814668289f;
+  r = fmaf(r, q, 0.229237331f);
+  r = fmaf(r, q, -0.0321202955f);
+  r = fmaf(r, q, 0.15242397f);
+  r = fmaf(r, q, 0.111656703f);
+  r = fmaf(r, q, 0.120269536f);
+  r = r * q * *g;
+  return z < 0.f ? r : 1.f - r;
 }
 
-__device__ __forceinline__ float activate(float z, int act) {
-  if (act == kActGelu) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-  if (act == kActRelu) return z > 0.f ? z : (z != z ? z : 0.f);
-  if (act == kActTanh) return tanhf(z);
-  return z;
+// tanh x = x (1 - x^2 / 3 + 2 x^4 / 15) near 0, where 1 - exp(-2 |x|) would lose digits.
+__device__ __forceinline__ float tanh16(float x) {
+  const float e = __builtin_amdgcn_exp2f(fabsf(x) * -2.8853900817779268f);
+  const float t = copysignf((1.f - e) * __builtin_amdgcn_rcpf(1.f + e), x);
+  const float x2 = x * x;
+  const float s = x * fmaf(x2, fmaf(x2, 0.13333333333333333f, -0.33333333333333333f), 1.f);
+  return fabsf(x) < 0.0625f ? s : t;
 }
 
-__device__ __forceinline__ float slope(float z, int act) {
-  if (act == kActGelu) return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
-  if (act == kActRelu) return z > 0.f ? 1.f : 0.f;
-  if (act == kActTanh) {
-    const float t = tanhf(z);
-    return 1.f - t * t;
+// Eight neighbouring values through an activation, or times its slope (the same branch for a whole launch).
+__device__ __forceinline__ void activate8(float* z, int act) {
+  if (act == kActGelu) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float g;
+      z[e] *= phi(z[e], &g);
+    }
+  } else if (act == kActRelu) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] = z[e] <= 0.f ? 0.f : z[e];  // (a NaN stays)
+  } else if (act == kActTanh) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] = tanh16(z[e]);
   }
-  return 1.f;
+}
+__device__ __forceinline__ void times_slope8(float* dy, const float* z, int act) {
+  if (act == kActGelu) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float g;
+      const float p = phi(z[e], &g);
+      dy[e] *= fmaf(z[e] * 0.39894228040143268f, g, p);
+    }
+  } else if (act == kActRelu) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dy[e] = z[e] > 0.f ? dy[e] : 0.f;
+  } else if (act == kActTanh) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float t = tanh16(z[e]);
+      dy[e] *= 1.f - t * t;
+    }
+  }
 }
 
 template <class T>
@@ -73,41 +98,62 @@ __device__ __forceinline__ void store8(T* p, const float* f) {
   *reinterpret_cast<typename Frag<T>::V*>(p) = v;
 }
 
-// The epilogue of 8 neighbouring sums of row i, columns j .. j + 7.
+// The epilogue of 8 neighbouring sums of row i, columns j .. j + 7, in place; pre receives them before the activation.
 template <class T>
-__device__ __forceinline__ void finish8(const GemmArgs& a, int i, int j, float* z) {
+__device__ __forceinline__ void finish8(const GemmArgs& a, int i, int j, float* z, float* pre) {
   if (a.bias != nullptr) {
     float b[8];
     load8((const T*)a.bias + j, b);
 #pragma unroll
     for (int e = 0; e < 8; ++e) z[e] += b[e];
   }
-  const int64_t at = (int64_t)i * a.n + j;
-  if (a.pre != nullptr) store8((T*)a.pre + at, z);
-  if (a.act != kActNone) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) z[e] = activate(z[e], a.act);
-  }
+  for (int e = 0; e < 8; ++e) pre[e] = z[e];
+  activate8(z, a.act);
   if (a.residual != nullptr) {
     float r[8];
     load8((const T*)a.residual + (int64_t)i * a.ld_res + j, r);
 #pragma unroll
     for (int e = 0; e < 8; ++e) z[e] += r[e];
   }
-  store8((T*)a.out + at, z);
 }
 
-template <class T, int TM, int TN, int RING, bool MS, bool NS>
-__global__ __launch_bounds__(kBlock, 2) void gemm_kernel(GemmArgs a) {
-  constexpr int LM = TM / 32, LN = TN / 32;           // 1 KiB loads a wave and stage
-  constexpr int BM = TM / 64, BN = TN / 64;           // 32 x 32 blocks a wave: 2 x 2 waves
-  constexpr int MBYTES = TM * 128, STAGE = (TM + TN) * 128;
+// Stores a 32 x 32 block of which lane l holds, of row l % 32, columns 8 g .. and 16 + 8 g ..
+// (g = l / 32): 16 lanes exchange their pieces with the next 16 so that four lanes write
+// 64 contiguous bytes of a row.
+template <class T>
+__device__ __forceinline__ void store_block(T* out, int64_t ld, int m, int n, int row0, int col0, const float* z0, const float* z1) {
+  typename Frag<T>::V v0, v1;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v0[e] = (T)z0[e], v1[e] = (T)z1[e];
+  u32x4 x = __builtin_bit_cast(u32x4, v0), y = __builtin_bit_cast(u32x4, v1);
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const auto s = __builtin_amdgcn_permlane16_swap(x[r], y[r], false, false);
+    x[r] = s[0], y[r] = s[1];
+  }
+  const int lane = threadIdx.x & 63;
+  const int row = row0 + (lane & 15), col = col0 + 16 * ((lane >> 4) & 1) + 8 * (lane >> 5);
+  if (col < n) {
+    T* to = out + (int64_t)row * ld + col;
+    if (row < m) *reinterpret_cast<u32x4*>(to) = x;
+    if (row + 16 < m) *reinterpret_cast<u32x4*>(to + 16 * ld) = y;
+  }
+}
+
+// WM x WN waves of BM x BN blocks of 32 x 32, RING stages in LDS.
+template <class T, int WM, int WN, int BM, int BN, int RING, bool MS, bool NS>
+__global__ __launch_bounds__(64 * WM * WN, (WM * BM + WN * BN) * RING <= 16 ? 2 : 1) void gemm_kernel(GemmArgs a) {
+  constexpr int W = WM * WN, TM = WM * BM * 32, TN = WN * BN * 32;
+  constexpr int MBYTES = TM * kDepth * 2, STAGE = (TM + TN) * kDepth * 2;
+  constexpr int LM = MBYTES / 1024 / W, LN = (STAGE - MBYTES) / 1024 / W;  // 1 KiB loads a wave and stage
+  static_assert(LM * 1024 * W == MBYTES && (LM + LN) * 1024 * W == STAGE, "whole loads");
   typedef typename Frag<T>::V V;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[RING * STAGE];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave & 1, wn = wave >> 1;
+  const int wm = wave % WM, wn = wave / WM;
   const int l32 = lane & 31, g = lane >> 5;
   const int p16 = lane >> 4, s16 = lane & 15;
 
@@ -129,17 +175,17 @@ __global__ __launch_bounds__(kBlock, 2) void gemm_kernel(GemmArgs a) {
   uint32_t vm[LM], vn[LN];
   int km[LM], kn[LN];  // reduction step of the load within a stage
   auto place = [&](int j, bool strided, int64_t ld, int first, int rows, uint32_t* voff, int* step) {
-    const int line = (wave + 4 * j) * 8 + (lane >> 3);
+    const int line = (wave + W * j) * 8 + (lane >> 3);
     const int piece = (lane & 7) ^ piece_swizzle(line);
     if (strided) {
-      const int col = line / 64 * 64 + piece * 8;
-      *voff = (uint32_t)((line & 63) * ld * 2) + (uint32_t)(col * 2);
+      const int col = line / kDepth * 64 + piece * 8;
+      *step = line % kDepth;
+      *voff = (uint32_t)(*step * ld * 2) + (uint32_t)(col * 2);
       if (first + col >= rows) *voff = kOutside;
-      *step = line & 63;
     } else {
+      *step = piece * 8;
       *voff = (uint32_t)(line * ld * 2) + (uint32_t)(piece * 16);
       if (first + line >= rows) *voff = kOutside;
-      *step = piece * 8;
     }
   };
 #pragma unroll
@@ -151,16 +197,16 @@ __global__ __launch_bounds__(kBlock, 2) void gemm_kernel(GemmArgs a) {
   const int64_t mstep = 2 * (MS ? kDepth * a.ldm : (int64_t)kDepth), nstep = 2 * (NS ? kDepth * a.ldn : (int64_t)kDepth);
   mbase += s_begin * mstep;
   nbase += s_begin * nstep;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)smem;
+  const uint32_t lds0 = lds_address(smem);
 
   int load_s = s_begin, load_buf = 0;
   auto load_stage = [&]() {
     const uint32_t at = lds0 + (uint32_t)(load_buf * STAGE + wave * 1024);
     const int left = a.k - load_s * kDepth;  // reduction steps from this stage on
 #pragma unroll
-    for (int j = 0; j < LM; ++j) load_lds(km[j] < left ? vm[j] : kOutside, mbase, at + j * 4096);
+    for (int j = 0; j < LM; ++j) load_lds(km[j] < left ? vm[j] : kOutside, mbase, at + j * (W * 1024));
 #pragma unroll
-    for (int j = 0; j < LN; ++j) load_lds(kn[j] < left ? vn[j] : kOutside, nbase, at + MBYTES + j * 4096);
+    for (int j = 0; j < LN; ++j) load_lds(kn[j] < left ? vn[j] : kOutside, nbase, at + MBYTES + j * (W * 1024));
     mbase += mstep;
     nbase += nstep;
     ++load_s;
@@ -173,14 +219,14 @@ __global__ __launch_bounds__(kBlock, 2) void gemm_kernel(GemmArgs a) {
       const int c = reorder ? ((s16 & 1) << 1) | ((s16 >> 1) & 1) : s16 & 3;
       const int col = r0 + 16 * (p16 & 1) + 4 * c;
       const int line = 16 * ks + 8 * (p16 >> 1) + (s16 >> 2);
-      const unsigned char* panel = t + (col >> 6) * 8192 + (col & 4) * 2;
+      const unsigned char* panel = t + (col >> 6) * (kDepth * 128) + (col & 4) * 2;
       const int piece = (col & 63) >> 3;
       const s16x4 lo = read_tr(panel + line * 128 + ((piece ^ piece_swizzle(line)) << 4));
       const s16x4 hi = read_tr(panel + (line + 4) * 128 + ((piece ^ piece_swizzle(line + 4)) << 4));
       return join_tr<T>(lo, hi);
     }
-    const int line = r0 + (reorder ? tile_row(l32) : l32);
-    return *reinterpret_cast<const V*>(t + line * 128 + (((2 * ks + g) ^ piece_swizzle(line)) << 4));
+    const int r = r0 + (reorder ? tile_row(l32) : l32);
+    return *reinterpret_cast<const V*>(t + row_offset<kDepth>(r, 2 * ks + g));
   };
 
   f32x16 acc[BM][BN];
@@ -208,7 +254,7 @@ __global__ __launch_bounds__(kBlock, 2) void gemm_kernel(GemmArgs a) {
     const unsigned char* tm = smem + buf * STAGE;
     const unsigned char* tn = tm + MBYTES;
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
+    for (int ks = 0; ks < kDepth / 16; ++ks) {
       V fm[BM], fn[BN];
 #pragma unroll
       for (int i = 0; i < BM; ++i) fm[i] = frag(tm, MS, (wm * BM + i) * 32, ks, false);
@@ -222,28 +268,37 @@ __global__ __launch_bounds__(kBlock, 2) void gemm_kernel(GemmArgs a) {
     buf = buf + 1 == RING ? 0 : buf + 1;
   }
 
-  // Lane: row i of the output, 8 neighbouring columns a half of its accumulator.
+  // Lane: a row of the output, two times 8 neighbouring columns of each block.
 #pragma unroll
   for (int i = 0; i < BM; ++i) {
-    const int row = m0 + (wm * BM + i) * 32 + l32;
+    const int row0 = m0 + (wm * BM + i) * 32, row = row0 + l32;
 #pragma unroll
-    for (int j = 0; j < BN; ++j)
+    for (int j = 0; j < BN; ++j) {
+      const int col0 = n0 + (wn * BN + j) * 32, col = col0 + 8 * g;
+      if (a.splits > 1) {
+        float* p = a.partial + ((int64_t)blockIdx.y * a.m + row) * a.n + col;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int col = n0 + (wn * BN + j) * 32 + 16 * h + 8 * g;
-        float z[8];
+        for (int h = 0; h < 2; ++h)
+          if (row < a.m && col + 16 * h < a.n) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) z[e] = acc[i][j][8 * h + e];
-        if (row < a.m && col < a.n) {
-          if (a.splits > 1) {
-            float* p = a.partial + ((int64_t)blockIdx.y * a.m + row) * a.n + col;
-            *reinterpret_cast<f32x4*>(p) = f32x4{z[0], z[1], z[2], z[3]};
-            *reinterpret_cast<f32x4*>(p + 4) = f32x4{z[4], z[5], z[6], z[7]};
-          } else {
-            finish8<T>(a, row, col, z);
+            for (int q = 0; q < 2; ++q) {
+              const int e = 8 * h + 4 * q;
+              *reinterpret_cast<f32x4*>(p + 16 * h + 4 * q) =
+                  f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+            }
           }
-        }
+      } else {
+        float z[16], pre[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z[e] = acc[i][j][e];
+        // rows and columns past the edge: those of the last ones again, not stored
+        const int r = min(row, a.m - 1);
+        finish8<T>(a, r, min(col, a.n - 8), z, pre);
+        finish8<T>(a, r, min(col + 16, a.n - 8), z + 8, pre + 8);
+        if (a.pre != nullptr) store_block((T*)a.pre, a.n, a.m, a.n, row0, col0, pre, pre + 8);
+        store_block((T*)a.out, a.n, a.m, a.n, row0, col0, z, z + 8);
       }
+    }
   }
 }
 
@@ -265,23 +320,27 @@ __global__ __launch_bounds__(kBlock) void gemm_join_kernel(GemmArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) z[e] += lo[e], z[4 + e] += hi[e];
   }
-  finish8<T>(a, (int)i, j, z);
+  float pre[8];
+  finish8<T>(a, (int)i, j, z, pre);
+  if (a.pre != nullptr) store8((T*)a.pre + i * a.n + j, pre);
+  store8((T*)a.out + i * a.n + j, z);
 }
 
-template <class T, int TM, int TN, int RING>
+template <class T, int WM, int WN, int BM, int BN, int RING>
 hipError_t launch_tiles(const GemmArgs& a, hipStream_t s) {
+  constexpr int TM = WM * BM * 32, TN = WN * BN * 32;
   const int tiles = ((a.m + TM - 1) / TM) * ((a.n + TN - 1) / TN);
-  const dim3 grid((tiles + 7) / 8 * 8, a.splits), block(kBlock);
+  const dim3 grid((tiles + 7) / 8 * 8, a.splits), block(64 * WM * WN);
   if (a.m_strided && a.n_strided)
-    hipLaunchKernelGGL((gemm_kernel<T, TM, TN, RING, true, true>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((gemm_kernel<T, WM, WN, BM, BN, RING, true, true>), grid, block, 0, s, a);
   else if (a.n_strided)
-    hipLaunchKernelGGL((gemm_kernel<T, TM, TN, RING, false, true>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((gemm_kernel<T, WM, WN, BM, BN, RING, false, true>), grid, block, 0, s, a);
   else
-    hipLaunchKernelGGL((gemm_kernel<T, TM, TN, RING, false, false>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((gemm_kernel<T, WM, WN, BM, BN, RING, false, false>), grid, block, 0, s, a);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && a.splits > 1) {
     const int64_t threads = (int64_t)a.m * (a.n / 8);
-    hipLaunchKernelGGL((gemm_join_kernel<T>), dim3((unsigned)((threads + kBlock - 1) / kBlock)), block, 0, s, a);
+    hipLaunchKernelGGL((gemm_join_kernel<T>), dim3((unsigned)((threads + kBlock - 1) / kBlock)), dim3(kBlock), 0, s, a);
     e = hipGetLastError();
   }
   return e;
@@ -289,50 +348,98 @@ hipError_t launch_tiles(const GemmArgs& a, hipStream_t s) {
 
 template <class T>
 hipError_t launch_typed(const GemmArgs& a, const GemmPlan& p, hipStream_t s) {
-  if (p.tm == 128) return launch_tiles<T, 128, 128, 2>(a, s);
-  return launch_tiles<T, 64, 64, 3>(a, s);
+  if (p.tile == 256) return launch_tiles<T, 2, 4, 4, 2, 2>(a, s);
+  if (p.tile == 128) return launch_tiles<T, 2, 2, 2, 2, 2>(a, s);
+  return launch_tiles<T, 2, 2, 1, 1, 3>(a, s);
 }
 
-// dz = dy act'(pre), 8 columns a thread, rows blockIdx.y, + gridDim.y, ...; column sums a part.
+// dz = dy act'(pre) and its column sums, bound by memory.  A workgroup has up to 256
+// pieces of 8 columns (blockIdx.x) and as many of its part's rows at a time as its threads
+// cover; it adds its row lanes' sums in LDS and writes one partial row.
 template <class T>
 __global__ __launch_bounds__(kBlock) void act_grad_kernel(ActGradArgs a) {
-  const int c = (blockIdx.x * kBlock + threadIdx.x) * 8;
-  if (c >= a.n) return;
+  __shared__ float red[kBlock * 8];
+  const int pieces = min(a.n / 8 - (int)blockIdx.x * kBlock, kBlock), lanes = kBlock / pieces;
+  const int p = threadIdx.x % pieces, rl = threadIdx.x / pieces;
+  const int c = (blockIdx.x * kBlock + p) * 8;
   float sum[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) sum[e] = 0.f;
-  for (int64_t r = blockIdx.y; r < a.m; r += gridDim.y) {
-    float g[8];
-    load8((const T*)a.dy + r * a.dy_stride + c, g);
-    if (a.act != kActNone) {
-      float z[8];
-      load8((const T*)a.pre + r * a.n + c, z);
+  const int64_t r0 = a.m * blockIdx.y / gridDim.y, r1 = a.m * (blockIdx.y + 1) / gridDim.y;
+  if (rl < lanes) {
+    const bool act = a.act != kActNone;
+    constexpr int U = 4;  // rows under way
+    for (int64_t r = r0 + rl; r < r1; r += U * lanes) {
+      typename Frag<T>::V g[U], z[U];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) g[e] *= slope(z[e], a.act);
-      store8((T*)a.dz + r * a.n + c, g);
+      for (int u = 0; u < U; ++u) {
+        const int64_t row = min(r + u * lanes, r1 - 1);
+        g[u] = *reinterpret_cast<const typename Frag<T>::V*>((const T*)a.dy + row * a.dy_stride + c);
+        if (act) z[u] = *reinterpret_cast<const typename Frag<T>::V*>((const T*)a.pre + row * a.n + c);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t row = r + u * lanes;
+        if (row < r1) {
+          float gf[8], zf[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) gf[e] = (float)g[u][e];
+          if (act) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) zf[e] = (float)z[u][e];
+            times_slope8(gf, zf, a.act);
+            store8((T*)a.dz + row * a.n + c, gf);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum[e] += gf[e];
+        }
+      }
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum[e] += g[e];
   }
-  if (a.partial != nullptr) {
-    float* p = a.partial + (int64_t)blockIdx.y * a.n + c;
-    *reinterpret_cast<f32x4*>(p) = f32x4{sum[0], sum[1], sum[2], sum[3]};
-    *reinterpret_cast<f32x4*>(p + 4) = f32x4{sum[4], sum[5], sum[6], sum[7]};
+  if (a.partial == nullptr) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) red[threadIdx.x * 8 + e] = sum[e];
+  __syncthreads();
+  float* out = a.partial + (int64_t)blockIdx.y * a.n + (int64_t)blockIdx.x * kBlock * 8;
+  for (int t = threadIdx.x; t < pieces * 8; t += kBlock) {
+    float s = 0.f;
+    for (int l = 0; l < lanes; ++l) s += red[l * pieces * 8 + t];
+    out[t] = s;
   }
 }
 
 }  // namespace
 
-GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, bool m_strided, bool n_strided, int cus) {
-  (void)m_strided, (void)n_strided;
-  GemmPlan p;
-  auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
-  p.tm = p.tn = tiles(128) >= cus ? 128 : 64;
-  // a reduction long enough is split where the tiles leave CUs idle
-  const int64_t t = tiles(p.tm), stages = (k + kDepth - 1) / kDepth;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(cus / std::max<int64_t>(t, 1), stages / 8));
-  p.ws_bytes = p.splits > 1 ? (int64_t)p.splits * m * n * 4 : 0;
-  return p;
+// Tiles of 256 x 256 (8 waves, one workgroup a CU), 128 x 128 and 64 x 64 (4 waves, two and three
+// workgroups a CU), and parts of the reduction where the tiles leave CUs idle: the choice of
+// least estimated time.  A CU runs its workgroups in rounds; a stage of a round costs what was
+// measured on long reductions (8192 x 8192, k = 2048: 1080, 850 and 480 TFLOP/s, that is 1.9,
+// 1.2 and 0.9 us with 1, 2 and 3 workgroups), a round 3 us more to fill and finish, and a split
+// 3 us and its sums' way to memory and back.  At 16384 x 2048, k = 768 that gives 256 x 256 (56 us
+// against 64 with 128 x 128), at 10007 x 768, k = 2048 128 x 128 (37 against 54), at 2048 x 768,
+// k = 16384 128 x 128 in 5 parts (62 against 68 for 256 x 256 in 10, 153 unsplit).
+GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int cus) {
+  static constexpr struct { int tile, wgs; double stage; } kTiles[] = {{256, 1, 1.9}, {128, 2, 1.2}, {64, 3, 0.9}};
+  const int64_t stages = (k + kDepth - 1) / kDepth;
+  GemmPlan best = {};
+  double least = 1e30;
+  for (const auto& t : kTiles) {
+    const int64_t tiles = ((m + t.tile - 1) / t.tile) * ((n + t.tile - 1) / t.tile);
+    for (int64_t splits = 1; splits <= 16 && (splits == 1 || splits * 8 <= stages); ++splits) {
+      const int64_t wgs = tiles * splits, full = wgs / (t.wgs * (int64_t)cus);
+      // a last round of few workgroups has more of a CU for each, but not below a stage's latency
+      const int64_t rest = (wgs - full * t.wgs * cus + cus - 1) / cus;
+      const double per = full * t.stage + (rest > 0 ? std::max(rest * t.stage / t.wgs, 0.5) : 0.0);
+      double us = (stages + splits - 1) / splits * per + 3.0 * (full + (rest > 0));
+      if (splits > 1) us += 3.0 + 2.0 * splits * m * n * 4 / 4e6;
+      if (us < least) {
+        least = us;
+        best.tile = t.tile, best.splits = (int)splits;
+        best.ws_bytes = splits > 1 ? splits * m * n * 4 : 0;
+      }
+    }
+  }
+  return best;
 }
 
 hipError_t launch_gemm(const GemmArgs& a, const GemmPlan& p, hipStream_t s) {
@@ -340,8 +447,8 @@ hipError_t launch_gemm(const GemmArgs& a, const GemmPlan& p, hipStream_t s) {
 }
 
 int act_grad_parts(int64_t m, int64_t n, int cus) {
-  const int64_t blocks = (n / 8 + kBlock - 1) / kBlock;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(m, 8 * cus / blocks));
+  const int64_t blocks = (n / 8 + kBlock - 1) / kBlock, lanes = std::max<int64_t>(1, kBlock / std::min<int64_t>(n / 8, kBlock));
+  return (int)std::max<int64_t>(1, std::min<int64_t>((m + lanes - 1) / lanes, 3 * cus / blocks));
 }
 
 hipError_t launch_act_grad(const ActGradArgs& a, hipStream_t s) {
@@ -351,7 +458,7 @@ hipError_t launch_act_grad(const ActGradArgs& a, hipStream_t s) {
   else
     hipLaunchKernelGGL(act_grad_kernel<__bf16>, grid, block, 0, s, a);
   hipError_t e = hipGetLastError();
-  if (e == hipSuccess && a.dbias != nullptr) e = launch_column_sums(a.partial, a.parts, a.n, a.n, a.type, a.dbias, s);
+  if (e == hipSuccess && a.dbias != nullptr) e = launch_column_sums(a.partial, a.parts, a.n, a.n, 0, a.type, a.dbias, nullptr, s);
   return e;
 }
 

@@ -42,6 +42,48 @@ struct Frag<__bf16> {
 
 __device__ __forceinline__ constexpr int piece_swizzle(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
 
+// Lines that hold two rows of 64 bytes: the same piece of 8 consecutive rows, and two
+// neighbouring pieces of 4 consecutive rows, lie on distinct banks.
+__device__ __forceinline__ constexpr int pair_swizzle(int line) { return ((line & 1) << 1) | ((line >> 1) & 1); }
+
+// Byte offset of a row's 16-byte piece in a tile of rows of WIDTH 16-bit columns (32, 64 or 128).
+template <int WIDTH>
+__device__ __forceinline__ int row_offset(int row, int piece) {
+  if constexpr (WIDTH == 32) {
+    const int line = row >> 1;
+    return line * 128 + ((((row & 1) * 4 + piece) ^ pair_swizzle(line)) << 4);
+  } else {
+    return row * (2 * WIDTH) + ((piece ^ piece_swizzle(row)) << 4);
+  }
+}
+
+// A byte offset past the end of every buffer: loads there give zeros.
+constexpr uint32_t kOutside = 0x80000000u;
+
+typedef int i32x4s __attribute__((ext_vector_type(4)));
+
+// 16 bytes a lane from base + voff into LDS at lds + 16 * lane; zeros where voff >= kOutside.
+__device__ __forceinline__ void load_lds(uint32_t voff, const unsigned char* base, uint32_t lds) {
+  const uint64_t b = (uint64_t)(uintptr_t)base;
+  const i32x4s rsrc = {__builtin_amdgcn_readfirstlane((int)(uint32_t)b),
+                       __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32) & 0xffff), (int)kOutside, 0x00020000};
+  const uint32_t m = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds);
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %2, %3, 0 offen lds\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "s"(m), "v"(voff), "s"(rsrc)
+      : "memory");
+}
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+
 // Row of a 32-row block that operand row m stands for.
 __device__ __forceinline__ constexpr int tile_row(int m) {
   return 16 * (m >> 4) + 8 * ((m >> 2) & 1) + 4 * ((m >> 3) & 1) + (m & 3);

@@ -172,21 +172,43 @@ __global__ __launch_bounds__(kBlock) void norm_backward_kernel(NormArgs a) {
     if (c < a.d) load_vec<T, VEC>(w + c, wf[i]);
   }
   const float inv_d = 1.f / (float)a.d;
-  for (int64_t row = (int64_t)blockIdx.x * kWaves + wave; row < a.n; row += (int64_t)gridDim.x * kWaves) {
+  const int64_t step = (int64_t)gridDim.x * kWaves;
+  typename Vec<T, VEC>::V xr[P], gr[P];  // the next row, under way while this one is computed
+  float mean_r = 0.f, rstd_r = 0.f;
+  auto fetch = [&](int64_t row) {
     const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_stride;
     const T* dy = reinterpret_cast<const T*>(a.dy) + row * a.dy_stride;
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    float h[P][VEC], g[P][VEC];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       const int c = (lane + 64 * i) * VEC;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) h[i][j] = mean, g[i][j] = 0.f;
       if (c < a.d) {
-        load_vec<T, VEC>(x + c, h[i]);
-        load_vec<T, VEC>(dy + c, g[i]);
+        xr[i] = *reinterpret_cast<const typename Vec<T, VEC>::V*>(x + c);
+        gr[i] = *reinterpret_cast<const typename Vec<T, VEC>::V*>(dy + c);
       }
     }
+    mean_r = a.mean[row];
+    rstd_r = a.rstd[row];
+  };
+  int64_t row = (int64_t)blockIdx.x * kWaves + wave;
+  if (row < a.n) fetch(row);
+  for (; row < a.n; row += step) {
+    const float mean = mean_r, rstd = rstd_r;
+    float h[P][VEC], g[P][VEC];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const bool in = (lane + 64 * i) * VEC < a.d;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        if constexpr (VEC == 1) {
+          h[i][j] = in ? (float)xr[i] : mean;
+          g[i][j] = in ? (float)gr[i] : 0.f;
+        } else {
+          h[i][j] = in ? (float)xr[i][j] : mean;
+          g[i][j] = in ? (float)gr[i][j] : 0.f;
+        }
+      }
+    }
+    if (row + step < a.n) fetch(row + step);
     float sg = 0.f, sgh = 0.f;
 #pragma unroll
     for (int i = 0; i < P; ++i)
@@ -270,28 +292,37 @@ __global__ __launch_bounds__(kBlock) void norm_columns_kernel(NormArgs a) {
   part[a.d + c] = db;
 }
 
-// 64 columns a workgroup, 16 waves over the partial rows; added in a fixed order.
+// Adds partial rows in a fixed order: 16 columns a workgroup, 64 threads a column, whose loads
+// (eight of them for 512 rows) are under way together; then a tree in LDS.
 template <class T>
-__global__ __launch_bounds__(1024) void column_sums_kernel(const float* partial, int parts, int64_t stride, int n, T* out) {
-  __shared__ float red[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = blockIdx.x * 64 + lane;
-  float s = 0.f;
-  if (c < n)
-    for (int p = wave; p < parts; p += 16) s += partial[p * stride + c];
-  red[wave][lane] = s;
-  __syncthreads();
-  if (wave == 0 && c < n) {
-    float t = 0.f;
+__global__ __launch_bounds__(1024) void column_sums_kernel(const float* partial, int parts, int64_t stride, int n, T* out,
+                                                           T* out2, int n1) {
+  __shared__ float red[64][17];
+  const int col = threadIdx.x & 15, lane = threadIdx.x >> 4;
+  const int c = blockIdx.x * 16 + col;
+  float s[8];
 #pragma unroll
-    for (int w = 0; w < 16; ++w) t += red[w][lane];
-    out[c] = (T)t;
+  for (int u = 0; u < 8; ++u) s[u] = 0.f;
+  if (c < n)
+    for (int p = lane; p < parts; p += 512)
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (p + 64 * u < parts) s[u] += partial[(p + 64 * u) * stride + c];
+  red[lane][col] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+#pragma unroll
+  for (int half = 32; half > 0; half >>= 1) {
+    __syncthreads();
+    if (lane < half) red[lane][col] += red[lane + half][col];
+  }
+  if (lane == 0 && c < n) {
+    T* to = c < n1 ? out + c : out2 + (c - n1);
+    *to = (T)red[0][col];
   }
 }
 
 template <class T>
 bool aligned_rows(const NormArgs& a, int vec, bool backward) {
-  auto ok = [&](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  auto ok = [&](const void* p) { return reinterpret_cast<uintptr_t>(p) % (vec * sizeof(T)) == 0; };
   if (a.d % vec != 0 || a.x_stride % vec != 0 || !ok(a.x) || !ok(a.weight)) return false;
   if (backward) return a.dy_stride % vec == 0 && ok(a.dy) && ok(a.dx);
   return ok(a.bias) && ok(a.y);
@@ -307,21 +338,25 @@ void launch_rows(const NormArgs& a, bool backward, hipStream_t s) {
     hipLaunchKernelGGL((norm_forward_kernel<T, VEC, P>), dim3((unsigned)((a.n + 3) / 4)), dim3(kBlock), 0, s, a);
 }
 
-// The fewest columns a lane that hold the row: 16-byte pieces where every row starts
-// on 16 bytes, single elements otherwise.
+// The fewest columns a lane that hold the row: pieces of 4 where every row starts on one,
+// single elements otherwise.  (Pieces of 8 of 16-bit rows leave a quarter of the lanes' second
+// piece empty at width 768, the registers with it.)
 template <class T>
 void launch_narrow(const NormArgs& a, bool backward, hipStream_t s) {
-  constexpr int VEC = 16 / sizeof(T);
   const int lanes = (a.d + 63) / 64;
-  if (aligned_rows<T>(a, VEC, backward)) {
-    if (lanes <= VEC)
-      launch_rows<T, VEC, 1>(a, backward, s);
-    else if (lanes <= 2 * VEC)
-      launch_rows<T, VEC, 2>(a, backward, s);
+  if (aligned_rows<T>(a, 4, backward)) {
+    if (lanes <= 4)
+      launch_rows<T, 4, 1>(a, backward, s);
+    else if (lanes <= 8)
+      launch_rows<T, 4, 2>(a, backward, s);
+    else if (lanes <= 12)
+      launch_rows<T, 4, 3>(a, backward, s);
     else if (lanes <= 16)
-      launch_rows<T, VEC, 16 / VEC>(a, backward, s);
+      launch_rows<T, 4, 4>(a, backward, s);
+    else if (lanes <= 24)
+      launch_rows<T, 4, 6>(a, backward, s);
     else
-      launch_rows<T, VEC, 32 / VEC>(a, backward, s);
+      launch_rows<T, 4, 8>(a, backward, s);
   } else {
     if (lanes <= 4)
       launch_rows<T, 1, 4>(a, backward, s);
@@ -355,17 +390,19 @@ void backward(const NormArgs& a, hipStream_t s) {
 int norm_backward_parts(int64_t n, int64_t d, int type, int cus) {
   (void)type;
   if (d > kRegWidth) return (int)std::min<int64_t>(n, 64);
-  return (int)std::min<int64_t>((n + 3) / 4, 2 * cus);
+  return (int)std::min<int64_t>((n + 3) / 4, 4 * cus);
 }
 
-hipError_t launch_column_sums(const float* partial, int parts, int64_t stride, int n, int type, void* out, hipStream_t s) {
-  const dim3 grid((n + 63) / 64), block(1024);
+hipError_t launch_column_sums(const float* partial, int parts, int64_t stride, int n1, int n2, int type, void* out, void* out2,
+                              hipStream_t s) {
+  const int n = n1 + n2;
+  const dim3 grid((n + 15) / 16), block(1024);
   if (type == kF16)
-    hipLaunchKernelGGL(column_sums_kernel<_Float16>, grid, block, 0, s, partial, parts, stride, n, (_Float16*)out);
+    hipLaunchKernelGGL(column_sums_kernel<_Float16>, grid, block, 0, s, partial, parts, stride, n, (_Float16*)out, (_Float16*)out2, n1);
   else if (type == kBF16)
-    hipLaunchKernelGGL(column_sums_kernel<__bf16>, grid, block, 0, s, partial, parts, stride, n, (__bf16*)out);
+    hipLaunchKernelGGL(column_sums_kernel<__bf16>, grid, block, 0, s, partial, parts, stride, n, (__bf16*)out, (__bf16*)out2, n1);
   else
-    hipLaunchKernelGGL(column_sums_kernel<float>, grid, block, 0, s, partial, parts, stride, n, (float*)out);
+    hipLaunchKernelGGL(column_sums_kernel<float>, grid, block, 0, s, partial, parts, stride, n, (float*)out, (float*)out2, n1);
   return hipGetLastError();
 }
 
@@ -387,10 +424,14 @@ hipError_t launch_norm_backward(const NormArgs& a, hipStream_t s) {
   else
     backward<float>(a, s);
   hipError_t e = hipGetLastError();
+  // the partial rows hold dweight's columns, then dbias's: one launch adds both
+  const int64_t stride = 2 * (int64_t)a.d;
+  if (e == hipSuccess && a.dweight != nullptr && a.dbias != nullptr)
+    return launch_column_sums(a.partial, a.parts, stride, a.d, a.d, a.type, a.dweight, a.dbias, s);
   if (e == hipSuccess && a.dweight != nullptr)
-    e = launch_column_sums(a.partial, a.parts, 2 * (int64_t)a.d, a.d, a.type, a.dweight, s);
+    e = launch_column_sums(a.partial, a.parts, stride, a.d, 0, a.type, a.dweight, nullptr, s);
   if (e == hipSuccess && a.dbias != nullptr)
-    e = launch_column_sums(a.partial + a.d, a.parts, 2 * (int64_t)a.d, a.d, a.type, a.dbias, s);
+    e = launch_column_sums(a.partial + a.d, a.parts, stride, a.d, 0, a.type, a.dbias, nullptr, s);
   return e;
 }
 

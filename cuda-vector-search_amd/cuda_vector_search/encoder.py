@@ -303,7 +303,7 @@ def _lengths(t, name: str, q):
 def _strided(t: torch.Tensor):
     """(tensor, strides) of [batch, position, head, width] with rows of 16-byte pieces; a copy where it has none."""
     strides = [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])]
-    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s % 8 for s in strides):
+    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s % 8 for s in strides) or strides[1] > 1 << 23:
         t = t.clone(memory_format=torch.contiguous_format)
         strides = list(t.stride()[:3])
     return t, _I64x3(*strides)

@@ -326,8 +326,8 @@ int cvs_linear_backward(const void* dy, const void* x, const void* w, const void
  * divide exact .. max_distance evenly in the logarithm (the last takes all further ones);
  * causal: per = buckets, and only the past counts; else per = buckets / 2 for keys at
  * or before the row, and another per for those after it.
- * Strides (batch, position, head) in elements, multiples of 8; width a multiple of 8, at
- * most 128; elements of a head contiguous; pointers 16-byte aligned.  Outputs are contiguous:
+ * Strides (batch, position, head) in elements, multiples of 8, a position's at most 2^23;
+ * width a multiple of 8, at most 128; elements of a head contiguous; pointers 16-byte aligned.  Outputs are contiguous:
  * out and dq [batch, q_len, heads, width], dk and dv [batch, k_len, k_heads, width],
  * lse (natural logarithm) [batch, heads, q_len], dbias_table [buckets, heads].
  */
