@@ -21,7 +21,7 @@ namespace {
 constexpr int kKeys = 64;  // keys of a tile
 
 template <class T, int DP, bool BIAS>
-__global__ __launch_bounds__(kBlock, 2) void attn_forward_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 3) void attn_forward_kernel(AttnArgs a) {
   typedef typename Frag<T>::V V;
   constexpr int KS = DP / 16, DB = DP / 32, TILE = kKeys * DP * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char sk[2][TILE], sv[2][TILE];
@@ -30,8 +30,8 @@ __global__ __launch_bounds__(kBlock, 2) void attn_forward_kernel(AttnArgs a) {
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int heads = a.batch * a.heads;
-  int block = blockIdx.x / heads;
-  if (a.causal) block = (a.lq + kAttnRows - 1) / kAttnRows - 1 - block;  // those with most keys first
+  // the last rows first: those see most keys when causal, and are of the longest sequences
+  const int block = (a.lq + kAttnRows - 1) / kAttnRows - 1 - blockIdx.x / heads;
   const int bh = blockIdx.x % heads;
   const int b = bh / a.heads, h = bh % a.heads, hk = h / (a.heads / a.k_heads);
   const int nk = key_count(a, b), nq = query_count(a, b), off = query_offset(a, b);
@@ -41,6 +41,23 @@ __global__ __launch_bounds__(kBlock, 2) void attn_forward_kernel(AttnArgs a) {
   const unsigned char* kbase = (const unsigned char*)a.k + 2 * (b * a.ks[0] + hk * a.ks[2]);
   const unsigned char* vbase = (const unsigned char*)a.v + 2 * (b * a.vs[0] + hk * a.vs[2]);
 
+  // this workgroup's keys: a part of those that some row of it sees
+  const int last_row = min(block * kAttnRows + kAttnRows, nq) - 1;
+  int end = last_row < block * kAttnRows ? 0 : nk;
+  if (a.causal) end = min(end, max(last_row + off + 1, 0));
+  const int tiles = (end + kKeys - 1) / kKeys;
+  int t0 = 0, t1 = tiles;
+  if (a.splits > 1) {  // (fewer than 2^23 tiles, at most 64 parts)
+    t0 = (int)((unsigned)tiles * blockIdx.y / (unsigned)a.splits);
+    t1 = (int)((unsigned)tiles * (blockIdx.y + 1) / (unsigned)a.splits);
+  }
+
+  const TileLoad<DP, kKeys> lk(2 * a.ks[1], a.d), lv(2 * a.vs[1], a.d);
+  auto load = [&](int t) {
+    lk.load(kbase, 2 * a.ks[1], t * kKeys, nk, sk[t & 1]);
+    lv.load(vbase, 2 * a.vs[1], t * kKeys, nk, sv[t & 1]);
+  };
+  if (t0 < t1) load(t0);
   V qf[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s) qf[s] = global_frag<T>(qrow, s, a.d, i < nq);
@@ -55,46 +72,51 @@ __global__ __launch_bounds__(kBlock, 2) void attn_forward_kernel(AttnArgs a) {
   float m = -__builtin_inff(), sum = 0.f;
   const float c = a.scale * kLog2e, slack = 8.f / c;
 
-  // this workgroup's keys: a part of those that some row of it sees
-  const int last_row = min(block * kAttnRows + kAttnRows, nq) - 1;
-  int end = last_row < block * kAttnRows ? 0 : nk;
-  if (a.causal) end = min(end, max(last_row + off + 1, 0));
-  const int tiles = (end + kKeys - 1) / kKeys;
-  const int t0 = (int)((int64_t)tiles * blockIdx.y / a.splits), t1 = (int)((int64_t)tiles * (blockIdx.y + 1) / a.splits);
-
-  const TileLoad<DP, kKeys> lk(2 * a.ks[1], a.d), lv(2 * a.vs[1], a.d);
-  auto load = [&](int t) {
-    lk.load(kbase, 2 * a.ks[1], t * kKeys, nk, sk[t & 1]);
-    lv.load(vbase, 2 * a.vs[1], t * kKeys, nk, sv[t & 1]);
-  };
-  if (t0 < t1) load(t0);
-  for (int t = t0; t < t1; ++t) {
+  // the tiles that a row of this wave sees a key of; through the others it only loads its share
+  int mine = r0 < nq ? t1 : t0;
+  if (a.causal) mine = max(t0, min(mine, (r0 + 32 + off + kKeys - 1) / kKeys));
+  for (int t = t0; t < mine; ++t) {
     const int buf = t & 1;
     tile_barrier();
     if (t + 1 < t1) load(t + 1);
     const int j0 = t * kKeys;
+    const int near = j0 - r0 - off;  // position of the tile's first key and the wave's first row
+    V rows[2][KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) rows[kb][s] = row_frag<T, DP>(sk[buf], kb * 32, s);
     f32x16 x[2];
     float shift = 0.f;  // a bias that all of the tile has
-    const int near = j0 - r0 - off;  // position of the tile's first key and the wave's first row
-    if (BIAS) {
-      const int reach = a.max_distance + kReach;
-      if (near - 31 >= a.max_distance || near + kKeys - 1 <= -a.max_distance) {
-        shift = tab[near > 0 ? 2 * reach : 0];
-        x[0] = x[1] = zero16();
-      } else {
-        const float* at = tab + (near - l32 + 8 * g + reach);
+    auto scores = [&]() {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+      for (int s = 0; s < KS; ++s)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) x[kb][e] = at[kb * 32 + elem_row(e, 0)];
-      }
-    } else {
+        for (int kb = 0; kb < 2; ++kb) x[kb] = Frag<T>::mfma(rows[kb][s], qf[s], x[kb]);
+    };
+    const int reach = a.max_distance + kReach;
+    if (!BIAS || near - 31 >= a.max_distance || near + kKeys - 1 <= -a.max_distance) {
+      if (BIAS) shift = tab[near > 0 ? 2 * reach : 0];
+      keep_order();
       x[0] = x[1] = zero16();
+      scores();
+    } else {
+      const float* at = tab + (near - l32 + 8 * g + reach);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[kb][e] = at[kb * 32 + elem_row(e, 0)];
+      keep_order();
+      scores();
     }
+    V cols[2][2][DB];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int s = 0; s < KS; ++s) x[kb] = Frag<T>::mfma(row_frag<T, DP>(sk[buf], kb * 32, s), qf[s], x[kb]);
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) cols[kb][s][d] = col_frag<T, DP>(sv[buf], kb * 32 + 16 * s, d * 32);
+    keep_order();
     if (j0 + kKeys > nk || (a.causal && near + kKeys - 1 > 0)) {
       const int seen = min(nk - 1, a.causal ? i + off : nk) - j0 - 8 * g;  // last key of the tile that the row sees
 #pragma unroll
@@ -107,7 +129,7 @@ __global__ __launch_bounds__(kBlock, 2) void attn_forward_kernel(AttnArgs a) {
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int e = 0; e < 16; ++e) top = fmaxf(top, x[kb][e]);
-    top = fmaxf(top, swap_halves(top)) + shift;
+    top = halves_max(top) + shift;
     if (__any(top > m + slack)) {
       const float next = fmaxf(m, top);
       const float fade = next == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((m - next) * c);
@@ -135,10 +157,14 @@ __global__ __launch_bounds__(kBlock, 2) void attn_forward_kernel(AttnArgs a) {
         const V p = pack8<T>(x[kb], s);
 #pragma unroll
         for (int d = 0; d < DB; ++d)
-          acc[d] = Frag<T>::mfma(col_frag<T, DP>(sv[buf], kb * 32 + 16 * s, d * 32), p, acc[d]);
+          acc[d] = Frag<T>::mfma(cols[kb][s][d], p, acc[d]);
       }
   }
-  sum += swap_halves(sum);
+  for (int t = max(mine, t0); t < t1; ++t) {
+    tile_barrier();
+    if (t + 1 < t1) load(t + 1);
+  }
+  sum = halves_sum(sum);
   if (i >= a.lq) return;
   if (i >= nq) sum = 0.f, m = -__builtin_inff();
   m *= c;  // to base-2 logarithms

@@ -63,8 +63,8 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int heads = a.batch * a.heads;
-  int block = blockIdx.x / heads;
-  if (a.causal) block = (a.lq + kAttnRows - 1) / kAttnRows - 1 - block;  // those with most keys first
+  // the last rows first: those see most keys when causal, and are of the longest sequences
+  const int block = (a.lq + kAttnRows - 1) / kAttnRows - 1 - blockIdx.x / heads;
   const int bh = blockIdx.x % heads;
   const int b = bh / a.heads, h = bh % a.heads, hk = h / (a.heads / a.k_heads);
   const int nk = key_count(a, b), nq = query_count(a, b), off = query_offset(a, b);
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
 #pragma unroll
     for (int j = 0; j < 8; ++j) delta = fmaf((float)gf[s][j], (float)of[j], delta);
   }
-  delta = one ? 0.f : delta + swap_halves(delta);
+  delta = one ? 0.f : halves_sum(delta);
   const int64_t row_at = (int64_t)bh * a.lq + i;
   float lse = kNever;
   if (i < nq) {
@@ -111,45 +111,90 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
   if (BIAS) {
     load_bias<T>(tab, a, h);
     for (int t = threadIdx.x; t < 4 * places; t += kBlock) tab[places + t] = 0.f;
-    for (int t = threadIdx.x; t < 4 * kSkew; t += kBlock) skew[t / kSkew][t % kSkew] = 0.f;
+    for (int t = threadIdx.x; t < kSkew; t += kBlock) reinterpret_cast<f32x4*>(&skew[0][0])[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
   f32x16 dq[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) dq[d] = zero16();
-  const f32x16 minus_delta = splat16(-delta);
   const float c = a.scale * kLog2e;
 
-  for (int t = 0; t < tiles; ++t) {
+  // the tiles that a row of this wave sees a key of; through the others it only loads its share
+  int mine = r0 < nq ? tiles : 0;
+  if (a.causal) mine = max(0, min(mine, (r0 + 32 + off + ROWS - 1) / ROWS));
+  for (int t = 0; t < mine; ++t) {
     const int buf = t & 1;
     tile_barrier();
     if (t + 1 < tiles) load(t + 1);
     f32x16 ds[KB], p[KB];
-    int near[KB];
+    float base[KB];
+    const int near0 = t * ROWS - r0 - off;  // position of the tile's first key and the wave's first row
+    V krows[KB][KS], vrows[KB][KS], kcols[KB][2][DB];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) krows[kb][s] = row_frag<T, DP>(sk[buf], kb * 32, s);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      const int j0 = t * ROWS + kb * 32;
-      near[kb] = j0 - r0 - off;
-      float base = -lse;
-      p[kb] = zero16();
+      const int near = near0 + kb * 32;
+      base[kb] = -lse;
       if (BIAS) {
-        if (near[kb] - 31 >= a.max_distance || near[kb] + 31 <= -a.max_distance) {
-          base += tab[near[kb] > 0 ? 2 * reach : 0] * c;
+        if (near - 31 >= a.max_distance || near + 31 <= -a.max_distance) {
+          base[kb] += tab[near > 0 ? 2 * reach : 0] * c;
+          p[kb] = zero16();
         } else {
-          const float* at = tab + (near[kb] - l32 + 8 * g + reach);
+          const float* at = tab + (near - l32 + 8 * g + reach);
 #pragma unroll
           for (int e = 0; e < 16; ++e) p[kb][e] = at[elem_row(e, 0)];
         }
+      } else {
+        p[kb] = zero16();
       }
-      ds[kb] = minus_delta;
+    }
+    auto read_vrows = [&]() {
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        p[kb] = Frag<T>::mfma(row_frag<T, DP>(sk[buf], kb * 32, s), qf[s], p[kb]);
-        ds[kb] = Frag<T>::mfma(row_frag<T, DP>(sv[buf], kb * 32, s), gf[s], ds[kb]);
-      }
+      for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) p[kb][e] = __builtin_amdgcn_exp2f(fmaf(p[kb][e], c, base));
-      if (j0 + 32 > nk || (a.causal && near[kb] + 31 > 0)) {
+        for (int kb = 0; kb < KB; ++kb) vrows[kb][s] = row_frag<T, DP>(sv[buf], kb * 32, s);
+    };
+    auto read_kcols = [&]() {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int d = 0; d < DB; ++d) kcols[kb][s][d] = col_frag<T, DP>(sk[buf], kb * 32 + 16 * s, d * 32);
+    };
+    if (DP <= 64) {
+      keep_order();
+      read_vrows();
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) p[kb] = Frag<T>::mfma(krows[kb][s], qf[s], p[kb]);
+    if (DP <= 64) {
+      keep_order();
+      read_kcols();
+    } else {  // no registers to read ahead with
+      read_vrows();
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) ds[kb] = splat16(-delta);
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) ds[kb] = Frag<T>::mfma(vrows[kb][s], gf[s], ds[kb]);
+    if (DP <= 64)
+      keep_order();
+    else
+      read_kcols();
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const int j0 = t * ROWS + kb * 32;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) p[kb][e] = __builtin_amdgcn_exp2f(fmaf(p[kb][e], c, base[kb]));
+      if (j0 + 32 > nk || (a.causal && near0 + kb * 32 + 31 > 0)) {
         const int seen = min(nk - 1, a.causal ? i + off : nk) - j0 - 8 * g;  // last key of the block that the row sees
 #pragma unroll
         for (int e = 0; e < 16; ++e) p[kb][e] = elem_row(e, 0) > seen ? 0.f : p[kb][e];
@@ -161,7 +206,7 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int e = 0; e < 16; ++e) sp += p[kb][e];
-      sp += swap_halves(sp);
+      sp = halves_sum(sp);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -169,7 +214,7 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
           p[kb][e] = sp == 0.f ? 0.f : p[kb][e] / sp;
           spd = fmaf(p[kb][e], ds[kb][e], spd);
         }
-      delta = spd + swap_halves(spd);
+      delta = halves_sum(spd);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -180,24 +225,28 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
 #pragma unroll
       for (int e = 0; e < 16; ++e) ds[kb][e] *= p[kb][e];
       if (BIAS) {
-        if (near[kb] + 31 <= -a.max_distance) {
+        const int near = near0 + kb * 32;
+        if (near + 31 <= -a.max_distance) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) before += ds[kb][e];
-        } else if (near[kb] - 31 >= a.max_distance) {
+        } else if (near - 31 >= a.max_distance) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) after += ds[kb][e];
         } else {
-          add_positions(skew[wave], sums + near[kb] - 31, ds[kb]);
+          add_positions(skew[wave], sums + near - 31, ds[kb]);
         }
       }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const V df = pack8<T>(ds[kb], s);
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
-          dq[d] = Frag<T>::mfma(col_frag<T, DP>(sk[buf], kb * 32 + 16 * s, d * 32), df, dq[d]);
+        for (int d = 0; d < DB; ++d) dq[d] = Frag<T>::mfma(kcols[kb][s][d], df, dq[d]);
       }
     }
+  }
+  for (int t = mine; t < tiles; ++t) {
+    tile_barrier();
+    if (t + 1 < tiles) load(t + 1);
   }
   if (i < a.lq) {
     const int64_t at = (((int64_t)b * a.lq + i) * a.heads + h) * a.d;
@@ -216,25 +265,31 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
       sums[reach] = after;
     }
     __syncthreads();
-    // bucket of a direction: distances edges[u] .. edges[u + 1] - 1 (the last: all further ones)
-    const int u = threadIdx.x % a.one_way, side = threadIdx.x / a.one_way;  // side 0: key at or before the query
-    if (threadIdx.x < a.buckets) {
-      float s = 0.f;
+    // bucket of a direction: distances edges[u] .. edges[u + 1] - 1 (the last: all further
+    // ones), a power of two of lanes to a bucket
+    int lanes = 2;
+    while (2 * lanes * a.buckets <= kBlock) lanes *= 2;
+    const int bucket = threadIdx.x / lanes, l = threadIdx.x % lanes;
+    float s = 0.f;
+    if (bucket < a.buckets) {
+      const int u = bucket % a.one_way, side = bucket / a.one_way;  // side 0: key at or before the query
       const int d0 = max((int)a.edges[u], side), d1 = u + 1 < a.one_way ? (int)a.edges[u + 1] : reach + 1;
-      for (int dist = d0; dist < d1; ++dist) {
+      for (int dist = d0 + l; dist < d1; dist += lanes) {
         const float* at = tab + places + reach + (side == 1 ? dist : -dist);
         s += (at[0] + at[places]) + (at[2 * places] + at[3 * places]);
       }
-      a.part_table[((int64_t)h * a.table_parts + (int64_t)b * (a.table_parts / a.batch) + block) * a.buckets + threadIdx.x] = s;
     }
+    for (int o = lanes / 2; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if (bucket < a.buckets && l == 0)
+      a.part_table[((int64_t)h * a.table_parts + (int64_t)b * (a.table_parts / a.batch) + block) * a.buckets + bucket] = s;
   }
 }
 
 // dk and dv of 128 keys (wave w: 32 of them as columns), over a part of the queries that see them.
 template <class T, int DP, bool BIAS>
-__global__ __launch_bounds__(kBlock, 2) void attn_backward_kv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kernel(AttnArgs a) {
   typedef typename Frag<T>::V V;
-  constexpr int KS = DP / 16, DB = DP / 32, ROWS = kTile<DP>, QB = ROWS / 32, TILE = ROWS * DP * 2;
+  constexpr int KS = DP / 16, DB = DP / 32, ROWS = 64, QB = ROWS / 32, TILE = ROWS * DP * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char sq[2][TILE], sg[2][TILE];
   __shared__ __attribute__((aligned(16))) float slse[2][ROWS], sdelta[2][ROWS];  // -log2 sums, -deltas
   extern __shared__ float tab[];
@@ -242,7 +297,9 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_kv_kernel(AttnArgs a)
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kheads = a.batch * a.k_heads, group = a.heads / a.k_heads;
-  const int bk = blockIdx.x % kheads, block = blockIdx.x / kheads;
+  // keys of most queries first: the first ones when causal, else those of the longest sequences
+  const int bk = blockIdx.x % kheads;
+  const int block = a.causal ? blockIdx.x / kheads : (a.lk + kAttnRows - 1) / kAttnRows - 1 - blockIdx.x / kheads;
   const int b = bk / a.k_heads, hk = bk % a.k_heads;
   const int nk = key_count(a, b), nq = query_count(a, b), off = query_offset(a, b);
   const int j0 = block * kAttnRows + wave * 32;
@@ -265,8 +322,12 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_kv_kernel(AttnArgs a)
   // tiles of queries that see a key of this workgroup, those of all heads in a row; this part's
   const int t0 = (a.causal ? max(block * kAttnRows - off, 0) : 0) / ROWS;
   const int nt = block * kAttnRows < nk ? max((nq + ROWS - 1) / ROWS - t0, 0) : 0;
-  int f0 = (int)((int64_t)nt * group * blockIdx.y / a.kv_parts);
-  const int f1 = (int)((int64_t)nt * group * (blockIdx.y + 1) / a.kv_parts);
+  int f0 = 0, f1 = nt * group;
+  if (a.kv_parts > 1) {
+    const int64_t all = f1;
+    f0 = (int)(all * blockIdx.y / a.kv_parts);
+    f1 = (int)(all * (blockIdx.y + 1) / a.kv_parts);
+  }
   const TileLoad<DP, ROWS> lq(2 * a.qs[1], a.d), lg(2 * a.dos[1], a.d);
   while (f0 < f1) {
     const int hh = f0 / nt, h = hk * group + hh;
@@ -290,30 +351,46 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_kv_kernel(AttnArgs a)
         stat = i < nq ? -delta[i] : 0.f;
       }
     };
-    load(first);
-    for (int t = first; t < last; ++t) {
-      const int buf = t & 1;
+    auto turn = [&](int t) {
       if (threadIdx.x < ROWS)
-        slse[buf][threadIdx.x] = stat;
+        slse[t & 1][threadIdx.x] = stat;
       else if (threadIdx.x < 2 * ROWS)
-        sdelta[buf][threadIdx.x - ROWS] = stat;
+        sdelta[t & 1][threadIdx.x - ROWS] = stat;
       tile_barrier();
       if (t + 1 < last) load(t + 1);
+    };
+    load(first);
+    // tiles that no key of this wave is seen from come first: it only loads its share of them
+    int mine = j0 < nk ? first : last;
+    if (a.causal) mine = min(last, max(mine, (j0 - off) / ROWS));
+    for (int t = first; t < mine; ++t) turn(t);
+    for (int t = mine; t < last; ++t) {
+      const int buf = t & 1;
+      turn(t);
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
         const int i0 = t * ROWS + qb * 32;
         const int near = j0 - i0 - off;
-        f32x16 p = zero16(), ds;
+        V qrows[KS], grows[KS], qcols[2][DB], gcols[2][DB];
+        f32x16 p, ds, base;
         float shift = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qrows[s] = row_frag<T, DP>(sq[buf], qb * 32, s);
         if (BIAS) {
           if (near - 31 >= a.max_distance || near + 31 <= -a.max_distance) {
             shift = tab[near > 0 ? 2 * reach : 0] * c;
+            p = zero16();
           } else {
             const float* at = tab + (near + l32 - 8 * g + reach);
 #pragma unroll
             for (int e = 0; e < 16; ++e) p[e] = at[-elem_row(e, 0)];
           }
+        } else {
+          p = zero16();
         }
+        keep_order();
+#pragma unroll
+        for (int s = 0; s < KS; ++s) grows[s] = row_frag<T, DP>(sg[buf], qb * 32, s);
         if (one) {
           ds = zero16();
         } else {
@@ -321,20 +398,27 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_kv_kernel(AttnArgs a)
           for (int e = 0; e < 16; ++e) ds[e] = sdelta[buf][qb * 32 + elem_row(e, g)];
         }
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          p = Frag<T>::mfma(row_frag<T, DP>(sq[buf], qb * 32, s), kf[s], p);
-          ds = Frag<T>::mfma(row_frag<T, DP>(sg[buf], qb * 32, s), vf[s], ds);
-        }
+        for (int s = 0; s < KS; ++s) p = Frag<T>::mfma(qrows[s], kf[s], p);
+        keep_order();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) base[e] = slse[buf][qb * 32 + elem_row(e, g)];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int d = 0; d < DB; ++d) gcols[s][d] = col_frag<T, DP>(sg[buf], qb * 32 + 16 * s, d * 32);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) ds = Frag<T>::mfma(grows[s], vf[s], ds);
+        keep_order();
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int d = 0; d < DB; ++d) qcols[s][d] = col_frag<T, DP>(sq[buf], qb * 32 + 16 * s, d * 32);
         if (one) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) ds[e] += sdelta[buf][qb * 32 + elem_row(e, g)];
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float base = slse[buf][qb * 32 + elem_row(e, g)];
-          if (BIAS) base += shift;
-          p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], c, base));
-        }
+        for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], c, BIAS ? base[e] + shift : base[e]));
         if (a.causal && near + 31 > 0) {
           const int seen = j - off - i0 - 8 * g;  // first row of the block that sees the key
 #pragma unroll
@@ -347,8 +431,8 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_kv_kernel(AttnArgs a)
           const V pf = pack8<T>(p, s), df = pack8<T>(ds, s);
 #pragma unroll
           for (int d = 0; d < DB; ++d) {
-            dv[d] = Frag<T>::mfma(col_frag<T, DP>(sg[buf], qb * 32 + 16 * s, d * 32), pf, dv[d]);
-            dk[d] = Frag<T>::mfma(col_frag<T, DP>(sq[buf], qb * 32 + 16 * s, d * 32), df, dk[d]);
+            dv[d] = Frag<T>::mfma(gcols[s][d], pf, dv[d]);
+            dk[d] = Frag<T>::mfma(qcols[s][d], df, dk[d]);
           }
         }
       }

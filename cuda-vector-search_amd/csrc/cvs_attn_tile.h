@@ -118,13 +118,23 @@ constexpr int kReach = 96;
 
 template <class T>
 __device__ __forceinline__ void load_bias(float* tab, const AttnArgs& a, int head) {
+  constexpr int N = (2 * (kMaxDistance + kReach) + kBlock) / kBlock;  // places a thread, all under way together
   const int reach = a.max_distance + kReach;
   const float unit = 1.f / a.scale;
-  for (int t = threadIdx.x; t <= 2 * reach; t += kBlock) {
-    const int rel = t - reach;
-    int u = a.bucket_of[min(abs(rel), a.max_distance)];
-    if (rel > 0) u = a.causal ? 0 : u + a.one_way;
-    tab[t] = (float)((const T*)a.table)[(int64_t)u * a.heads + head] * unit;
+  int u[N];
+  float v[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int rel = min((int)threadIdx.x + n * kBlock, 2 * reach) - reach;
+    u[n] = a.bucket_of[min(abs(rel), a.max_distance)];
+    if (rel > 0) u[n] = a.causal ? 0 : u[n] + a.one_way;
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n) v[n] = (float)((const T*)a.table)[u[n] * a.heads + head] * unit;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int t = threadIdx.x + n * kBlock;
+    if (t <= 2 * reach) tab[t] = v[n];
   }
 }
 

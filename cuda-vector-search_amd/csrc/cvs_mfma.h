@@ -113,8 +113,19 @@ __device__ __forceinline__ typename Frag<T>::V pack8(const f32x16& v, int s) {
   return r;
 }
 
-__device__ __forceinline__ float swap_halves(float v) {  // lane l's value from lane l ^ 32
-  return __shfl_xor(v, 32);
+// Maximum and sum of lane l's value and lane l ^ 32's.
+__device__ __forceinline__ float halves_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
+__device__ __forceinline__ float halves_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Nothing moves across: LDS reads stay ahead of the products they are to wait under.  (Left
+// to itself the compiler reads one operand, waits for it and multiplies, to save
+// registers.)
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0); }
 
 }  // namespace cvs
