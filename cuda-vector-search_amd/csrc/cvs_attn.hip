@@ -175,20 +175,196 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 3) void attn_forward_kernel(A
       a.part_ml[2 * (blockIdx.y * rows + at)] = m;
       a.part_ml[2 * (blockIdx.y * rows + at) + 1] = sum;
     }
-    float* o = a.part_out + (blockIdx.y * rows + at) * a.d;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int col = d * 32 + 16 * (q >> 1) + 8 * g + 4 * (q & 1);
-        if (col < a.d)
-          *reinterpret_cast<f32x4*>(o + col) = f32x4{acc[d][4 * q], acc[d][4 * q + 1], acc[d][4 * q + 2], acc[d][4 * q + 3]};
-      }
+    store_part_row<DP>(a.part_out + (blockIdx.y * rows + at) * a.d, acc, a.d);
     return;
   }
   if (a.lse != nullptr && g == 0) a.lse[at] = sum == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(sum)) * kLn2;
   store_head_row<T, DP>((T*)a.out + ((int64_t)(b * (int64_t)a.lq + i) * a.heads + h) * a.d, acc,
                         sum == 0.f ? 0.f : 1.f / sum, a.d);
+}
+
+// Few query rows (single tokens, a pooling query) over many keys, bound by reading the keys.
+// The rows of the query heads that share a key head (of one head where there is a
+// bias) are the columns of one block, at most 32.  Each wave walks key tiles of its own, 32
+// keys, through buffers of its own, with no barrier, its next tile's loads under way (64 KiB a
+// CU); the waves' sums are joined at the end.  (8 x 12 heads of 64, one row over up to 8191 keys:
+// 36 us in the kernel above, where three of four waves had no rows.)
+template <class T, int DP, bool BIAS>
+__global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_rows_kernel(AttnArgs a) {
+  typedef typename Frag<T>::V V;
+  constexpr int KS = DP / 16, DB = DP / 32, TILE = 32 * DP * 2, LOADS = TILE / 1024;
+  // per wave: two tiles of keys and of values; at the end its sums
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[4][2][2][TILE];
+  __shared__ float stat[4][2][32];
+  extern __shared__ float tab[];
+
+  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = a.heads / a.k_heads, gcols = BIAS ? 1 : group;  // query heads of a block
+  const int blocks = a.heads / gcols;
+  const int b = blockIdx.x / blocks, h0 = blockIdx.x % blocks * gcols, hk = h0 / group;
+  const int nk = key_count(a, b), nq = query_count(a, b), off = query_offset(a, b);
+  const int i = l32 % a.lq, h = h0 + l32 / a.lq;
+  const bool row = l32 < a.lq * gcols;  // this lane's column is a row of a head
+  const unsigned char* kbase = (const unsigned char*)a.k + 2 * (b * a.ks[0] + hk * a.ks[2]);
+  const unsigned char* vbase = (const unsigned char*)a.v + 2 * (b * a.vs[0] + hk * a.vs[2]);
+
+  int end = nq > 0 ? nk : 0;
+  if (a.causal) end = min(end, max(nq + off, 0));
+  const int tiles = (end + 31) / 32;
+  int t0 = 0, t1 = tiles;
+  if (a.splits > 1) {
+    t0 = (int)((unsigned)tiles * blockIdx.y / (unsigned)a.splits);
+    t1 = (int)((unsigned)tiles * (blockIdx.y + 1) / (unsigned)a.splits);
+  }
+  const TileLoad<DP, 32, 1> lk(2 * a.ks[1], a.d), lv(2 * a.vs[1], a.d);
+  auto load = [&](int t, int buf) {
+    lk.load(kbase, 2 * a.ks[1], t * 32, nk, smem[wave][buf][0]);
+    lv.load(vbase, 2 * a.vs[1], t * 32, nk, smem[wave][buf][1]);
+  };
+  int t = t0 + wave, buf = 0;
+  if (t < t1) load(t, 0);
+  V qf[KS];
+  const unsigned char* qrow = (const unsigned char*)a.q + 2 * (b * a.qs[0] + i * a.qs[1] + h * a.qs[2]);
+#pragma unroll
+  for (int s = 0; s < KS; ++s) qf[s] = global_frag<T>(qrow, s, a.d, row && i < nq);
+  if (BIAS) {
+    load_bias<T>(tab, a, h0);
+    __syncthreads();
+  }
+
+  f32x16 acc[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) acc[d] = zero16();
+  float m = -__builtin_inff(), sum = 0.f;
+  const float c = a.scale * kLog2e, slack = 8.f / c;
+  const int reach = a.max_distance + kReach;
+  wait_vmcnt_lgkm0<0>();
+  for (; t < t1; t += 4, buf ^= 1) {
+    wait_vmcnt_lgkm0<63>();  // the reads of the buffer to be loaded next
+    asm volatile("" ::: "memory");
+    if (t + 4 < t1) {
+      load(t + 4, buf ^ 1);
+      wait_vmcnt_lgkm0<2 * LOADS>();
+    } else {
+      wait_vmcnt_lgkm0<0>();
+    }
+    asm volatile("" ::: "memory");
+    const unsigned char* sk = smem[wave][buf][0];
+    const unsigned char* sv = smem[wave][buf][1];
+    const int j0 = t * 32, near = j0 - off;
+    V rows[KS], cols[2][DB];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) rows[s] = row_frag<T, DP>(sk, 0, s);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) cols[s][d] = col_frag<T, DP>(sv, 16 * s, d * 32);
+    f32x16 x = zero16();
+    float shift = 0.f;
+    if (BIAS) {
+      if (near - 31 >= a.max_distance || near + 31 <= -a.max_distance) {
+        shift = tab[near > 0 ? 2 * reach : 0];
+      } else {
+        const float* at = tab + (near - l32 + 8 * g + reach);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = at[elem_row(e, 0)];
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) x = Frag<T>::mfma(rows[s], qf[s], x);
+    if (j0 + 32 > nk || (a.causal && near + 31 > 0)) {
+      const int seen = min(nk - 1, a.causal ? i + off : nk) - j0 - 8 * g;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] = elem_row(e, 0) > seen ? -__builtin_inff() : x[e];
+    }
+    float top = x[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
+    top = halves_max(top) + shift;
+    if (__any(top > m + slack)) {
+      const float next = fmaxf(m, top);
+      const float fade = next == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((m - next) * c);
+      m = next;
+      sum *= fade;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[d][e] *= fade;
+    }
+    const float base = m == -__builtin_inff() ? shift * c : (shift - m) * c;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], c, base));
+      sum += x[e];
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const V p = pack8<T>(x, s);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) acc[d] = Frag<T>::mfma(cols[s][d], p, acc[d]);
+    }
+  }
+  // join the waves: sums relative to the largest of their m, column by column
+  sum = halves_sum(sum);
+  if (g == 0) stat[wave][0][l32] = m, stat[wave][1][l32] = sum;
+  wait_vmcnt_lgkm0<0>();
+  __syncthreads();  // (every wave is done with the tiles, too)
+  float top = -__builtin_inff();
+#pragma unroll
+  for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[w][0][l32]);
+  const float base = top == -__builtin_inff() ? 0.f : top;
+  const float fade = __builtin_amdgcn_exp2f((m - base) * c);
+  float* sums = reinterpret_cast<float*>(smem[wave]);  // [32 columns][DP], the pieces of 4 in an order by column
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int piece = (d * 32 + 16 * (q >> 1) + 8 * g + 4 * (q & 1)) / 4;
+      *reinterpret_cast<f32x4*>(sums + l32 * DP + ((piece ^ (l32 & 7)) * 4)) =
+          f32x4{acc[d][4 * q], acc[d][4 * q + 1], acc[d][4 * q + 2], acc[d][4 * q + 3]} * fade;
+    }
+  __syncthreads();
+  const int64_t rows = (int64_t)a.batch * a.heads * a.lq;
+  for (int u = threadIdx.x; u < a.lq * gcols * (DP / 8); u += kBlock) {
+    const int col = u / (DP / 8), c8 = u % (DP / 8) * 8;
+    if (c8 >= a.d) continue;
+    const int ci = col % a.lq, ch = h0 + col / a.lq;
+    const int64_t at = ((int64_t)b * a.heads + ch) * a.lq + ci;
+    float ct = -__builtin_inff(), cs = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) ct = fmaxf(ct, stat[w][0][col]);
+    const float cb = ct == -__builtin_inff() ? 0.f : ct;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) cs += stat[w][1][col] * __builtin_amdgcn_exp2f((stat[w][0][col] - cb) * c);
+    if (ci >= nq) ct = -__builtin_inff(), cs = 0.f;
+    float z[8];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        s += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(smem[w]) + col * DP + (((c8 / 4 + half) ^ (col & 7)) * 4));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[4 * half + e] = s[e];
+    }
+    if (a.splits > 1) {
+      float* o = a.part_out + (blockIdx.y * rows + at) * a.d + c8;
+      *reinterpret_cast<f32x4*>(o) = f32x4{z[0], z[1], z[2], z[3]};
+      *reinterpret_cast<f32x4*>(o + 4) = f32x4{z[4], z[5], z[6], z[7]};
+      if (c8 == 0) {
+        a.part_ml[2 * (blockIdx.y * rows + at)] = ct * c;
+        a.part_ml[2 * (blockIdx.y * rows + at) + 1] = cs;
+      }
+    } else {
+      const float inv = cs == 0.f ? 0.f : 1.f / cs;
+      V v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (T)(z[e] * inv);
+      *reinterpret_cast<V*>((T*)a.out + (((int64_t)b * a.lq + ci) * a.heads + ch) * a.d + c8) = v;
+      if (c8 == 0 && a.lse != nullptr) a.lse[at] = cs == 0.f ? -__builtin_inff() : (ct * c + __builtin_amdgcn_logf(cs)) * kLn2;
+    }
+  }
 }
 
 // Joins the parts of the keys: one wave a query row.
@@ -224,11 +400,23 @@ __global__ __launch_bounds__(kBlock) void attn_join_kernel(AttnArgs a) {
   if (a.lse != nullptr && lane == 0) a.lse[at] = sum == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
+// Whether the rows of a block of heads are few enough for one block's columns.
+bool few_rows(const AttnArgs& a) { return (int64_t)a.lq * (a.table != nullptr ? 1 : a.heads / a.k_heads) <= 32; }
+
+int64_t workgroups(const AttnArgs& a) {
+  if (few_rows(a)) return (int64_t)a.batch * (a.table != nullptr ? a.heads : a.k_heads);
+  return (a.lq + kAttnRows - 1) / kAttnRows * (int64_t)a.batch * a.heads;
+}
+
 template <class T, int DP>
 void launch_width(const AttnArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)((a.lq + kAttnRows - 1) / kAttnRows * (int64_t)a.batch * a.heads), a.splits), block(kBlock);
+  const dim3 grid((unsigned)workgroups(a), a.splits), block(kBlock);
   const size_t tab = (2 * (a.max_distance + kReach) + 1) * sizeof(float);
-  if (a.table != nullptr)
+  if (few_rows(a) && a.table != nullptr)
+    hipLaunchKernelGGL((attn_rows_kernel<T, DP, true>), grid, block, tab, s, a);
+  else if (few_rows(a))
+    hipLaunchKernelGGL((attn_rows_kernel<T, DP, false>), grid, block, 0, s, a);
+  else if (a.table != nullptr)
     hipLaunchKernelGGL((attn_forward_kernel<T, DP, true>), grid, block, tab, s, a);
   else
     hipLaunchKernelGGL((attn_forward_kernel<T, DP, false>), grid, block, 0, s, a);
@@ -253,10 +441,11 @@ hipError_t forward(const AttnArgs& a, hipStream_t s) {
 
 }  // namespace
 
+// Parts of the keys: enough for two workgroups a CU, of at least 4 tiles of 64 (or 4 a wave
+// of 32) each.
 int attn_splits(const AttnArgs& a, int cus) {
-  const int64_t wgs = (a.lq + kAttnRows - 1) / kAttnRows * (int64_t)a.batch * a.heads;
-  const int64_t tiles = (a.lk + kKeys - 1) / kKeys;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / std::max<int64_t>(wgs, 1), tiles / 4, (int64_t)64}));
+  const int64_t least = few_rows(a) ? 4 * 4 * 32 : 4 * kKeys;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / std::max<int64_t>(workgroups(a), 1), a.lk / least, (int64_t)64}));
 }
 
 hipError_t launch_attn_forward(const AttnArgs& a, hipStream_t s) {

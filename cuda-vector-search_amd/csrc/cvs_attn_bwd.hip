@@ -79,14 +79,22 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
   const int last_row = min(block * kAttnRows + kAttnRows, nq) - 1;
   int end = last_row < block * kAttnRows ? 0 : nk;
   if (a.causal) end = min(end, max(last_row + off + 1, 0));
-  const int tiles = (end + ROWS - 1) / ROWS;
+  const int all = (end + ROWS - 1) / ROWS;
   const bool one = nk <= ROWS;  // a row's keys are all in one tile
+  // this workgroup's part of the tiles (fewer than 2^24, at most 64 parts); the first part writes
+  // delta, or the last one, which then has the one tile
+  int t0 = 0, tiles = all;
+  if (a.q_parts > 1) {
+    t0 = (int)((unsigned)all * blockIdx.y / (unsigned)a.q_parts);
+    tiles = (int)((unsigned)all * (blockIdx.y + 1) / (unsigned)a.q_parts);
+  }
+  const bool writes_delta = (int)blockIdx.y == (one ? a.q_parts - 1 : 0);
   const TileLoad<DP, ROWS> lk(2 * a.ks[1], a.d), lv(2 * a.vs[1], a.d);
   auto load = [&](int t) {
     lk.load(kbase, 2 * a.ks[1], t * ROWS, nk, sk[t & 1]);
     lv.load(vbase, 2 * a.vs[1], t * ROWS, nk, sv[t & 1]);
   };
-  if (tiles > 0) load(0);
+  if (t0 < tiles) load(t0);
 
   V qf[KS], gf[KS];
   float delta = 0.f;
@@ -120,9 +128,9 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
   const float c = a.scale * kLog2e;
 
   // the tiles that a row of this wave sees a key of; through the others it only loads its share
-  int mine = r0 < nq ? tiles : 0;
-  if (a.causal) mine = max(0, min(mine, (r0 + 32 + off + ROWS - 1) / ROWS));
-  for (int t = 0; t < mine; ++t) {
+  int mine = r0 < nq ? tiles : t0;
+  if (a.causal) mine = max(t0, min(mine, (r0 + 32 + off + ROWS - 1) / ROWS));
+  for (int t = t0; t < mine; ++t) {
     const int buf = t & 1;
     tile_barrier();
     if (t + 1 < tiles) load(t + 1);
@@ -250,8 +258,11 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
   }
   if (i < a.lq) {
     const int64_t at = (((int64_t)b * a.lq + i) * a.heads + h) * a.d;
-    store_head_row<T, DP>((T*)a.dq + at, dq, a.scale, a.d);
-    if (g == 0) a.delta[row_at] = delta;
+    if (a.q_parts > 1)
+      store_part_row<DP>(a.part_q + (int64_t)blockIdx.y * a.batch * a.lq * a.heads * a.d + at, dq, a.d);
+    else
+      store_head_row<T, DP>((T*)a.dq + at, dq, a.scale, a.d);
+    if (g == 0 && writes_delta) a.delta[row_at] = delta;
   }
   if (BIAS) {
 #pragma unroll
@@ -281,7 +292,8 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
     }
     for (int o = lanes / 2; o > 0; o >>= 1) s += __shfl_xor(s, o);
     if (bucket < a.buckets && l == 0)
-      a.part_table[((int64_t)h * a.table_parts + (int64_t)b * (a.table_parts / a.batch) + block) * a.buckets + bucket] = s;
+      a.part_table[((int64_t)h * a.table_parts + ((int64_t)b * a.q_parts + blockIdx.y) * ((a.lq + kAttnRows - 1) / kAttnRows) +
+                    block) * a.buckets + bucket] = s;
   }
 }
 
@@ -447,39 +459,31 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
   if (a.kv_parts > 1) {
     const int64_t all = (int64_t)a.batch * a.lk * a.k_heads * a.d;
     float* to = a.part_kv + 2 * blockIdx.y * all + at;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int col = d * 32 + 16 * (q >> 1) + 8 * g + 4 * (q & 1);
-        if (col < a.d) {
-          *reinterpret_cast<f32x4*>(to + col) = f32x4{dk[d][4 * q], dk[d][4 * q + 1], dk[d][4 * q + 2], dk[d][4 * q + 3]};
-          *reinterpret_cast<f32x4*>(to + all + col) = f32x4{dv[d][4 * q], dv[d][4 * q + 1], dv[d][4 * q + 2], dv[d][4 * q + 3]};
-        }
-      }
+    store_part_row<DP>(to, dk, a.d);
+    store_part_row<DP>(to + all, dv, a.d);
     return;
   }
   store_head_row<T, DP>((T*)a.dk + at, dk, a.scale, a.d);
   store_head_row<T, DP>((T*)a.dv + at, dv, 1.f, a.d);
 }
 
-// Adds the parts of dk (blockIdx.y 0) or dv in order: 8 values a thread.
+// Adds `parts` of n values, `stride` apart, in order: 8 a thread; blockIdx.y: the second of two sums beside each other.
 template <class T>
-__global__ __launch_bounds__(kBlock) void attn_join_kv_kernel(AttnArgs a) {
-  const int64_t all = (int64_t)a.batch * a.lk * a.k_heads * a.d;
+__global__ __launch_bounds__(kBlock) void attn_join_grads_kernel(const float* part, int parts, int64_t stride, int64_t n, float scale0,
+                                                                 T* out0, T* out1) {
   const int64_t at = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * 8;
-  if (at >= all) return;
+  if (at >= n) return;
   f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
-  for (int p = 0; p < a.kv_parts; ++p) {
-    const f32x4* from = reinterpret_cast<const f32x4*>(a.part_kv + (2 * p + blockIdx.y) * all + at);
+  for (int p = 0; p < parts; ++p) {
+    const f32x4* from = reinterpret_cast<const f32x4*>(part + p * stride + blockIdx.y * n + at);
     lo += from[0];
     hi += from[1];
   }
-  const float scale = blockIdx.y == 0 ? a.scale : 1.f;
+  const float scale = blockIdx.y == 0 ? scale0 : 1.f;
   typename Frag<T>::V v;
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[e] = (T)(lo[e] * scale), v[4 + e] = (T)(hi[e] * scale);
-  *reinterpret_cast<typename Frag<T>::V*>((T*)(blockIdx.y == 0 ? a.dk : a.dv) + at) = v;
+  *reinterpret_cast<typename Frag<T>::V*>((blockIdx.y == 0 ? out0 : out1) + at) = v;
 }
 
 // dtable[bucket, h]: the workgroups' sums in order; 64 lanes a (bucket, head).
@@ -499,15 +503,17 @@ hipError_t launch_width(const AttnArgs& a, hipStream_t s) {
   const int64_t qblocks = (a.lq + kAttnRows - 1) / kAttnRows, kblocks = (a.lk + kAttnRows - 1) / kAttnRows;
   const size_t tab = BIAS ? (2 * (a.max_distance + kReach) + 1) * sizeof(float) : 0;
   if (qblocks > 0)
-    hipLaunchKernelGGL((attn_backward_q_kernel<T, DP, BIAS>), dim3((unsigned)(qblocks * a.batch * a.heads)), dim3(kBlock),
-                       5 * tab, s, a);
+    hipLaunchKernelGGL((attn_backward_q_kernel<T, DP, BIAS>), dim3((unsigned)(qblocks * a.batch * a.heads), a.q_parts),
+                       dim3(kBlock), 5 * tab, s, a);
   if (kblocks > 0)
     hipLaunchKernelGGL((attn_backward_kv_kernel<T, DP, BIAS>), dim3((unsigned)(kblocks * a.batch * a.k_heads), a.kv_parts),
                        dim3(kBlock), tab, s, a);
-  if (a.kv_parts > 1) {
-    const int64_t threads = (int64_t)a.batch * a.lk * a.k_heads * a.d / 8;
-    hipLaunchKernelGGL(attn_join_kv_kernel<T>, dim3((unsigned)((threads + kBlock - 1) / kBlock), 2), dim3(kBlock), 0, s, a);
-  }
+  auto join = [&](const float* part, int parts, int64_t n, int sums, float scale, void* out0, void* out1) {
+    const dim3 grid((unsigned)((n / 8 + kBlock - 1) / kBlock), sums);
+    hipLaunchKernelGGL(attn_join_grads_kernel<T>, grid, dim3(kBlock), 0, s, part, parts, sums * n, n, scale, (T*)out0, (T*)out1);
+  };
+  if (a.q_parts > 1) join(a.part_q, a.q_parts, (int64_t)a.batch * a.lq * a.heads * a.d, 1, a.scale, a.dq, nullptr);
+  if (a.kv_parts > 1) join(a.part_kv, a.kv_parts, (int64_t)a.batch * a.lk * a.k_heads * a.d, 2, a.scale, a.dk, a.dv);
   return hipGetLastError();
 }
 
@@ -529,8 +535,12 @@ hipError_t backward(const AttnArgs& a, hipStream_t s) {
 
 }  // namespace
 
-// Parts of the queries for dk and dv: enough workgroups for four rounds' balance where keys
-// are few or causal rows make their work unequal, of at least 8 tiles each.
+// Parts of the keys for dq, and of the queries for dk and dv: enough workgroups for two (dq)
+// or four rounds' balance (dk, dv: causal work is unequal) of the CUs, of at least 8 tiles each.
+int attn_q_parts(const AttnArgs& a, int cus) {
+  const int64_t wgs = (a.lq + kAttnRows - 1) / kAttnRows * (int64_t)a.batch * a.heads;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / wgs, a.lk / 512, (int64_t)64}));
+}
 int attn_kv_parts(const AttnArgs& a, int cus) {
   const int64_t wgs = (a.lk + kAttnRows - 1) / kAttnRows * (int64_t)a.batch * a.k_heads;
   const int64_t tiles = (a.lq + 63) / 64 * (int64_t)(a.heads / a.k_heads);

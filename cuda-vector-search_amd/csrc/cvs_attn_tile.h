@@ -12,21 +12,21 @@ namespace cvs {
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
-// Loads of tiles of ROWS rows of a head straight into LDS, by the four waves of a workgroup:
-// a lane's place in each 1 KiB load is the same in every tile.  Rows from `rows` on and
-// columns from `d` on become zeros.
-template <int DP, int ROWS>
+// Loads of tiles of ROWS rows of a head straight into LDS, by the four waves of a workgroup
+// (WAVES = 1: by one, for itself): a lane's place in each 1 KiB load is the same in every
+// tile.  Rows from `rows` on and columns from `d` on become zeros.
+template <int DP, int ROWS, int WAVES = 4>
 struct TileLoad {
-  static constexpr int N = ROWS * DP * 2 / 4096;
-  static_assert(N * 4096 == ROWS * DP * 2, "whole loads");
+  static constexpr int N = ROWS * DP * 2 / 1024 / WAVES;
+  static_assert(N * WAVES * 1024 == ROWS * DP * 2, "whole loads");
   uint32_t at[N];
   int row[N];
 
   __device__ __forceinline__ TileLoad(int64_t stride_bytes, int d) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = WAVES > 1 ? threadIdx.x >> 6 : 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int line = (wave + 4 * i) * 8 + (lane >> 3), slot = lane & 7;
+      const int line = (wave + WAVES * i) * 8 + (lane >> 3), slot = lane & 7;
       int piece;
       if constexpr (DP == 32) {
         const int x = slot ^ pair_swizzle(line);
@@ -42,10 +42,10 @@ struct TileLoad {
   // Rows first .. first + ROWS - 1 of the head at `base` (its row 0) to the tile at `lds`.
   __device__ __forceinline__ void load(const unsigned char* base, int64_t stride_bytes, int first, int rows,
                                        const unsigned char* lds) const {
-    const uint32_t to = lds_address(lds) + (threadIdx.x >> 6) * 1024;
+    const uint32_t to = lds_address(lds) + (WAVES > 1 ? threadIdx.x >> 6 : 0) * 1024;
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      load_lds(first + row[i] < rows ? at[i] : kOutside, base + first * stride_bytes, to + i * 4096);
+      load_lds(first + row[i] < rows ? at[i] : kOutside, base + first * stride_bytes, to + i * (WAVES * 1024));
   }
 };
 
@@ -107,6 +107,19 @@ __device__ __forceinline__ void store_head_row(T* row, const f32x16* acc, float 
         for (int j = 0; j < 8; ++j) v[j] = (T)(acc[b][8 * h + j] * scale);
         *reinterpret_cast<typename Frag<T>::V*>(row + c) = v;
       }
+    }
+}
+
+// The same, unscaled, to fp32 partial sums.
+template <int DP>
+__device__ __forceinline__ void store_part_row(float* row, const f32x16* acc, int d) {
+  const int g = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int c = b * 32 + 16 * (q >> 1) + 8 * g + 4 * (q & 1);
+      if (c < d) *reinterpret_cast<f32x4*>(row + c) = f32x4{acc[b][4 * q], acc[b][4 * q + 1], acc[b][4 * q + 2], acc[b][4 * q + 3]};
     }
 }
 

@@ -120,12 +120,15 @@ struct AttnArgs {
   int64_t dos[3];
   float* delta;                   // [batch, heads, lq] sum(dout out)
   void *dq, *dk, *dv, *dtable;
-  float* part_table;              // [heads, batch * query blocks, buckets]
+  int q_parts;                    // parts of the keys that dq is summed over
+  float* part_q;                  // [q_parts, batch, lq, heads, d] when q_parts > 1
+  float* part_table;              // [heads, batch * q_parts * query blocks, buckets]
   int table_parts;
   int kv_parts;                   // parts of the queries that dk and dv are summed over
   float* part_kv;                 // [kv_parts, 2, batch, lk, k_heads, d] when kv_parts > 1
 };
 constexpr int kAttnRows = 128;    // query (or key) rows of a workgroup
+int attn_q_parts(const AttnArgs& a, int cus);
 int attn_kv_parts(const AttnArgs& a, int cus);
 int attn_splits(const AttnArgs& a, int cus);
 hipError_t launch_attn_forward(const AttnArgs& a, hipStream_t s);

@@ -156,8 +156,8 @@ AttnArgs attn_args(const cvs_attention* p) {
 }
 
 struct AttnPlan {
-  int splits = 1, table_parts = 0, kv_parts = 1;
-  int64_t part_kv = 0, part_out = 0, part_ml = 0, delta = 0, part_table = 0, bytes = 0;
+  int splits = 1, table_parts = 0, kv_parts = 1, q_parts = 1;
+  int64_t part_kv = 0, part_q = 0, part_out = 0, part_ml = 0, delta = 0, part_table = 0, bytes = 0;
 };
 
 AttnPlan plan_attention(const AttnArgs& a, bool backward, int cus) {
@@ -166,8 +166,10 @@ AttnPlan plan_attention(const AttnArgs& a, bool backward, int cus) {
   const int64_t rows = (int64_t)a.batch * a.heads * a.lq;
   if (backward) {
     p.delta = at, at += up256(rows * 4);
+    p.q_parts = rows == 0 ? 1 : attn_q_parts(a, cus);
+    if (p.q_parts > 1) p.part_q = at, at += up256(p.q_parts * rows * a.d * 4);
     if (a.table != nullptr) {
-      p.table_parts = a.batch * ((a.lq + kAttnRows - 1) / kAttnRows);
+      p.table_parts = a.batch * p.q_parts * ((a.lq + kAttnRows - 1) / kAttnRows);
       p.part_table = at, at += up256((int64_t)a.heads * p.table_parts * a.buckets * 4);
     }
     p.kv_parts = rows == 0 || a.lk == 0 ? 1 : attn_kv_parts(a, cus);
@@ -401,7 +403,8 @@ int cvs_attention_backward(const cvs_attention* p, const void* dout, const int64
   a.delta = reinterpret_cast<float*>(ws + plan.delta);
   a.part_table = reinterpret_cast<float*>(ws + plan.part_table);
   a.table_parts = plan.table_parts;
-  a.kv_parts = plan.kv_parts;
+  a.kv_parts = plan.kv_parts, a.q_parts = plan.q_parts;
+  a.part_q = reinterpret_cast<float*>(ws + plan.part_q);
   a.part_kv = reinterpret_cast<float*>(ws + plan.part_kv);
   return done(launch_attn_backward(a, s), "attention backward launch");
 }
