@@ -19,22 +19,22 @@ namespace cvs {
 namespace {
 
 constexpr int kDepth = 64;                    // reduction steps of a stage
-// The normal distribution's Phi(-t), t >= 0, is exp(-t^2 / 2) times a smooth function, here
-// a polynomial in q = 1 / (1 + 0.3 t) fitted for least relative error: within 2.2e-6 of
-// Phi for t <= 6, 6e-5 to 14, where Phi is below 1e-44.  (The error function of the
-// math library costs some 40 instructions; with it the epilogue of 16384 x 2048, k = 768,
-// took three times as long as the products.)  *g receives exp(-t^2 / 2).
-__device__ __forceinline__ float phi(float z, float* g) {
+// The normal distribution's Phi(z).  log2 Phi(-t), t >= 0, is nearly a parabola: a
+// polynomial of degree 7 in t, fitted on [0, 7] for least error where t Phi(-t) is visible, gives
+// Phi(-t) within 3.7e-6 of itself for t <= 3, 7e-5 for t <= 6, and below 1e-9, on its
+// way to 0, from there.  (The error function of the math library costs some 40 instructions; a
+// rational function times exp(-t^2 / 2) took 22 where this takes 15, and the epilogue of
+// 16384 x 2048, k = 768 is bound by them.)
+__device__ __forceinline__ float phi(float z) {
   const float t = fabsf(z);
-  const float q = __builtin_amdgcn_rcpf(fmaf(0.3f, t, 1.f));
-  *g = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
-  float r = -0.0814668289f;
-  r = fmaf(r, q, 0.229237331f);
-  r = fmaf(r, q, -0.0321202955f);
-  r = fmaf(r, q, 0.15242397f);
-  r = fmaf(r, q, 0.111656703f);
-  r = fmaf(r, q, 0.120269536f);
-  r = r * q * *g;
+  float r = -1.56350917e-06f;
+  r = fmaf(r, t, 5.67471386e-05f);
+  r = fmaf(r, t, -0.000897089475f);
+  r = fmaf(r, t, 0.00839532736f);
+  r = fmaf(r, t, -0.053766588f);
+  r = fmaf(r, t, -0.458625503f);
+  r = fmaf(r, t, -1.15119633f);
+  r = __builtin_amdgcn_exp2f(fmaf(r, t, -1.f));
   return z < 0.f ? r : 1.f - r;
 }
 
@@ -51,10 +51,7 @@ __device__ __forceinline__ float tanh16(float x) {
 __device__ __forceinline__ void activate8(float* z, int act) {
   if (act == kActGelu) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float g;
-      z[e] *= phi(z[e], &g);
-    }
+    for (int e = 0; e < 8; ++e) z[e] *= phi(z[e]);
   } else if (act == kActRelu) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) z[e] = z[e] <= 0.f ? 0.f : z[e];  // (a NaN stays)
@@ -67,9 +64,8 @@ __device__ __forceinline__ void times_slope8(float* dy, const float* z, int act)
   if (act == kActGelu) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      float g;
-      const float p = phi(z[e], &g);
-      dy[e] *= fmaf(z[e] * 0.39894228040143268f, g, p);
+      const float g = __builtin_amdgcn_exp2f(z[e] * z[e] * -0.72134752044448170f);
+      dy[e] *= fmaf(z[e] * 0.39894228040143268f, g, phi(z[e]));
     }
   } else if (act == kActRelu) {
 #pragma unroll
@@ -413,13 +409,13 @@ __global__ __launch_bounds__(kBlock) void act_grad_kernel(ActGradArgs a) {
 // Tiles of 256 x 256 (8 waves, one workgroup a CU), 128 x 128 and 64 x 64 (4 waves, two and three
 // workgroups a CU), and parts of the reduction where the tiles leave CUs idle: the choice of
 // least estimated time.  A CU runs its workgroups in rounds; a stage of a round costs what was
-// measured on long reductions (8192 x 8192, k = 2048: 1080, 850 and 480 TFLOP/s, that is 1.9,
-// 1.2 and 0.9 us with 1, 2 and 3 workgroups), a round 3 us more to fill and finish, and a split
+// measured on long reductions (8192 x 8192, k = 2048: 1080, 850 and 480 TFLOP/s, that is 1.8 to
+// 2.0, 1.2 and 0.9 us with 1, 2 and 3 workgroups), a round 3 us more to fill and finish, and a split
 // 3 us and its sums' way to memory and back.  At 16384 x 2048, k = 768 that gives 256 x 256 (56 us
 // against 64 with 128 x 128), at 10007 x 768, k = 2048 128 x 128 (37 against 54), at 2048 x 768,
 // k = 16384 128 x 128 in 5 parts (62 against 68 for 256 x 256 in 10, 153 unsplit).
 GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int cus) {
-  static constexpr struct { int tile, wgs; double stage; } kTiles[] = {{256, 1, 1.9}, {128, 2, 1.2}, {64, 3, 0.9}};
+  static constexpr struct { int tile, wgs; double stage; } kTiles[] = {{256, 1, 1.8}, {128, 2, 1.2}, {64, 3, 0.9}};
   const int64_t stages = (k + kDepth - 1) / kDepth;
   GemmPlan best = {};
   double least = 1e30;
