@@ -153,15 +153,19 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * BM + WN * BN) * RING <= 16 ? 2 
   const int l32 = lane & 31, g = lane >> 5;
   const int p16 = lane >> 4, s16 = lane & 15;
 
-  // Tiles in an order that gives each XCD (consecutive workgroups go round the 8 of
-  // them) neighbouring tiles, columns first: they share rows of M in its L2.
+  // Tiles in an order that gives each XCD (consecutive workgroups go round the 8 of them)
+  // neighbouring ones, in blocks of 4 tile rows, down the columns: the tiles under way
+  // in an XCD share rows of both operands in its L2.
+  constexpr int kRows = 4;
   const int tiles_n = (a.n + TN - 1) / TN, tiles_m = (a.m + TM - 1) / TM;
   const int tiles = tiles_n * tiles_m;
   const int per = (tiles + 7) / 8;
   const int local = blockIdx.x >> 3;
   const int tile = (blockIdx.x & 7) * per + local;
   if (local >= per || tile >= tiles) return;
-  const int m0 = tile / tiles_n * TM, n0 = tile % tiles_n * TN;
+  const int strip = tile / (kRows * tiles_n), in_strip = tile - strip * kRows * tiles_n;
+  const int rows = min(kRows, tiles_m - strip * kRows);
+  const int m0 = (strip * kRows + in_strip % rows) * TM, n0 = in_strip / rows * TN;
 
   const int stages = (a.k + kDepth - 1) / kDepth;
   const int s_begin = (int)((int64_t)stages * blockIdx.y / a.splits);
@@ -233,35 +237,87 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * BM + WN * BN) * RING <= 16 ? 2 
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
+  auto read = [&](int stage, int ks, V* fm, V* fn) {
+    const unsigned char* tm = smem + stage * STAGE;
 #pragma unroll
-  for (int s = 0; s < RING - 1; ++s)
-    if (s_begin + s < s_end) load_stage();
-
+    for (int i = 0; i < BM; ++i) fm[i] = frag(tm, MS, (wm * BM + i) * 32, ks, false);
+#pragma unroll
+    for (int j = 0; j < BN; ++j) fn[j] = frag(tm + MBYTES, NS, (wn * BN + j) * 32, ks, true);
+  };
+  auto multiply = [&](const V* fm, const V* fn) {
+#pragma unroll
+    for (int i = 0; i < BM; ++i)
+#pragma unroll
+      for (int j = 0; j < BN; ++j) acc[i][j] = Frag<T>::mfma(fn[j], fm[i], acc[i][j]);
+  };
   int buf = 0;
-  for (int s = s_begin; s < s_end; ++s) {
-    // this stage's loads are in; those of the next RING - 2 may still be under way
-    if (RING > 2 && s + 1 < s_end)
-      wait_vmcnt_lgkm0<(RING - 2) * (LM + LN)>();
-    else
+  if constexpr (W == 8) {
+    // Two waves a SIMD, half a turn apart: while one reads the operands of two depth steps, the
+    // other multiplies its own, and a barrier ends each such phase.  (Both at their own pace,
+    // a barrier a stage: 16384 x 768, k = 2048 59 us instead of 52, 16384 x 2048, k = 768 with
+    // gelu 83 instead of 77.)  The late waves are one phase behind; a stage's buffer is loaded
+    // again from the phase on after the late waves' last read of it, and its loads have landed,
+    // by each wave's own wait, before the barrier that the early waves' first read follows.
+    static_assert(RING == 2, "two stages");
+    const bool late = wave >= W / 2;
+    auto phase_end = [&](bool landed) {
+      keep_order();
+      if (landed)
+        wait_vmcnt_lgkm0<0>();
+      else
+        wait_vmcnt_lgkm0<63>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      keep_order();
+    };
+    if (s_begin < s_end) load_stage();
+    if (s_begin + 1 < s_end) {
+      load_stage();
+      wait_vmcnt_lgkm0<LM + LN>();
+    } else {
       wait_vmcnt_lgkm0<0>();
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (load_s < s_end) load_stage();  // into the buffer that every wave has left
-    const unsigned char* tm = smem + buf * STAGE;
-    const unsigned char* tn = tm + MBYTES;
-#pragma unroll
-    for (int ks = 0; ks < kDepth / 16; ++ks) {
-      V fm[BM], fn[BN];
-#pragma unroll
-      for (int i = 0; i < BM; ++i) fm[i] = frag(tm, MS, (wm * BM + i) * 32, ks, false);
-#pragma unroll
-      for (int j = 0; j < BN; ++j) fn[j] = frag(tn, NS, (wn * BN + j) * 32, ks, true);
-#pragma unroll
-      for (int i = 0; i < BM; ++i)
-#pragma unroll
-        for (int j = 0; j < BN; ++j) acc[i][j] = Frag<T>::mfma(fn[j], fm[i], acc[i][j]);
     }
-    buf = buf + 1 == RING ? 0 : buf + 1;
+    __builtin_amdgcn_s_barrier();
+    if (late) __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    for (int s = s_begin; s < s_end; ++s) {
+      if (s > s_begin && load_s < s_end) load_stage();
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        V fm[2][BM], fn[2][BN];
+        read(buf, 2 * half, fm[0], fn[0]);
+        read(buf, 2 * half + 1, fm[1], fn[1]);
+        phase_end(half == 1 && late);
+        __builtin_amdgcn_s_setprio(1);
+        multiply(fm[0], fn[0]);
+        multiply(fm[1], fn[1]);
+        __builtin_amdgcn_s_setprio(0);
+        phase_end(half == 1 && !late);
+      }
+      buf ^= 1;
+    }
+    if (!late) __builtin_amdgcn_s_barrier();
+  } else {
+#pragma unroll
+    for (int s = 0; s < RING - 1; ++s)
+      if (s_begin + s < s_end) load_stage();
+    for (int s = s_begin; s < s_end; ++s) {
+      // this stage's loads are in; those of the next RING - 2 may still be under way
+      if (RING > 2 && s + 1 < s_end)
+        wait_vmcnt_lgkm0<(RING - 2) * (LM + LN)>();
+      else
+        wait_vmcnt_lgkm0<0>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (load_s < s_end) load_stage();  // into the buffer that every wave has left
+#pragma unroll
+      for (int ks = 0; ks < kDepth / 16; ++ks) {
+        V fm[BM], fn[BN];
+        read(buf, ks, fm, fn);
+        multiply(fm, fn);
+      }
+      buf = buf + 1 == RING ? 0 : buf + 1;
+    }
   }
 
   // Lane: a row of the output, two times 8 neighbouring columns of each block.
@@ -344,7 +400,7 @@ hipError_t launch_tiles(const GemmArgs& a, hipStream_t s) {
 
 template <class T>
 hipError_t launch_typed(const GemmArgs& a, const GemmPlan& p, hipStream_t s) {
-  if (p.tile == 256) return launch_tiles<T, 2, 4, 4, 2, 2>(a, s);
+  if (p.tile == 256) return launch_tiles<T, 4, 2, 2, 4, 2>(a, s);
   if (p.tile == 128) return launch_tiles<T, 2, 2, 2, 2, 2>(a, s);
   return launch_tiles<T, 2, 2, 1, 1, 3>(a, s);
 }
