@@ -297,9 +297,23 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
   }
 }
 
-// dk and dv of 128 keys (wave w: 32 of them as columns), over a part of the queries that see them.
+// dtable[bucket, h]: the q kernel's workgroups' sums in order; a wave a (bucket, head).
+template <class T>
+__device__ __forceinline__ void add_table(const AttnArgs& a, int at) {
+  if (at >= a.buckets * a.heads) return;
+  const int bucket = at % a.buckets, h = at / a.buckets, lane = threadIdx.x & 63;
+  const float* p = a.part_table + (int64_t)h * a.table_parts * a.buckets + bucket;
+  float s = 0.f;
+  for (int t = lane; t < a.table_parts; t += 64) s += p[(int64_t)t * a.buckets];
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
+  if (lane == 0) ((T*)a.dtable)[(int64_t)bucket * a.heads + h] = (T)s;
+}
+
+// dk and dv of 128 keys (wave w: 32 of them as columns), over a part of the queries that see
+// them.  Where there is a bias, the workgroups from `key_wgs` on add up its table's gradient.
 template <class T, int DP, bool BIAS>
-__global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kernel(AttnArgs a, int key_wgs) {
   typedef typename Frag<T>::V V;
   constexpr int KS = DP / 16, DB = DP / 32, ROWS = 64, QB = ROWS / 32, TILE = ROWS * DP * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char sq[2][TILE], sg[2][TILE];
@@ -308,6 +322,10 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
 
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (BIAS && (int)blockIdx.x >= key_wgs) {
+    if (blockIdx.y == 0) add_table<T>(a, ((int)blockIdx.x - key_wgs) * 4 + wave);
+    return;
+  }
   const int kheads = a.batch * a.k_heads, group = a.heads / a.k_heads;
   // keys of most queries first: the first ones when causal, else those of the longest sequences
   const int bk = blockIdx.x % kheads;
@@ -486,18 +504,6 @@ __global__ __launch_bounds__(kBlock) void attn_join_grads_kernel(const float* pa
   *reinterpret_cast<typename Frag<T>::V*>((blockIdx.y == 0 ? out0 : out1) + at) = v;
 }
 
-// dtable[bucket, h]: the workgroups' sums in order; 64 lanes a (bucket, head).
-template <class T>
-__global__ __launch_bounds__(64) void attn_table_kernel(AttnArgs a) {
-  const int bucket = blockIdx.x % a.buckets, h = blockIdx.x / a.buckets;
-  const float* p = a.part_table + (int64_t)h * a.table_parts * a.buckets + bucket;
-  float s = 0.f;
-  for (int t = threadIdx.x; t < a.table_parts; t += 64) s += p[(int64_t)t * a.buckets];
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
-  if (threadIdx.x == 0) ((T*)a.dtable)[(int64_t)bucket * a.heads + h] = (T)s;
-}
-
 template <class T, int DP, bool BIAS>
 hipError_t launch_width(const AttnArgs& a, hipStream_t s) {
   const int64_t qblocks = (a.lq + kAttnRows - 1) / kAttnRows, kblocks = (a.lk + kAttnRows - 1) / kAttnRows;
@@ -505,9 +511,10 @@ hipError_t launch_width(const AttnArgs& a, hipStream_t s) {
   if (qblocks > 0)
     hipLaunchKernelGGL((attn_backward_q_kernel<T, DP, BIAS>), dim3((unsigned)(qblocks * a.batch * a.heads), a.q_parts),
                        dim3(kBlock), 5 * tab, s, a);
-  if (kblocks > 0)
-    hipLaunchKernelGGL((attn_backward_kv_kernel<T, DP, BIAS>), dim3((unsigned)(kblocks * a.batch * a.k_heads), a.kv_parts),
-                       dim3(kBlock), tab, s, a);
+  const int64_t key_wgs = kblocks * a.batch * a.k_heads, all_wgs = key_wgs + (BIAS ? (a.buckets * a.heads + 3) / 4 : 0);
+  if (all_wgs > 0)
+    hipLaunchKernelGGL((attn_backward_kv_kernel<T, DP, BIAS>), dim3((unsigned)all_wgs, a.kv_parts), dim3(kBlock), tab, s, a,
+                       (int)key_wgs);
   auto join = [&](const float* part, int parts, int64_t n, int sums, float scale, void* out0, void* out1) {
     const dim3 grid((unsigned)((n / 8 + kBlock - 1) / kBlock), sums);
     hipLaunchKernelGGL(attn_join_grads_kernel<T>, grid, dim3(kBlock), 0, s, part, parts, sums * n, n, scale, (T*)out0, (T*)out1);
@@ -526,11 +533,7 @@ hipError_t launch_bias(const AttnArgs& a, hipStream_t s) {
 
 template <class T>
 hipError_t backward(const AttnArgs& a, hipStream_t s) {
-  if (a.table == nullptr) return launch_bias<T, false>(a, s);
-  const hipError_t e = launch_bias<T, true>(a, s);
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(attn_table_kernel<T>, dim3(a.buckets * a.heads), dim3(64), 0, s, a);
-  return hipGetLastError();
+  return a.table == nullptr ? launch_bias<T, false>(a, s) : launch_bias<T, true>(a, s);
 }
 
 }  // namespace

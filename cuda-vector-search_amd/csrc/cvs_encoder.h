@@ -66,6 +66,8 @@ struct GemmPlan {
 };
 GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int cus);
 hipError_t launch_gemm(const GemmArgs& a, const GemmPlan& p, hipStream_t s);
+// Two products, with partial sums apart; one launch where their tiles are alike.  a: N strided, b: both.
+hipError_t launch_gemm_pair(const GemmArgs& a, const GemmPlan& pa, const GemmArgs& b, const GemmPlan& pb, hipStream_t s);
 
 // dz = dy act'(pre) ([m, n], when act is not none and dz not null) and the column
 // sums of dz (dbias, when not null).
@@ -78,7 +80,7 @@ struct ActGradArgs {
   const void* pre;        // [m, n] contiguous
   void* dz;
   void* dbias;
-  float* partial;         // [parts, n]
+  float* partial;         // [parts, n] when parts > 1
   int parts;
 };
 int act_grad_parts(int64_t m, int64_t n, int cus);

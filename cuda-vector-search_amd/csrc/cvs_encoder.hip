@@ -74,7 +74,7 @@ int check_rows(const void* p, int64_t stride, int64_t width, const char* what) {
 struct LinearBackwardPlan {
   GemmPlan dx, dw;
   int parts;
-  int64_t dz, partial, gemm, bytes;  // offsets, then all
+  int64_t dz, partial, gemm, gemm_dw, bytes;  // offsets, then all
 };
 
 LinearBackwardPlan plan_linear_backward(int64_t m, int64_t k, int64_t n, int act, int cus) {
@@ -85,7 +85,8 @@ LinearBackwardPlan plan_linear_backward(int64_t m, int64_t k, int64_t n, int act
   int64_t at = 0;
   p.dz = at, at += act == CVS_ACT_NONE ? 0 : up256(m * n * 2);
   p.partial = at, at += up256((int64_t)p.parts * n * 4);
-  p.gemm = at, at += up256(std::max(p.dx.ws_bytes, p.dw.ws_bytes));
+  p.gemm = at, at += up256(p.dx.ws_bytes);
+  p.gemm_dw = at, at += up256(p.dw.ws_bytes);
   p.bytes = at;
   return p;
 }
@@ -307,7 +308,7 @@ int cvs_linear_backward(const void* dy, const void* x, const void* w, const void
   if (act != CVS_ACT_NONE || dbias != nullptr) {
     ActGradArgs g = {};
     g.type = type, g.act = act, g.m = m, g.n = (int)n, g.dy = dy, g.dy_stride = dy_stride, g.pre = pre;
-    g.dbias = dbias, g.partial = dbias != nullptr ? reinterpret_cast<float*>(ws + p.partial) : nullptr, g.parts = p.parts;
+    g.dbias = dbias, g.partial = reinterpret_cast<float*>(ws + p.partial), g.parts = p.parts;
     if (act != CVS_ACT_NONE) {
       g.dz = ws + p.dz;
       dz = g.dz, dz_stride = n;
@@ -315,23 +316,24 @@ int cvs_linear_backward(const void* dy, const void* x, const void* w, const void
     const hipError_t e = launch_act_grad(g, s);
     if (e != hipSuccess) return hip_fail(e, "linear backward launch");
   }
-  GemmArgs a = {};
-  a.type = type, a.partial = reinterpret_cast<float*>(ws + p.gemm);
-  if (dx != nullptr) {  // dz [m, n] x w [n, k]
-    a.m = (int)m, a.n = (int)k, a.k = (int)n;
-    a.M = dz, a.ldm = dz_stride, a.m_strided = false, a.N = w, a.ldn = k, a.n_strided = true;
-    a.out = dx, a.splits = p.dx.splits;
-    const hipError_t e = launch_gemm(a, p.dx, s);
-    if (e != hipSuccess) return hip_fail(e, "linear backward launch");
-  }
-  if (dw != nullptr) {  // dz^T [n, m] x x [m, k]
-    a.m = (int)n, a.n = (int)k, a.k = (int)m;
-    a.M = dz, a.ldm = dz_stride, a.m_strided = true, a.N = x, a.ldn = x_stride, a.n_strided = true;
-    a.out = dw, a.splits = p.dw.splits;
-    const hipError_t e = launch_gemm(a, p.dw, s);
-    if (e != hipSuccess) return hip_fail(e, "linear backward launch");
-  }
-  return CVS_OK;
+  GemmArgs x_args = {}, w_args = {};
+  x_args.type = w_args.type = type;
+  // dx = dz [m, n] x w [n, k]
+  x_args.m = (int)m, x_args.n = (int)k, x_args.k = (int)n;
+  x_args.M = dz, x_args.ldm = dz_stride, x_args.m_strided = false, x_args.N = w, x_args.ldn = k, x_args.n_strided = true;
+  x_args.out = dx, x_args.splits = p.dx.splits, x_args.partial = reinterpret_cast<float*>(ws + p.gemm);
+  // dw = dz^T [n, m] x x [m, k]
+  w_args.m = (int)n, w_args.n = (int)k, w_args.k = (int)m;
+  w_args.M = dz, w_args.ldm = dz_stride, w_args.m_strided = true, w_args.N = x, w_args.ldn = x_stride, w_args.n_strided = true;
+  w_args.out = dw, w_args.splits = p.dw.splits, w_args.partial = reinterpret_cast<float*>(ws + p.gemm_dw);
+  hipError_t e = hipSuccess;
+  if (dx != nullptr && dw != nullptr)
+    e = launch_gemm_pair(x_args, p.dx, w_args, p.dw, s);
+  else if (dx != nullptr)
+    e = launch_gemm(x_args, p.dx, s);
+  else if (dw != nullptr)
+    e = launch_gemm(w_args, p.dw, s);
+  return done(e, "linear backward launch");
 }
 
 int cvs_attention_plan(const cvs_attention* p, int backward, int device, int64_t* workspace_bytes) {

@@ -137,15 +137,22 @@ __device__ __forceinline__ void store_block(T* out, int64_t ld, int m, int n, in
   }
 }
 
-// WM x WN waves of BM x BN blocks of 32 x 32, RING stages in LDS.
+// Workgroups of a product: tiles rounded up to a multiple of 8, times the parts of the reduction.
+__host__ __device__ inline int gemm_grid(const GemmArgs& a, int tm, int tn) {
+  return (((a.m + tm - 1) / tm) * ((a.n + tn - 1) / tn) + 7) / 8 * 8 * a.splits;
+}
+
+template <int WM, int WN, int BM, int BN, int RING>
+constexpr int gemm_lds() { return RING * (WM * BM + WN * BN) * 32 * kDepth * 2; }
+
+// Workgroup `id` of a product: WM x WN waves of BM x BN blocks of 32 x 32, RING stages in LDS (smem).
 template <class T, int WM, int WN, int BM, int BN, int RING, bool MS, bool NS>
-__global__ __launch_bounds__(64 * WM * WN, (WM * BM + WN * BN) * RING <= 16 ? 2 : 1) void gemm_kernel(GemmArgs a) {
+__device__ __forceinline__ void gemm_tile(const GemmArgs& a, int id, unsigned char* smem) {
   constexpr int W = WM * WN, TM = WM * BM * 32, TN = WN * BN * 32;
   constexpr int MBYTES = TM * kDepth * 2, STAGE = (TM + TN) * kDepth * 2;
   constexpr int LM = MBYTES / 1024 / W, LN = (STAGE - MBYTES) / 1024 / W;  // 1 KiB loads a wave and stage
   static_assert(LM * 1024 * W == MBYTES && (LM + LN) * 1024 * W == STAGE, "whole loads");
   typedef typename Frag<T>::V V;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[RING * STAGE];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -160,16 +167,16 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * BM + WN * BN) * RING <= 16 ? 2 
   const int tiles_n = (a.n + TN - 1) / TN, tiles_m = (a.m + TM - 1) / TM;
   const int tiles = tiles_n * tiles_m;
   const int per = (tiles + 7) / 8;
-  const int local = blockIdx.x >> 3;
-  const int tile = (blockIdx.x & 7) * per + local;
-  if (local >= per || tile >= tiles) return;
+  const int split = id / (8 * per);
+  const int tile = (id & 7) * per + (id - split * 8 * per) / 8;
+  if (tile >= tiles) return;
   const int strip = tile / (kRows * tiles_n), in_strip = tile - strip * kRows * tiles_n;
   const int rows = min(kRows, tiles_m - strip * kRows);
   const int m0 = (strip * kRows + in_strip % rows) * TM, n0 = in_strip / rows * TN;
 
   const int stages = (a.k + kDepth - 1) / kDepth;
-  const int s_begin = (int)((int64_t)stages * blockIdx.y / a.splits);
-  const int s_end = (int)((int64_t)stages * (blockIdx.y + 1) / a.splits);
+  const int s_begin = (int)((int64_t)stages * split / a.splits);
+  const int s_end = (int)((int64_t)stages * (split + 1) / a.splits);
 
   // This lane's place in each 1 KiB load: line and 16-byte piece of the tile.
   uint32_t vm[LM], vn[LN];
@@ -328,7 +335,7 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * BM + WN * BN) * RING <= 16 ? 2 
     for (int j = 0; j < BN; ++j) {
       const int col0 = n0 + (wn * BN + j) * 32, col = col0 + 8 * g;
       if (a.splits > 1) {
-        float* p = a.partial + ((int64_t)blockIdx.y * a.m + row) * a.n + col;
+        float* p = a.partial + ((int64_t)split * a.m + row) * a.n + col;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           if (row < a.m && col + 16 * h < a.n) {
@@ -352,6 +359,24 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * BM + WN * BN) * RING <= 16 ? 2 
       }
     }
   }
+}
+
+template <class T, int WM, int WN, int BM, int BN, int RING, bool MS, bool NS>
+__global__ __launch_bounds__(64 * WM * WN, (WM * BM + WN * BN) * RING <= 16 ? 2 : 1) void gemm_kernel(GemmArgs a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[gemm_lds<WM, WN, BM, BN, RING>()];
+  gemm_tile<T, WM, WN, BM, BN, RING, MS, NS>(a, blockIdx.x, smem);
+}
+
+// Two products that share an operand, dx (first) and dW, in one launch: neither fills the GPU
+// where the rows are few.
+template <class T, int WM, int WN, int BM, int BN, int RING>
+__global__ __launch_bounds__(64 * WM * WN, (WM * BM + WN * BN) * RING <= 16 ? 2 : 1) void gemm_pair_kernel(GemmArgs a, GemmArgs b) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[gemm_lds<WM, WN, BM, BN, RING>()];
+  const int first = gemm_grid(a, WM * BM * 32, WN * BN * 32);
+  if ((int)blockIdx.x < first)
+    gemm_tile<T, WM, WN, BM, BN, RING, false, true>(a, blockIdx.x, smem);
+  else
+    gemm_tile<T, WM, WN, BM, BN, RING, true, true>(b, blockIdx.x - first, smem);
 }
 
 // Adds the parts of a split reduction, in order, and finishes: 8 columns a thread.
@@ -378,23 +403,34 @@ __global__ __launch_bounds__(kBlock) void gemm_join_kernel(GemmArgs a) {
   store8((T*)a.out + i * a.n + j, z);
 }
 
+template <class T>
+hipError_t launch_join(const GemmArgs& a, hipStream_t s) {
+  const int64_t threads = (int64_t)a.m * (a.n / 8);
+  hipLaunchKernelGGL((gemm_join_kernel<T>), dim3((unsigned)((threads + kBlock - 1) / kBlock)), dim3(kBlock), 0, s, a);
+  return hipGetLastError();
+}
+
 template <class T, int WM, int WN, int BM, int BN, int RING>
 hipError_t launch_tiles(const GemmArgs& a, hipStream_t s) {
-  constexpr int TM = WM * BM * 32, TN = WN * BN * 32;
-  const int tiles = ((a.m + TM - 1) / TM) * ((a.n + TN - 1) / TN);
-  const dim3 grid((tiles + 7) / 8 * 8, a.splits), block(64 * WM * WN);
+  const dim3 grid(gemm_grid(a, WM * BM * 32, WN * BN * 32)), block(64 * WM * WN);
   if (a.m_strided && a.n_strided)
     hipLaunchKernelGGL((gemm_kernel<T, WM, WN, BM, BN, RING, true, true>), grid, block, 0, s, a);
   else if (a.n_strided)
     hipLaunchKernelGGL((gemm_kernel<T, WM, WN, BM, BN, RING, false, true>), grid, block, 0, s, a);
   else
     hipLaunchKernelGGL((gemm_kernel<T, WM, WN, BM, BN, RING, false, false>), grid, block, 0, s, a);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess && a.splits > 1 ? launch_join<T>(a, s) : e;
+}
+
+template <class T, int WM, int WN, int BM, int BN, int RING>
+hipError_t launch_pair(const GemmArgs& a, const GemmArgs& b, hipStream_t s) {
+  constexpr int TM = WM * BM * 32, TN = WN * BN * 32;
+  hipLaunchKernelGGL((gemm_pair_kernel<T, WM, WN, BM, BN, RING>), dim3(gemm_grid(a, TM, TN) + gemm_grid(b, TM, TN)),
+                     dim3(64 * WM * WN), 0, s, a, b);
   hipError_t e = hipGetLastError();
-  if (e == hipSuccess && a.splits > 1) {
-    const int64_t threads = (int64_t)a.m * (a.n / 8);
-    hipLaunchKernelGGL((gemm_join_kernel<T>), dim3((unsigned)((threads + kBlock - 1) / kBlock)), dim3(kBlock), 0, s, a);
-    e = hipGetLastError();
-  }
+  if (e == hipSuccess && a.splits > 1) e = launch_join<T>(a, s);
+  if (e == hipSuccess && b.splits > 1) e = launch_join<T>(b, s);
   return e;
 }
 
@@ -405,15 +441,26 @@ hipError_t launch_typed(const GemmArgs& a, const GemmPlan& p, hipStream_t s) {
   return launch_tiles<T, 2, 2, 1, 1, 3>(a, s);
 }
 
+template <class T>
+hipError_t launch_typed_pair(const GemmArgs& a, const GemmArgs& b, const GemmPlan& p, hipStream_t s) {
+  if (p.tile == 128) return launch_pair<T, 2, 2, 2, 2, 2>(a, b, s);
+  return launch_pair<T, 2, 2, 1, 1, 3>(a, b, s);
+}
+
+// Pieces of 8 columns of a workgroup of act_grad_kernel: few for few rows, which one part then
+// has, so that it writes dbias itself.
+__host__ __device__ inline int act_grad_width(int64_t m, int n) { return m <= 256 ? 16 : min(n / 8, kBlock); }
+
 // dz = dy act'(pre) and its column sums, bound by memory.  A workgroup has up to 256
 // pieces of 8 columns (blockIdx.x) and as many of its part's rows at a time as its threads
 // cover; it adds its row lanes' sums in LDS and writes one partial row.
 template <class T>
 __global__ __launch_bounds__(kBlock) void act_grad_kernel(ActGradArgs a) {
   __shared__ float red[kBlock * 8];
-  const int pieces = min(a.n / 8 - (int)blockIdx.x * kBlock, kBlock), lanes = kBlock / pieces;
+  const int width = act_grad_width(a.m, a.n);
+  const int pieces = min(a.n / 8 - (int)blockIdx.x * width, width), lanes = kBlock / pieces;
   const int p = threadIdx.x % pieces, rl = threadIdx.x / pieces;
-  const int c = (blockIdx.x * kBlock + p) * 8;
+  const int c = (blockIdx.x * width + p) * 8;
   float sum[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) sum[e] = 0.f;
@@ -448,15 +495,18 @@ __global__ __launch_bounds__(kBlock) void act_grad_kernel(ActGradArgs a) {
       }
     }
   }
-  if (a.partial == nullptr) return;
+  if (a.dbias == nullptr) return;
 #pragma unroll
   for (int e = 0; e < 8; ++e) red[threadIdx.x * 8 + e] = sum[e];
   __syncthreads();
-  float* out = a.partial + (int64_t)blockIdx.y * a.n + (int64_t)blockIdx.x * kBlock * 8;
+  const int64_t col0 = (int64_t)blockIdx.x * width * 8;
   for (int t = threadIdx.x; t < pieces * 8; t += kBlock) {
     float s = 0.f;
     for (int l = 0; l < lanes; ++l) s += red[l * pieces * 8 + t];
-    out[t] = s;
+    if (gridDim.y == 1)
+      ((T*)a.dbias)[col0 + t] = (T)s;
+    else
+      a.partial[(int64_t)blockIdx.y * a.n + col0 + t] = s;
   }
 }
 
@@ -498,19 +548,30 @@ hipError_t launch_gemm(const GemmArgs& a, const GemmPlan& p, hipStream_t s) {
   return a.type == kF16 ? launch_typed<_Float16>(a, p, s) : launch_typed<__bf16>(a, p, s);
 }
 
+hipError_t launch_gemm_pair(const GemmArgs& a, const GemmPlan& pa, const GemmArgs& b, const GemmPlan& pb, hipStream_t s) {
+  if (pa.tile == pb.tile && pa.tile < 256)
+    return a.type == kF16 ? launch_typed_pair<_Float16>(a, b, pa, s) : launch_typed_pair<__bf16>(a, b, pa, s);
+  const hipError_t e = launch_gemm(a, pa, s);
+  return e == hipSuccess ? launch_gemm(b, pb, s) : e;
+}
+
 int act_grad_parts(int64_t m, int64_t n, int cus) {
-  const int64_t blocks = (n / 8 + kBlock - 1) / kBlock, lanes = std::max<int64_t>(1, kBlock / std::min<int64_t>(n / 8, kBlock));
+  const int64_t width = act_grad_width(m, (int)n);
+  if (m <= 256) return 1;
+  const int64_t blocks = (n / 8 + width - 1) / width, lanes = kBlock / width;
   return (int)std::max<int64_t>(1, std::min<int64_t>((m + lanes - 1) / lanes, 3 * cus / blocks));
 }
 
 hipError_t launch_act_grad(const ActGradArgs& a, hipStream_t s) {
-  const dim3 grid((a.n / 8 + kBlock - 1) / kBlock, a.parts), block(kBlock);
+  const int width = act_grad_width(a.m, a.n);
+  const dim3 grid((a.n / 8 + width - 1) / width, a.parts), block(kBlock);
   if (a.type == kF16)
     hipLaunchKernelGGL(act_grad_kernel<_Float16>, grid, block, 0, s, a);
   else
     hipLaunchKernelGGL(act_grad_kernel<__bf16>, grid, block, 0, s, a);
   hipError_t e = hipGetLastError();
-  if (e == hipSuccess && a.dbias != nullptr) e = launch_column_sums(a.partial, a.parts, a.n, a.n, 0, a.type, a.dbias, nullptr, s);
+  if (e == hipSuccess && a.dbias != nullptr && a.parts > 1)
+    e = launch_column_sums(a.partial, a.parts, a.n, a.n, 0, a.type, a.dbias, nullptr, s);
   return e;
 }
 

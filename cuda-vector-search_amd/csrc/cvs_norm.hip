@@ -235,6 +235,7 @@ __global__ __launch_bounds__(kBlock) void norm_backward_kernel(NormArgs a) {
     }
   }
   float* part = a.partial + (int64_t)blockIdx.x * 2 * a.d;
+  const bool alone = gridDim.x == 1;  // the sums are the gradients
 #pragma unroll
   for (int i = 0; i < P; ++i) {
 #pragma unroll
@@ -245,7 +246,14 @@ __global__ __launch_bounds__(kBlock) void norm_backward_kernel(NormArgs a) {
       __syncthreads();
       for (int t = threadIdx.x; t < 64 * VEC; t += kBlock) {
         const int c = i * 64 * VEC + t;
-        if (c < a.d) part[which * (int64_t)a.d + c] = (red[0][t] + red[1][t]) + (red[2][t] + red[3][t]);
+        if (c < a.d) {
+          const float s = (red[0][t] + red[1][t]) + (red[2][t] + red[3][t]);
+          T* out = reinterpret_cast<T*>(which ? a.dbias : a.dweight);
+          if (!alone)
+            part[which * (int64_t)a.d + c] = s;
+          else if (out != nullptr)
+            out[c] = (T)s;
+        }
       }
     }
   }
@@ -390,6 +398,7 @@ void backward(const NormArgs& a, hipStream_t s) {
 int norm_backward_parts(int64_t n, int64_t d, int type, int cus) {
   (void)type;
   if (d > kRegWidth) return (int)std::min<int64_t>(n, 64);
+  if (n <= 32) return 1;  // a launch for the sums would take longer than eight rows a wave
   return (int)std::min<int64_t>((n + 3) / 4, 4 * cus);
 }
 
@@ -424,6 +433,7 @@ hipError_t launch_norm_backward(const NormArgs& a, hipStream_t s) {
   else
     backward<float>(a, s);
   hipError_t e = hipGetLastError();
+  if (a.parts == 1 && a.d <= kRegWidth) return e;
   // the partial rows hold dweight's columns, then dbias's: one launch adds both
   const int64_t stride = 2 * (int64_t)a.d;
   if (e == hipSuccess && a.dweight != nullptr && a.dbias != nullptr)

@@ -93,6 +93,11 @@ def _workspace(lib, key, device, plan):
     return torch.empty(size, dtype=torch.uint8, device=device) if size else None
 
 
+def _new(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous memory for a result of t's shape and type."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -120,10 +125,10 @@ def layer_norm_forward(x, weight, bias=None, eps: float = 1e-5, stats: bool = Tr
     width = _norm_args(x, weight, bias)
     lib = _ext.load().lib
     r = _rows(x, width, False)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _new(x)
     mean = rstd = None
     if stats:
-        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
         rstd = torch.empty_like(mean)
     weight = weight.contiguous()
     bias = None if bias is None else bias.contiguous()
@@ -142,7 +147,7 @@ def layer_norm_backward(dy, x, weight, mean, rstd):
     r, g = _rows(x, width, False), _rows(dy, width, False)
     n = r.shape[0]
     mean, rstd = _stats(mean, "mean", x, x.shape[:-1]), _stats(rstd, "rstd", x, x.shape[:-1])
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = _new(x)
     if n == 0:
         return dx, torch.zeros_like(weight), torch.zeros_like(weight)
     weight = weight.contiguous()
@@ -216,7 +221,7 @@ def linear_forward(x, weight, bias=None, activation=None, residual=None, keep_pr
     lib = _ext.load().lib
     r = _rows(x, k, True)
     m = r.shape[0]
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(shape)
     pre = torch.empty_like(y) if keep_pre else None
     if m == 0:
         return y, pre
@@ -248,10 +253,10 @@ def linear_backward(dy, x, weight, activation=None, pre=None, needs=(True, True,
     lib = _ext.load().lib
     r, g = _rows(x, k, True), _rows(dy, n, True)
     m = r.shape[0]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if needs[0] else None
-    new = torch.zeros if m == 0 else torch.empty
-    dweight = new((n, k), dtype=x.dtype, device=x.device) if needs[1] else None
-    dbias = new((n,), dtype=x.dtype, device=x.device) if needs[2] else None
+    dx = _new(x) if needs[0] else None
+    new = x.new_zeros if m == 0 else x.new_empty
+    dweight = new((n, k)) if needs[1] else None
+    dbias = new((n,)) if needs[2] else None
     if m == 0:
         return dx, dweight, dbias
     weight = _packed(weight)
@@ -414,8 +419,8 @@ def attention_forward(q, k, v, bias_table=None, key_lengths=None, query_lengths=
     """
     a, call, hold = _attention_args(q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance)
     lib = _ext.load().lib
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    sums = torch.empty((a.batch, a.heads, a.q_len), dtype=torch.float32, device=q.device) if lse else None
+    out = _new(q)
+    sums = q.new_empty((a.batch, a.heads, a.q_len), dtype=torch.float32) if lse else None
     dev = q.device.index
     ws = _attention_workspace(lib, a, call, False, q.device)
     _check(lib.cvs_attention_forward(ctypes.byref(a), out.data_ptr(), _ptr(sums), _ptr(ws), 0 if ws is None else ws.numel(),
@@ -434,7 +439,7 @@ def attention_backward(dout, q, k, v, out, lse, bias_table=None, key_lengths=Non
     lib = _ext.load().lib
     dout, dout_stride = _strided(dout)
     out = _packed(out)
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    dq, dk, dv = _new(q), _new(k), _new(v)
     dtable = None if bias_table is None else torch.empty_like(hold[3])
     if a.batch == 0 or (a.q_len == 0 and a.k_len == 0):
         return dq, dk, dv, None if dtable is None else dtable.zero_()
