@@ -94,8 +94,8 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 3) void attn_forward_kernel(A
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) x[kb] = Frag<T>::mfma(rows[kb][s], qf[s], x[kb]);
     };
-    const int reach = a.max_distance + kReach;
-    if (!BIAS || near - 31 >= a.max_distance || near + kKeys - 1 <= -a.max_distance) {
+    const int reach = a.far + kReach;
+    if (!BIAS || near - 31 >= a.far || near + kKeys - 1 <= -a.far) {
       if (BIAS) shift = tab[near > 0 ? 2 * reach : 0];
       keep_order();
       x[0] = x[1] = zero16();
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_rows_kernel(Attn
   for (int d = 0; d < DB; ++d) acc[d] = zero16();
   float m = -__builtin_inff(), sum = 0.f;
   const float c = a.scale * kLog2e, slack = 8.f / c;
-  const int reach = a.max_distance + kReach;
+  const int reach = a.far + kReach;
   wait_vmcnt_lgkm0<0>();
   for (; t < t1; t += 4, buf ^= 1) {
     wait_vmcnt_lgkm0<63>();  // the reads of the buffer to be loaded next
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_rows_kernel(Attn
     f32x16 x = zero16();
     float shift = 0.f;
     if (BIAS) {
-      if (near - 31 >= a.max_distance || near + 31 <= -a.max_distance) {
+      if (near - 31 >= a.far || near + 31 <= -a.far) {
         shift = tab[near > 0 ? 2 * reach : 0];
       } else {
         const float* at = tab + (near - l32 + 8 * g + reach);
@@ -411,7 +411,7 @@ int64_t workgroups(const AttnArgs& a) {
 template <class T, int DP>
 void launch_width(const AttnArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)workgroups(a), a.splits), block(kBlock);
-  const size_t tab = (2 * (a.max_distance + kReach) + 1) * sizeof(float);
+  const size_t tab = (2 * (a.far + kReach) + 1) * sizeof(float);
   if (few_rows(a) && a.table != nullptr)
     hipLaunchKernelGGL((attn_rows_kernel<T, DP, true>), grid, block, tab, s, a);
   else if (few_rows(a))

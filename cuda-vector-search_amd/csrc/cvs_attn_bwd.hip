@@ -37,12 +37,15 @@ constexpr int kTile = DP > 64 ? 32 : 64;
 // instead took 192 cycles each: 281 us of 32 sequences of up to 512, 12 heads of 64.)
 constexpr int kSkewPitch = 36, kSkew = 64 * kSkewPitch;
 
-__device__ __forceinline__ void add_positions(float* skew, float* sums, const f32x16& ds) {
+__device__ __forceinline__ void put_positions(float* skew, const f32x16& ds) {
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   float* to = skew + (8 * g - l32 + 31) * kSkewPitch + l32;
 #pragma unroll
   for (int e = 0; e < 16; ++e) to[elem_row(e, 0) * kSkewPitch] = ds[e];
   __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+}
+__device__ __forceinline__ void take_positions(const float* skew, float* sums) {
+  const int lane = threadIdx.x & 63;
   const f32x4* from = reinterpret_cast<const f32x4*>(skew + lane * kSkewPitch);
   f32x4 s = from[0];
 #pragma unroll
@@ -113,9 +116,9 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
     lse = a.lse[row_at] * kLog2e;
     if (lse == -__builtin_inff()) lse = kNever;  // a row that sees nothing
   }
-  const int reach = a.max_distance + kReach, places = 2 * reach + 1;
+  const int reach = a.far + kReach, places = 2 * reach + 1;
   float* sums = tab + places + wave * places + reach;  // by position, this wave's
-  float before = 0.f, after = 0.f;                     // positions all <= -max_distance, all >= max_distance
+  float before = 0.f, after = 0.f;                     // positions all <= -far, all >= far
   if (BIAS) {
     load_bias<T>(tab, a, h);
     for (int t = threadIdx.x; t < 4 * places; t += kBlock) tab[places + t] = 0.f;
@@ -147,7 +150,7 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
       const int near = near0 + kb * 32;
       base[kb] = -lse;
       if (BIAS) {
-        if (near - 31 >= a.max_distance || near + 31 <= -a.max_distance) {
+        if (near - 31 >= a.far || near + 31 <= -a.far) {
           base[kb] += tab[near > 0 ? 2 * reach : 0] * c;
           p[kb] = zero16();
         } else {
@@ -230,25 +233,33 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
     }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
+      const int near = near0 + kb * 32;
+      const bool in_range = near + 31 > -a.far && near - 31 < a.far;
 #pragma unroll
       for (int e = 0; e < 16; ++e) ds[kb][e] *= p[kb][e];
       if (BIAS) {
-        const int near = near0 + kb * 32;
-        if (near + 31 <= -a.max_distance) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) before += ds[kb][e];
-        } else if (near - 31 >= a.max_distance) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) after += ds[kb][e];
+        if (in_range) {
+          put_positions(skew[wave], ds[kb]);
         } else {
-          add_positions(skew[wave], sums + near - 31, ds[kb]);
+          float s = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s += ds[kb][e];
+          if (near < 0)
+            before += s;
+          else
+            after += s;
         }
+        keep_order();  // (the sums' places settle in LDS under the products)
       }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const V df = pack8<T>(ds[kb], s);
 #pragma unroll
         for (int d = 0; d < DB; ++d) dq[d] = Frag<T>::mfma(kcols[kb][s][d], df, dq[d]);
+      }
+      if (BIAS) {
+        keep_order();
+        if (in_range) take_positions(skew[wave], sums + near - 31);
       }
     }
   }
@@ -346,7 +357,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
 #pragma unroll
   for (int d = 0; d < DB; ++d) dk[d] = dv[d] = zero16();
   const float c = a.scale * kLog2e;
-  const int reach = a.max_distance + kReach;
+  const int reach = a.far + kReach;
   const bool one = nk <= ROWS;  // delta is dout . v's own sum: subtracted as it stands
 
   // tiles of queries that see a key of this workgroup, those of all heads in a row; this part's
@@ -407,7 +418,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
 #pragma unroll
         for (int s = 0; s < KS; ++s) qrows[s] = row_frag<T, DP>(sq[buf], qb * 32, s);
         if (BIAS) {
-          if (near - 31 >= a.max_distance || near + 31 <= -a.max_distance) {
+          if (near - 31 >= a.far || near + 31 <= -a.far) {
             shift = tab[near > 0 ? 2 * reach : 0] * c;
             p = zero16();
           } else {
@@ -507,7 +518,7 @@ __global__ __launch_bounds__(kBlock) void attn_join_grads_kernel(const float* pa
 template <class T, int DP, bool BIAS>
 hipError_t launch_width(const AttnArgs& a, hipStream_t s) {
   const int64_t qblocks = (a.lq + kAttnRows - 1) / kAttnRows, kblocks = (a.lk + kAttnRows - 1) / kAttnRows;
-  const size_t tab = BIAS ? (2 * (a.max_distance + kReach) + 1) * sizeof(float) : 0;
+  const size_t tab = BIAS ? (2 * (a.far + kReach) + 1) * sizeof(float) : 0;
   if (qblocks > 0)
     hipLaunchKernelGGL((attn_backward_q_kernel<T, DP, BIAS>), dim3((unsigned)(qblocks * a.batch * a.heads), a.q_parts),
                        dim3(kBlock), 5 * tab, s, a);

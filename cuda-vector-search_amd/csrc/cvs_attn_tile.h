@@ -124,22 +124,23 @@ __device__ __forceinline__ void store_part_row(float* row, const f32x16* acc, in
 }
 
 // A head's learned bias by relative position, in LDS, in units of unscaled scores (so that it
-// is what a block of scores starts from): tab[rel + reach], reach = max_distance + kReach.  A
-// block of 32 queries and up to 64 keys that has a position nearer than max_distance has
-// none further than max_distance + kReach; other blocks have one bias throughout.
+// is what a block of scores starts from): tab[rel + reach], reach = far + kReach, far being
+// the smallest distance of the last bucket.  A block of 32 queries and up to 64 keys that has
+// a position nearer than far has none further than far + kReach; other blocks have one
+// bias throughout.
 constexpr int kReach = 96;
 
 template <class T>
 __device__ __forceinline__ void load_bias(float* tab, const AttnArgs& a, int head) {
   constexpr int N = (2 * (kMaxDistance + kReach) + kBlock) / kBlock;  // places a thread, all under way together
-  const int reach = a.max_distance + kReach;
+  const int reach = a.far + kReach;
   const float unit = 1.f / a.scale;
   int u[N];
   float v[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     const int rel = min((int)threadIdx.x + n * kBlock, 2 * reach) - reach;
-    u[n] = a.bucket_of[min(abs(rel), a.max_distance)];
+    u[n] = a.bucket_of[min(abs(rel), a.far)];
     if (rel > 0) u[n] = a.causal ? 0 : u[n] + a.one_way;
   }
 #pragma unroll

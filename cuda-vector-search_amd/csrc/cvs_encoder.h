@@ -108,6 +108,7 @@ struct AttnArgs {
   // learned bias by relative position
   const void* table;              // [buckets, heads] or null
   int buckets, max_distance;
+  int far;                             // smallest distance of the last bucket
   int one_way;                          // buckets of one direction
   unsigned char bucket_of[kMaxDistance + 1];   // a direction's bucket by distance (the last: all further ones)
   unsigned short edges[kMaxBuckets + 1];       // smallest distance of each, then one past max_distance

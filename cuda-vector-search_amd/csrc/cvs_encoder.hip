@@ -148,6 +148,7 @@ AttnArgs attn_args(const cvs_attention* p) {
     for (int t = 1; t < wide; ++t)
       a.edges[exact + t] = (unsigned short)std::ceil(exact * std::pow((double)a.max_distance / exact, (double)t / wide) - 1e-9);
     a.edges[a.one_way] = (unsigned short)(a.max_distance + 1);
+    a.far = a.edges[a.one_way - 1];
     for (int dist = 0, u = 0; dist <= a.max_distance; ++dist) {
       while (u + 1 < a.one_way && a.edges[u + 1] <= dist) ++u;
       a.bucket_of[dist] = (unsigned char)u;
