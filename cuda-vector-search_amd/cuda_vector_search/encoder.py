@@ -81,7 +81,7 @@ def _row_stride(r: torch.Tensor) -> int:
     return r.stride(0) if r.shape[0] > 1 else r.shape[1]
 
 
-def _workspace(lib, key, device, plan):
+def _workspace(key, like, plan):
     """Scratch of a call: its size by ``plan`` (asked once for each set of sizes)."""
     size = _plans.get(key)
     if size is None:
@@ -90,7 +90,7 @@ def _workspace(lib, key, device, plan):
         if len(_plans) >= 4096:
             _plans.clear()
         size = _plans[key] = int(out.value)
-    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    return like.new_empty(size, dtype=torch.uint8) if size else None
 
 
 def _new(t: torch.Tensor) -> torch.Tensor:
@@ -153,7 +153,7 @@ def layer_norm_backward(dy, x, weight, mean, rstd):
     weight = weight.contiguous()
     dweight, dbias = torch.empty_like(weight), torch.empty_like(weight)
     dev, code = x.device.index, TYPES[x.dtype]
-    ws = _workspace(lib, ("norm", n, width, code, dev), x.device,
+    ws = _workspace(("norm", n, width, code, dev), x,
                     lambda out: lib.cvs_layer_norm_backward_plan(n, width, code, dev, out))
     _check(lib.cvs_layer_norm_backward(g.data_ptr(), r.data_ptr(), weight.data_ptr(), mean.data_ptr(), rstd.data_ptr(), n,
                                        width, _row_stride(g), _row_stride(r), code, dx.data_ptr(), dweight.data_ptr(),
@@ -229,7 +229,7 @@ def linear_forward(x, weight, bias=None, activation=None, residual=None, keep_pr
     bias = None if bias is None else _packed(bias)
     res = None if residual is None else _rows(residual, n, True)
     dev = x.device.index
-    ws = _workspace(lib, ("linear", m, k, n, dev), x.device, lambda out: lib.cvs_linear_plan(m, k, n, dev, out))
+    ws = _workspace(("linear", m, k, n, dev), x, lambda out: lib.cvs_linear_plan(m, k, n, dev, out))
     _check(lib.cvs_linear(r.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(res), m, k, n, _row_stride(r),
                           0 if res is None else _row_stride(res), ACTIVATIONS[activation], TYPES[x.dtype], y.data_ptr(),
                           _ptr(pre), _ptr(ws), 0 if ws is None else ws.numel(), dev, _ext.raw_stream(dev)))
@@ -261,7 +261,7 @@ def linear_backward(dy, x, weight, activation=None, pre=None, needs=(True, True,
         return dx, dweight, dbias
     weight = _packed(weight)
     dev, act = x.device.index, ACTIVATIONS[activation]
-    ws = _workspace(lib, ("linear backward", m, k, n, act, dev), x.device,
+    ws = _workspace(("linear backward", m, k, n, act, dev), x,
                     lambda out: lib.cvs_linear_backward_plan(m, k, n, act, dev, out))
     _check(lib.cvs_linear_backward(g.data_ptr(), r.data_ptr(), weight.data_ptr(), _ptr(pre), m, k, n, _row_stride(g),
                                    _row_stride(r), act, TYPES[x.dtype], _ptr(dx), _ptr(dweight), _ptr(dbias), _ptr(ws),
@@ -389,15 +389,15 @@ def _attention_args(q, k, v, bias_table, key_lengths, query_lengths, query_start
     return a, call, hold
 
 
-def _attention_workspace(lib, a, call, backward: bool, device):
+def _attention_workspace(lib, a, call, backward: bool, q):
     size = None if call is None else call.bytes[backward]
     if size is None:
         out = _I64(0)
-        _check(lib.cvs_attention_plan(ctypes.byref(a), backward, device.index, ctypes.byref(out)))
+        _check(lib.cvs_attention_plan(ctypes.byref(a), backward, q.device.index, ctypes.byref(out)))
         size = int(out.value)
         if call is not None:
             call.bytes[backward] = size
-    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    return q.new_empty(size, dtype=torch.uint8) if size else None
 
 
 def attention_forward(q, k, v, bias_table=None, key_lengths=None, query_lengths=None, query_start=None,
@@ -422,7 +422,7 @@ def attention_forward(q, k, v, bias_table=None, key_lengths=None, query_lengths=
     out = _new(q)
     sums = q.new_empty((a.batch, a.heads, a.q_len), dtype=torch.float32) if lse else None
     dev = q.device.index
-    ws = _attention_workspace(lib, a, call, False, q.device)
+    ws = _attention_workspace(lib, a, call, False, q)
     _check(lib.cvs_attention_forward(ctypes.byref(a), out.data_ptr(), _ptr(sums), _ptr(ws), 0 if ws is None else ws.numel(),
                                      dev, _ext.raw_stream(dev)))
     return out, sums
@@ -444,7 +444,7 @@ def attention_backward(dout, q, k, v, out, lse, bias_table=None, key_lengths=Non
     if a.batch == 0 or (a.q_len == 0 and a.k_len == 0):
         return dq, dk, dv, None if dtable is None else dtable.zero_()
     dev = q.device.index
-    ws = _attention_workspace(lib, a, call, True, q.device)
+    ws = _attention_workspace(lib, a, call, True, q)
     _check(lib.cvs_attention_backward(ctypes.byref(a), dout.data_ptr(), dout_stride, out.data_ptr(), lse.data_ptr(),
                                       dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dtable), _ptr(ws),
                                       0 if ws is None else ws.numel(), dev, _ext.raw_stream(dev)))
