@@ -55,6 +55,7 @@ int check_linear(int64_t m, int64_t k, int64_t n) {
   if (k < 8 || n < 8 || k % 8 != 0 || n % 8 != 0)
     return fail(CVS_ERR_INVALID, "linear takes feature counts that are multiples of 8 (zero-pad them)");
   if (k > (1 << 20) || n > (1 << 20)) return fail(CVS_ERR_INVALID, "linear takes at most 2^20 features");
+  if (m * std::max(k, n) > ((int64_t)1 << 36)) return fail(CVS_ERR_INVALID, "linear: more than 2^36 values in a matrix");
   return CVS_OK;
 }
 
@@ -105,7 +106,7 @@ int check_attention(const cvs_attention* p) {
   if (p->heads > 65536 || p->batch > INT_MAX / p->heads)
     return fail(CVS_ERR_INVALID, "attention: too many heads");
   for (const int64_t len : {p->q_len, p->k_len})
-    if ((len + kAttnRows - 1) / kAttnRows * p->batch * p->heads > INT_MAX || p->batch * len * p->heads > ((int64_t)1 << 35))
+    if ((len + kAttnRows - 1) / kAttnRows * p->batch * p->heads >= (1 << 23))  // (a launch has fewer than 2^32 threads)
       return fail(CVS_ERR_INVALID, "attention: too many rows");
   if (!(p->scale > 0) || !std::isfinite((float)p->scale)) return fail(CVS_ERR_INVALID, "attention: scale must be positive and finite");
   if (p->bias_table != nullptr) {

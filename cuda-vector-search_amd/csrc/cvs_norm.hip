@@ -263,23 +263,24 @@ __global__ __launch_bounds__(kBlock) void norm_backward_kernel(NormArgs a) {
 template <class T>
 __global__ __launch_bounds__(kBlock) void norm_backward_wide_kernel(NormArgs a) {
   __shared__ float scratch[kBlock / kWave];
-  const int64_t row = blockIdx.x;
-  const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_stride;
-  const T* dy = reinterpret_cast<const T*>(a.dy) + row * a.dy_stride;
-  const T* w = reinterpret_cast<const T*>(a.weight);
-  const float mean = a.mean[row], rstd = a.rstd[row];
-  float sg = 0.f, sgh = 0.f;
-  for (int c = threadIdx.x; c < a.d; c += kBlock) {
-    const float g = (float)dy[c] * (float)w[c];
-    sg += g;
-    sgh = fmaf(g, ((float)x[c] - mean) * rstd, sgh);
+  for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
+    const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_stride;
+    const T* dy = reinterpret_cast<const T*>(a.dy) + row * a.dy_stride;
+    const T* w = reinterpret_cast<const T*>(a.weight);
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    float sg = 0.f, sgh = 0.f;
+    for (int c = threadIdx.x; c < a.d; c += kBlock) {
+      const float g = (float)dy[c] * (float)w[c];
+      sg += g;
+      sgh = fmaf(g, ((float)x[c] - mean) * rstd, sgh);
+    }
+    const float inv_d = 1.f / (float)a.d;
+    const float mg = block_sum(sg, scratch) * inv_d;
+    const float mgh = block_sum(sgh, scratch) * inv_d;
+    T* dx = reinterpret_cast<T*>(a.dx) + row * a.d;
+    for (int c = threadIdx.x; c < a.d; c += kBlock)
+      dx[c] = (T)(rstd * ((float)dy[c] * (float)w[c] - mg - ((float)x[c] - mean) * rstd * mgh));
   }
-  const float inv_d = 1.f / (float)a.d;
-  const float mg = block_sum(sg, scratch) * inv_d;
-  const float mgh = block_sum(sgh, scratch) * inv_d;
-  T* dx = reinterpret_cast<T*>(a.dx) + row * a.d;
-  for (int c = threadIdx.x; c < a.d; c += kBlock)
-    dx[c] = (T)(rstd * ((float)dy[c] * (float)w[c] - mg - ((float)x[c] - mean) * rstd * mgh));
 }
 
 // Partial column sums of wide rows: workgroup (x: 256 columns, y: part of the rows).
@@ -346,9 +347,9 @@ void launch_rows(const NormArgs& a, bool backward, hipStream_t s) {
     hipLaunchKernelGGL((norm_forward_kernel<T, VEC, P>), dim3((unsigned)((a.n + 3) / 4)), dim3(kBlock), 0, s, a);
 }
 
-// The fewest columns a lane that hold the row: pieces of 4 where every row starts on one,
-// single elements otherwise.  (Pieces of 8 of 16-bit rows leave a quarter of the lanes' second
-// piece empty at width 768, the registers with it.)
+// The fewest columns a lane that hold the row: pieces of 4, or of 2, where every row starts on
+// one, single elements otherwise.  (Pieces of 8 of 16-bit rows leave a quarter of the lanes'
+// second piece empty at width 768, the registers with it.)
 template <class T>
 void launch_narrow(const NormArgs& a, bool backward, hipStream_t s) {
   const int lanes = (a.d + 63) / 64;
@@ -365,9 +366,16 @@ void launch_narrow(const NormArgs& a, bool backward, hipStream_t s) {
       launch_rows<T, 4, 6>(a, backward, s);
     else
       launch_rows<T, 4, 8>(a, backward, s);
+  } else if (aligned_rows<T>(a, 2, backward)) {
+    if (lanes <= 6)
+      launch_rows<T, 2, 3>(a, backward, s);
+    else if (lanes <= 16)
+      launch_rows<T, 2, 8>(a, backward, s);
+    else
+      launch_rows<T, 2, 16>(a, backward, s);
   } else {
-    if (lanes <= 4)
-      launch_rows<T, 1, 4>(a, backward, s);
+    if (lanes <= 6)
+      launch_rows<T, 1, 6>(a, backward, s);
     else if (lanes <= 16)
       launch_rows<T, 1, 16>(a, backward, s);
     else
@@ -388,7 +396,7 @@ void backward(const NormArgs& a, hipStream_t s) {
   if (a.d <= kRegWidth) {
     launch_narrow<T>(a, true, s);
   } else {
-    hipLaunchKernelGGL(norm_backward_wide_kernel<T>, dim3((unsigned)a.n), dim3(kBlock), 0, s, a);
+    hipLaunchKernelGGL(norm_backward_wide_kernel<T>, dim3((unsigned)std::min<int64_t>(a.n, 1 << 20)), dim3(kBlock), 0, s, a);
     hipLaunchKernelGGL(norm_columns_kernel<T>, dim3((a.d + kBlock - 1) / kBlock, a.parts), dim3(kBlock), 0, s, a);
   }
 }
@@ -417,14 +425,26 @@ hipError_t launch_column_sums(const float* partial, int parts, int64_t stride, i
   return hipGetLastError();
 }
 
-hipError_t launch_norm_forward(const NormArgs& a, hipStream_t s) {
-  if (a.type == kF16)
-    forward<_Float16>(a, s);
-  else if (a.type == kBF16)
-    forward<__bf16>(a, s);
-  else
-    forward<float>(a, s);
-  return hipGetLastError();
+hipError_t launch_norm_forward(const NormArgs& all, hipStream_t s) {
+  // (a launch has fewer than 2^32 threads: rows in pieces)
+  constexpr int64_t kRows = 1 << 23;
+  const int64_t size = all.type == kF32 ? 4 : 2;
+  for (int64_t r = 0; r < all.n; r += kRows) {
+    NormArgs a = all;
+    a.n = std::min(kRows, all.n - r);
+    a.x = static_cast<const char*>(all.x) + r * all.x_stride * size;
+    a.y = static_cast<char*>(all.y) + r * all.d * size;
+    if (all.mean != nullptr) a.mean = all.mean + r, a.rstd = all.rstd + r;
+    if (a.type == kF16)
+      forward<_Float16>(a, s);
+    else if (a.type == kBF16)
+      forward<__bf16>(a, s);
+    else
+      forward<float>(a, s);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_norm_backward(const NormArgs& a, hipStream_t s) {
