@@ -52,6 +52,8 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 3) void attn_forward_kernel(A
     t1 = (int)((unsigned)tiles * (blockIdx.y + 1) / (unsigned)a.splits);
   }
 
+  BiasLoad<T> bias;
+  if (BIAS) bias.buckets(a);
   const TileLoad<DP, kKeys> lk(2 * a.ks[1], a.d), lv(2 * a.vs[1], a.d);
   auto load = [&](int t) {
     lk.load(kbase, 2 * a.ks[1], t * kKeys, nk, sk[t & 1]);
@@ -61,7 +63,10 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 3) void attn_forward_kernel(A
   V qf[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s) qf[s] = global_frag<T>(qrow, s, a.d, i < nq);
-  if (BIAS) load_bias<T>(tab, a, h);
+  if (BIAS) {
+    bias.values(a, h);
+    bias.store(a, tab);
+  }
 
   f32x16 acc[DB];
 #pragma unroll
@@ -217,6 +222,8 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_rows_kernel(Attn
     t0 = (int)((unsigned)tiles * blockIdx.y / (unsigned)a.splits);
     t1 = (int)((unsigned)tiles * (blockIdx.y + 1) / (unsigned)a.splits);
   }
+  BiasLoad<T> bias;
+  if (BIAS) bias.buckets(a);
   const TileLoad<DP, 32, 1> lk(2 * a.ks[1], a.d), lv(2 * a.vs[1], a.d);
   auto load = [&](int t, int buf) {
     lk.load(kbase, 2 * a.ks[1], t * 32, nk, smem[wave][buf][0]);
@@ -229,7 +236,8 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_rows_kernel(Attn
 #pragma unroll
   for (int s = 0; s < KS; ++s) qf[s] = global_frag<T>(qrow, s, a.d, row && i < nq);
   if (BIAS) {
-    load_bias<T>(tab, a, h0);
+    bias.values(a, h0);
+    bias.store(a, tab);
     __syncthreads();
   }
 

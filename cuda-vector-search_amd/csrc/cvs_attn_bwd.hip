@@ -92,6 +92,8 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
     tiles = (int)((unsigned)all * (blockIdx.y + 1) / (unsigned)a.q_parts);
   }
   const bool writes_delta = (int)blockIdx.y == (one ? a.q_parts - 1 : 0);
+  BiasLoad<T> bias;
+  if (BIAS) bias.buckets(a);
   const TileLoad<DP, ROWS> lk(2 * a.ks[1], a.d), lv(2 * a.vs[1], a.d);
   auto load = [&](int t) {
     lk.load(kbase, 2 * a.ks[1], t * ROWS, nk, sk[t & 1]);
@@ -99,31 +101,33 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
   };
   if (t0 < tiles) load(t0);
 
-  V qf[KS], gf[KS];
-  float delta = 0.f;
+  // the first loads are all on their way before one is waited for: the keys' and values' tiles,
+  // the bias, the rows, and under them shared memory is cleared
+  V qf[KS], gf[KS], of[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
     qf[s] = global_frag<T>(qrow, s, a.d, i < nq);
     gf[s] = global_frag<T>(grow, s, a.d, i < nq);
-    const V of = global_frag<T>(orow, s, a.d, i < nq);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) delta = fmaf((float)gf[s][j], (float)of[j], delta);
+    of[s] = global_frag<T>(orow, s, a.d, i < nq);
   }
-  delta = one ? 0.f : halves_sum(delta);
   const int64_t row_at = (int64_t)bh * a.lq + i;
-  float lse = kNever;
-  if (i < nq) {
-    lse = a.lse[row_at] * kLog2e;
-    if (lse == -__builtin_inff()) lse = kNever;  // a row that sees nothing
-  }
+  float lse = i < nq ? a.lse[row_at] * kLog2e : kNever;
+  if (BIAS) bias.values(a, h);
   const int reach = a.far + kReach, places = 2 * reach + 1;
   float* sums = tab + places + wave * places + reach;  // by position, this wave's
   float before = 0.f, after = 0.f;                     // positions all <= -far, all >= far
   if (BIAS) {
-    load_bias<T>(tab, a, h);
     for (int t = threadIdx.x; t < 4 * places; t += kBlock) tab[places + t] = 0.f;
     for (int t = threadIdx.x; t < kSkew; t += kBlock) reinterpret_cast<f32x4*>(&skew[0][0])[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    bias.store(a, tab);
   }
+  float delta = 0.f;
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) delta = fmaf((float)gf[s][j], (float)of[s][j], delta);
+  delta = one ? 0.f : halves_sum(delta);
+  if (lse == -__builtin_inff()) lse = kNever;  // a row that sees nothing
 
   f32x16 dq[DB];
 #pragma unroll
@@ -296,6 +300,7 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
     if (bucket < a.buckets) {
       const int u = bucket % a.one_way, side = bucket / a.one_way;  // side 0: key at or before the query
       const int d0 = max((int)a.edges[u], side), d1 = u + 1 < a.one_way ? (int)a.edges[u + 1] : reach + 1;
+#pragma unroll 4
       for (int dist = d0 + l; dist < d1; dist += lanes) {
         const float* at = tab + places + reach + (side == 1 ? dist : -dist);
         s += (at[0] + at[places]) + (at[2 * places] + at[3 * places]);
@@ -370,6 +375,8 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
     f1 = (int)(all * (blockIdx.y + 1) / a.kv_parts);
   }
   const TileLoad<DP, ROWS> lq(2 * a.qs[1], a.d), lg(2 * a.dos[1], a.d);
+  BiasLoad<T> bias;
+  if (BIAS) bias.buckets(a);
   while (f0 < f1) {
     const int hh = f0 / nt, h = hk * group + hh;
     const int first = t0 + f0 % nt, last = min(t0 + nt, first + f1 - f0);  // this head's
@@ -379,7 +386,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
     const float* lse = a.lse + ((int64_t)b * a.heads + h) * a.lq;
     const float* delta = a.delta + ((int64_t)b * a.heads + h) * a.lq;
     __syncthreads();  // the last head's tiles and bias have been read
-    if (BIAS) load_bias<T>(tab, a, h);
+    if (BIAS) bias.values(a, h);
     float stat = 0.f;  // threads 0 .. ROWS - 1: -log2 sum of a row, the next ROWS: -delta
     auto load = [&](int t) {
       lq.load(qbase, 2 * a.qs[1], t * ROWS, nq, sq[t & 1]);
@@ -401,6 +408,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
       if (t + 1 < last) load(t + 1);
     };
     load(first);
+    if (BIAS) bias.store(a, tab);
     // tiles that no key of this wave is seen from come first: it only loads its share of them
     int mine = j0 < nk ? first : last;
     if (a.causal) mine = min(last, max(mine, (j0 - off) / ROWS));

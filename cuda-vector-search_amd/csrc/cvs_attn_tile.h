@@ -130,27 +130,36 @@ __device__ __forceinline__ void store_part_row(float* row, const f32x16* acc, in
 // bias throughout.
 constexpr int kReach = 96;
 
+// Two dependent loads from memory, in steps that a kernel puts its other first loads between.
 template <class T>
-__device__ __forceinline__ void load_bias(float* tab, const AttnArgs& a, int head) {
-  constexpr int N = (2 * (kMaxDistance + kReach) + kBlock) / kBlock;  // places a thread, all under way together
-  const int reach = a.far + kReach;
-  const float unit = 1.f / a.scale;
+struct BiasLoad {
+  static constexpr int N = (2 * (kMaxDistance + kReach) + kBlock) / kBlock;  // places a thread
   int u[N];
   float v[N];
+
+  __device__ __forceinline__ void buckets(const AttnArgs& a) {
+    const int reach = a.far + kReach;
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const int rel = min((int)threadIdx.x + n * kBlock, 2 * reach) - reach;
-    u[n] = a.bucket_of[min(abs(rel), a.far)];
-    if (rel > 0) u[n] = a.causal ? 0 : u[n] + a.one_way;
+    for (int n = 0; n < N; ++n) {
+      const int rel = min((int)threadIdx.x + n * kBlock, 2 * reach) - reach;
+      u[n] = a.bucket_of[min(abs(rel), a.far)];
+      if (rel > 0) u[n] = a.causal ? 0 : u[n] + a.one_way;
+    }
   }
+  __device__ __forceinline__ void values(const AttnArgs& a, int head) {
+    const float unit = 1.f / a.scale;
 #pragma unroll
-  for (int n = 0; n < N; ++n) v[n] = (float)((const T*)a.table)[u[n] * a.heads + head] * unit;
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const int t = threadIdx.x + n * kBlock;
-    if (t <= 2 * reach) tab[t] = v[n];
+    for (int n = 0; n < N; ++n) v[n] = (float)((const T*)a.table)[u[n] * a.heads + head] * unit;
   }
-}
+  __device__ __forceinline__ void store(const AttnArgs& a, float* tab) const {
+    const int reach = a.far + kReach;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int t = threadIdx.x + n * kBlock;
+      if (t <= 2 * reach) tab[t] = v[n];
+    }
+  }
+};
 
 __device__ __forceinline__ int key_count(const AttnArgs& a, int b) {
   return a.key_lengths == nullptr ? a.lk : min(max(a.key_lengths[b], 0), a.lk);
