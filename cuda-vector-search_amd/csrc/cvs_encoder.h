@@ -60,8 +60,8 @@ struct GemmArgs {
   int splits;
 };
 struct GemmPlan {
-  int tile;     // rows and columns of a workgroup's tile
-  int splits;   // parts of the reduction
+  int tile, tile_n;  // rows and columns of a workgroup's tile
+  int splits;        // parts of the reduction
   int64_t ws_bytes;
 };
 GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int cus);

@@ -436,7 +436,7 @@ hipError_t launch_pair(const GemmArgs& a, const GemmArgs& b, hipStream_t s) {
 
 template <class T>
 hipError_t launch_typed(const GemmArgs& a, const GemmPlan& p, hipStream_t s) {
-  if (p.tile == 256) return launch_tiles<T, 4, 2, 2, 4, 2>(a, s);
+  if (p.tile == 256) return p.tile_n == 256 ? launch_tiles<T, 4, 2, 2, 4, 2>(a, s) : launch_tiles<T, 4, 2, 2, 3, 2>(a, s);
   if (p.tile == 128) return launch_tiles<T, 2, 2, 2, 2, 2>(a, s);
   return launch_tiles<T, 2, 2, 1, 1, 3>(a, s);
 }
@@ -512,23 +512,27 @@ __global__ __launch_bounds__(kBlock) void act_grad_kernel(ActGradArgs a) {
 
 }  // namespace
 
-// Tiles of 256 x 256 (8 waves, one workgroup a CU), 128 x 128 and 64 x 64 (4 waves, two and three
-// workgroups a CU), and parts of the reduction where the tiles leave CUs idle: the choice of
-// least estimated time.  A CU runs its workgroups in rounds; a stage of a round costs what was
+// Tiles of 256 x 256 and 256 x 192 (8 waves, one workgroup a CU), 128 x 128 and 64 x 64 (4 waves,
+// two and three workgroups a CU), and parts of the reduction where the tiles leave CUs idle: the
+// choice of least estimated time.  A CU runs its workgroups in rounds; every XCD has an eighth of
+// the tiles, rounded up, and all their parts (33 tiles in 7 parts are 35 workgroups on 32 CUs, two
+// rounds: 100 us where 128 x 128 takes 60).  A stage of a round costs what was
 // measured on long reductions (8192 x 8192, k = 2048: 1080, 850 and 480 TFLOP/s, that is 1.8 to
-// 2.0, 1.2 and 0.9 us with 1, 2 and 3 workgroups), a round 3 us more to fill and finish, and a split
-// 3 us and its sums' way to memory and back.  At 16384 x 2048, k = 768 that gives 256 x 256 (56 us
-// against 64 with 128 x 128), at 10007 x 768, k = 2048 128 x 128 (37 against 54), at 2048 x 768,
-// k = 16384 128 x 128 in 5 parts (62 against 68 for 256 x 256 in 10, 153 unsplit).
+// 2.0, 1.2 and 0.9 us with 1, 2 and 3 workgroups; 256 x 192 has 1.7), a round 3 us more to fill
+// and finish, and a split 3 us and its sums' way to memory and back.  At 16384 x 2048, k = 768
+// that gives 256 x 256 (56 us against 64 with 128 x 128), at 16384 x 768, k = 2048 256 x 192 (its
+// 256 tiles 57 us, 192 of 256 x 256 63), at 10007 x 768, k = 2048 128 x 128 (37 against 54 for
+// 256 x 256), at 2048 x 768, k = 16384 128 x 128 in 5 parts (67 with the join, 256 x 192 in 8 72).
 GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int cus) {
-  static constexpr struct { int tile, wgs; double stage; } kTiles[] = {{256, 1, 1.8}, {128, 2, 1.2}, {64, 3, 0.9}};
+  static constexpr struct { int m, n, wgs; double stage; } kTiles[] = {
+      {256, 256, 1, 1.8}, {256, 192, 1, 1.7}, {128, 128, 2, 1.2}, {64, 64, 3, 0.9}};
   const int64_t stages = (k + kDepth - 1) / kDepth;
   GemmPlan best = {};
   double least = 1e30;
   for (const auto& t : kTiles) {
-    const int64_t tiles = ((m + t.tile - 1) / t.tile) * ((n + t.tile - 1) / t.tile);
+    const int64_t tiles = ((m + t.m - 1) / t.m) * ((n + t.n - 1) / t.n);
     for (int64_t splits = 1; splits <= 16 && (splits == 1 || splits * 8 <= stages); ++splits) {
-      const int64_t wgs = tiles * splits, full = wgs / (t.wgs * (int64_t)cus);
+      const int64_t wgs = (tiles + 7) / 8 * 8 * splits, full = wgs / (t.wgs * (int64_t)cus);
       // a last round of few workgroups has more of a CU for each, but not below a stage's latency
       const int64_t rest = (wgs - full * t.wgs * cus + cus - 1) / cus;
       const double per = full * t.stage + (rest > 0 ? std::max(rest * t.stage / t.wgs, 0.5) : 0.0);
@@ -536,7 +540,7 @@ GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int cus) {
       if (splits > 1) us += 3.0 + 2.0 * splits * m * n * 4 / 4e6;
       if (us < least) {
         least = us;
-        best.tile = t.tile, best.splits = (int)splits;
+        best.tile = t.m, best.tile_n = t.n, best.splits = (int)splits;
         best.ws_bytes = splits > 1 ? splits * m * n * 4 : 0;
       }
     }

@@ -93,7 +93,10 @@ def test_layer_norm_empty_and_odd_values(eng):
 
 LINEAR = [(1, 8, 8, None, F16), (23, 384, 1536, "gelu", F16), (64, 64, 64, "relu", BF16), (65, 72, 136, "tanh", F16),
           (300, 768, 104, "gelu", BF16), (129, 200, 520, None, F16), (1000, 384, 384, "gelu", F16), (7, 2048, 768, None, BF16),
-          (2049, 264, 1000, "gelu", BF16), (4100, 128, 1032, None, F16), (4500, 640, 1160, "relu", BF16)]
+          (2049, 264, 1000, "gelu", BF16), (4100, 128, 1032, None, F16), (4500, 640, 1160, "relu", BF16),
+          # sizes whose products take the larger tiles, whole and in parts
+          (6478, 64, 1752, "gelu", BF16), (5956, 1976, 64, "tanh", F16), (404, 3728, 3240, None, BF16), (8303, 2440, 392, "gelu", F16),
+          (8486, 64, 912, "tanh", F16), (6669, 1192, 64, "gelu", BF16), (416, 2328, 3408, "relu", F16), (6171, 520, 3296, None, F16)]
 
 
 @pytest.mark.parametrize("m,k,n,act,dtype", LINEAR)
