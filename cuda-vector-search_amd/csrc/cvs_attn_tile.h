@@ -34,7 +34,7 @@ struct TileLoad {
       } else if constexpr (DP == 64) {
         row[i] = line, piece = slot ^ piece_swizzle(line);
       } else {
-        row[i] = line >> 1, piece = ((line & 1) * 8 + slot) ^ piece_swizzle(line >> 1);
+        row[i] = line >> 1, piece = ((line & 1) * 8 + slot) ^ wide_swizzle(line >> 1);
       }
       at[i] = piece * 8 < d ? (uint32_t)(row[i] * (int)stride_bytes + piece * 16) : kOutside;
     }

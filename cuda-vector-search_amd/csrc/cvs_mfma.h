@@ -7,10 +7,11 @@
 // following product of depth 16 takes from that lane, and 16 contiguous bytes for
 // a store.
 //
-// LDS tiles are lines of 128 bytes in 16-byte pieces; slot s of line r holds piece
-// s ^ piece_swizzle(r).  Both ways of reading a tile are then free of bank
-// conflicts: the same piece of 8 consecutive lines (rows as operand rows), and two
-// neighbouring pieces of 4 consecutive lines (transposing reads, rows as depth).
+// LDS tiles are lines of 128 bytes in 16-byte pieces, slot s of line r holding piece
+// s ^ piece_swizzle(r).  LDS serves 256 bytes a cycle, from two neighbouring lines' slots.
+// Both ways of reading a tile take each of the 16 once: the same piece of 16 consecutive
+// rows (operand rows; 16 lanes a cycle), and four neighbouring pieces of 4 consecutive rows
+// (transposing reads, rows as depth; 32 lanes of 8 bytes a cycle).
 #pragma once
 
 #include "cvs_common.h"
@@ -40,11 +41,11 @@ struct Frag<__bf16> {
   }
 };
 
-__device__ __forceinline__ constexpr int piece_swizzle(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
-
-// Lines that hold two rows of 64 bytes: the same piece of 8 consecutive rows, and two
-// neighbouring pieces of 4 consecutive rows, lie on distinct banks.
-__device__ __forceinline__ constexpr int pair_swizzle(int line) { return ((line & 1) << 1) | ((line >> 1) & 1); }
+__device__ __forceinline__ constexpr int piece_swizzle(int r) { return (((r >> 1) & 1) << 2) | ((r >> 2) & 3); }
+// Rows of 256 bytes, two lines: of 16 pieces.
+__device__ __forceinline__ constexpr int wide_swizzle(int r) { return ((r & 3) << 2) | ((r >> 2) & 3); }
+// Lines that hold two rows of 64 bytes.
+__device__ __forceinline__ constexpr int pair_swizzle(int line) { return (line >> 1) & 3; }
 
 // Byte offset of a row's 16-byte piece in a tile of rows of WIDTH 16-bit columns (32, 64 or 128).
 template <int WIDTH>
@@ -52,8 +53,10 @@ __device__ __forceinline__ int row_offset(int row, int piece) {
   if constexpr (WIDTH == 32) {
     const int line = row >> 1;
     return line * 128 + ((((row & 1) * 4 + piece) ^ pair_swizzle(line)) << 4);
+  } else if constexpr (WIDTH == 64) {
+    return row * 128 + ((piece ^ piece_swizzle(row)) << 4);
   } else {
-    return row * (2 * WIDTH) + ((piece ^ piece_swizzle(row)) << 4);
+    return row * 256 + ((piece ^ wide_swizzle(row)) << 4);
   }
 }
 
