@@ -334,10 +334,10 @@ __device__ __forceinline__ void add_table(const AttnArgs& a, int at) {
 
 // dk and dv of 128 keys (wave w: 32 of them as columns), over a part of the queries that see
 // them.  Where there is a bias, the workgroups from `key_wgs` on add up its table's gradient.
-// The keys' rows of both operands and both sums stay in registers (at width 128 some 420 of them, one
-// workgroup a CU); the queries' tiles are read from LDS twice, as rows and transposed, which takes
-// LDS about as long as the matrix cores take for the four products.  2 x 4096, 16 heads on 4 of
-// 128, causal: 382 us, 0.72 PFLOP/s of its products; 64 x 512, 12 heads of 64: 165 us, with a bias 180 to 190.
+// The keys' rows of both operands and both sums stay in registers, at width 128 some 420 of them:
+// one wave a SIMD then, whose products (36% of the time), exponentials and packing follow one
+// another.  2 x 4096, 16 heads on 4 of 128, causal: 382 us, 0.72 PFLOP/s of its four products;
+// 64 x 512, 12 heads of 64, two workgroups a CU: 165 us, with a bias 180 to 190.
 template <class T, int DP, bool BIAS>
 __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kernel(AttnArgs a, int key_wgs) {
   typedef typename Frag<T>::V V;
