@@ -295,10 +295,8 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& a, int id, unsigned ch
         read(buf, 2 * half, fm[0], fn[0]);
         read(buf, 2 * half + 1, fm[1], fn[1]);
         phase_end(half == 1 && late);
-        __builtin_amdgcn_s_setprio(1);
         multiply(fm[0], fn[0]);
         multiply(fm[1], fn[1]);
-        __builtin_amdgcn_s_setprio(0);
         phase_end(half == 1 && !late);
       }
       buf ^= 1;
