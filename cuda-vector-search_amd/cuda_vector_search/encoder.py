@@ -13,15 +13,18 @@ These three are differentiable.  ``*_forward`` and ``*_backward`` are the passes
 themselves, for programs that keep the saved tensors on their own.  Tensors are float16
 or bfloat16 (``layer_norm``: float32 too), all of one type; results have it too, with
 fp32 sums inside.  A refused argument raises ``RuntimeError`` with the reason; there
-is no torch fallback.
+is no torch fallback.  Forward-mode derivatives and proxy tracing are refused too;
+``torch.jit.trace`` records the three as Python calls.
 """
 
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _ext
@@ -37,6 +40,43 @@ _plans: dict = {}  # workspace bytes by operator and sizes (a pure function of t
 def _check(rc: int) -> None:
     if rc != 0:
         raise _ext.load()._error(rc)
+
+
+def _library():
+    """The library, to be written with through pointers: not while torch's proxies record, which
+    would see only the allocations (and replay those: results of memory nobody wrote)."""
+    if torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise RuntimeError("encoder operators cannot be traced by proxies")
+    return _ext.load().lib
+
+
+def _has_tangent(*values) -> bool:
+    return forward_ad._current_level >= 0 and any(
+        isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in values)
+
+
+def _bare(passes):
+    """A pass of its own, which no autograd function announces to torch: refused where a trace
+    records or a tensor carries a tangent.  ``.inner`` is the pass itself."""
+
+    @functools.wraps(passes)
+    def call(*args, **kwargs):
+        if torch._C._get_tracing_state() is not None:
+            raise RuntimeError(f"{passes.__name__} cannot be traced; {passes.__name__.rsplit('_', 1)[0]} can")
+        if _has_tangent(*args, *kwargs.values()):
+            raise RuntimeError(f"{passes.__name__} has no forward-mode derivative")
+        return passes(*args, **kwargs)
+
+    call.inner = passes
+    return call
+
+
+def _through_autograd(*tensors) -> bool:
+    """Whether torch has to see the call: to differentiate it, backwards or (which it refuses)
+    forwards, or to record it in a trace."""
+    if torch._C._get_tracing_state() is not None or _has_tangent(*tensors):
+        return True
+    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
 
 
 def _tensor(t, name: str, like=None, shape=None) -> None:
@@ -118,12 +158,13 @@ def _norm_args(x, weight, bias):
     return width
 
 
+@_bare
 def layer_norm_forward(x, weight, bias=None, eps: float = 1e-5, stats: bool = True):
     """(y, mean, rstd) of the rows of ``x`` [..., width]: y = (x - mean) rstd weight + bias
     with rstd = 1 / sqrt(variance + eps).  mean and rstd are float32 [...] for the
     backward pass, None without ``stats``."""
     width = _norm_args(x, weight, bias)
-    lib = _ext.load().lib
+    lib = _library()
     r = _rows(x, width, False)
     y = _new(x)
     mean = rstd = None
@@ -139,11 +180,12 @@ def layer_norm_forward(x, weight, bias=None, eps: float = 1e-5, stats: bool = Tr
     return y, mean, rstd
 
 
+@_bare
 def layer_norm_backward(dy, x, weight, mean, rstd):
     """(dx, dweight, dbias) of ``layer_norm_forward`` for ``dy``, of x's shape."""
     width = _norm_args(x, weight, None)
     _tensor(dy, "dy", x, x.shape)
-    lib = _ext.load().lib
+    lib = _library()
     r, g = _rows(x, width, False), _rows(dy, width, False)
     n = r.shape[0]
     mean, rstd = _stats(mean, "mean", x, x.shape[:-1]), _stats(rstd, "rstd", x, x.shape[:-1])
@@ -165,7 +207,7 @@ def layer_norm_backward(dy, x, weight, mean, rstd):
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = layer_norm_forward(x, weight, bias, eps)
+        y, mean, rstd = layer_norm_forward.inner(x, weight, bias, eps)
         ctx.save_for_backward(x, weight, mean, rstd)
         ctx.biased = bias is not None
         return y
@@ -173,19 +215,15 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        dx, dweight, dbias = layer_norm_backward(dy, *ctx.saved_tensors)
+        dx, dweight, dbias = layer_norm_backward.inner(dy, *ctx.saved_tensors)
         return dx, dweight, dbias if ctx.biased else None, None
-
-
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
 
 
 def layer_norm(x, weight, bias=None, eps: float = 1e-5):
     """Layer norm over the last dimension of ``x``; ``weight`` and ``bias`` are [width]."""
-    if _wants_grad(x, weight, bias):
+    if _through_autograd(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, eps)
-    return layer_norm_forward(x, weight, bias, eps, stats=False)[0]
+    return layer_norm_forward.inner(x, weight, bias, eps, stats=False)[0]
 
 
 # ---- matrix product with its epilogue ----------------------------------------------
@@ -208,6 +246,7 @@ def _linear_args(x, weight, activation):
     return n, k
 
 
+@_bare
 def linear_forward(x, weight, bias=None, activation=None, residual=None, keep_pre: bool = False):
     """(y, pre): y = activation(x weight^T + bias) + residual for ``x`` [..., k] and ``weight``
     [n, k].  ``activation``: None, "gelu" (by the error function), "relu" or "tanh".
@@ -218,7 +257,7 @@ def linear_forward(x, weight, bias=None, activation=None, residual=None, keep_pr
         _tensor(bias, "bias", x, (n,))
     if residual is not None:
         _tensor(residual, "residual", x, shape)
-    lib = _ext.load().lib
+    lib = _library()
     r = _rows(x, k, True)
     m = r.shape[0]
     y = x.new_empty(shape)
@@ -236,6 +275,7 @@ def linear_forward(x, weight, bias=None, activation=None, residual=None, keep_pr
     return y, pre
 
 
+@_bare
 def linear_backward(dy, x, weight, activation=None, pre=None, needs=(True, True, True)):
     """(dx, dweight, dbias) of ``linear_forward`` for ``dy``; the residual's gradient is ``dy``
     itself.  ``pre`` is what the forward pass kept (not needed without an
@@ -250,7 +290,7 @@ def linear_backward(dy, x, weight, activation=None, pre=None, needs=(True, True,
         pre = _packed(pre)
     else:
         pre = None
-    lib = _ext.load().lib
+    lib = _library()
     r, g = _rows(x, k, True), _rows(dy, n, True)
     m = r.shape[0]
     dx = _new(x) if needs[0] else None
@@ -272,7 +312,7 @@ def linear_backward(dy, x, weight, activation=None, pre=None, needs=(True, True,
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, activation, residual):
-        y, pre = linear_forward(x, weight, bias, activation, residual, keep_pre=activation is not None)
+        y, pre = linear_forward.inner(x, weight, bias, activation, residual, keep_pre=activation is not None)
         ctx.save_for_backward(x, weight, pre)
         ctx.activation = activation
         return y
@@ -281,16 +321,16 @@ class _Linear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, weight, pre = ctx.saved_tensors
-        dx, dweight, dbias = linear_backward(dy, x, weight, ctx.activation, pre, ctx.needs_input_grad[:3])
+        dx, dweight, dbias = linear_backward.inner(dy, x, weight, ctx.activation, pre, ctx.needs_input_grad[:3])
         return dx, dweight, dbias, None, dy if ctx.needs_input_grad[4] else None
 
 
 def linear(x, weight, bias=None, activation=None, residual=None):
     """activation(x weight^T + bias) + residual; ``x`` [..., k], ``weight`` [n, k], feature
     counts multiples of 8."""
-    if _wants_grad(x, weight, bias, residual):
+    if _through_autograd(x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, activation, residual)
-    return linear_forward(x, weight, bias, activation, residual)[0]
+    return linear_forward.inner(x, weight, bias, activation, residual)[0]
 
 
 # ---- attention -----------------------------------------------------------------------
@@ -400,6 +440,7 @@ def _attention_workspace(lib, a, call, backward: bool, q):
     return q.new_empty(size, dtype=torch.uint8) if size else None
 
 
+@_bare
 def attention_forward(q, k, v, bias_table=None, key_lengths=None, query_lengths=None, query_start=None,
                       causal: bool = False, scale=None, max_distance: int = 128, lse: bool = True):
     """(out, lse) of softmax attention: ``q`` [batch, q_len, heads, width], ``k`` and ``v``
@@ -418,7 +459,7 @@ def attention_forward(q, k, v, bias_table=None, key_lengths=None, query_lengths=
     buckets for the past, else the first half for keys at or before the row.
     """
     a, call, hold = _attention_args(q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance)
-    lib = _ext.load().lib
+    lib = _library()
     out = _new(q)
     sums = q.new_empty((a.batch, a.heads, a.q_len), dtype=torch.float32) if lse else None
     dev = q.device.index
@@ -428,6 +469,7 @@ def attention_forward(q, k, v, bias_table=None, key_lengths=None, query_lengths=
     return out, sums
 
 
+@_bare
 def attention_backward(dout, q, k, v, out, lse, bias_table=None, key_lengths=None, query_lengths=None, query_start=None,
                        causal: bool = False, scale=None, max_distance: int = 128):
     """(dq, dk, dv, dbias_table) of ``attention_forward`` for ``dout``, from its ``out`` and ``lse``;
@@ -436,7 +478,7 @@ def attention_backward(dout, q, k, v, out, lse, bias_table=None, key_lengths=Non
     _tensor(dout, "dout", q, q.shape)
     _tensor(out, "out", q, q.shape)
     lse = _stats(lse, "lse", q, (a.batch, a.heads, a.q_len))
-    lib = _ext.load().lib
+    lib = _library()
     dout, dout_stride = _strided(dout)
     out = _packed(out)
     dq, dk, dv = _new(q), _new(k), _new(v)
@@ -454,7 +496,7 @@ def attention_backward(dout, q, k, v, out, lse, bias_table=None, key_lengths=Non
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance):
-        out, lse = attention_forward(q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance)
+        out, lse = attention_forward.inner(q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance)
         ctx.save_for_backward(q, k, v, out, lse, bias_table, key_lengths, query_lengths, query_start)
         ctx.more = (causal, scale, max_distance)
         return out
@@ -463,13 +505,13 @@ class _Attention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, *masks = ctx.saved_tensors
-        return (*attention_backward(dout, q, k, v, out, lse, *masks, *ctx.more), None, None, None, None, None, None)
+        return (*attention_backward.inner(dout, q, k, v, out, lse, *masks, *ctx.more), None, None, None, None, None, None)
 
 
 def attention(q, k, v, bias_table=None, key_lengths=None, query_lengths=None, query_start=None, causal: bool = False,
               scale=None, max_distance: int = 128):
     """Softmax attention, [batch, q_len, heads, width]; arguments as ``attention_forward``'s."""
     args = (q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance)
-    if _wants_grad(q, k, v, bias_table):
+    if _through_autograd(q, k, v, bias_table):
         return _Attention.apply(*args)
-    return attention_forward(*args, lse=False)[0]
+    return attention_forward.inner(*args, lse=False)[0]
