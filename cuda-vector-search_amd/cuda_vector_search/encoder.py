@@ -22,6 +22,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import operator
 
 import torch
 from torch.autograd import forward_ad
@@ -389,6 +390,10 @@ def _attention_check(q, k, v, bias_table, scale) -> None:
 
 def _attention_args(q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance):
     """(AttentionArgs, its _AttentionCall or None, tensors it points into) after the checks."""
+    # values, not tensors that hold them: those are found by identity and may have changed since
+    scale = None if scale is None else float(scale)
+    causal = bool(causal)
+    max_distance = 0 if bias_table is None else operator.index(max_distance)
     try:
         key = (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype, q.device, k.device,
                v.device, causal, scale, max_distance,
@@ -406,7 +411,7 @@ def _attention_args(q, k, v, bias_table, key_lengths, query_lengths, query_start
         k, a.k_stride = _strided(k)
         v, a.v_stride = _strided(v)
         a.scale = 1.0 / math.sqrt(a.width) if scale is None else scale
-        a.type, a.causal = TYPES[q.dtype], bool(causal)
+        a.type, a.causal = TYPES[q.dtype], causal
         a.buckets, a.max_distance = (0, 0) if bias_table is None else (bias_table.shape[0], max_distance)
         call = None
         if key is not None and q is given[0] and k is given[1] and v is given[2]:
