@@ -9,7 +9,10 @@
 // by transposing reads.  Probabilities are rounded to the inputs' type (as the matrix
 // cores take them); scores, maxima, sums and the output's sum are fp32.
 //
-// A row that sees no key gets zeros, and -inf as its log sum.
+// A row that sees no key gets zeros, and -inf as its log sum.  Keys past the last one that a
+// workgroup's rows see are not read (a cache's places not yet written); a value that is not
+// finite, of a key that a later row of the same workgroup sees, does reach the earlier rows,
+// as 0 times it.
 #include <algorithm>
 
 #include "cvs_attn_tile.h"
@@ -61,8 +64,8 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 3) void attn_forward_kernel(A
   if (BIAS) bias.buckets(a);
   const TileLoad<DP, kKeys> lk(2 * a.ks[1], a.d), lv(2 * a.vs[1], a.d);
   auto load = [&](int t) {
-    lk.load(kbase, 2 * a.ks[1], t * kKeys, nk, sk[t & 1]);
-    lv.load(vbase, 2 * a.vs[1], t * kKeys, nk, sv[t & 1]);
+    lk.load(kbase, 2 * a.ks[1], t * kKeys, end, sk[t & 1]);
+    lv.load(vbase, 2 * a.vs[1], t * kKeys, end, sv[t & 1]);
   };
   if (t0 < t1) load(t0);
   V qf[KS];
@@ -188,6 +191,10 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 3) void attn_forward_kernel(A
     store_part_row<DP>(a.part_out + (blockIdx.y * rows + at) * a.d, acc, a.d);
     return;
   }
+  if (sum == 0.f) {  // (the sums may be NaN: 0 times a value that other rows see)
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[d] = zero16();
+  }
   if (a.lse != nullptr && g == 0) a.lse[at] = sum == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(sum)) * kLn2;
   store_head_row<T, DP>((T*)a.out + ((int64_t)(b * (int64_t)a.lq + i) * a.heads + h) * a.d, acc,
                         sum == 0.f ? 0.f : 1.f / sum, a.d);
@@ -233,8 +240,8 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_rows_kernel(Attn
   if (BIAS) bias.buckets(a);
   const TileLoad<DP, 32, 1> lk(2 * a.ks[1], a.d), lv(2 * a.vs[1], a.d);
   auto load = [&](int t, int buf) {
-    lk.load(kbase, 2 * a.ks[1], t * 32, nk, smem[wave][buf][0]);
-    lv.load(vbase, 2 * a.vs[1], t * 32, nk, smem[wave][buf][1]);
+    lk.load(kbase, 2 * a.ks[1], t * 32, end, smem[wave][buf][0]);
+    lv.load(vbase, 2 * a.vs[1], t * 32, end, smem[wave][buf][1]);
   };
   int t = t0 + wave, buf = 0;
   if (t < t1) load(t, 0);
@@ -375,7 +382,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_rows_kernel(Attn
       const float inv = cs == 0.f ? 0.f : 1.f / cs;
       V v;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = (T)(z[e] * inv);
+      for (int e = 0; e < 8; ++e) v[e] = (T)(cs == 0.f ? 0.f : z[e] * inv);
       *reinterpret_cast<V*>((T*)a.out + (((int64_t)b * a.lq + ci) * a.heads + ch) * a.d + c8) = v;
       if (c8 == 0 && a.lse != nullptr) a.lse[at] = cs == 0.f ? -__builtin_inff() : (ct * c + __builtin_amdgcn_logf(cs)) * kLn2;
     }
@@ -396,6 +403,7 @@ __global__ __launch_bounds__(kBlock) void attn_join_kernel(AttnArgs a) {
   const int c = 2 * lane;
   for (int s = 0; s < a.splits; ++s) {
     const float* ml = a.part_ml + 2 * (s * rows + at);
+    if (ml[1] == 0.f) continue;  // nothing seen there, and its sums may be NaN
     const float f = __builtin_amdgcn_exp2f(ml[0] - base);
     sum = fmaf(f, ml[1], sum);
     if (c < a.d) {

@@ -14,6 +14,8 @@
 // the bias, dout . v from -delta.  Probabilities and ds are rounded to the inputs' type for
 // those products; everything else is fp32.
 //
+// Rows that see nothing, and keys that no row sees, are not read, and have no gradient.
+//
 // Rows that see at most one tile of keys take delta from the probabilities themselves,
 // normalised again: where few keys leave ds small beside its terms, the rounding of
 // out would be most of it.
@@ -102,22 +104,23 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
   if (BIAS) bias.buckets(a);
   const TileLoad<DP, ROWS> lk(2 * a.ks[1], a.d), lv(2 * a.vs[1], a.d);
   auto load = [&](int t) {
-    lk.load(kbase, 2 * a.ks[1], t * ROWS, nk, sk[t & 1]);
-    lv.load(vbase, 2 * a.vs[1], t * ROWS, nk, sv[t & 1]);
+    lk.load(kbase, 2 * a.ks[1], t * ROWS, end, sk[t & 1]);
+    lv.load(vbase, 2 * a.vs[1], t * ROWS, end, sv[t & 1]);
   };
   if (t0 < tiles) load(t0);
 
   // the first loads are all on their way before one is waited for: the keys' and values' tiles,
   // the bias, the rows, and under them shared memory is cleared
   V qf[KS], gf[KS], of[KS];
+  const bool in = i >= first_row(a, off) && i < nq;
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
-    qf[s] = global_frag<T>(qrow, s, a.d, i < nq);
-    gf[s] = global_frag<T>(grow, s, a.d, i < nq);
-    of[s] = global_frag<T>(orow, s, a.d, i < nq);
+    qf[s] = global_frag<T>(qrow, s, a.d, in);
+    gf[s] = global_frag<T>(grow, s, a.d, in);
+    of[s] = global_frag<T>(orow, s, a.d, in);
   }
   const int64_t row_at = (int64_t)bh * a.lq + i;
-  float lse = i < nq ? a.lse[row_at] * kLog2e : kNever;
+  float lse = in ? a.lse[row_at] * kLog2e : kNever;
   if (BIAS) bias.values(a, h);
   const int reach = a.far + kReach, places = 2 * reach + 1;
   float* sums = tab + places + wave * places + reach;  // by position, this wave's
@@ -133,7 +136,8 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
 #pragma unroll
     for (int j = 0; j < 8; ++j) delta = fmaf((float)gf[s][j], (float)of[s][j], delta);
   delta = one ? 0.f : halves_sum(delta);
-  if (lse == -__builtin_inff()) lse = kNever;  // a row that sees nothing
+  const bool blind = !in || lse == -__builtin_inff();  // a row that sees nothing
+  if (blind) lse = kNever;
 
   f32x16 dq[DB];
 #pragma unroll
@@ -277,6 +281,11 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
     tile_barrier();
     if (t + 1 < tiles) load(t + 1);
   }
+  if (blind) {  // (the sums may be NaN: 0 times a value that other rows see)
+    delta = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) dq[d] = zero16();
+  }
   if (i < a.lq) {
     const int64_t at = (((int64_t)b * a.lq + i) * a.heads + h) * a.d;
     if (a.q_parts > 1)
@@ -362,11 +371,12 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
   const int j = j0 + l32;
   const unsigned char* krow = (const unsigned char*)a.k + 2 * (b * a.ks[0] + j * a.ks[1] + hk * a.ks[2]);
   const unsigned char* vrow = (const unsigned char*)a.v + 2 * (b * a.vs[0] + j * a.vs[1] + hk * a.vs[2]);
+  const int row0 = min(first_row(a, off), nq), seen_keys = seen_count(a, nk, nq, off);
   V kf[KS], vf[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
-    kf[s] = global_frag<T>(krow, s, a.d, j < nk);
-    vf[s] = global_frag<T>(vrow, s, a.d, j < nk);
+    kf[s] = global_frag<T>(krow, s, a.d, j < seen_keys);
+    vf[s] = global_frag<T>(vrow, s, a.d, j < seen_keys);
   }
   f32x16 dk[DB], dv[DB];
 #pragma unroll
@@ -377,7 +387,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
 
   // tiles of queries that see a key of this workgroup, those of all heads in a row; this part's
   const int t0 = (a.causal ? max(block * kAttnRows - off, 0) : 0) / ROWS;
-  const int nt = block * kAttnRows < nk ? max((nq + ROWS - 1) / ROWS - t0, 0) : 0;
+  const int nt = block * kAttnRows < seen_keys ? max((nq + ROWS - 1) / ROWS - t0, 0) : 0;
   int f0 = 0, f1 = nt * group;
   if (a.kv_parts > 1) {
     const int64_t all = f1;
@@ -399,14 +409,14 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
     if (BIAS) bias.values(a, h);
     float stat = 0.f;  // threads 0 .. ROWS - 1: -log2 sum of a row, the next ROWS: -delta
     auto load = [&](int t) {
-      lq.load(qbase, 2 * a.qs[1], t * ROWS, nq, sq[t & 1]);
-      lg.load(gbase, 2 * a.dos[1], t * ROWS, nq, sg[t & 1]);
+      lq.load(qbase, 2 * a.qs[1], t * ROWS, nq, sq[t & 1], row0);
+      lg.load(gbase, 2 * a.dos[1], t * ROWS, nq, sg[t & 1], row0);
       const int i = t * ROWS + threadIdx.x % ROWS;
       if (threadIdx.x < ROWS) {
-        stat = i < nq ? -lse[i] * kLog2e : -kNever;
+        stat = i >= row0 && i < nq ? -lse[i] * kLog2e : -kNever;
         if (stat == __builtin_inff()) stat = -kNever;  // a row that sees nothing
       } else if (threadIdx.x < 2 * ROWS) {
-        stat = i < nq ? -delta[i] : 0.f;
+        stat = i >= row0 && i < nq ? -delta[i] : 0.f;
       }
     };
     auto turn = [&](int t) {
@@ -420,7 +430,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
     load(first);
     if (BIAS) bias.store(a, tab);
     // tiles that no key of this wave is seen from come first: it only loads its share of them
-    int mine = j0 < nk ? first : last;
+    int mine = j0 < seen_keys ? first : last;
     if (a.causal) mine = min(last, max(mine, (j0 - off) / ROWS));
     for (int t = first; t < mine; ++t) turn(t);
     for (int t = mine; t < last; ++t) {
@@ -498,7 +508,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
     }
   }
   if (j >= a.lk) return;
-  if (j >= nk) {
+  if (j >= seen_keys) {
 #pragma unroll
     for (int d = 0; d < DB; ++d) dk[d] = dv[d] = zero16();
   }

@@ -14,7 +14,8 @@ constexpr float kLn2 = 0.69314718055994530942f;
 
 // Loads of tiles of ROWS rows of a head straight into LDS, by the four waves of a workgroup
 // (WAVES = 1: by one, for itself): a lane's place in each 1 KiB load is the same in every
-// tile.  Rows from `rows` on and columns from `d` on become zeros.
+// tile.  Rows from `rows` on, rows before `low` and columns from `d` on become zeros: whatever lies
+// there (0 times a NaN is one) is not read.
 template <int DP, int ROWS, int WAVES = 4>
 struct TileLoad {
   static constexpr int N = ROWS * DP * 2 / 1024 / WAVES;
@@ -39,13 +40,13 @@ struct TileLoad {
       at[i] = piece * 8 < d ? (uint32_t)(row[i] * (int)stride_bytes + piece * 16) : kOutside;
     }
   }
-  // Rows first .. first + ROWS - 1 of the head at `base` (its row 0) to the tile at `lds`.
+  // Rows first .. first + ROWS - 1 of the head at `base` (its row 0) to the tile at `lds`; 0 <= low <= rows.
   __device__ __forceinline__ void load(const unsigned char* base, int64_t stride_bytes, int first, int rows,
-                                       const unsigned char* lds) const {
+                                       const unsigned char* lds, int low = 0) const {
     const uint32_t to = lds_address(lds) + (WAVES > 1 ? threadIdx.x >> 6 : 0) * 1024;
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      load_lds(first + row[i] < rows ? at[i] : kOutside, base + first * stride_bytes, to + i * (WAVES * 1024));
+      load_lds((unsigned)(first - low + row[i]) < (unsigned)(rows - low) ? at[i] : kOutside, base + first * stride_bytes, to + i * (WAVES * 1024));
   }
 };
 
@@ -169,6 +170,11 @@ __device__ __forceinline__ int query_count(const AttnArgs& a, int b) {
 }
 __device__ __forceinline__ int query_offset(const AttnArgs& a, int b) {
   return a.query_start == nullptr ? a.lk - a.lq : min(max(a.query_start[b], -(1 << 29)), 1 << 29);
+}
+// The first row that sees a key, were there any, and the end of the keys that some row sees.
+__device__ __forceinline__ int first_row(const AttnArgs& a, int off) { return a.causal ? max(-off, 0) : 0; }
+__device__ __forceinline__ int seen_count(const AttnArgs& a, int nk, int nq, int off) {
+  return a.causal ? min(nk, max(nq + off, 0)) : nk;
 }
 
 }  // namespace cvs
