@@ -43,17 +43,22 @@ def _check(rc: int) -> None:
         raise _ext.load()._error(rc)
 
 
+_tracing = torch._C._get_tracing_state
+_mode = torch._C._get_dispatch_mode
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
+
+
 def _library():
     """The library, to be written with through pointers: not while torch's proxies record, which
     would see only the allocations (and replay those: results of memory nobody wrote)."""
-    if torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+    if _mode(_PROXY) is not None:
         raise RuntimeError("encoder operators cannot be traced by proxies")
     return _ext.load().lib
 
 
-def _has_tangent(*values) -> bool:
-    return forward_ad._current_level >= 0 and any(
-        isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in values)
+def _has_tangent(values) -> bool:
+    """(Where forward_ad._current_level says that there may be any.)"""
+    return any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in values)
 
 
 def _bare(passes):
@@ -62,9 +67,9 @@ def _bare(passes):
 
     @functools.wraps(passes)
     def call(*args, **kwargs):
-        if torch._C._get_tracing_state() is not None:
+        if _tracing() is not None:
             raise RuntimeError(f"{passes.__name__} cannot be traced; {passes.__name__.rsplit('_', 1)[0]} can")
-        if _has_tangent(*args, *kwargs.values()):
+        if forward_ad._current_level >= 0 and _has_tangent((*args, *kwargs.values())):
             raise RuntimeError(f"{passes.__name__} has no forward-mode derivative")
         return passes(*args, **kwargs)
 
@@ -75,7 +80,7 @@ def _bare(passes):
 def _through_autograd(*tensors) -> bool:
     """Whether torch has to see the call: to differentiate it, backwards or (which it refuses)
     forwards, or to record it in a trace."""
-    if torch._C._get_tracing_state() is not None or _has_tangent(*tensors):
+    if _tracing() is not None or (forward_ad._current_level >= 0 and _has_tangent(tensors)):
         return True
     return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
 
