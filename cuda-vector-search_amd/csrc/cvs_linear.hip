@@ -73,8 +73,10 @@ __device__ __forceinline__ void times_slope8(float* dy, const float* z, int act)
   } else if (act == kActTanh) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float t = tanh16(z[e]);
-      dy[e] *= 1.f - t * t;
+      // 1 - tanh^2 = 4 x / (1 + x)^2 with x = exp(-2 |z|), which keeps its digits far out
+      const float x = __builtin_amdgcn_exp2f(fabsf(z[e]) * -2.8853900817779268f);
+      const float r = __builtin_amdgcn_rcpf(1.f + x);
+      dy[e] *= 4.f * x * r * r;
     }
   }
 }
