@@ -403,13 +403,13 @@ __global__ __launch_bounds__(kBlock) void attn_join_kernel(AttnArgs a) {
   const int c = 2 * lane;
   for (int s = 0; s < a.splits; ++s) {
     const float* ml = a.part_ml + 2 * (s * rows + at);
-    if (ml[1] == 0.f) continue;  // nothing seen there, and its sums may be NaN
+    const bool seen = ml[1] != 0.f;  // (where nothing was, the sums may be NaN; a select, so that the loads go together)
     const float f = __builtin_amdgcn_exp2f(ml[0] - base);
     sum = fmaf(f, ml[1], sum);
     if (c < a.d) {
       const float* o = a.part_out + (s * rows + at) * a.d + c;
-      o0 = fmaf(f, o[0], o0);
-      o1 = fmaf(f, o[1], o1);
+      o0 = fmaf(f, seen ? o[0] : 0.f, o0);
+      o1 = fmaf(f, seen ? o[1] : 0.f, o1);
     }
   }
   const int i = (int)(at % a.lq);
