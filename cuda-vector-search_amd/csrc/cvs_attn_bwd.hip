@@ -16,9 +16,10 @@
 //
 // Rows that see nothing, and keys that no row sees, are not read, and have no gradient.
 //
-// Rows that see at most one tile of keys take delta from the probabilities themselves,
-// normalised again: where few keys leave ds small beside its terms, the rounding of
-// out would be most of it.
+// Where all of a wave's rows see at most the first tile of keys (sequences of that many keys, the
+// first rows of causal ones) they take delta from the probabilities themselves, normalised
+// again: few keys leave ds small beside its terms, and the rounding of out would be most of
+// it.  (The rows after them take it from out, with that rounding.)
 #include <algorithm>
 
 #include "cvs_attn_tile.h"
@@ -91,15 +92,16 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
   int end = last_row < block * kAttnRows ? 0 : nk;
   if (a.causal) end = min(end, max(last_row + off + 1, 0));
   const int all = (end + ROWS - 1) / ROWS;
-  const bool one = nk <= ROWS;  // a row's keys are all in one tile
+  // this wave's rows see keys of the first tile only
+  const bool one = (a.causal ? min(nk, r0 + 32 + off) : nk) <= ROWS;
   // this workgroup's part of the tiles (fewer than 2^24, at most 64 parts); the first part writes
-  // delta, or the last one, which then has the one tile
+  // delta, or, where the wave's rows take it from the first tile, the part that has it
   int t0 = 0, tiles = all;
   if (a.q_parts > 1) {
     t0 = (int)((unsigned)all * blockIdx.y / (unsigned)a.q_parts);
     tiles = (int)((unsigned)all * (blockIdx.y + 1) / (unsigned)a.q_parts);
   }
-  const bool writes_delta = (int)blockIdx.y == (one ? a.q_parts - 1 : 0);
+  const bool writes_delta = one && all > 0 ? t0 == 0 && tiles > 0 : blockIdx.y == 0;
   BiasLoad<T> bias;
   if (BIAS) bias.buckets(a);
   const TileLoad<DP, ROWS> lk(2 * a.ks[1], a.d), lv(2 * a.vs[1], a.d);
@@ -383,7 +385,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
   for (int d = 0; d < DB; ++d) dk[d] = dv[d] = zero16();
   const float c = a.scale * kLog2e;
   const int reach = a.far + kReach;
-  const bool one = nk <= ROWS;  // delta is dout . v's own sum: subtracted as it stands
+  const bool one = nk <= ROWS;  // delta is made of dout . v's own sums: subtracted as they stand, so that one key leaves 0
 
   // tiles of queries that see a key of this workgroup, those of all heads in a row; this part's
   const int t0 = (a.causal ? max(block * kAttnRows - off, 0) : 0) / ROWS;
