@@ -30,6 +30,70 @@ namespace {
 
 constexpr float kNever = __builtin_inff();
 
+// float16 holds ds of long rows and small gradients only as subnormals (p of 1 / 3000 times
+// dout . v of 2^-12 has few digits left: dq off by 2%), so probabilities are taken times 2^10
+// there, by their exponent, and sums divided at the end: what a ds then loses is 2^-35 at
+// most, and 8192 of them, each against an operand of 1 and times a scale of 1/8, come to half the
+// spacing of the result's own subnormals.  A ds past 2^5 takes less than 2^10: the q kernel
+// lowers the exponent of a column (a query) when a tile brings one, and leaves each workgroup's
+// largest for the kv kernel, which takes one factor for a key head from those.  (The pass
+// of 32 sequences of up to 512, 12 heads of 64, bias, 112 us against 109 without any of this, causal
+// 2 x 4096, 16 heads on 4 of 128, 579 both; with a column's own exponent in the kv kernel too 606.)
+template <class T>
+constexpr int kLift = 0;
+template <>
+constexpr int kLift<_Float16> = 10;
+template <class T>
+constexpr float kUnlift = 1.f / (1 << kLift<T>);
+constexpr int kTop = 15;  // lifted values stay below 2^15, or the sums of a rounding more
+
+// The exponent that brings values of at most `top` below 2^kTop.
+__device__ __forceinline__ int room(float top) { return kTop - __builtin_amdgcn_frexp_expf(top); }
+
+__device__ __forceinline__ float largest(const f32x16& v, float top) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(v[e]));
+  return top;
+}
+template <int DB>
+__device__ __forceinline__ void times(f32x16* sums, float factor) {
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sums[d][e] *= factor;
+}
+// A column's state in the q kernel.
+struct Lifted {
+  float lift, unit = 1.f;  // its exponent; what a value times 2^kLift is of one times 2^lift
+  float peak = 0.f;        // its largest value so far, times 2^lift
+};
+
+// Lowers the exponents of columns whose values, of which this lane's largest is `top`, pass 2^kTop,
+// with these values and the sums so far.
+template <int DB, int N>
+__device__ __forceinline__ void fit_half(float top, Lifted& c, f32x16* sums, f32x16* ds) {
+  c.peak = fmaxf(c.peak, top);
+  if (__builtin_expect(__any(top > (float)(1 << kTop)), 0)) {
+    const int past = max(-room(halves_max(top)), 0);
+    const float change = ldexpf(1.f, -past);
+    c.lift -= past;
+    c.unit = ldexpf(c.unit, past);
+    c.peak *= change;
+    times<DB>(sums, change);
+    times<N>(ds, change);
+  }
+}
+// The wave's largest, in every lane: across its halves and quarters, then around each 16 lanes.
+__device__ __forceinline__ float wave_max(float v) {
+  v = halves_max(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x128, 0xf, 0xf, false)));
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x124, 0xf, 0xf, false)));
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x122, 0xf, 0xf, false)));
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x121, 0xf, 0xf, false)));
+}
+
 // Rows of a streamed tile: 64, or 32 of width 128 (two workgroups' tiles fit a CU's LDS).
 template <int DP>
 constexpr int kTile = DP > 64 ? 32 : 64;
@@ -70,6 +134,7 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
   constexpr int KS = DP / 16, DB = DP / 32, ROWS = kTile<DP>, KB = ROWS / 32, TILE = ROWS * DP * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char sk[2][TILE], sv[2][TILE];
   __shared__ __attribute__((aligned(16))) float skew[BIAS ? 4 : 1][BIAS ? kSkew : 4];
+  __shared__ float peaks[4];
   extern __shared__ float tab[];  // bias by position, then the waves' sums by position
 
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
@@ -145,6 +210,7 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
 #pragma unroll
   for (int d = 0; d < DB; ++d) dq[d] = zero16();
   const float c = a.scale * kLog2e;
+  Lifted col = {kLift<T>};  // of this column's probabilities and ds
 
   // the tiles that a row of this wave sees a key of; through the others it only loads its share
   int mine = r0 < nq ? tiles : t0;
@@ -164,7 +230,7 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       const int near = near0 + kb * 32;
-      base[kb] = -lse;
+      base[kb] = col.lift - lse;
       if (BIAS) {
         if (near - 31 >= a.far || near + 31 <= -a.far) {
           base[kb] += tab[near > 0 ? 2 * reach : 0] * c;
@@ -240,6 +306,7 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
         for (int e = 0; e < 16; ++e) {
           p[kb][e] = sp == 0.f ? 0.f : p[kb][e] / sp;
           spd = fmaf(p[kb][e], ds[kb][e], spd);
+          if (kLift<T> != 0) p[kb][e] *= __builtin_amdgcn_exp2f(col.lift);
         }
       delta = halves_sum(spd);
 #pragma unroll
@@ -247,19 +314,38 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
 #pragma unroll
         for (int e = 0; e < 16; ++e) ds[kb][e] -= delta;
     }
+    if constexpr (kLift<T> != 0) {
+      float top = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) ds[kb][e] *= p[kb][e];
+        top = largest(ds[kb], top);
+      }
+      fit_half<DB, KB>(top, col, dq, ds);
+    }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       const int near = near0 + kb * 32;
       const bool in_range = near + 31 > -a.far && near - 31 < a.far;
+      if constexpr (kLift<T> == 0) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) ds[kb][e] *= p[kb][e];
+        for (int e = 0; e < 16; ++e) ds[kb][e] *= p[kb][e];
+      }
       if (BIAS) {
         if (in_range) {
-          put_positions(skew[wave], ds[kb]);
+          if (kLift<T> == 0 || !__any(col.unit != 1.f)) {
+            put_positions(skew[wave], ds[kb]);
+          } else {
+            f32x16 alike = ds[kb];
+            times<1>(&alike, col.unit);
+            put_positions(skew[wave], alike);
+          }
         } else {
           float s = 0.f;
 #pragma unroll
           for (int e = 0; e < 16; ++e) s += ds[kb][e];
+          if (kLift<T> != 0) s *= col.unit;
           if (near < 0)
             before += s;
           else
@@ -290,11 +376,22 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
   }
   if (i < a.lq) {
     const int64_t at = (((int64_t)b * a.lq + i) * a.heads + h) * a.d;
-    if (a.q_parts > 1)
+    const float undo = kUnlift<T> * col.unit;
+    if (a.q_parts > 1) {
+      if (kLift<T> != 0) times<DB>(dq, undo);
       store_part_row<DP>(a.part_q + (int64_t)blockIdx.y * a.batch * a.lq * a.heads * a.d + at, dq, a.d);
-    else
-      store_head_row<T, DP>((T*)a.dq + at, dq, a.scale, a.d);
+    } else {
+      store_head_row<T, DP>((T*)a.dq + at, dq, a.scale * undo, a.d);
+    }
     if (g == 0 && writes_delta) a.delta[row_at] = delta;
+  }
+  if constexpr (kLift<T> != 0) {
+    const float top = wave_max(col.peak * col.unit * kUnlift<T>);
+    if (lane == 0) peaks[wave] = top;
+    __syncthreads();
+    const int blocks = (a.lq + kAttnRows - 1) / kAttnRows;
+    if (threadIdx.x == 0)
+      a.part_peak[((int64_t)bh * a.q_parts + blockIdx.y) * blocks + block] = fmaxf(fmaxf(peaks[0], peaks[1]), fmaxf(peaks[2], peaks[3]));
   }
   if (BIAS) {
 #pragma unroll
@@ -326,7 +423,7 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
     for (int o = lanes / 2; o > 0; o >>= 1) s += __shfl_xor(s, o);
     if (bucket < a.buckets && l == 0)
       a.part_table[((int64_t)h * a.table_parts + ((int64_t)b * a.q_parts + blockIdx.y) * ((a.lq + kAttnRows - 1) / kAttnRows) +
-                    block) * a.buckets + bucket] = s;
+                    block) * a.buckets + bucket] = s * kUnlift<T>;
   }
 }
 
@@ -354,7 +451,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
   typedef typename Frag<T>::V V;
   constexpr int KS = DP / 16, DB = DP / 32, ROWS = 64, QB = ROWS / 32, TILE = ROWS * DP * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char sq[2][TILE], sg[2][TILE];
-  __shared__ __attribute__((aligned(16))) float slse[2][ROWS], sdelta[2][ROWS];  // -log2 sums, -deltas
+  __shared__ __attribute__((aligned(16))) float slse[2][ROWS], sdelta[2][ROWS];  // kLift - log2 sums, -deltas
   extern __shared__ float tab[];
 
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
@@ -374,6 +471,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
   const unsigned char* krow = (const unsigned char*)a.k + 2 * (b * a.ks[0] + j * a.ks[1] + hk * a.ks[2]);
   const unsigned char* vrow = (const unsigned char*)a.v + 2 * (b * a.vs[0] + j * a.vs[1] + hk * a.vs[2]);
   const int row0 = min(first_row(a, off), nq), seen_keys = seen_count(a, nk, nq, off);
+  float shrink = 1.f;  // of this workgroup's ds, where they would not fit
   V kf[KS], vf[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
@@ -423,7 +521,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
     };
     auto turn = [&](int t) {
       if (threadIdx.x < ROWS)
-        slse[t & 1][threadIdx.x] = stat;
+        slse[t & 1][threadIdx.x] = stat + kLift<T>;
       else if (threadIdx.x < 2 * ROWS)
         sdelta[t & 1][threadIdx.x - ROWS] = stat;
       tile_barrier();
@@ -431,6 +529,14 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
     };
     load(first);
     if (BIAS) bias.store(a, tab);
+    if constexpr (kLift<T> != 0) {  // (under the first tile's loads)
+      const int64_t count = (int64_t)group * a.q_parts * ((a.lq + kAttnRows - 1) / kAttnRows);
+      const float* from = a.part_peak + bk * count;
+      float peak = 0.f;  // of the heads that share this one
+      for (int64_t t = lane; t < count; t += 64) peak = fmaxf(peak, from[t]);
+      const int past = __builtin_amdgcn_readfirstlane(kLift<T> - room(wave_max(peak)));
+      shrink = ldexpf(1.f, -max(past, 0));
+    }
     // tiles that no key of this wave is seen from come first: it only loads its share of them
     int mine = j0 < seen_keys ? first : last;
     if (a.causal) mine = min(last, max(mine, (j0 - off) / ROWS));
@@ -497,6 +603,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) ds[e] *= p[e];
+        if (kLift<T> != 0 && shrink != 1.f) times<1>(&ds, shrink);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const V pf = pack8<T>(p, s), df = pack8<T>(ds, s);
@@ -515,15 +622,17 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
     for (int d = 0; d < DB; ++d) dk[d] = dv[d] = zero16();
   }
   const int64_t at = (((int64_t)b * a.lk + j) * a.k_heads + hk) * a.d;
+  const float undo = kUnlift<T> / shrink;
   if (a.kv_parts > 1) {
+    if (kLift<T> != 0) times<DB>(dk, undo), times<DB>(dv, kUnlift<T>);
     const int64_t all = (int64_t)a.batch * a.lk * a.k_heads * a.d;
     float* to = a.part_kv + 2 * blockIdx.y * all + at;
     store_part_row<DP>(to, dk, a.d);
     store_part_row<DP>(to + all, dv, a.d);
     return;
   }
-  store_head_row<T, DP>((T*)a.dk + at, dk, a.scale, a.d);
-  store_head_row<T, DP>((T*)a.dv + at, dv, 1.f, a.d);
+  store_head_row<T, DP>((T*)a.dk + at, dk, a.scale * undo, a.d);
+  store_head_row<T, DP>((T*)a.dv + at, dv, kUnlift<T>, a.d);
 }
 
 // Adds `parts` of n values, `stride` apart, in order: 8 a thread; blockIdx.y: the second of two sums

@@ -125,6 +125,7 @@ struct AttnArgs {
   void *dq, *dk, *dv, *dtable;
   int q_parts;                    // parts of the keys that dq is summed over
   float* part_q;                  // [q_parts, batch, lq, heads, d] when q_parts > 1
+  float* part_peak;               // [batch, heads, q_parts, query blocks] largest |ds| (float16)
   float* part_table;              // [heads, batch * q_parts * query blocks, buckets]
   int table_parts;
   int kv_parts;                   // parts of the queries that dk and dv are summed over

@@ -160,7 +160,7 @@ AttnArgs attn_args(const cvs_attention* p) {
 
 struct AttnPlan {
   int splits = 1, table_parts = 0, kv_parts = 1, q_parts = 1;
-  int64_t part_kv = 0, part_q = 0, part_out = 0, part_ml = 0, delta = 0, part_table = 0, bytes = 0;
+  int64_t part_kv = 0, part_q = 0, part_out = 0, part_ml = 0, delta = 0, part_peak = 0, part_table = 0, bytes = 0;
 };
 
 AttnPlan plan_attention(const AttnArgs& a, bool backward, int cus) {
@@ -171,6 +171,8 @@ AttnPlan plan_attention(const AttnArgs& a, bool backward, int cus) {
     p.delta = at, at += up256(rows * 4);
     p.q_parts = rows == 0 ? 1 : attn_q_parts(a, cus);
     if (p.q_parts > 1) p.part_q = at, at += up256(p.q_parts * rows * a.d * 4);
+    if (a.type == CVS_TYPE_F16)
+      p.part_peak = at, at += up256((int64_t)a.batch * a.heads * p.q_parts * ((a.lq + kAttnRows - 1) / kAttnRows) * 4);
     if (a.table != nullptr) {
       p.table_parts = a.batch * p.q_parts * ((a.lq + kAttnRows - 1) / kAttnRows);
       p.part_table = at, at += up256((int64_t)a.heads * p.table_parts * a.buckets * 4);
@@ -405,6 +407,7 @@ int cvs_attention_backward(const cvs_attention* p, const void* dout, const int64
   for (int i = 0; i < 3; ++i) a.dos[i] = dout_stride[i];
   a.dq = dq, a.dk = dk, a.dv = dv, a.dtable = dbias_table;
   a.delta = reinterpret_cast<float*>(ws + plan.delta);
+  a.part_peak = reinterpret_cast<float*>(ws + plan.part_peak);
   a.part_table = reinterpret_cast<float*>(ws + plan.part_table);
   a.table_parts = plan.table_parts;
   a.kv_parts = plan.kv_parts, a.q_parts = plan.q_parts;
