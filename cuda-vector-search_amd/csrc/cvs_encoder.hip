@@ -51,12 +51,16 @@ int64_t norm_ws(int64_t n, int64_t d, int type, int cus) {
 // ---- matrix product ----------------------------------------------------------------
 
 int check_linear(int64_t m, int64_t k, int64_t n) {
-  if (m < 0 || m >= INT_MAX) return fail(CVS_ERR_INVALID, "too many rows");
+  if (m < 0 || m > INT_MAX - 255) return fail(CVS_ERR_INVALID, "too many rows");  // (rows of the last tile count on past m)
   if (k < 8 || n < 8 || k % 8 != 0 || n % 8 != 0)
     return fail(CVS_ERR_INVALID, "linear takes feature counts that are multiples of 8 (zero-pad them)");
   if (k > (1 << 20) || n > (1 << 20)) return fail(CVS_ERR_INVALID, "linear takes at most 2^20 features");
   if (m * std::max(k, n) > ((int64_t)1 << 36)) return fail(CVS_ERR_INVALID, "linear: more than 2^36 values in a matrix");
   return CVS_OK;
+}
+
+int check_plan(const GemmPlan& p) {
+  return p.splits > 0 ? CVS_OK : fail(CVS_ERR_INVALID, "linear: too many rows and features for a launch");
 }
 
 int check_linear_types(int act, int type) {
@@ -246,7 +250,9 @@ int cvs_linear_plan(int64_t m, int64_t k, int64_t n, int device, int64_t* worksp
   DevInfo di;
   int rc = dev_info(device, &di);
   if (rc == CVS_OK) rc = check_linear(m, k, n);
-  if (rc == CVS_OK) *workspace_bytes = m == 0 ? 0 : plan_gemm(m, n, k, di.cus).ws_bytes;
+  GemmPlan p = {};
+  if (rc == CVS_OK && m > 0) rc = check_plan(p = plan_gemm(m, n, k, di.cus));
+  if (rc == CVS_OK) *workspace_bytes = p.ws_bytes;
   return rc;
 }
 
@@ -265,7 +271,8 @@ int cvs_linear(const void* x, const void* w, const void* bias, const void* resid
   if (!aligned16(w) || !aligned16(bias) || !aligned16(y) || !aligned16(pre))
     return fail(CVS_ERR_INVALID, "linear: pointers must be 16-byte aligned");
   const GemmPlan p = plan_gemm(m, n, k, di.cus);
-  rc = check_workspace(workspace, workspace_bytes, p.ws_bytes);
+  rc = check_plan(p);
+  if (rc == CVS_OK) rc = check_workspace(workspace, workspace_bytes, p.ws_bytes);
   if (rc != CVS_OK) return rc;
   DeviceGuard guard(device);
   if (guard.err != hipSuccess) return hip_fail(guard.err, "hipSetDevice");
@@ -281,7 +288,13 @@ int cvs_linear_backward_plan(int64_t m, int64_t k, int64_t n, int act, int devic
   DevInfo di;
   int rc = dev_info(device, &di);
   if (rc == CVS_OK) rc = check_linear(m, k, n);
-  if (rc == CVS_OK) *workspace_bytes = m == 0 ? 0 : plan_linear_backward(m, k, n, act, di.cus).bytes;
+  LinearBackwardPlan p = {};
+  if (rc == CVS_OK && m > 0) {
+    p = plan_linear_backward(m, k, n, act, di.cus);
+    rc = check_plan(p.dx);
+    if (rc == CVS_OK) rc = check_plan(p.dw);
+  }
+  if (rc == CVS_OK) *workspace_bytes = p.bytes;
   return rc;
 }
 
@@ -301,7 +314,9 @@ int cvs_linear_backward(const void* dy, const void* x, const void* w, const void
   if (!aligned16(w) || !aligned16(pre) || !aligned16(dx) || !aligned16(dw) || !aligned16(dbias))
     return fail(CVS_ERR_INVALID, "linear: pointers must be 16-byte aligned");
   const LinearBackwardPlan p = plan_linear_backward(m, k, n, act, di.cus);
-  rc = check_workspace(workspace, workspace_bytes, p.bytes);
+  rc = check_plan(p.dx);
+  if (rc == CVS_OK) rc = check_plan(p.dw);
+  if (rc == CVS_OK) rc = check_workspace(workspace, workspace_bytes, p.bytes);
   if (rc != CVS_OK) return rc;
   DeviceGuard guard(device);
   if (guard.err != hipSuccess) return hip_fail(guard.err, "hipSetDevice");

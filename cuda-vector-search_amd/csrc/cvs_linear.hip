@@ -19,6 +19,7 @@ namespace cvs {
 namespace {
 
 constexpr int kDepth = 64;                    // reduction steps of a stage
+constexpr int64_t kLaunchThreads = (int64_t)1 << 32;
 // The normal distribution's Phi(z).  log2 Phi(-t), t >= 0, is nearly a parabola: a
 // polynomial of degree 7 in t, fitted on [0, 7] for least error where t Phi(-t) is visible, gives
 // Phi(-t) within 3.7e-6 of itself for t <= 3, 7e-5 for t <= 6, and below 1e-9, on its
@@ -523,9 +524,12 @@ __global__ __launch_bounds__(kBlock) void act_grad_kernel(ActGradArgs a) {
 // that gives 256 x 256 (56 us against 64 with 128 x 128), at 16384 x 768, k = 2048 256 x 192 (its
 // 256 tiles 57 us, 192 of 256 x 256 63), at 10007 x 768, k = 2048 128 x 128 (37 against 54 for
 // 256 x 256), at 2048 x 768, k = 16384 128 x 128 in 5 parts (67 with the join, 256 x 192 in 8 72).
+//
+// A launch has fewer than 2^32 threads: choices of more are passed over, and where that leaves none
+// (splits 0), there is no plan.
 GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int cus) {
-  static constexpr struct { int m, n, wgs; double stage; } kTiles[] = {
-      {256, 256, 1, 1.8}, {256, 192, 1, 1.7}, {128, 128, 2, 1.2}, {64, 64, 3, 0.9}};
+  static constexpr struct { int m, n, wgs, threads; double stage; } kTiles[] = {
+      {256, 256, 1, 512, 1.8}, {256, 192, 1, 512, 1.7}, {128, 128, 2, 256, 1.2}, {64, 64, 3, 256, 0.9}};
   const int64_t stages = (k + kDepth - 1) / kDepth;
   GemmPlan best = {};
   double least = 1e30;
@@ -533,6 +537,7 @@ GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int cus) {
     const int64_t tiles = ((m + t.m - 1) / t.m) * ((n + t.n - 1) / t.n);
     for (int64_t splits = 1; splits <= 16 && (splits == 1 || splits * 8 <= stages); ++splits) {
       const int64_t wgs = (tiles + 7) / 8 * 8 * splits, full = wgs / (t.wgs * (int64_t)cus);
+      if (wgs * t.threads >= kLaunchThreads || (splits > 1 && m * (n / 8) + kBlock > kLaunchThreads)) break;
       // a last round of few workgroups has more of a CU for each, but not below a stage's latency
       const int64_t rest = (wgs - full * t.wgs * cus + cus - 1) / cus;
       const double per = full * t.stage + (rest > 0 ? std::max(rest * t.stage / t.wgs, 0.5) : 0.0);
@@ -553,7 +558,8 @@ hipError_t launch_gemm(const GemmArgs& a, const GemmPlan& p, hipStream_t s) {
 }
 
 hipError_t launch_gemm_pair(const GemmArgs& a, const GemmPlan& pa, const GemmArgs& b, const GemmPlan& pb, hipStream_t s) {
-  if (pa.tile == pb.tile && pa.tile < 256)
+  const int64_t both = (int64_t)gemm_grid(a, pa.tile, pa.tile_n) + gemm_grid(b, pb.tile, pb.tile_n);
+  if (pa.tile == pb.tile && pa.tile < 256 && both * 256 < kLaunchThreads)
     return a.type == kF16 ? launch_typed_pair<_Float16>(a, b, pa, s) : launch_typed_pair<__bf16>(a, b, pa, s);
   const hipError_t e = launch_gemm(a, pa, s);
   return e == hipSuccess ? launch_gemm(b, pb, s) : e;

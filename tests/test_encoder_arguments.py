@@ -31,3 +31,36 @@ def test_a_scale_changed_in_place_counts(eng):
         for a, b in zip(encoder.attention_backward(v, q, k, v, out, lse, scale=scale, causal=causal)[:3],
                         encoder.attention_backward(v, q, k, v, out, lse, scale=s, causal=c)[:3]):
             assert torch.equal(a, b), f"gradient, scale {s}, causal {c}"
+
+
+def plan(name, *sizes):
+    """(status, workspace bytes) of a plan entry: no launch."""
+    out = ctypes.c_int64(-1)
+    rc = getattr(_ext.load().lib, name)(*sizes, 0, ctypes.byref(out))
+    return rc, out.value
+
+
+def test_linear_rows_that_no_launch_takes(eng):
+    """2^31 - 256 rows and more are refused before a tile's last row passes an int; so are
+    sizes whose tiles are 2^32 threads; the ones below have plans."""
+    for m in (2**31 - 2, 2**31 - 255, 2**31 - 257):  # (the last: 2^23 tiles of 512 threads)
+        assert plan("cvs_linear_plan", m, 8, 8)[0] != 0 and "rows" in str(_ext.load()._error(1))
+        assert plan("cvs_linear_backward_plan", m, 8, 8, 0)[0] != 0
+    for m in (2**31 - 2**12, 2**30 + 5, 2**24):
+        rc, size = plan("cvs_linear_plan", m, 8, 8)
+        assert rc == 0 and size == 0
+        assert plan("cvs_linear_backward_plan", m, 8, 8, 0)[0] == 0
+
+
+def test_linear_of_two_to_the_thirty_rows(eng):
+    """Offsets past 2^32 in either matrix: the last rows, and some before, against the same rows alone."""
+    m = 2**30 + 5
+    x = torch.randn(m, 8, device="cuda", dtype=F16)
+    w = half(8, 8)
+    y = encoder.linear(x, w)
+    dx = encoder.linear_backward(x, x, w, needs=(True, False, False))[0]
+    for at in (0, 2**29 - 70, 2**30 - 100, m - 333):
+        rows = x[at:at + 333].contiguous()
+        assert torch.equal(y[at:at + 333], encoder.linear(rows, w))
+        assert torch.equal(dx[at:at + 333], encoder.linear_backward(rows, rows, w, needs=(True, False, False))[0])
+        assert torch.allclose(y[at:at + 333].float(), rows.float() @ w.float().T, atol=2e-2, rtol=1e-2)
