@@ -112,7 +112,8 @@ int check_attention(const cvs_attention* p) {
   for (const int64_t len : {p->q_len, p->k_len})
     if ((len + kAttnRows - 1) / kAttnRows * p->batch * p->heads >= (1 << 23))  // (a launch has fewer than 2^32 threads)
       return fail(CVS_ERR_INVALID, "attention: too many rows");
-  if (!(p->scale > 0) || !std::isfinite((float)p->scale)) return fail(CVS_ERR_INVALID, "attention: scale must be positive and finite");
+  // (the kernels hold biases in units of unscaled scores, bias / scale)
+  if (!(p->scale >= 0x1p-100 && p->scale <= 0x1p100)) return fail(CVS_ERR_INVALID, "attention: scale must be positive, from 2^-100 to 2^100");
   if (p->bias_table != nullptr) {
     const int64_t one = p->causal ? p->buckets : p->buckets / 2;
     if (p->buckets < 4 || p->buckets > kMaxBuckets || p->buckets % 2 != 0)

@@ -337,7 +337,7 @@ typedef struct cvs_attention {
   int64_t batch, q_len, k_len, heads, k_heads, width;
   const void *q, *k, *v;
   int64_t q_stride[3], k_stride[3], v_stride[3];
-  double scale; /* positive */
+  double scale; /* 2^-100 to 2^100 */
   int type;     /* CVS_TYPE_F16 or CVS_TYPE_BF16 */
   int causal;
   const int32_t* key_lengths;   /* [batch] or NULL: k_len */

@@ -8,6 +8,7 @@ import math
 import pytest
 import torch
 
+import encoder_oracle as o
 from cuda_vector_search import _ext, encoder
 
 pytestmark = pytest.mark.gpu
@@ -64,3 +65,20 @@ def test_linear_of_two_to_the_thirty_rows(eng):
         assert torch.equal(y[at:at + 333], encoder.linear(rows, w))
         assert torch.equal(dx[at:at + 333], encoder.linear_backward(rows, rows, w, needs=(True, False, False))[0])
         assert torch.allclose(y[at:at + 333].float(), rows.float() @ w.float().T, atol=2e-2, rtol=1e-2)
+
+
+def test_scales_that_fp32_cannot_divide_by(eng):
+    """A bias is held divided by the scale: where that is infinite the call was answered with NaN."""
+    q, k, v = half(1, 40, 2, 32), half(1, 40, 2, 32), half(1, 40, 2, 32)
+    table = half(8, 2)
+    for scale in (1e-45, 1e-300, 2.0**-101, 1e38, math.inf, -1.0):
+        with pytest.raises(RuntimeError, match="scale"):
+            encoder.attention(q, k, v, table, scale=scale, max_distance=9)
+    ref = dict(table=table.double().cpu(), max_distance=9)
+    args = [t.double().cpu() for t in (q, k, v)]
+    out, lse = encoder.attention_forward(q, k, v, table, scale=2.0**-100, max_distance=9)
+    o.within(out, o.attention(*args, 2.0**-100, **ref)[0], o.attention_bounds(*args, 2.0**-100, F16, **ref)[0], "out")
+    grads = encoder.attention_backward(v, q, k, v, out, lse, table, scale=2.0**-100, max_distance=9)
+    for a, r, b in zip(grads, o.attention_grads(args[2], *args, 2.0**-100, **ref),
+                       o.attention_grad_bounds(args[2], *args, 2.0**-100, F16, **ref)):
+        o.within(a, r, b, "gradient")
