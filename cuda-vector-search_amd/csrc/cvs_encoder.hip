@@ -220,7 +220,7 @@ int cvs_layer_norm_backward_plan(int64_t n, int64_t d, int type, int device, int
   DevInfo di;
   int rc = dev_info(device, &di);
   if (rc == CVS_OK) rc = check_norm(n, d, type);
-  if (rc == CVS_OK) *workspace_bytes = norm_ws(n, d, type, di.cus);
+  if (rc == CVS_OK && workspace_bytes != nullptr) *workspace_bytes = norm_ws(n, d, type, di.cus);
   return rc;
 }
 
@@ -253,7 +253,7 @@ int cvs_linear_plan(int64_t m, int64_t k, int64_t n, int device, int64_t* worksp
   if (rc == CVS_OK) rc = check_linear(m, k, n);
   GemmPlan p = {};
   if (rc == CVS_OK && m > 0) rc = check_plan(p = plan_gemm(m, n, k, di.cus));
-  if (rc == CVS_OK) *workspace_bytes = p.ws_bytes;
+  if (rc == CVS_OK && workspace_bytes != nullptr) *workspace_bytes = p.ws_bytes;
   return rc;
 }
 
@@ -295,7 +295,7 @@ int cvs_linear_backward_plan(int64_t m, int64_t k, int64_t n, int act, int devic
     rc = check_plan(p.dx);
     if (rc == CVS_OK) rc = check_plan(p.dw);
   }
-  if (rc == CVS_OK) *workspace_bytes = p.bytes;
+  if (rc == CVS_OK && workspace_bytes != nullptr) *workspace_bytes = p.bytes;
   return rc;
 }
 
@@ -360,7 +360,7 @@ int cvs_attention_plan(const cvs_attention* p, int backward, int device, int64_t
   DevInfo di;
   int rc = dev_info(device, &di);
   if (rc == CVS_OK) rc = check_attention(p);
-  if (rc == CVS_OK) *workspace_bytes = plan_attention(attn_args(p), backward != 0, di.cus).bytes;
+  if (rc == CVS_OK && workspace_bytes != nullptr) *workspace_bytes = plan_attention(attn_args(p), backward != 0, di.cus).bytes;
   return rc;
 }
 

@@ -82,3 +82,15 @@ def test_scales_that_fp32_cannot_divide_by(eng):
     for a, r, b in zip(grads, o.attention_grads(args[2], *args, 2.0**-100, **ref),
                        o.attention_grad_bounds(args[2], *args, 2.0**-100, F16, **ref)):
         o.within(a, r, b, "gradient")
+
+
+def test_plans_without_a_place_for_the_size(eng):
+    """As the search's plans: a null pointer asks only whether there is a plan."""
+    lib = _ext.load().lib
+    assert lib.cvs_layer_norm_backward_plan(100, 64, 0, 0, None) == 0
+    assert lib.cvs_linear_plan(100, 64, 64, 0, None) == 0
+    assert lib.cvs_linear_backward_plan(100, 64, 64, 1, 0, None) == 0
+    a = _ext.AttentionArgs(batch=1, q_len=8, k_len=8, heads=1, k_heads=1, width=16, scale=1.0)
+    assert lib.cvs_attention_plan(ctypes.byref(a), 0, 0, None) == 0
+    assert lib.cvs_attention_plan(ctypes.byref(a), 1, 0, None) == 0
+    assert lib.cvs_attention_plan(None, 1, 0, None) != 0
