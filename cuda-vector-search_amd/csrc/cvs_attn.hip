@@ -25,8 +25,8 @@ constexpr int kKeys = 64;  // keys of a tile
 
 // Two LDS buffers of 64 keys and values, two or three workgroups a CU (which fill each other's
 // exponentials and waits with products), queries and sums in registers.  Bound by the vector
-// instructions between the products: 2 x 8192, 12 heads of 64, 0.82 PFLOP/s; 2 x 4096, 16 heads
-// of 128, 0.92; at short sequences by a workgroup's start and end (64 x up to 512, 12 heads
+// instructions between the products: 2 x 8192, 12 heads of 64, 469 us, 0.88 PFLOP/s; 2 x 4096, 16 heads
+// of 128, 270 us, 1.02; at short sequences by a workgroup's start and end (64 x up to 512, 12 heads
 // of 64, bias: 57 us).
 template <class T, int DP, bool BIAS>
 __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 3) void attn_forward_kernel(AttnArgs a) {

@@ -125,8 +125,8 @@ __device__ __forceinline__ void take_positions(const float* skew, float* sums) {
 // rows stay in registers, tiles of keys and values come into two LDS buffers in turn, and two
 // workgroups a CU fill each other's waits.  Bound by issue of the matrix and vector instructions
 // of a block, one after the other in a wave (the softmax's exponentials, the packing; with a bias
-// also the positions' sums): 2 x 4096, 16 heads of 128, causal 232 us, 0.89 PFLOP/s of its three
-// products; 64 x 512, 12 heads of 64, 125 us, with a bias 166 to 180; at short sequences by a
+// also the positions' sums): 2 x 4096, 16 heads of 128, causal 217 us, 0.95 PFLOP/s of its three
+// products; 64 x 512, 12 heads of 64, 122 us, with a bias 156; at short sequences by a
 // workgroup's start and end, some 7 us (32 sequences of up to 512, 12 heads of 64, bias: 58 us).
 template <class T, int DP, bool BIAS>
 __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) {
@@ -443,9 +443,9 @@ __device__ __forceinline__ void add_table(const AttnArgs& a, int at) {
 // dk and dv of 128 keys (wave w: 32 of them as columns), over a part of the queries that see
 // them.  Where there is a bias, the workgroups from `key_wgs` on add up its table's gradient.
 // The keys' rows of both operands and both sums stay in registers, at width 128 some 420 of them:
-// one wave a SIMD then, whose products (36% of the time), exponentials and packing follow one
-// another.  2 x 4096, 16 heads on 4 of 128, causal: 382 us, 0.72 PFLOP/s of its four products;
-// 64 x 512, 12 heads of 64, two workgroups a CU: 165 us, with a bias 180 to 190.
+// one wave a SIMD then, whose products (37% of the time), exponentials and packing follow one
+// another.  2 x 4096, 16 heads on 4 of 128, causal: 329 us, 0.84 PFLOP/s of its four products;
+// 64 x 512, 12 heads of 64, two workgroups a CU: 148 us, with a bias 156.
 template <class T, int DP, bool BIAS>
 __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kernel(AttnArgs a, int key_wgs) {
   typedef typename Frag<T>::V V;
@@ -636,7 +636,8 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
 }
 
 // Adds `parts` of n values, `stride` apart, in order: 8 a thread; blockIdx.y: the second of two sums
-// beside each other.  Bound by memory: dk and dv of 8192 x 4 heads of 128 in 2 parts 12.7 us, 5.9 TB/s.
+// beside each other.  dk and dv of 8192 x 4 heads of 128 in 2 parts, 67 MB read and 17 written: 12.9 us,
+// 6.5 TB/s, more than memory's 5.1, so that part of the sums still comes from the cache.
 template <class T>
 __global__ __launch_bounds__(kBlock) void attn_join_grads_kernel(const float* part, int parts, int64_t stride, int64_t n, float scale0,
                                                                  T* out0, T* out1) {
@@ -692,8 +693,9 @@ hipError_t backward(const AttnArgs& a, hipStream_t s) {
 // Parts of the keys for dq, and of the queries for dk and dv: enough workgroups for two of a CU,
 // of at least 8 tiles each.  (dq of 128 rows over 8192 keys, 8 heads of 64: the backward pass 35 us,
 // 141 with whole rows; dk and dv of 128 keys from 8192 rows: 39 us, 207 whole.  Causal, 2 x 4096 of
-// 16 heads on 4 of 128, 256 workgroups of unequal work: the pass 572 us in 2 parts, 600 in 4, whose
-// sums weigh more than their balance gains, 790 whole.)
+// 16 heads on 4 of 128, 256 workgroups of unequal work: the pass 563 us in 2 parts, 590 in 4, whose
+// sums weigh more than their balance gains, 790 whole; not causal 1060 and 1094; 2000 rows, 12 heads
+// of 64 81 and 85; but causal 8192 rows, 8 heads on 1 of 128 932 for two workgroups a CU and 874 for four.)
 int attn_q_parts(const AttnArgs& a, int cus) {
   const int64_t wgs = (a.lq + kAttnRows - 1) / kAttnRows * (int64_t)a.batch * a.heads;
   return (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / wgs, a.lk / 512, (int64_t)64}));

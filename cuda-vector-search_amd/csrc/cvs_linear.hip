@@ -264,8 +264,9 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& a, int id, unsigned ch
   if constexpr (W == 8) {
     // Two waves a SIMD, half a turn apart: while one reads the operands of two depth steps, the
     // other multiplies its own, and a barrier ends each such phase.  (Both at their own pace,
-    // a barrier a stage: 16384 x 768, k = 2048 59 us instead of 52, 16384 x 2048, k = 768 with
-    // gelu 83 instead of 77.)  The late waves are one phase behind; a stage's buffer is loaded
+    // a barrier a stage: dW of 32768 x 2048, k = 2048 268 us instead of 248, dx of 32768 x 2048, k = 1024 123
+    // instead of 118, 8192 x 8192, k = 2048 240 instead of 234; short reductions gain nothing,
+    // 16384 x 2048, k = 768 52.5 instead of 54.)  The late waves are one phase behind; a stage's buffer is loaded
     // again from the phase on after the late waves' last read of it, and its loads have landed,
     // by each wave's own wait, before the barrier that the early waves' first read follows.
     static_assert(RING == 2, "two stages");
@@ -521,9 +522,10 @@ __global__ __launch_bounds__(kBlock) void act_grad_kernel(ActGradArgs a) {
 // measured on long reductions (8192 x 8192, k = 2048: 1080, 850 and 480 TFLOP/s, that is 1.8 to
 // 2.0, 1.2 and 0.9 us with 1, 2 and 3 workgroups; 256 x 192 has 1.7), a round 3 us more to fill
 // and finish, and a split 3 us and its sums' way to memory and back.  At 16384 x 2048, k = 768
-// that gives 256 x 256 (56 us against 64 with 128 x 128), at 16384 x 768, k = 2048 256 x 192 (its
-// 256 tiles 57 us, 192 of 256 x 256 63), at 10007 x 768, k = 2048 128 x 128 (37 against 54 for
-// 256 x 256), at 2048 x 768, k = 16384 128 x 128 in 5 parts (67 with the join, 256 x 192 in 8 72).
+// that gives 256 x 256 (calls of the product alone, back to back: 54 us, with 128 x 128 58), at
+// 16384 x 768, k = 2048 256 x 192 (its 256 tiles 48 us, 192 of 256 x 256 52), at 10007 x 768, k = 2048
+// 128 x 128 (35, 256 x 256 47), at 2048 x 768, k = 16384 128 x 128 in 5 parts (61 with the join,
+// 256 x 192 in parts 65).
 //
 // A launch has fewer than 2^32 threads: choices of more are passed over, and where that leaves none
 // (splits 0), there is no plan.

@@ -461,7 +461,8 @@ def attention_forward(q, k, v, bias_table=None, key_lengths=None, query_lengths=
     position i + start, start = ``query_start[b]`` (by default k_len - q_len: the last row at the
     last key), and sees key j when j < ``key_lengths[b]`` and, if ``causal``, j <= i + start.
     Rows at or past ``query_lengths[b]`` see nothing; a row that sees nothing has out 0 and
-    lse -inf.  ``scale`` is from 2^-100 to 2^100, by default width ** -0.5.
+    lse -inf.  What lies in keys that no row sees (a cache's places not yet written)
+    reaches no result.  ``scale`` is from 2^-100 to 2^100, by default width ** -0.5.
 
     ``bias_table`` [buckets, heads] adds bias_table[bucket(j - i - start), h] to the score.
     Buckets: half of a direction's for one distance each, the others evenly in the

@@ -298,7 +298,8 @@ int cvs_layer_norm_backward(const void* dy, const void* x, const void* weight, c
  * y[m, n] = act(x w^T + bias) + residual for x [m, k], w [n, k]: bias [n], residual [m, n]
  * (rows residual_stride elements apart) and pre [m, n] (receives x w^T + bias, which the
  * backward pass takes) may be NULL.  Types CVS_TYPE_F16 and CVS_TYPE_BF16; k, n and the
- * strides are multiples of 8, pointers 16-byte aligned.  m may be anything.
+ * strides are multiples of 8, pointers 16-byte aligned.  m is below 2^31 - 255, and its tiles
+ * fit a launch (2^31 - 4096 rows of 8 do).
  */
 int cvs_linear_plan(int64_t m, int64_t k, int64_t n, int device, int64_t* workspace_bytes);
 int cvs_linear(const void* x, const void* w, const void* bias, const void* residual, int64_t m, int64_t k, int64_t n,
@@ -320,7 +321,8 @@ int cvs_linear_backward(const void* dy, const void* x, const void* w, const void
  * reads key head h / (heads / k_heads).  Row i of a sequence stands at key position
  * i + start (query_start[b], or k_len - q_len) and sees key j when j < key_lengths[b]
  * and, if causal, j <= i + start; rows at or past query_lengths[b] see nothing.  A row
- * that sees nothing has output 0 and log sum -inf.
+ * that sees nothing has output 0 and log sum -inf.  What lies in keys that no row
+ * sees (a cache's places not yet written) reaches no result.
  *   score[i, j] = scale * q_i . k_j + bias_table[bucket(j - i - start)][h]
  * bucket: distances below exact = per / 2 have one each, the per - exact others
  * divide exact .. max_distance evenly in the logarithm (the last takes all further ones);
