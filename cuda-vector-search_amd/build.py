@@ -43,13 +43,13 @@ FLAGS = [
 ]
 
 SOURCES = ["cvs_scan.hip", "cvs_gscan.hip", "cvs_scan_q8.hip", "cvs_select.hip", "cvs_rowtopk.hip", "cvs_gemv.hip", "cvs_prep.hip", "cvs_q8.hip",
-           "cvs_norm.hip", "cvs_linear.hip", "cvs_attn.hip", "cvs_attn_bwd.hip", "cvs_encoder.hip", "cvs_capi.hip"]
+           "cvs_norm.hip", "cvs_linear.hip", "cvs_gated.hip", "cvs_linear_int8.hip", "cvs_attn.hip", "cvs_attn_bwd.hip", "cvs_encoder.hip", "cvs_capi.hip"]
 
 # Per-source extra flags.  The scan keeps its MFMA accumulators in VGPRs (the
 # query fragments are pinned in AGPRs explicitly): the epilogue then reads the
 # scores without 64 v_accvgpr_read per tile (measured 3-6% faster scan).
-MFMA_SOURCES = ["cvs_scan.hip", "cvs_gscan.hip", "cvs_scan_q8.hip", "cvs_linear.hip", "cvs_attn.hip",
-                "cvs_attn_bwd.hip"]  # kernels whose MFMA results the build checks
+MFMA_SOURCES = ["cvs_scan.hip", "cvs_gscan.hip", "cvs_scan_q8.hip", "cvs_linear.hip", "cvs_gated.hip",
+                "cvs_linear_int8.hip", "cvs_attn.hip", "cvs_attn_bwd.hip"]  # kernels whose MFMA results the build checks
 EXTRA = {"cvs_scan.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "cvs_scan_q8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 

@@ -8,7 +8,7 @@
 namespace cvs {
 
 enum ElemType : int { kF16 = 0, kBF16 = 1, kF32 = 2 };
-enum Activation : int { kActNone = 0, kActGelu = 1, kActRelu = 2, kActTanh = 3 };
+enum Activation : int { kActNone = 0, kActGelu = 1, kActRelu = 2, kActTanh = 3, kActSilu = 4, kActSigmoid = 5 };  // (the last two: gates)
 
 // ---- layer norm ----------------------------------------------------------------
 struct NormArgs {
@@ -59,15 +59,65 @@ struct GemmArgs {
   float* partial;         // [splits, m, n] when splits > 1
   int splits;
 };
+// The other kinds of product (cvs_gemm_tile.h); partial is [splits, m, 2, n] when gated, whole numbers when int8.
+struct GemmKindArgs : GemmArgs {
+  const void* N2;         // gated: the second factor's weight; two parts: N of the second part
+  const void* bias2;      // gated: [n] or null
+  int64_t m_second;       // two parts: elements from M's first part to its second
+  const float* row_scale; // int8: [m]
+  const float* col_scale; // int8: [n]
+};
 struct GemmPlan {
   int tile, tile_n;  // rows and columns of a workgroup's tile
   int splits;        // parts of the reduction
   int64_t ws_bytes;
 };
+struct TileChoice { int m, n, wgs, threads; double stage; };  // a tile, workgroups of it a CU, us a stage
+// The choice of least estimated time; sums: fp32 sums of an output where the reduction is split.
+GemmPlan plan_tiles(const TileChoice* choices, int count, int64_t m, int64_t n, int64_t stages, int sums, int cus);
 GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int cus);
 hipError_t launch_gemm(const GemmArgs& a, const GemmPlan& p, hipStream_t s);
 // Two products, with partial sums apart; one launch where their tiles are alike.  a: N strided, b: both.
 hipError_t launch_gemm_pair(const GemmArgs& a, const GemmPlan& pa, const GemmArgs& b, const GemmPlan& pb, hipStream_t s);
+
+// The gated product's forward pass (out [m, n], pre [m, 2 n] or null) and dx of its backward pass:
+// dz [m, 2 n] times both weights.
+GemmPlan plan_gated(int64_t m, int64_t n, int64_t k, int cus);
+hipError_t launch_gated(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s);
+GemmPlan plan_two_parts(int64_t m, int64_t n, int64_t k, int cus);
+hipError_t launch_two_parts(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s);
+
+// dz = [dy up act'(gate), dy act(gate)] ([m, 2 n], contiguous) of pre = [gate, up], and dz's column sums.
+struct GatedGradArgs {
+  int type, act;
+  int64_t m;
+  int n;
+  const void* dy;
+  int64_t dy_stride;
+  const void* pre;
+  void* dz;
+  void* dgate_bias;       // [n] or null
+  void* dup_bias;
+  float* partial;         // [parts, 2, n] when either is not null
+  int parts;
+};
+int gated_grad_parts(int64_t m, int64_t n, int cus);
+hipError_t launch_gated_grad(const GatedGradArgs& a, hipStream_t s);
+
+// Rows in 8-bit whole numbers with a scale each, and the product of such operands (ldm, ldn and k in
+// 16-bit units: pairs of values).
+struct QuantArgs {
+  int type;
+  int64_t n;
+  int d;
+  const void* x;
+  int64_t x_stride;
+  signed char* values;    // [n, d]
+  float* scales;          // [n]
+};
+hipError_t launch_quantize(const QuantArgs& a, hipStream_t s);
+GemmPlan plan_int8(int64_t m, int64_t n, int64_t k, int cus);
+hipError_t launch_int8(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s);
 
 // dz = dy act'(pre) ([m, n], when act is not none and dz not null) and the column
 // sums of dz (dbias, when not null).

@@ -96,6 +96,81 @@ LinearBackwardPlan plan_linear_backward(int64_t m, int64_t k, int64_t n, int act
   return p;
 }
 
+// ---- gated product -----------------------------------------------------------------
+
+int check_gated_types(int act, int type) {
+  if (type != CVS_TYPE_F16 && type != CVS_TYPE_BF16) return fail(CVS_ERR_INVALID, "gated linear takes float16 or bfloat16");
+  if (act < CVS_ACT_NONE || act > CVS_ACT_SIGMOID) return fail(CVS_ERR_INVALID, "unknown activation %d", act);
+  return CVS_OK;
+}
+
+// (twice n values a row: dz, pre)
+int check_gated(int64_t m, int64_t k, int64_t n) {
+  const int rc = check_linear(m, k, n);
+  return rc == CVS_OK && n > (1 << 19) ? fail(CVS_ERR_INVALID, "gated linear takes at most 2^19 output features") : rc;
+}
+
+struct GatedBackwardPlan {
+  GemmPlan dx, dw, one;  // one: a single weight's gradient
+  int parts;
+  int64_t dz, partial, gemm, bytes;  // offsets, then all
+};
+
+GatedBackwardPlan plan_gated_backward(int64_t m, int64_t k, int64_t n, int cus) {
+  GatedBackwardPlan p;
+  p.dx = plan_two_parts(m, k, n, cus);
+  p.dw = plan_gemm(2 * n, k, m, cus);
+  p.one = plan_gemm(n, k, m, cus);
+  p.parts = gated_grad_parts(m, n, cus);
+  int64_t at = 0;
+  p.dz = at, at += up256(2 * m * n * 2);
+  p.partial = at, at += up256((int64_t)p.parts * 2 * n * 4);
+  p.gemm = at, at += up256(std::max({p.dx.ws_bytes, p.dw.ws_bytes, p.one.ws_bytes}));  // (one product after the other)
+  p.bytes = at;
+  return p;
+}
+
+int check_gated_plan(const GatedBackwardPlan& p) {
+  int rc = check_plan(p.dx);
+  if (rc == CVS_OK) rc = check_plan(p.dw);
+  return rc == CVS_OK ? check_plan(p.one) : rc;
+}
+
+// ---- 8-bit product -----------------------------------------------------------------
+
+int check_quantize(int64_t n, int64_t d, int type) {
+  if (type != CVS_TYPE_F16 && type != CVS_TYPE_BF16) return fail(CVS_ERR_INVALID, "8-bit rows are made of float16 or bfloat16");
+  if (n < 0 || n > INT_MAX - 255) return fail(CVS_ERR_INVALID, "too many rows");
+  if (d < 16 || d % 16 != 0 || d > (1 << 17))
+    return fail(CVS_ERR_INVALID, "8-bit rows have a multiple of 16 values, at most 2^17 (zero-pad them)");
+  // (a launch has fewer than 2^32 threads: rows of a wave each, or a workgroup)
+  if (n * (d <= 4096 ? 64 : 256) + 256 >= ((int64_t)1 << 32)) return fail(CVS_ERR_INVALID, "too many rows");
+  return CVS_OK;
+}
+
+int check_int8(int64_t m, int64_t k, int64_t n, int act, int type) {
+  int rc = check_quantize(m, k, type);
+  if (rc == CVS_OK) rc = check_linear(m, k, n);
+  if (rc == CVS_OK) rc = check_linear_types(act, type);
+  return rc;
+}
+
+struct Int8Plan {
+  GemmPlan product;
+  int64_t values, scales, gemm, bytes;  // offsets, then all
+};
+
+Int8Plan plan_linear_int8(int64_t m, int64_t k, int64_t n, int cus) {
+  Int8Plan p;
+  p.product = plan_int8(m, n, k, cus);
+  int64_t at = 0;
+  p.values = at, at += up256(m * k);
+  p.scales = at, at += up256(m * 4);
+  p.gemm = at, at += up256(p.product.ws_bytes);
+  p.bytes = at;
+  return p;
+}
+
 // ---- attention ---------------------------------------------------------------------
 
 int check_attention(const cvs_attention* p) {
@@ -354,6 +429,172 @@ int cvs_linear_backward(const void* dy, const void* x, const void* w, const void
   else if (dw != nullptr)
     e = launch_gemm(w_args, p.dw, s);
   return done(e, "linear backward launch");
+}
+
+int cvs_gated_linear_plan(int64_t m, int64_t k, int64_t n, int device, int64_t* workspace_bytes) {
+  DevInfo di;
+  int rc = dev_info(device, &di);
+  if (rc == CVS_OK) rc = check_gated(m, k, n);
+  GemmPlan p = {};
+  if (rc == CVS_OK && m > 0) rc = check_plan(p = plan_gated(m, n, k, di.cus));
+  if (rc == CVS_OK && workspace_bytes != nullptr) *workspace_bytes = p.ws_bytes;
+  return rc;
+}
+
+int cvs_gated_linear(const void* x, const void* gate, const void* up, const void* gate_bias, const void* up_bias, int64_t m,
+                     int64_t k, int64_t n, int64_t x_stride, int act, int type, void* y, void* pre, void* workspace,
+                     int64_t workspace_bytes, int device, void* stream) {
+  DevInfo di;
+  int rc = gfx950(device, &di);
+  if (rc == CVS_OK) rc = check_gated(m, k, n);
+  if (rc == CVS_OK) rc = check_gated_types(act, type);
+  if (rc != CVS_OK || m == 0) return rc;
+  if (x == nullptr || gate == nullptr || up == nullptr || y == nullptr) return fail(CVS_ERR_INVALID, "gated linear: null pointer");
+  rc = check_rows(x, x_stride, k, "x");
+  if (rc != CVS_OK) return rc;
+  if (!aligned16(gate) || !aligned16(up) || !aligned16(gate_bias) || !aligned16(up_bias) || !aligned16(y) || !aligned16(pre))
+    return fail(CVS_ERR_INVALID, "gated linear: pointers must be 16-byte aligned");
+  const GemmPlan p = plan_gated(m, n, k, di.cus);
+  rc = check_plan(p);
+  if (rc == CVS_OK) rc = check_workspace(workspace, workspace_bytes, p.ws_bytes);
+  if (rc != CVS_OK) return rc;
+  DeviceGuard guard(device);
+  if (guard.err != hipSuccess) return hip_fail(guard.err, "hipSetDevice");
+  GemmKindArgs a = {};
+  a.type = type, a.m = (int)m, a.n = (int)n, a.k = (int)k;
+  a.M = x, a.ldm = x_stride, a.N = gate, a.N2 = up, a.ldn = k;
+  a.bias = gate_bias, a.bias2 = up_bias, a.act = act;
+  a.pre = pre, a.out = y, a.partial = reinterpret_cast<float*>(workspace), a.splits = p.splits;
+  return done(launch_gated(a, p, reinterpret_cast<hipStream_t>(stream)), "gated linear launch");
+}
+
+int cvs_gated_linear_backward_plan(int64_t m, int64_t k, int64_t n, int device, int64_t* workspace_bytes) {
+  DevInfo di;
+  int rc = dev_info(device, &di);
+  if (rc == CVS_OK) rc = check_gated(m, k, n);
+  GatedBackwardPlan p = {};
+  if (rc == CVS_OK && m > 0) rc = check_gated_plan(p = plan_gated_backward(m, k, n, di.cus));
+  if (rc == CVS_OK && workspace_bytes != nullptr) *workspace_bytes = p.bytes;
+  return rc;
+}
+
+int cvs_gated_linear_backward(const void* dy, const void* x, const void* gate, const void* up, const void* pre, int64_t m,
+                              int64_t k, int64_t n, int64_t dy_stride, int64_t x_stride, int act, int type, void* dx,
+                              void* dgate, void* dup, void* dgate_bias, void* dup_bias, void* workspace,
+                              int64_t workspace_bytes, int device, void* stream) {
+  DevInfo di;
+  int rc = gfx950(device, &di);
+  if (rc == CVS_OK) rc = check_gated(m, k, n);
+  if (rc == CVS_OK) rc = check_gated_types(act, type);
+  if (rc != CVS_OK || m == 0) return rc;
+  if (dy == nullptr || x == nullptr || gate == nullptr || up == nullptr || pre == nullptr)
+    return fail(CVS_ERR_INVALID, "gated linear: null pointer");
+  rc = check_rows(dy, dy_stride, n, "dy");
+  if (rc == CVS_OK) rc = check_rows(x, x_stride, k, "x");
+  if (rc != CVS_OK) return rc;
+  if (!aligned16(gate) || !aligned16(up) || !aligned16(pre) || !aligned16(dx) || !aligned16(dgate) || !aligned16(dup) ||
+      !aligned16(dgate_bias) || !aligned16(dup_bias))
+    return fail(CVS_ERR_INVALID, "gated linear: pointers must be 16-byte aligned");
+  const GatedBackwardPlan p = plan_gated_backward(m, k, n, di.cus);
+  rc = check_gated_plan(p);
+  if (rc == CVS_OK) rc = check_workspace(workspace, workspace_bytes, p.bytes);
+  if (rc != CVS_OK) return rc;
+  DeviceGuard guard(device);
+  if (guard.err != hipSuccess) return hip_fail(guard.err, "hipSetDevice");
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
+  GatedGradArgs g = {};
+  g.type = type, g.act = act, g.m = m, g.n = (int)n, g.dy = dy, g.dy_stride = dy_stride, g.pre = pre;
+  g.dz = ws + p.dz, g.dgate_bias = dgate_bias, g.dup_bias = dup_bias;
+  g.partial = reinterpret_cast<float*>(ws + p.partial), g.parts = p.parts;
+  hipError_t e = launch_gated_grad(g, s);
+  float* sums = reinterpret_cast<float*>(ws + p.gemm);
+  if (e == hipSuccess && dx != nullptr) {  // dx = dg [m, n] gate [n, k] + du up
+    GemmKindArgs a = {};
+    a.type = type, a.m = (int)m, a.n = (int)k, a.k = (int)n;
+    a.M = g.dz, a.ldm = 2 * n, a.m_second = n, a.N = gate, a.N2 = up, a.ldn = k, a.n_strided = true;
+    a.out = dx, a.partial = sums, a.splits = p.dx.splits;
+    e = launch_two_parts(a, p.dx, s);
+  }
+  // dgate = dg^T x, dup = du^T x: one product of 2 n rows where they lie one behind the other
+  auto weight = [&](int64_t first, int64_t rows, const GemmPlan& plan, void* out) {
+    GemmArgs a = {};
+    a.type = type, a.m = (int)rows, a.n = (int)k, a.k = (int)m;
+    a.M = static_cast<unsigned char*>(g.dz) + 2 * first, a.ldm = 2 * n, a.m_strided = true;
+    a.N = x, a.ldn = x_stride, a.n_strided = true;
+    a.out = out, a.partial = sums, a.splits = plan.splits;
+    return launch_gemm(a, plan, s);
+  };
+  if (e == hipSuccess && dgate != nullptr && dup == static_cast<unsigned char*>(dgate) + 2 * n * k) {
+    e = weight(0, 2 * n, p.dw, dgate);
+  } else {
+    if (e == hipSuccess && dgate != nullptr) e = weight(0, n, p.one, dgate);
+    if (e == hipSuccess && dup != nullptr) e = weight(n, n, p.one, dup);
+  }
+  return done(e, "gated linear backward launch");
+}
+
+int cvs_quantize_rows(const void* x, int64_t n, int64_t d, int64_t x_stride, int type, void* values, float* scales, int device,
+                      void* stream) {
+  DevInfo di;
+  int rc = gfx950(device, &di);
+  if (rc == CVS_OK) rc = check_quantize(n, d, type);
+  if (rc != CVS_OK || n == 0) return rc;
+  if (x == nullptr || values == nullptr || scales == nullptr) return fail(CVS_ERR_INVALID, "quantize rows: null pointer");
+  rc = check_rows(x, x_stride, d, "x");
+  if (rc == CVS_OK && !aligned16(values)) rc = fail(CVS_ERR_INVALID, "quantize rows: values must be 16-byte aligned");
+  if (rc != CVS_OK) return rc;
+  DeviceGuard guard(device);
+  if (guard.err != hipSuccess) return hip_fail(guard.err, "hipSetDevice");
+  QuantArgs a = {};
+  a.type = type, a.n = n, a.d = (int)d, a.x = x, a.x_stride = x_stride;
+  a.values = static_cast<signed char*>(values), a.scales = scales;
+  return done(launch_quantize(a, reinterpret_cast<hipStream_t>(stream)), "quantize rows launch");
+}
+
+int cvs_linear_int8_plan(int64_t m, int64_t k, int64_t n, int device, int64_t* workspace_bytes) {
+  DevInfo di;
+  int rc = dev_info(device, &di);
+  if (rc == CVS_OK) rc = check_int8(m, k, n, CVS_ACT_NONE, CVS_TYPE_F16);
+  Int8Plan p = {};
+  if (rc == CVS_OK && m > 0) rc = check_plan((p = plan_linear_int8(m, k, n, di.cus)).product);
+  if (rc == CVS_OK && workspace_bytes != nullptr) *workspace_bytes = p.bytes;
+  return rc;
+}
+
+int cvs_linear_int8(const void* x, const void* w, const float* w_scales, const void* bias, const void* residual, int64_t m,
+                    int64_t k, int64_t n, int64_t x_stride, int64_t residual_stride, int act, int type, void* y,
+                    void* workspace, int64_t workspace_bytes, int device, void* stream) {
+  DevInfo di;
+  int rc = gfx950(device, &di);
+  if (rc == CVS_OK) rc = check_int8(m, k, n, act, type);
+  if (rc != CVS_OK || m == 0) return rc;
+  if (x == nullptr || w == nullptr || w_scales == nullptr || y == nullptr) return fail(CVS_ERR_INVALID, "linear int8: null pointer");
+  rc = check_rows(x, x_stride, k, "x");
+  if (rc == CVS_OK && residual != nullptr) rc = check_rows(residual, residual_stride, n, "residual");
+  if (rc != CVS_OK) return rc;
+  if (!aligned16(w) || !aligned16(w_scales) || !aligned16(bias) || !aligned16(y))
+    return fail(CVS_ERR_INVALID, "linear int8: pointers must be 16-byte aligned");
+  const Int8Plan p = plan_linear_int8(m, k, n, di.cus);
+  rc = check_plan(p.product);
+  if (rc == CVS_OK) rc = check_workspace(workspace, workspace_bytes, p.bytes);
+  if (rc != CVS_OK) return rc;
+  DeviceGuard guard(device);
+  if (guard.err != hipSuccess) return hip_fail(guard.err, "hipSetDevice");
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
+  QuantArgs q = {};
+  q.type = type, q.n = m, q.d = (int)k, q.x = x, q.x_stride = x_stride;
+  q.values = reinterpret_cast<signed char*>(ws + p.values), q.scales = reinterpret_cast<float*>(ws + p.scales);
+  hipError_t e = launch_quantize(q, s);
+  if (e != hipSuccess) return hip_fail(e, "linear int8 launch");
+  GemmKindArgs a = {};
+  a.type = type, a.m = (int)m, a.n = (int)n, a.k = (int)(k / 2);
+  a.M = q.values, a.ldm = k / 2, a.N = w, a.ldn = k / 2;
+  a.row_scale = q.scales, a.col_scale = w_scales;
+  a.bias = bias, a.residual = residual, a.ld_res = residual_stride, a.act = act;
+  a.out = y, a.partial = reinterpret_cast<float*>(ws + p.gemm), a.splits = p.product.splits;
+  return done(launch_int8(a, p.product, s), "linear int8 launch");
 }
 
 int cvs_attention_plan(const cvs_attention* p, int backward, int device, int64_t* workspace_bytes) {

@@ -1,0 +1,244 @@
+// The gated feed-forward block: both projections, the activation and the product in one
+// kernel, and its backward pass.
+//
+//   y = act(g) * u,  g = x Wg^T + bg,  u = x Wu^T + bu  (pre = [g, u], rounded, for the backward pass)
+//   dg = dy * u * act'(g),  du = dy * act(g)            (dz = [dg, du], rounded, and its column sums)
+//   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x
+//
+// Forward, a tile of the product has as many columns of g as of u, the same ones, so that g and
+// u meet in a wave's registers.  Backward, dx is one sum over two reductions and both weights'
+// gradients are one product whose rows are dz's 2 n columns (cvs_linear.hip's).
+#include <algorithm>
+
+#include "cvs_gemm_tile.h"
+
+namespace cvs {
+
+namespace {
+
+template <class T, int WM, int WN, int BM, int BN, int RING, int WGS, bool NS, int KIND>
+__global__ __launch_bounds__(64 * WM * WN, WGS) void gemm_kind_kernel(GemmKindArgs a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[gemm_lds<WM, WN, BM, BN, RING>()];
+  gemm_tile<T, WM, WN, BM, BN, RING, false, NS, KIND>(a, blockIdx.x, smem);
+}
+
+// Adds the parts of a split reduction, in order, and finishes: 8 columns a thread.
+template <class T>
+__global__ __launch_bounds__(kBlock) void gated_join_kernel(GemmKindArgs a) {
+  const int64_t at = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  const int pieces = a.n / 8;
+  const int64_t i = at / pieces;
+  if (i >= a.m) return;
+  const int j = (int)(at - i * pieces) * 8;
+  const int64_t plane = (int64_t)a.m * a.n * 2;
+  float z[2][8], h[8];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[u][e] = 0.f;
+  const float* p = a.partial + i * 2 * a.n + j;
+  for (int s = 0; s < a.splits; ++s, p += plane)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float* from = p + (u == 0 ? 0 : a.n);
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(from), hi = *reinterpret_cast<const f32x4*>(from + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[u][e] += lo[e], z[u][4 + e] += hi[e];
+    }
+  finish_gated8<T>(a, j, z[0], z[1], h);
+  if (a.pre != nullptr) {
+    store8((T*)a.pre + i * 2 * a.n + j, z[0]);
+    store8((T*)a.pre + i * 2 * a.n + a.n + j, z[1]);
+  }
+  store8((T*)a.out + i * a.n + j, h);
+}
+
+template <class T>
+__global__ __launch_bounds__(kBlock) void two_parts_join_kernel(GemmKindArgs a) {
+  const int64_t at = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * 8, plane = (int64_t)a.m * a.n;
+  if (at >= plane) return;
+  float z[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) z[e] = 0.f;
+  const float* p = a.partial + at;
+  for (int s = 0; s < a.splits; ++s, p += plane) {
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[e] += lo[e], z[4 + e] += hi[e];
+  }
+  store8((T*)a.out + at, z);
+}
+
+template <class T, int WM, int WN, int BM, int BN, int RING, int WGS, bool NS, int KIND>
+void launch_tiles(const GemmKindArgs& a, hipStream_t s) {
+  const dim3 grid(gemm_grid(a, WM * BM * 32, WN * BN * (KIND == kGated ? 16 : 32))), block(64 * WM * WN);
+  hipLaunchKernelGGL((gemm_kind_kernel<T, WM, WN, BM, BN, RING, WGS, NS, KIND>), grid, block, 0, s, a);
+}
+
+dim3 join_grid(const GemmKindArgs& a) { return dim3((unsigned)(((int64_t)a.m * (a.n / 8) + kBlock - 1) / kBlock)); }
+
+template <class T>
+hipError_t gated(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s) {
+  if (p.tile == 256)
+    launch_tiles<T, 4, 2, 2, 4, 2, 1, false, kGated>(a, s);
+  else if (p.tile == 128)
+    launch_tiles<T, 2, 2, 2, 2, 2, 2, false, kGated>(a, s);
+  else
+    launch_tiles<T, 2, 2, 1, 2, 3, 2, false, kGated>(a, s);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.splits == 1) return e;
+  hipLaunchKernelGGL(gated_join_kernel<T>, join_grid(a), dim3(kBlock), 0, s, a);
+  return hipGetLastError();
+}
+
+template <class T>
+hipError_t two_parts(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s) {
+  if (p.tile == 256 && p.tile_n == 256)
+    launch_tiles<T, 4, 2, 2, 4, 2, 1, true, kTwoParts>(a, s);
+  else if (p.tile == 256)
+    launch_tiles<T, 4, 2, 2, 3, 2, 1, true, kTwoParts>(a, s);
+  else if (p.tile == 128)
+    launch_tiles<T, 2, 2, 2, 2, 2, 2, true, kTwoParts>(a, s);
+  else
+    launch_tiles<T, 2, 2, 1, 1, 3, 2, true, kTwoParts>(a, s);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.splits == 1) return e;
+  hipLaunchKernelGGL(two_parts_join_kernel<T>, join_grid(a), dim3(kBlock), 0, s, a);
+  return hipGetLastError();
+}
+
+// du = dy act(g) and dg = dy u act'(g) of 8 values (the same branch for a whole launch).
+__device__ __forceinline__ void gate_grads8(const float* dy, const float* g, const float* u, int act, float* dg, float* du) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) dg[e] = dy[e] * u[e];
+  if (act == kActSilu || act == kActSigmoid) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      // s and 1 - s, each with its digits however small
+      const float x = __builtin_amdgcn_exp2f(fabsf(g[e]) * -kLog2e), r = __builtin_amdgcn_rcpf(1.f + x);
+      const float s = g[e] < 0.f ? x * r : r, rest = g[e] < 0.f ? r : x * r;
+      du[e] = dy[e] * (act == kActSilu ? g[e] * s : s);
+      dg[e] *= act == kActSilu ? s * fmaf(g[e], rest, 1.f) : s * rest;
+    }
+  } else if (act == kActNone) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) du[e] = dy[e] * g[e];
+  } else {
+    float h[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = g[e];
+    activate8(h, act);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) du[e] = dy[e] * h[e];
+    times_slope8(dg, g, act);
+  }
+}
+
+// Pieces of 8 columns of a workgroup, as act_grad_kernel's: few for few rows.
+__host__ __device__ inline int gated_grad_width(int64_t m, int n) { return m <= 256 ? 16 : min(n / 8, kBlock); }
+
+// dz and its column sums, bound by memory: three values in, two out.  A workgroup has up to 256
+// pieces of 8 columns (blockIdx.x) and as many of its part's rows at a time as its threads cover.
+template <class T>
+__global__ __launch_bounds__(kBlock) void gated_grad_kernel(GatedGradArgs a) {
+  __shared__ float red[kBlock * 8];
+  const int width = gated_grad_width(a.m, a.n);
+  const int pieces = min(a.n / 8 - (int)blockIdx.x * width, width), lanes = kBlock / pieces;
+  const int p = threadIdx.x % pieces, rl = threadIdx.x / pieces;
+  const int c = (blockIdx.x * width + p) * 8;
+  float sum[2][8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum[0][e] = sum[1][e] = 0.f;
+  const int64_t r0 = a.m * blockIdx.y / gridDim.y, r1 = a.m * (blockIdx.y + 1) / gridDim.y;
+  if (rl < lanes) {
+    constexpr int U = 4;  // rows under way
+    for (int64_t r = r0 + rl; r < r1; r += U * lanes) {
+      typename Frag<T>::V d[U], g[U], z[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t row = min(r + u * lanes, r1 - 1);
+        d[u] = *reinterpret_cast<const typename Frag<T>::V*>((const T*)a.dy + row * a.dy_stride + c);
+        g[u] = *reinterpret_cast<const typename Frag<T>::V*>((const T*)a.pre + row * 2 * a.n + c);
+        z[u] = *reinterpret_cast<const typename Frag<T>::V*>((const T*)a.pre + row * 2 * a.n + a.n + c);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t row = r + u * lanes;
+        if (row < r1) {
+          float df[8], gf[8], uf[8], dg[8], du[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) df[e] = (float)d[u][e], gf[e] = (float)g[u][e], uf[e] = (float)z[u][e];
+          gate_grads8(df, gf, uf, a.act, dg, du);
+          store8((T*)a.dz + row * 2 * a.n + c, dg);
+          store8((T*)a.dz + row * 2 * a.n + a.n + c, du);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum[0][e] += dg[e], sum[1][e] += du[e];
+        }
+      }
+    }
+  }
+  if (a.dgate_bias == nullptr && a.dup_bias == nullptr) return;
+  const int64_t col0 = (int64_t)blockIdx.x * width * 8;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) red[threadIdx.x * 8 + e] = sum[u][e];
+    __syncthreads();
+    T* out = (T*)(u == 0 ? a.dgate_bias : a.dup_bias);
+    for (int t = threadIdx.x; t < pieces * 8; t += kBlock) {
+      float s = 0.f;
+      for (int l = 0; l < lanes; ++l) s += red[l * pieces * 8 + t];
+      if (gridDim.y > 1)
+        a.partial[((int64_t)blockIdx.y * 2 + u) * a.n + col0 + t] = s;
+      else if (out != nullptr)
+        out[col0 + t] = (T)s;
+    }
+  }
+}
+
+}  // namespace
+
+// Tiles of 256 x (128 + 128) (8 waves, one workgroup a CU), 128 x (64 + 64) (two) and 64 x (64 + 64) (two),
+// with the costs of plan_gemm's products of as many blocks.
+GemmPlan plan_gated(int64_t m, int64_t n, int64_t k, int cus) {
+  static constexpr TileChoice kTiles[] = {{256, 128, 1, 512, 1.8}, {128, 64, 2, 256, 1.2}, {64, 64, 2, 256, 0.9}};
+  return plan_tiles(kTiles, 3, m, n, (k + kDepth - 1) / kDepth, 2, cus);
+}
+
+hipError_t launch_gated(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s) {
+  return a.type == kF16 ? gated<_Float16>(a, p, s) : gated<__bf16>(a, p, s);
+}
+
+GemmPlan plan_two_parts(int64_t m, int64_t n, int64_t k, int cus) {
+  static constexpr TileChoice kTiles[] = {{256, 256, 1, 512, 1.8}, {256, 192, 1, 512, 1.7}, {128, 128, 2, 256, 1.2}, {64, 64, 3, 256, 0.9}};
+  return plan_tiles(kTiles, 4, m, n, 2 * ((k + kDepth - 1) / kDepth), 1, cus);
+}
+
+hipError_t launch_two_parts(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s) {
+  return a.type == kF16 ? two_parts<_Float16>(a, p, s) : two_parts<__bf16>(a, p, s);
+}
+
+int gated_grad_parts(int64_t m, int64_t n, int cus) {
+  if (m <= 256) return 1;
+  const int64_t width = gated_grad_width(m, (int)n);
+  const int64_t blocks = (n / 8 + width - 1) / width, lanes = kBlock / width;
+  return (int)std::max<int64_t>(1, std::min<int64_t>((m + lanes - 1) / lanes, 3 * cus / blocks));
+}
+
+hipError_t launch_gated_grad(const GatedGradArgs& a, hipStream_t s) {
+  const int width = gated_grad_width(a.m, a.n);
+  const dim3 grid((a.n / 8 + width - 1) / width, a.parts), block(kBlock);
+  if (a.type == kF16)
+    hipLaunchKernelGGL(gated_grad_kernel<_Float16>, grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL(gated_grad_kernel<__bf16>, grid, block, 0, s, a);
+  hipError_t e = hipGetLastError();
+  const int first = a.dgate_bias != nullptr ? a.n : 0, second = a.dup_bias != nullptr ? a.n : 0;
+  if (e == hipSuccess && a.parts > 1 && first + second > 0)
+    e = launch_column_sums(a.partial + (first > 0 ? 0 : a.n), a.parts, 2 * a.n, first > 0 ? first : second, first > 0 ? second : 0,
+                           a.type, first > 0 ? a.dgate_bias : a.dup_bias, first > 0 ? a.dup_bias : nullptr, s);
+  return e;
+}
+
+}  // namespace cvs

@@ -1,0 +1,217 @@
+// Matrix product of 8-bit whole numbers: each row of x (a token) is taken in units of
+// its own scale, each row of the weight (a channel) comes in units of its own, and
+//
+//   y[i, j] = act(sx_i sw_j sum_r qx(i, r) qw(j, r) + bias[j]) + residual[i, j],
+//   sx_i = max_r |x(i, r)| / 127,  qx(i, r) = x(i, r) / sx_i to the nearest whole number, ties to the even one.
+//
+// The sum is whole and exact in 32 bits up to k = 2^17 (127 * 128 * 2^17 < 2^31), in any order.
+#include <algorithm>
+
+#include "cvs_gemm_tile.h"
+
+namespace cvs {
+
+namespace {
+
+// The largest magnitude of 16-bit floats by their bits: NaN and infinities come out on top.
+template <class T>
+struct Top;
+template <>
+struct Top<_Float16> {
+  static constexpr uint32_t kInf = 0x7c00;
+  static __device__ __forceinline__ float value(uint32_t bits) { return (float)__builtin_bit_cast(_Float16, (uint16_t)bits); }
+};
+template <>
+struct Top<__bf16> {
+  static constexpr uint32_t kInf = 0x7f80;
+  static __device__ __forceinline__ float value(uint32_t bits) { return __uint_as_float(bits << 16); }
+};
+
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ u16x2 top_of(const u32x4& v, u16x2 top) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v[e] & 0x7fff7fffu));
+  return top;
+}
+
+// A row's scale and what turns its values into whole numbers.  The quotient 127 x / top is exact
+// where it is a tie: 127 x is (18 bits), the division's remainder too, and one step of it from the
+// reciprocal's estimate leaves an error far below a tie's distance from any other quotient (2^-12 at
+// least: top has 11 bits).  Both are brought to where top is 0.5 to 1, out of the subnormals.
+struct RowUnit {
+  float scale, top, inv;
+  int shift;
+  bool finite;
+
+  template <class T>
+  __device__ __forceinline__ static RowUnit of(uint32_t bits) {
+    RowUnit u;
+    u.finite = bits < Top<T>::kInf;
+    const float top = u.finite ? Top<T>::value(bits) : 0.f;
+    u.scale = u.finite ? top / 127.f : __builtin_nanf("");
+    u.shift = -__builtin_amdgcn_frexp_expf(top);
+    u.top = ldexpf(top, u.shift);
+    u.inv = top > 0.f ? __builtin_amdgcn_rcpf(u.top) : 0.f;
+    return u;
+  }
+  // The whole number in the low byte (of the sum with 1.5 * 2^23, whose spacing is 1).
+  __device__ __forceinline__ uint32_t whole(float x) const {
+    const float t = 127.f * ldexpf(x, shift);
+    const float q = t * inv;
+    return __float_as_uint(fmaf(fmaf(-q, top, t), inv, q) + 12582912.f);
+  }
+  template <class T>
+  __device__ __forceinline__ u32x4 whole16(const u32x4& lo, const u32x4& hi) const {
+    const auto a = __builtin_bit_cast(typename Frag<T>::V, lo), b = __builtin_bit_cast(typename Frag<T>::V, hi);
+    u32x4 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = whole((float)(e < 2 ? a[4 * e + i] : b[4 * e - 8 + i]));
+      const uint32_t low = __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0400u), high = __builtin_amdgcn_perm(w[3], w[2], 0x04000c0cu);
+      r[e] = finite ? low | high : 0u;
+    }
+    return r;
+  }
+};
+
+// Rows of up to 1024 P values, a wave each, held in registers.
+template <class T, int P>
+__global__ __launch_bounds__(kBlock) void quantize_kernel(QuantArgs a) {
+  const int64_t row = (int64_t)blockIdx.x * (kBlock / kWave) + (threadIdx.x >> 6);
+  if (row >= a.n) return;
+  const int lane = threadIdx.x & 63;
+  const T* x = (const T*)a.x + row * a.x_stride;
+  u32x4 lo[P], hi[P];
+  u16x2 top = {0, 0};
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int c = (p * 64 + lane) * 16;
+    lo[p] = hi[p] = u32x4{0, 0, 0, 0};
+    if (c < a.d) {
+      lo[p] = *reinterpret_cast<const u32x4*>(x + c);
+      hi[p] = *reinterpret_cast<const u32x4*>(x + c + 8);
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < P; ++p) top = top_of(hi[p], top_of(lo[p], top));
+  uint32_t bits = max((uint32_t)top[0], (uint32_t)top[1]);
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) bits = max(bits, (uint32_t)__shfl_xor((int)bits, s));
+  const RowUnit u = RowUnit::of<T>(bits);
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int c = (p * 64 + lane) * 16;
+    if (c < a.d) *reinterpret_cast<u32x4*>(a.values + row * a.d + c) = u.whole16<T>(lo[p], hi[p]);
+  }
+  if (lane == 0) a.scales[row] = u.scale;
+}
+
+// Longer rows, a workgroup each, read twice.
+template <class T>
+__global__ __launch_bounds__(kBlock) void quantize_long_kernel(QuantArgs a) {
+  __shared__ uint32_t tops[4];
+  const int64_t row = blockIdx.x;
+  const T* x = (const T*)a.x + row * a.x_stride;
+  u16x2 top = {0, 0};
+  for (int c = threadIdx.x * 16; c < a.d; c += kBlock * 16)
+    top = top_of(*reinterpret_cast<const u32x4*>(x + c + 8), top_of(*reinterpret_cast<const u32x4*>(x + c), top));
+  uint32_t bits = max((uint32_t)top[0], (uint32_t)top[1]);
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) bits = max(bits, (uint32_t)__shfl_xor((int)bits, s));
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = bits;
+  __syncthreads();
+  const RowUnit u = RowUnit::of<T>(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
+  for (int c = threadIdx.x * 16; c < a.d; c += kBlock * 16)
+    *reinterpret_cast<u32x4*>(a.values + row * a.d + c) =
+        u.whole16<T>(*reinterpret_cast<const u32x4*>(x + c), *reinterpret_cast<const u32x4*>(x + c + 8));
+  if (threadIdx.x == 0) a.scales[row] = u.scale;
+}
+
+template <class T>
+void quantize(const QuantArgs& a, hipStream_t s) {
+  const dim3 waves((unsigned)((a.n + 3) / 4)), block(kBlock);
+  if (a.d <= 1024)
+    hipLaunchKernelGGL((quantize_kernel<T, 1>), waves, block, 0, s, a);
+  else if (a.d <= 2048)
+    hipLaunchKernelGGL((quantize_kernel<T, 2>), waves, block, 0, s, a);
+  else if (a.d <= 4096)
+    hipLaunchKernelGGL((quantize_kernel<T, 4>), waves, block, 0, s, a);
+  else
+    hipLaunchKernelGGL(quantize_long_kernel<T>, dim3((unsigned)a.n), block, 0, s, a);
+}
+
+template <class T, int WM, int WN, int BM, int BN, int RING, int WGS>
+__global__ __launch_bounds__(64 * WM * WN, WGS) void gemm_int8_kernel(GemmKindArgs a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[gemm_lds<WM, WN, BM, BN, RING>()];
+  gemm_tile<T, WM, WN, BM, BN, RING, false, false, kInt8>(a, blockIdx.x, smem);
+}
+
+// Adds the parts of a split reduction and finishes: 8 columns a thread.
+template <class T>
+__global__ __launch_bounds__(kBlock) void int8_join_kernel(GemmKindArgs a) {
+  const int64_t at = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  const int pieces = a.n / 8;
+  const int64_t i = at / pieces;
+  if (i >= a.m) return;
+  const int j = (int)(at - i * pieces) * 8;
+  const int64_t plane = (int64_t)a.m * a.n;
+  i32x4 lo = {0, 0, 0, 0}, hi = lo;
+  const float* p = a.partial + i * a.n + j;
+  for (int s = 0; s < a.splits; ++s, p += plane) {
+    lo += *reinterpret_cast<const i32x4*>(p);
+    hi += *reinterpret_cast<const i32x4*>(p + 4);
+  }
+  float z[8], pre[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) z[e] = (float)lo[e], z[4 + e] = (float)hi[e];
+  unscale8(a, (int)i, j, z);
+  finish8<T>(a, (int)i, j, z, pre);
+  store8((T*)a.out + i * a.n + j, z);
+}
+
+template <class T, int WM, int WN, int BM, int BN, int RING, int WGS>
+void launch_tiles(const GemmKindArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((gemm_int8_kernel<T, WM, WN, BM, BN, RING, WGS>), dim3(gemm_grid(a, WM * BM * 32, WN * BN * 32)),
+                     dim3(64 * WM * WN), 0, s, a);
+}
+
+template <class T>
+hipError_t product(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s) {
+  if (p.tile == 256 && p.tile_n == 256)
+    launch_tiles<T, 4, 2, 2, 4, 2, 1>(a, s);
+  else if (p.tile == 256)
+    launch_tiles<T, 4, 2, 2, 3, 2, 1>(a, s);
+  else if (p.tile == 128)
+    launch_tiles<T, 2, 2, 2, 2, 2, 2>(a, s);
+  else
+    launch_tiles<T, 2, 2, 1, 1, 3, 2>(a, s);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.splits == 1) return e;
+  hipLaunchKernelGGL(int8_join_kernel<T>, dim3((unsigned)(((int64_t)a.m * (a.n / 8) + kBlock - 1) / kBlock)), dim3(kBlock), 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_quantize(const QuantArgs& a, hipStream_t s) {
+  if (a.type == kF16)
+    quantize<_Float16>(a, s);
+  else
+    quantize<__bf16>(a, s);
+  return hipGetLastError();
+}
+
+// plan_gemm's tiles: a stage of 64 16-bit units is 128 values.
+GemmPlan plan_int8(int64_t m, int64_t n, int64_t k, int cus) {
+  static constexpr TileChoice kTiles[] = {{256, 256, 1, 512, 1.8}, {256, 192, 1, 512, 1.7}, {128, 128, 2, 256, 1.2}, {64, 64, 3, 256, 0.9}};
+  return plan_tiles(kTiles, 4, m, n, (k / 2 + kDepth - 1) / kDepth, 1, cus);
+}
+
+hipError_t launch_int8(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s) {
+  return a.type == kF16 ? product<_Float16>(a, p, s) : product<__bf16>(a, p, s);
+}
+
+}  // namespace cvs

@@ -194,6 +194,13 @@ def _bind_encoder(lib: ctypes.CDLL) -> None:
         "cvs_linear": [vp] * 4 + [i64] * 5 + [i32, i32, vp, vp, vp, i64, i32, vp],
         "cvs_linear_backward_plan": [i64, i64, i64, i32, i32, out],
         "cvs_linear_backward": [vp] * 4 + [i64] * 5 + [i32, i32, vp, vp, vp, vp, i64, i32, vp],
+        "cvs_gated_linear_plan": [i64, i64, i64, i32, out],
+        "cvs_gated_linear": [vp] * 5 + [i64] * 4 + [i32, i32, vp, vp, vp, i64, i32, vp],
+        "cvs_gated_linear_backward_plan": [i64, i64, i64, i32, out],
+        "cvs_gated_linear_backward": [vp] * 5 + [i64] * 5 + [i32, i32] + [vp] * 6 + [i64, i32, vp],
+        "cvs_quantize_rows": [vp, i64, i64, i64, i32, vp, vp, i32, vp],
+        "cvs_linear_int8_plan": [i64, i64, i64, i32, out],
+        "cvs_linear_int8": [vp] * 5 + [i64] * 5 + [i32, i32, vp, vp, i64, i32, vp],
         "cvs_attention_plan": [att, i32, i32, out],
         "cvs_attention_forward": [att, vp, vp, vp, i64, i32, vp],
         "cvs_attention_backward": [att, vp, out, vp, vp, vp, vp, vp, vp, vp, i64, i32, vp],

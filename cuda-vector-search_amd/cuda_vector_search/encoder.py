@@ -6,15 +6,19 @@ these operators.  Each runs hand-written gfx950 kernels (``libcvs_hip.so`` throu
 
 * ``layer_norm(x, weight, bias)``;
 * ``linear(x, weight, bias, activation, residual)``, a matrix product with its epilogue;
+* ``gated_linear(x, gate, up, ...)``, the gated feed-forward block's two products, activation
+  and product;
 * ``attention(q, k, v, ...)``, softmax attention over sequences of differing lengths,
-  causal or not, with shared key heads and a learned bias by relative position.
+  causal or not, with shared key heads and a learned bias by relative position;
+* ``linear_int8(x, values, scales, ...)``, for serving: ``linear`` of a weight that
+  ``quantize_rows`` laid out, in products of 8-bit whole numbers.
 
-These three are differentiable.  ``*_forward`` and ``*_backward`` are the passes
+All but the last are differentiable.  ``*_forward`` and ``*_backward`` are the passes
 themselves, for programs that keep the saved tensors on their own.  Tensors are float16
 or bfloat16 (``layer_norm``: float32 too), all of one type; results have it too, with
 fp32 sums inside.  A refused argument raises ``RuntimeError`` with the reason; there
 is no torch fallback.  Forward-mode derivatives and proxy tracing are refused too;
-``torch.jit.trace`` records the three as Python calls.
+``torch.jit.trace`` records the differentiable ones as Python calls.
 """
 
 from __future__ import annotations
@@ -32,6 +36,7 @@ from . import _ext
 
 TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 ACTIVATIONS = {None: 0, "gelu": 1, "relu": 2, "tanh": 3}
+GATES = {**ACTIVATIONS, "silu": 4, "sigmoid": 5}
 _I64 = ctypes.c_int64
 _I64x3 = _I64 * 3
 
@@ -74,6 +79,20 @@ def _bare(passes):
         return passes(*args, **kwargs)
 
     call.inner = passes
+    return call
+
+
+def _serving(call_):
+    """A call without a gradient: refused where torch would want one, or records a trace."""
+
+    @functools.wraps(call_)
+    def call(*args, **kwargs):
+        if _tracing() is not None:
+            raise RuntimeError(f"{call_.__name__} cannot be traced")
+        if _through_autograd(*args, *kwargs.values()):
+            raise RuntimeError(f"{call_.__name__} has no derivative: call it under torch.no_grad()")
+        return call_(*args, **kwargs)
+
     return call
 
 
@@ -337,6 +356,182 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     if _through_autograd(x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, activation, residual)
     return linear_forward.inner(x, weight, bias, activation, residual)[0]
+
+
+# ---- the gated feed-forward block ------------------------------------------------------
+
+
+def _gated_args(x, gate, up, activation):
+    _tensor(x, "x")
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError("gated_linear takes float16 or bfloat16")
+    if activation not in GATES:
+        raise ValueError(f"activation must be one of {list(GATES)}")
+    if x.dim() < 1:
+        raise RuntimeError("x must be [..., in_features]")
+    _tensor(gate, "gate", x)
+    if gate.dim() != 2 or gate.shape[1] != x.shape[-1]:
+        raise RuntimeError("gate must be [out_features, in_features], as wide as x")
+    _tensor(up, "up", x, gate.shape)
+    n, k = gate.shape
+    if k < 8 or n < 8 or k % 8 or n % 8:
+        raise RuntimeError("gated_linear takes feature counts that are multiples of 8 (zero-pad them)")
+    return n, k
+
+
+@_bare
+def gated_linear_forward(x, gate, up, gate_bias=None, up_bias=None, activation="silu", keep_pre: bool = False):
+    """(y, pre): y = activation(x gate^T + gate_bias) * (x up^T + up_bias) for ``x`` [..., k], ``gate``
+    and ``up`` [n, k] (halves of one weight, say).  ``activation``: "silu" (z sigmoid(z)),
+    "gelu" (by the error function), "sigmoid", "relu", "tanh" or None.  pre [..., 2 n] is both products,
+    the gate's first, for the backward pass, None without ``keep_pre``."""
+    n, k = _gated_args(x, gate, up, activation)
+    biases = []
+    for name, bias in (("gate_bias", gate_bias), ("up_bias", up_bias)):
+        if bias is not None:
+            _tensor(bias, name, x, (n,))
+            bias = _packed(bias)
+        biases.append(bias)
+    lib = _library()
+    r = _rows(x, k, True)
+    m = r.shape[0]
+    y = x.new_empty((*x.shape[:-1], n))
+    pre = x.new_empty((*x.shape[:-1], 2 * n)) if keep_pre else None
+    if m == 0:
+        return y, pre
+    gate, up = _packed(gate), _packed(up)
+    dev = x.device.index
+    ws = _workspace(("gated", m, k, n, dev), x, lambda out: lib.cvs_gated_linear_plan(m, k, n, dev, out))
+    _check(lib.cvs_gated_linear(r.data_ptr(), gate.data_ptr(), up.data_ptr(), _ptr(biases[0]), _ptr(biases[1]), m, k, n,
+                                _row_stride(r), GATES[activation], TYPES[x.dtype], y.data_ptr(), _ptr(pre), _ptr(ws),
+                                0 if ws is None else ws.numel(), dev, _ext.raw_stream(dev)))
+    return y, pre
+
+
+@_bare
+def gated_linear_backward(dy, x, gate, up, pre, activation="silu", needs=(True, True, True, True, True)):
+    """(dx, dgate, dup, dgate_bias, dup_bias) of ``gated_linear_forward`` for ``dy``, from the ``pre`` that
+    it kept.  Gradients that ``needs`` leaves out are None."""
+    n, k = _gated_args(x, gate, up, activation)
+    _tensor(dy, "dy", x, (*x.shape[:-1], n))
+    _tensor(pre, "pre", x, (*x.shape[:-1], 2 * n))
+    lib = _library()
+    r, g = _rows(x, k, True), _rows(dy, n, True)
+    m = r.shape[0]
+    dx = _new(x) if needs[0] else None
+    new = x.new_zeros if m == 0 else x.new_empty
+    if needs[1] and needs[2]:
+        both = new((2, n, k))  # (one behind the other: one product)
+        dgate, dup = both[0], both[1]
+    else:
+        dgate, dup = (new((n, k)) if need else None for need in needs[1:3])
+    dgate_bias, dup_bias = (new((n,)) if need else None for need in needs[3:5])
+    grads = dx, dgate, dup, dgate_bias, dup_bias
+    if m == 0 or all(t is None for t in grads):
+        return grads
+    pre, gate, up = _packed(pre), _packed(gate), _packed(up)
+    dev = x.device.index
+    ws = _workspace(("gated backward", m, k, n, dev), x, lambda out: lib.cvs_gated_linear_backward_plan(m, k, n, dev, out))
+    _check(lib.cvs_gated_linear_backward(g.data_ptr(), r.data_ptr(), gate.data_ptr(), up.data_ptr(), pre.data_ptr(), m, k, n,
+                                         _row_stride(g), _row_stride(r), GATES[activation], TYPES[x.dtype],
+                                         *(_ptr(t) for t in grads), _ptr(ws), 0 if ws is None else ws.numel(), dev,
+                                         _ext.raw_stream(dev)))
+    return grads
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, up, gate_bias, up_bias, activation):
+        y, pre = gated_linear_forward.inner(x, gate, up, gate_bias, up_bias, activation, keep_pre=True)
+        ctx.save_for_backward(x, gate, up, pre)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return (*gated_linear_backward.inner(dy, *ctx.saved_tensors, ctx.activation, ctx.needs_input_grad[:5]), None)
+
+
+def gated_linear(x, gate, up, gate_bias=None, up_bias=None, activation="silu"):
+    """activation(x gate^T + gate_bias) * (x up^T + up_bias); arguments as ``gated_linear_forward``'s."""
+    if _through_autograd(x, gate, up, gate_bias, up_bias):
+        return _GatedLinear.apply(x, gate, up, gate_bias, up_bias, activation)
+    return gated_linear_forward.inner(x, gate, up, gate_bias, up_bias, activation)[0]
+
+
+# ---- products of 8-bit whole numbers ---------------------------------------------------
+
+
+def _int8_width(k) -> None:
+    if k < 16 or k % 16 or k > 1 << 17:
+        raise RuntimeError("8-bit rows have a multiple of 16 values, at most 2^17 (zero-pad them)")
+
+
+@_serving
+def quantize_rows(x):
+    """(values, scales) of the rows of ``x`` [..., k]: scales float32 [...], a row's largest magnitude / 127;
+    values int8 [..., k], the row in units of its scale to the nearest whole number, ties to the
+    even one.  A row of zeros has scale 0, one with a value that is not finite scale NaN and values 0."""
+    _tensor(x, "x")
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError("quantize_rows takes float16 or bfloat16")
+    if x.dim() < 1:
+        raise RuntimeError("x must be [..., k]")
+    k = x.shape[-1]
+    _int8_width(k)
+    lib = _library()
+    r = _rows(x, k, True)
+    values = x.new_empty(x.shape, dtype=torch.int8)
+    scales = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    dev = x.device.index
+    if r.shape[0]:
+        _check(lib.cvs_quantize_rows(r.data_ptr(), r.shape[0], k, _row_stride(r), TYPES[x.dtype], values.data_ptr(),
+                                     scales.data_ptr(), dev, _ext.raw_stream(dev)))
+    return values, scales
+
+
+@_serving
+def linear_int8(x, values, scales, bias=None, activation=None, residual=None):
+    """activation(x weight^T + bias) + residual for ``x`` [..., k] and a weight [n, k] in 8-bit whole numbers, ``values``
+    (int8 [n, k]) times ``scales`` (float32 [n], its channels'), as ``quantize_rows`` lays them out once.  x's rows
+    (its tokens) are taken in 8-bit whole numbers too, by the same rule, inside; sums are whole and exact.
+    k is a multiple of 16, n of 8.  No derivative."""
+    _tensor(x, "x")
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError("linear_int8 takes float16 or bfloat16")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {list(ACTIVATIONS)}")
+    if x.dim() < 1:
+        raise RuntimeError("x must be [..., in_features]")
+    if not (isinstance(values, torch.Tensor) and values.device == x.device and values.dtype == torch.int8
+            and values.dim() == 2 and values.shape[1] == x.shape[-1]):
+        raise RuntimeError("values must be int8 [out_features, in_features] on the same device, as wide as x")
+    n, k = values.shape
+    _int8_width(k)
+    if n < 8 or n % 8:
+        raise RuntimeError("linear_int8 takes a multiple of 8 output features (zero-pad them)")
+    scales = _packed(_stats(scales, "scales", x, (n,)))
+    shape = (*x.shape[:-1], n)
+    if bias is not None:
+        _tensor(bias, "bias", x, (n,))
+    if residual is not None:
+        _tensor(residual, "residual", x, shape)
+    lib = _library()
+    r = _rows(x, k, True)
+    m = r.shape[0]
+    y = x.new_empty(shape)
+    if m == 0:
+        return y
+    values = _packed(values)
+    bias = None if bias is None else _packed(bias)
+    res = None if residual is None else _rows(residual, n, True)
+    dev = x.device.index
+    ws = _workspace(("int8", m, k, n, dev), x, lambda out: lib.cvs_linear_int8_plan(m, k, n, dev, out))
+    _check(lib.cvs_linear_int8(r.data_ptr(), values.data_ptr(), scales.data_ptr(), _ptr(bias), _ptr(res), m, k, n,
+                               _row_stride(r), 0 if res is None else _row_stride(res), ACTIVATIONS[activation], TYPES[x.dtype],
+                               y.data_ptr(), _ptr(ws), 0 if ws is None else ws.numel(), dev, _ext.raw_stream(dev)))
+    return y
 
 
 # ---- attention -----------------------------------------------------------------------

@@ -293,6 +293,8 @@ int cvs_layer_norm_backward(const void* dy, const void* x, const void* weight, c
 #define CVS_ACT_GELU 1 /* z * (1 + erf(z / sqrt 2)) / 2 */
 #define CVS_ACT_RELU 2
 #define CVS_ACT_TANH 3
+#define CVS_ACT_SILU 4    /* z / (1 + exp(-z)); this and the next: gated products only */
+#define CVS_ACT_SIGMOID 5 /* 1 / (1 + exp(-z)) */
 
 /*
  * y[m, n] = act(x w^T + bias) + residual for x [m, k], w [n, k]: bias [n], residual [m, n]
@@ -315,6 +317,47 @@ int cvs_linear_backward_plan(int64_t m, int64_t k, int64_t n, int act, int devic
 int cvs_linear_backward(const void* dy, const void* x, const void* w, const void* pre, int64_t m, int64_t k, int64_t n,
                         int64_t dy_stride, int64_t x_stride, int act, int type, void* dx, void* dw, void* dbias,
                         void* workspace, int64_t workspace_bytes, int device, void* stream);
+
+/*
+ * The gated feed-forward block: y[m, n] = act(x gate^T + gate_bias) * (x up^T + up_bias) for x [m, k],
+ * gate and up [n, k] (contiguous), biases [n] (either may be NULL), any CVS_ACT_*; pre [m, 2 n]
+ * (may be NULL) receives both products, the gate's n columns first, which the backward pass takes.
+ * As cvs_linear otherwise; n is at most 2^19.
+ */
+int cvs_gated_linear_plan(int64_t m, int64_t k, int64_t n, int device, int64_t* workspace_bytes);
+int cvs_gated_linear(const void* x, const void* gate, const void* up, const void* gate_bias, const void* up_bias, int64_t m,
+                     int64_t k, int64_t n, int64_t x_stride, int act, int type, void* y, void* pre, void* workspace,
+                     int64_t workspace_bytes, int device, void* stream);
+
+/*
+ * Gradients of cvs_gated_linear for dy [m, n] (rows dy_stride elements apart): dx [m, k], dgate and dup
+ * [n, k], dgate_bias and dup_bias [n], each of which may be NULL.  Both weights' are one product where
+ * dup lies right behind dgate.
+ */
+int cvs_gated_linear_backward_plan(int64_t m, int64_t k, int64_t n, int device, int64_t* workspace_bytes);
+int cvs_gated_linear_backward(const void* dy, const void* x, const void* gate, const void* up, const void* pre, int64_t m,
+                              int64_t k, int64_t n, int64_t dy_stride, int64_t x_stride, int act, int type, void* dx,
+                              void* dgate, void* dup, void* dgate_bias, void* dup_bias, void* workspace,
+                              int64_t workspace_bytes, int device, void* stream);
+
+/*
+ * Rows in 8-bit whole numbers: scales[i] = max_r |x[i, r]| / 127 (fp32), values[i, r] = 127 x[i, r] / max_r |x[i, r]|
+ * to the nearest whole number, ties to the even one, values [n, d] contiguous.  A row of zeros has scale 0;
+ * one with a value that is not finite has scale NaN and values 0.  d is a multiple of 16, at most 2^17, x of
+ * CVS_TYPE_F16 or CVS_TYPE_BF16, its stride a multiple of 8.
+ */
+int cvs_quantize_rows(const void* x, int64_t n, int64_t d, int64_t x_stride, int type, void* values, float* scales, int device,
+                      void* stream);
+
+/*
+ * y[m, n] = act(x w^T + bias) + residual with x's rows (tokens) in 8-bit whole numbers as cvs_quantize_rows
+ * makes them, inside, and w [n, k] given so, w_scales [n] (channels): whole sums, exact.  y, bias
+ * and residual are of x's type; k is a multiple of 16, at most 2^17; n and the strides multiples of 8.
+ */
+int cvs_linear_int8_plan(int64_t m, int64_t k, int64_t n, int device, int64_t* workspace_bytes);
+int cvs_linear_int8(const void* x, const void* w, const float* w_scales, const void* bias, const void* residual, int64_t m,
+                    int64_t k, int64_t n, int64_t x_stride, int64_t residual_stride, int act, int type, void* y,
+                    void* workspace, int64_t workspace_bytes, int device, void* stream);
 
 /*
  * Softmax attention with an optional learned bias by relative position.  Query head h
