@@ -28,7 +28,7 @@ constexpr int kKeys = 64;  // keys of a tile
 // instructions between the products: 2 x 8192, 12 heads of 64, 469 us, 0.88 PFLOP/s; 2 x 4096, 16 heads
 // of 128, 270 us, 1.02; at short sequences by a workgroup's start and end (64 x up to 512, 12 heads
 // of 64, bias: 57 us).
-template <class T, int DP, bool BIAS>
+template <class T, int DP, bool BIAS, bool WIN>
 __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 3) void attn_forward_kernel(AttnArgs a) {
   typedef typename Frag<T>::V V;
   constexpr int KS = DP / 16, DB = DP / 32, TILE = kKeys * DP * 2;
@@ -53,7 +53,12 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 3) void attn_forward_kernel(A
   const int last_row = min(block * kAttnRows + kAttnRows, nq) - 1;
   int end = last_row < block * kAttnRows ? 0 : nk;
   if (a.causal) end = min(end, max(last_row + off + 1, 0));
-  const int tiles = (end + kKeys - 1) / kKeys;
+  int tiles = (end + kKeys - 1) / kKeys;
+  WindowTiles<kKeys> win;
+  if constexpr (WIN) {
+    win = WindowTiles<kKeys>(a, nk, block * kAttnRows + off, last_row + off);
+    tiles = win.count;
+  }
   int t0 = 0, t1 = tiles;
   if (a.splits > 1) {  // (fewer than 2^23 tiles, at most 64 parts)
     t0 = (int)((unsigned)tiles * blockIdx.y / (unsigned)a.splits);
@@ -64,8 +69,14 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 3) void attn_forward_kernel(A
   if (BIAS) bias.buckets(a);
   const TileLoad<DP, kKeys> lk(2 * a.ks[1], a.d), lv(2 * a.vs[1], a.d);
   auto load = [&](int t) {
-    lk.load(kbase, 2 * a.ks[1], t * kKeys, end, sk[t & 1]);
-    lv.load(vbase, 2 * a.vs[1], t * kKeys, end, sv[t & 1]);
+    if constexpr (WIN) {
+      const int first = win.tile(t) * kKeys;
+      lk.load_window(kbase, 2 * a.ks[1], first, win.end, sk[t & 1], win.low, win.head);
+      lv.load_window(vbase, 2 * a.vs[1], first, win.end, sv[t & 1], win.low, win.head);
+    } else {
+      lk.load(kbase, 2 * a.ks[1], t * kKeys, end, sk[t & 1]);
+      lv.load(vbase, 2 * a.vs[1], t * kKeys, end, sv[t & 1]);
+    }
   };
   if (t0 < t1) load(t0);
   V qf[KS];
@@ -87,12 +98,13 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 3) void attn_forward_kernel(A
 
   // the tiles that a row of this wave sees a key of; through the others it only loads its share
   int mine = r0 < nq ? t1 : t0;
-  if (a.causal) mine = max(t0, min(mine, (r0 + 32 + off + kKeys - 1) / kKeys));
+  if (!WIN && a.causal) mine = max(t0, min(mine, (r0 + 32 + off + kKeys - 1) / kKeys));
   for (int t = t0; t < mine; ++t) {
     const int buf = t & 1;
     tile_barrier();
     if (t + 1 < t1) load(t + 1);
-    const int j0 = t * kKeys;
+    const int j0 = (WIN ? win.tile(t) : t) * kKeys;
+    if (WIN && !window_meets(a, j0, kKeys, r0 + off, min(r0 + 31, nq - 1) + off)) continue;
     const int near = j0 - r0 - off;  // position of the tile's first key and the wave's first row
     V rows[2][KS];
 #pragma unroll
@@ -130,7 +142,13 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 3) void attn_forward_kernel(A
 #pragma unroll
         for (int d = 0; d < DB; ++d) cols[kb][s][d] = col_frag<T, DP>(sv[buf], kb * 32 + 16 * s, d * 32);
     keep_order();
-    if (j0 + kKeys > nk || (a.causal && near + kKeys - 1 > 0)) {
+    if constexpr (WIN) {
+      if (j0 + kKeys > nk || near + kKeys - 1 > a.after || near < 31 - a.before) {
+        const WindowMask mask(a, nk, i + off, j0 + 8 * g);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) mask.apply(x[kb], kb * 32, j0 < a.sinks, -__builtin_inff());
+      }
+    } else if (j0 + kKeys > nk || (a.causal && near + kKeys - 1 > 0)) {
       const int seen = min(nk - 1, a.causal ? i + off : nk) - j0 - 8 * g;  // last key of the tile that the row sees
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
@@ -208,7 +226,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 3) void attn_forward_kernel(A
 // 23 us, 5.4 TB/s of keys and values; 36 us in the kernel above, where three of four waves had no
 // rows.  One sequence of 23, 12 heads of 32, with a bias: 5.2 us, the latency of the bias's two
 // dependent loads, the keys' tile and a launch.)
-template <class T, int DP, bool BIAS>
+template <class T, int DP, bool BIAS, bool WIN>
 __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_rows_kernel(AttnArgs a) {
   typedef typename Frag<T>::V V;
   constexpr int KS = DP / 16, DB = DP / 32, TILE = 32 * DP * 2, LOADS = TILE / 1024;
@@ -230,7 +248,12 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_rows_kernel(Attn
 
   int end = nq > 0 ? nk : 0;
   if (a.causal) end = min(end, max(nq + off, 0));
-  const int tiles = (end + 31) / 32;
+  int tiles = (end + 31) / 32;
+  WindowTiles<32> win;
+  if constexpr (WIN) {
+    win = WindowTiles<32>(a, nk, off, nq - 1 + off);
+    tiles = win.count;
+  }
   int t0 = 0, t1 = tiles;
   if (a.splits > 1) {
     t0 = (int)((unsigned)tiles * blockIdx.y / (unsigned)a.splits);
@@ -240,8 +263,14 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_rows_kernel(Attn
   if (BIAS) bias.buckets(a);
   const TileLoad<DP, 32, 1> lk(2 * a.ks[1], a.d), lv(2 * a.vs[1], a.d);
   auto load = [&](int t, int buf) {
-    lk.load(kbase, 2 * a.ks[1], t * 32, end, smem[wave][buf][0]);
-    lv.load(vbase, 2 * a.vs[1], t * 32, end, smem[wave][buf][1]);
+    if constexpr (WIN) {
+      const int first = win.tile(t) * 32;
+      lk.load_window(kbase, 2 * a.ks[1], first, win.end, smem[wave][buf][0], win.low, win.head);
+      lv.load_window(vbase, 2 * a.vs[1], first, win.end, smem[wave][buf][1], win.low, win.head);
+    } else {
+      lk.load(kbase, 2 * a.ks[1], t * 32, end, smem[wave][buf][0]);
+      lv.load(vbase, 2 * a.vs[1], t * 32, end, smem[wave][buf][1]);
+    }
   };
   int t = t0 + wave, buf = 0;
   if (t < t1) load(t, 0);
@@ -274,7 +303,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_rows_kernel(Attn
     asm volatile("" ::: "memory");
     const unsigned char* sk = smem[wave][buf][0];
     const unsigned char* sv = smem[wave][buf][1];
-    const int j0 = t * 32, near = j0 - off;
+    const int j0 = (WIN ? win.tile(t) : t) * 32, near = j0 - off;
     V rows[KS], cols[2][DB];
 #pragma unroll
     for (int s = 0; s < KS; ++s) rows[s] = row_frag<T, DP>(sk, 0, s);
@@ -295,7 +324,10 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_rows_kernel(Attn
     }
 #pragma unroll
     for (int s = 0; s < KS; ++s) x = Frag<T>::mfma(rows[s], qf[s], x);
-    if (j0 + 32 > nk || (a.causal && near + 31 > 0)) {
+    if constexpr (WIN) {
+      if (j0 + 32 > nk || near + 31 > a.after || near < nq - 1 - a.before)
+        WindowMask(a, nk, i + off, j0 + 8 * g).apply(x, 0, j0 < a.sinks, -__builtin_inff());
+    } else if (j0 + 32 > nk || (a.causal && near + 31 > 0)) {
       const int seen = min(nk - 1, a.causal ? i + off : nk) - j0 - 8 * g;
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[e] = elem_row(e, 0) > seen ? -__builtin_inff() : x[e];
@@ -431,18 +463,26 @@ int64_t workgroups(const AttnArgs& a) {
   return (a.lq + kAttnRows - 1) / kAttnRows * (int64_t)a.batch * a.heads;
 }
 
-template <class T, int DP>
-void launch_width(const AttnArgs& a, hipStream_t s) {
+template <class T, int DP, bool WIN>
+void launch_window(const AttnArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)workgroups(a), a.splits), block(kBlock);
   const size_t tab = (2 * (a.far + kReach) + 1) * sizeof(float);
   if (few_rows(a) && a.table != nullptr)
-    hipLaunchKernelGGL((attn_rows_kernel<T, DP, true>), grid, block, tab, s, a);
+    hipLaunchKernelGGL((attn_rows_kernel<T, DP, true, WIN>), grid, block, tab, s, a);
   else if (few_rows(a))
-    hipLaunchKernelGGL((attn_rows_kernel<T, DP, false>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((attn_rows_kernel<T, DP, false, WIN>), grid, block, 0, s, a);
   else if (a.table != nullptr)
-    hipLaunchKernelGGL((attn_forward_kernel<T, DP, true>), grid, block, tab, s, a);
+    hipLaunchKernelGGL((attn_forward_kernel<T, DP, true, WIN>), grid, block, tab, s, a);
   else
-    hipLaunchKernelGGL((attn_forward_kernel<T, DP, false>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((attn_forward_kernel<T, DP, false, WIN>), grid, block, 0, s, a);
+}
+
+template <class T, int DP>
+void launch_width(const AttnArgs& a, hipStream_t s) {
+  if (a.windowed)
+    launch_window<T, DP, true>(a, s);
+  else
+    launch_window<T, DP, false>(a, s);
 }
 
 template <class T>
@@ -469,7 +509,9 @@ hipError_t forward(const AttnArgs& a, hipStream_t s) {
 // up to 8191 keys, 12 heads of 64: 23 us and 5 for the join, 40 whole.)
 int attn_splits(const AttnArgs& a, int cus) {
   const int64_t least = few_rows(a) ? 4 * 4 * 32 : 4 * kKeys;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / std::max<int64_t>(workgroups(a), 1), a.lk / least, (int64_t)64}));
+  int64_t keys = a.lk;  // that a workgroup walks
+  if (a.windowed) keys = std::min(keys, (int64_t)a.sinks + a.before + a.after + std::min(a.lq, kAttnRows));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / std::max<int64_t>(workgroups(a), 1), keys / least, (int64_t)64}));
 }
 
 hipError_t launch_attn_forward(const AttnArgs& a, hipStream_t s) {

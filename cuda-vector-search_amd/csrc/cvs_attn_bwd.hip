@@ -128,7 +128,7 @@ __device__ __forceinline__ void take_positions(const float* skew, float* sums) {
 // also the positions' sums): 2 x 4096, 16 heads of 128, causal 217 us, 0.95 PFLOP/s of its three
 // products; 64 x 512, 12 heads of 64, 122 us, with a bias 156; at short sequences by a
 // workgroup's start and end, some 7 us (32 sequences of up to 512, 12 heads of 64, bias: 58 us).
-template <class T, int DP, bool BIAS>
+template <class T, int DP, bool BIAS, bool WIN>
 __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) {
   typedef typename Frag<T>::V V;
   constexpr int KS = DP / 16, DB = DP / 32, ROWS = kTile<DP>, KB = ROWS / 32, TILE = ROWS * DP * 2;
@@ -156,9 +156,18 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
   const int last_row = min(block * kAttnRows + kAttnRows, nq) - 1;
   int end = last_row < block * kAttnRows ? 0 : nk;
   if (a.causal) end = min(end, max(last_row + off + 1, 0));
-  const int all = (end + ROWS - 1) / ROWS;
+  int all = (end + ROWS - 1) / ROWS;
+  WindowTiles<ROWS> win;
+  int row_first, row_end;  // the rows that see a key of a window
+  const bool narrow = WIN && window_narrow(a);
   // this wave's rows see keys of the first tile only
-  const bool one = (a.causal ? min(nk, r0 + 32 + off) : nk) <= ROWS;
+  bool one = (a.causal ? min(nk, r0 + 32 + off) : nk) <= ROWS;
+  if constexpr (WIN) {
+    win = WindowTiles<ROWS>(a, nk, block * kAttnRows + off, last_row + off);
+    all = win.count;
+    window_rows(a, nk, nq, off, row_first, row_end);
+    one = !narrow && (one || (!a.causal && min(nk, max(r0 + 32 + off + a.after, a.sinks)) <= ROWS));
+  }
   // this workgroup's part of the tiles (fewer than 2^24, at most 64 parts); the first part writes
   // delta, or, where the wave's rows take it from the first tile, the part that has it
   int t0 = 0, tiles = all;
@@ -171,15 +180,21 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
   if (BIAS) bias.buckets(a);
   const TileLoad<DP, ROWS> lk(2 * a.ks[1], a.d), lv(2 * a.vs[1], a.d);
   auto load = [&](int t) {
-    lk.load(kbase, 2 * a.ks[1], t * ROWS, end, sk[t & 1]);
-    lv.load(vbase, 2 * a.vs[1], t * ROWS, end, sv[t & 1]);
+    if constexpr (WIN) {
+      const int first = win.tile(t) * ROWS;
+      lk.load_window(kbase, 2 * a.ks[1], first, win.end, sk[t & 1], win.low, win.head);
+      lv.load_window(vbase, 2 * a.vs[1], first, win.end, sv[t & 1], win.low, win.head);
+    } else {
+      lk.load(kbase, 2 * a.ks[1], t * ROWS, end, sk[t & 1]);
+      lv.load(vbase, 2 * a.vs[1], t * ROWS, end, sv[t & 1]);
+    }
   };
   if (t0 < tiles) load(t0);
 
   // the first loads are all on their way before one is waited for: the keys' and values' tiles,
   // the bias, the rows, and under them shared memory is cleared
   V qf[KS], gf[KS], of[KS];
-  const bool in = i >= first_row(a, off) && i < nq;
+  const bool in = WIN ? i >= row_first && i < row_end : i >= first_row(a, off) && i < nq;
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
     qf[s] = global_frag<T>(qrow, s, a.d, in);
@@ -212,16 +227,69 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
   const float c = a.scale * kLog2e;
   Lifted col = {kLift<T>};  // of this column's probabilities and ds
 
+  if (WIN && narrow) {
+    // delta = peak + sum p (dp - peak) / sum p with the largest dp as peak: of one key it is dp itself
+    float sp = 0.f, spd = 0.f, peak = -kNever;
+    for (int t = 0; t < all; ++t) {  // (one part)
+      tile_barrier();
+      if (t + 1 < all) load(t + 1);
+      const int tile0 = win.tile(t) * ROWS;
+      if (r0 >= nq || !window_meets(a, tile0, ROWS, r0 + off, min(r0 + 31, nq - 1) + off)) continue;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const int j0 = tile0 + kb * 32, near = j0 - r0 - off;
+        f32x16 p = zero16(), dp = zero16();
+        float base = -lse;
+        if (BIAS) {
+          if (near - 31 >= a.far || near + 31 <= -a.far) {
+            base += tab[near > 0 ? 2 * reach : 0] * c;
+          } else {
+            const float* at = tab + (near - l32 + 8 * g + reach);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) p[e] = at[elem_row(e, 0)];
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < KS; ++s) p = Frag<T>::mfma(row_frag<T, DP>(sk[t & 1], kb * 32, s), qf[s], p);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) dp = Frag<T>::mfma(row_frag<T, DP>(sv[t & 1], kb * 32, s), gf[s], dp);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], c, base));
+        const WindowMask mask(a, nk, i + off, j0 + 8 * g);
+        mask.apply(p, 0, j0 < a.sinks, 0.f);
+        float top = -kNever;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = p[e] > 0.f ? fmaxf(top, dp[e]) : top;
+        top = fmaxf(peak, halves_max(top));
+        if (top > peak) {
+          spd = peak == -kNever ? 0.f : fmaf(sp, peak - top, spd);
+          peak = top;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          sp += p[e];
+          spd = fmaf(p[e], p[e] > 0.f ? dp[e] - peak : 0.f, spd);
+        }
+      }
+    }
+    sp = halves_sum(sp), spd = halves_sum(spd);
+    delta = sp > 0.f ? peak + spd / sp : 0.f;
+    tile_barrier();
+    if (t0 < tiles) load(t0);
+  }
+
   // the tiles that a row of this wave sees a key of; through the others it only loads its share
   int mine = r0 < nq ? tiles : t0;
-  if (a.causal) mine = max(t0, min(mine, (r0 + 32 + off + ROWS - 1) / ROWS));
+  if (!WIN && a.causal) mine = max(t0, min(mine, (r0 + 32 + off + ROWS - 1) / ROWS));
   for (int t = t0; t < mine; ++t) {
     const int buf = t & 1;
     tile_barrier();
     if (t + 1 < tiles) load(t + 1);
+    const int tile0 = (WIN ? win.tile(t) : t) * ROWS;
+    if (WIN && !window_meets(a, tile0, ROWS, r0 + off, min(r0 + 31, nq - 1) + off)) continue;
     f32x16 ds[KB], p[KB];
     float base[KB];
-    const int near0 = t * ROWS - r0 - off;  // position of the tile's first key and the wave's first row
+    const int near0 = tile0 - r0 - off;  // position of the tile's first key and the wave's first row
     V krows[KB][KS], vrows[KB][KS], kcols[KB][2][DB];
 #pragma unroll
     for (int s = 0; s < KS; ++s)
@@ -273,7 +341,7 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
       read_vrows();
     }
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) ds[kb] = splat16(-delta);
+    for (int kb = 0; kb < KB; ++kb) ds[kb] = splat16(WIN && narrow ? 0.f : -delta);
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -284,10 +352,14 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
       read_kcols();
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      const int j0 = t * ROWS + kb * 32;
+      const int j0 = tile0 + kb * 32;
 #pragma unroll
       for (int e = 0; e < 16; ++e) p[kb][e] = __builtin_amdgcn_exp2f(fmaf(p[kb][e], c, base[kb]));
-      if (j0 + 32 > nk || (a.causal && near0 + kb * 32 + 31 > 0)) {
+      if constexpr (WIN) {
+        const int near = near0 + kb * 32;
+        if (j0 + 32 > nk || near + 31 > a.after || near < 31 - a.before)
+          WindowMask(a, nk, i + off, j0 + 8 * g).apply(p[kb], 0, j0 < a.sinks, 0.f);
+      } else if (j0 + 32 > nk || (a.causal && near0 + kb * 32 + 31 > 0)) {
         const int seen = min(nk - 1, a.causal ? i + off : nk) - j0 - 8 * g;  // last key of the block that the row sees
 #pragma unroll
         for (int e = 0; e < 16; ++e) p[kb][e] = elem_row(e, 0) > seen ? 0.f : p[kb][e];
@@ -309,6 +381,12 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
           if (kLift<T> != 0) p[kb][e] *= __builtin_amdgcn_exp2f(col.lift);
         }
       delta = halves_sum(spd);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) ds[kb][e] -= delta;
+    }
+    if (WIN && narrow) {  // (delta is of these very sums: subtracted as they stand)
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -446,7 +524,7 @@ __device__ __forceinline__ void add_table(const AttnArgs& a, int at) {
 // one wave a SIMD then, whose products (37% of the time), exponentials and packing follow one
 // another.  2 x 4096, 16 heads on 4 of 128, causal: 329 us, 0.84 PFLOP/s of its four products;
 // 64 x 512, 12 heads of 64, two workgroups a CU: 148 us, with a bias 156.
-template <class T, int DP, bool BIAS>
+template <class T, int DP, bool BIAS, bool WIN>
 __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kernel(AttnArgs a, int key_wgs) {
   typedef typename Frag<T>::V V;
   constexpr int KS = DP / 16, DB = DP / 32, ROWS = 64, QB = ROWS / 32, TILE = ROWS * DP * 2;
@@ -470,24 +548,36 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
   const int j = j0 + l32;
   const unsigned char* krow = (const unsigned char*)a.k + 2 * (b * a.ks[0] + j * a.ks[1] + hk * a.ks[2]);
   const unsigned char* vrow = (const unsigned char*)a.v + 2 * (b * a.vs[0] + j * a.vs[1] + hk * a.vs[2]);
-  const int row0 = min(first_row(a, off), nq), seen_keys = seen_count(a, nk, nq, off);
+  int row0 = min(first_row(a, off), nq), row1 = nq, seen_keys = seen_count(a, nk, nq, off);  // rows that see a key, keys that are seen
+  if constexpr (WIN) {
+    window_rows(a, nk, nq, off, row0, row1);
+    seen_keys = row1 > row0 ? min(nk, max(row1 - 1 + off + a.after + 1, 0)) : 0;  // (by the window; from its first row's on)
+  }
+  const int seen_low = WIN ? row0 + off - a.before : 0;
+  const bool seen = j < seen_keys && (!WIN || j >= seen_low);
   float shrink = 1.f;  // of this workgroup's ds, where they would not fit
   V kf[KS], vf[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
-    kf[s] = global_frag<T>(krow, s, a.d, j < seen_keys);
-    vf[s] = global_frag<T>(vrow, s, a.d, j < seen_keys);
+    kf[s] = global_frag<T>(krow, s, a.d, seen);
+    vf[s] = global_frag<T>(vrow, s, a.d, seen);
   }
   f32x16 dk[DB], dv[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) dk[d] = dv[d] = zero16();
   const float c = a.scale * kLog2e;
   const int reach = a.far + kReach;
-  const bool one = nk <= ROWS;  // delta is made of dout . v's own sums: subtracted as they stand, so that one key leaves 0
+  // delta is made of dout . v's own sums: subtracted as they stand, so that one key leaves 0
+  const bool one = nk <= ROWS || (WIN && window_narrow(a));
 
   // tiles of queries that see a key of this workgroup, those of all heads in a row; this part's
-  const int t0 = (a.causal ? max(block * kAttnRows - off, 0) : 0) / ROWS;
-  const int nt = block * kAttnRows < seen_keys ? max((nq + ROWS - 1) / ROWS - t0, 0) : 0;
+  int t0 = (a.causal ? max(block * kAttnRows - off, 0) : 0) / ROWS;
+  int nt = block * kAttnRows < seen_keys ? max((nq + ROWS - 1) / ROWS - t0, 0) : 0;
+  if constexpr (WIN) {  // (the first keys' gradients are attn_backward_sinks_kernel's)
+    const int lo = max(row0, block * kAttnRows - off - a.after), hi = min(row1, block * kAttnRows + kAttnRows - off + a.before);
+    t0 = lo / ROWS;
+    nt = block * kAttnRows < seen_keys && block * kAttnRows + kAttnRows > a.sinks && lo < hi ? (hi + ROWS - 1) / ROWS - t0 : 0;
+  }
   int f0 = 0, f1 = nt * group;
   if (a.kv_parts > 1) {
     const int64_t all = f1;
@@ -509,14 +599,14 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
     if (BIAS) bias.values(a, h);
     float stat = 0.f;  // threads 0 .. ROWS - 1: -log2 sum of a row, the next ROWS: -delta
     auto load = [&](int t) {
-      lq.load(qbase, 2 * a.qs[1], t * ROWS, nq, sq[t & 1], row0);
-      lg.load(gbase, 2 * a.dos[1], t * ROWS, nq, sg[t & 1], row0);
+      lq.load(qbase, 2 * a.qs[1], t * ROWS, row1, sq[t & 1], row0);
+      lg.load(gbase, 2 * a.dos[1], t * ROWS, row1, sg[t & 1], row0);
       const int i = t * ROWS + threadIdx.x % ROWS;
       if (threadIdx.x < ROWS) {
-        stat = i >= row0 && i < nq ? -lse[i] * kLog2e : -kNever;
+        stat = i >= row0 && i < row1 ? -lse[i] * kLog2e : -kNever;
         if (stat == __builtin_inff()) stat = -kNever;  // a row that sees nothing
       } else if (threadIdx.x < 2 * ROWS) {
-        stat = i >= row0 && i < nq ? -delta[i] : 0.f;
+        stat = i >= row0 && i < row1 ? -delta[i] : 0.f;
       }
     };
     auto turn = [&](int t) {
@@ -539,11 +629,12 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
     }
     // tiles that no key of this wave is seen from come first: it only loads its share of them
     int mine = j0 < seen_keys ? first : last;
-    if (a.causal) mine = min(last, max(mine, (j0 - off) / ROWS));
+    if (!WIN && a.causal) mine = min(last, max(mine, (j0 - off) / ROWS));
     for (int t = first; t < mine; ++t) turn(t);
     for (int t = mine; t < last; ++t) {
       const int buf = t & 1;
       turn(t);
+      if (WIN && (t * ROWS > j0 + 31 - off + a.before || t * ROWS + ROWS <= j0 - off - a.after)) continue;
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
         const int i0 = t * ROWS + qb * 32;
@@ -596,7 +687,14 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], c, BIAS ? base[e] + shift : base[e]));
-        if (a.causal && near + 31 > 0) {
+        if constexpr (WIN) {
+          if (near + 31 > a.after || near < 31 - a.before) {
+            const int low = j - off - a.after - i0 - 8 * g;  // first row of the block that sees the key
+            const unsigned span = a.after + a.before;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) p[e] = (unsigned)(elem_row(e, 0) - low) <= span ? p[e] : 0.f;
+          }
+        } else if (a.causal && near + 31 > 0) {
           const int seen = j - off - i0 - 8 * g;  // first row of the block that sees the key
 #pragma unroll
           for (int e = 0; e < 16; ++e) p[e] = elem_row(e, 0) < seen ? 0.f : p[e];
@@ -616,8 +714,8 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
       }
     }
   }
-  if (j >= a.lk) return;
-  if (j >= seen_keys) {
+  if (j >= a.lk || (WIN && j < a.sinks)) return;
+  if (!seen) {
 #pragma unroll
     for (int d = 0; d < DB; ++d) dk[d] = dv[d] = zero16();
   }
@@ -633,6 +731,190 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
   }
   store_head_row<T, DP>((T*)a.dk + at, dk, a.scale * undo, a.d);
   store_head_row<T, DP>((T*)a.dv + at, dv, kUnlift<T>, a.d);
+}
+
+// dk and dv of the first keys, which rows see from anywhere: 32 keys as columns, each wave walking row tiles of
+// its own (32 rows, of all heads that share the key head, one after the other) through buffers of its own, with
+// no barrier, its next tile's loads under way; the waves' sums are joined at the end.  A part of
+// the rows (blockIdx.y) each; parts are added by attn_join_sinks_kernel.
+template <class T, int DP, bool BIAS>
+__global__ __launch_bounds__(kBlock, 1) void attn_backward_sinks_kernel(AttnArgs a) {
+  typedef typename Frag<T>::V V;
+  constexpr int KS = DP / 16, DB = DP / 32, TILE = 32 * DP * 2, LOADS = TILE / 1024;
+  // per wave: two tiles of q and of dout; at the end its sums
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[4][2][2][TILE];
+  __shared__ __attribute__((aligned(16))) float stats[4][2][32];  // kLift - log2 sums, -deltas
+
+  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kheads = a.batch * a.k_heads, group = a.heads / a.k_heads;
+  const int bk = blockIdx.x % kheads, block = blockIdx.x / kheads;
+  const int b = bk / a.k_heads, hk = bk % a.k_heads;
+  const int nk = key_count(a, b), nq = query_count(a, b), off = query_offset(a, b);
+  const int j0 = block * 32, j = j0 + l32;
+  int row0, row1;
+  window_rows(a, nk, nq, off, row0, row1);
+  const int heads_seen = min(a.sinks, a.causal ? min(nk, max(row1 + off, 0)) : nk);  // keys of these that some row sees
+  const bool seen = row0 < row1 && j < heads_seen;
+  const unsigned char* krow = (const unsigned char*)a.k + 2 * (b * a.ks[0] + j * a.ks[1] + hk * a.ks[2]);
+  const unsigned char* vrow = (const unsigned char*)a.v + 2 * (b * a.vs[0] + j * a.vs[1] + hk * a.vs[2]);
+  V kf[KS], vf[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    kf[s] = global_frag<T>(krow, s, a.d, seen);
+    vf[s] = global_frag<T>(vrow, s, a.d, seen);
+  }
+  f32x16 dk[DB], dv[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) dk[d] = dv[d] = zero16();
+  const float c = a.scale * kLog2e;
+  float shrink = 1.f;  // of ds, where they would not fit (as the kv kernel's)
+  if constexpr (kLift<T> != 0) {
+    const int64_t count = (int64_t)group * a.q_parts * ((a.lq + kAttnRows - 1) / kAttnRows);
+    const float* from = a.part_peak + bk * count;
+    float peak = 0.f;
+    for (int64_t t = lane; t < count; t += 64) peak = fmaxf(peak, from[t]);
+    shrink = ldexpf(1.f, -max(__builtin_amdgcn_readfirstlane(kLift<T> - room(wave_max(peak))), 0));
+  }
+
+  // row tiles of all heads in a row; this part's, of which each wave takes every fourth
+  const int t0 = (a.causal ? max(row0, j0 - off) : row0) / 32;
+  const int nt = row0 < row1 && j0 < heads_seen ? max((row1 + 31) / 32 - t0, 0) : 0;
+  const int64_t all = (int64_t)nt * group;
+  const int64_t f0 = all * blockIdx.y / a.sink_parts, f1 = all * (blockIdx.y + 1) / a.sink_parts;
+  const TileLoad<DP, 32, 1> lq(2 * a.qs[1], a.d), lg(2 * a.dos[1], a.d);
+  float stat = 0.f;  // lanes 0 .. 31: -log2 sum of a row, the others: -delta
+  auto load = [&](int64_t f, int buf) {
+    const int h = hk * group + (int)(f / nt), t = t0 + (int)(f % nt);
+    lq.load((const unsigned char*)a.q + 2 * (b * a.qs[0] + h * a.qs[2]), 2 * a.qs[1], t * 32, row1, smem[wave][buf][0], row0);
+    lg.load((const unsigned char*)a.dout + 2 * (b * a.dos[0] + h * a.dos[2]), 2 * a.dos[1], t * 32, row1, smem[wave][buf][1], row0);
+    const int i = t * 32 + l32;
+    const int64_t at = ((int64_t)b * a.heads + h) * a.lq + i;
+    const bool in = i >= row0 && i < row1;
+    if (g == 0) {
+      stat = in ? -a.lse[at] * kLog2e : -kNever;
+      if (stat == __builtin_inff()) stat = -kNever;  // a row that sees nothing
+    } else {
+      stat = in ? -a.delta[at] : 0.f;
+    }
+  };
+  int64_t f = f0 + wave;
+  int buf = 0;
+  if (f < f1) load(f, 0);
+  for (; f < f1; f += 4, buf ^= 1) {
+    wait_vmcnt_lgkm0<0>();  // this tile's loads, and the reads of the buffers to be loaded next
+    asm volatile("" ::: "memory");
+    stats[wave][g][l32] = g == 0 ? stat + kLift<T> : stat;
+    if (f + 4 < f1) load(f + 4, buf ^ 1);
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    const unsigned char* sq = smem[wave][buf][0];
+    const unsigned char* sg = smem[wave][buf][1];
+    const int h = hk * group + (int)(f / nt), i0 = (t0 + (int)(f % nt)) * 32;
+    const int near = j0 - i0 - off;
+    f32x16 p = zero16(), ds;
+    float shift = 0.f;
+    if (BIAS) {
+      const float unit = 1.f / a.scale;
+      const T* table = (const T*)a.table + h;
+      auto bias = [&](int rel) {
+        int u = a.bucket_of[min(abs(rel), a.far)];
+        if (rel > 0) u = a.causal ? 0 : u + a.one_way;
+        return (float)table[(int64_t)u * a.heads] * unit;
+      };
+      if (near - 31 >= a.far || near + 31 <= -a.far) {
+        shift = bias(near) * c;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[e] = bias(near + l32 - elem_row(e, g));
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) p = Frag<T>::mfma(row_frag<T, DP>(sq, 0, s), kf[s], p);
+    ds = zero16();  // (delta may be made of dout . v's own sums: subtracted as they stand)
+#pragma unroll
+    for (int s = 0; s < KS; ++s) ds = Frag<T>::mfma(row_frag<T, DP>(sg, 0, s), vf[s], ds);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) ds[e] += stats[wave][1][elem_row(e, g)];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], c, stats[wave][0][elem_row(e, g)] + shift));
+    if (a.causal && near + 31 > 0) {
+      const int first = j - off - i0 - 8 * g;  // first row of the block that sees the key
+#pragma unroll
+      for (int e = 0; e < 16; ++e) p[e] = elem_row(e, 0) < first ? 0.f : p[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) ds[e] *= p[e];
+    if (kLift<T> != 0 && shrink != 1.f) times<1>(&ds, shrink);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const V pf = pack8<T>(p, s), df = pack8<T>(ds, s);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        dv[d] = Frag<T>::mfma(col_frag<T, DP>(sg, 16 * s, d * 32), pf, dv[d]);
+        dk[d] = Frag<T>::mfma(col_frag<T, DP>(sq, 16 * s, d * 32), df, dk[d]);
+      }
+    }
+  }
+  // join the waves: [2][32 columns][DP] each, the pieces of 4 in an order by column
+  wait_vmcnt_lgkm0<0>();
+  float* sums = reinterpret_cast<float*>(smem[wave]);
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x16& acc = u == 0 ? dk[d] : dv[d];
+        const int piece = (d * 32 + 16 * (q >> 1) + 8 * g + 4 * (q & 1)) / 4;
+        *reinterpret_cast<f32x4*>(sums + (u * 32 + l32) * DP + ((piece ^ (l32 & 7)) * 4)) =
+            f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+      }
+  __syncthreads();
+  const float undo_k = kUnlift<T> / shrink, undo_v = kUnlift<T>;
+  const int64_t plane = (int64_t)a.batch * a.sinks * a.k_heads * a.d;
+  for (int t = threadIdx.x; t < 2 * 32 * (DP / 8); t += kBlock) {
+    const int u = t / (32 * (DP / 8)), col = t / (DP / 8) % 32, c8 = t % (DP / 8) * 8;
+    if (c8 >= a.d || j0 + col >= a.sinks) continue;
+    float z[8];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        s += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(smem[w]) + (u * 32 + col) * DP + (((c8 / 4 + half) ^ (col & 7)) * 4));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[4 * half + e] = j0 + col < heads_seen ? s[e] * (u == 0 ? undo_k : undo_v) : 0.f;
+    }
+    if (a.sink_parts > 1) {
+      float* o = a.part_sinks + (2 * blockIdx.y + u) * plane + (((int64_t)b * a.sinks + j0 + col) * a.k_heads + hk) * a.d + c8;
+      *reinterpret_cast<f32x4*>(o) = f32x4{z[0], z[1], z[2], z[3]};
+      *reinterpret_cast<f32x4*>(o + 4) = f32x4{z[4], z[5], z[6], z[7]};
+    } else {
+      V v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (T)(u == 0 ? z[e] * a.scale : z[e]);
+      *reinterpret_cast<V*>((T*)(u == 0 ? a.dk : a.dv) + (((int64_t)b * a.lk + j0 + col) * a.k_heads + hk) * a.d + c8) = v;
+    }
+  }
+}
+
+// Adds the parts of the first keys' dk and dv, in order: 8 values a thread.
+template <class T>
+__global__ __launch_bounds__(kBlock) void attn_join_sinks_kernel(AttnArgs a) {
+  const int64_t row = (int64_t)a.sinks * a.k_heads * a.d, plane = a.batch * row;
+  const int64_t at = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * 8;
+  if (at >= plane) return;
+  f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+  for (int p = 0; p < a.sink_parts; ++p) {
+    const f32x4* from = reinterpret_cast<const f32x4*>(a.part_sinks + (2 * p + blockIdx.y) * plane + at);
+    lo += from[0];
+    hi += from[1];
+  }
+  const float scale = blockIdx.y == 0 ? a.scale : 1.f;
+  typename Frag<T>::V v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = (T)(lo[e] * scale), v[4 + e] = (T)(hi[e] * scale);
+  *reinterpret_cast<typename Frag<T>::V*>((T*)(blockIdx.y == 0 ? a.dk : a.dv) + at / row * a.lk * a.k_heads * a.d + at % row) = v;
 }
 
 // Adds `parts` of n values, `stride` apart, in order: 8 a thread; blockIdx.y: the second of two sums
@@ -656,16 +938,16 @@ __global__ __launch_bounds__(kBlock) void attn_join_grads_kernel(const float* pa
   *reinterpret_cast<typename Frag<T>::V*>((blockIdx.y == 0 ? out0 : out1) + at) = v;
 }
 
-template <class T, int DP, bool BIAS>
-hipError_t launch_width(const AttnArgs& a, hipStream_t s) {
+template <class T, int DP, bool BIAS, bool WIN>
+hipError_t launch_window(const AttnArgs& a, hipStream_t s) {
   const int64_t qblocks = (a.lq + kAttnRows - 1) / kAttnRows, kblocks = (a.lk + kAttnRows - 1) / kAttnRows;
   const size_t tab = BIAS ? (2 * (a.far + kReach) + 1) * sizeof(float) : 0;
   if (qblocks > 0)
-    hipLaunchKernelGGL((attn_backward_q_kernel<T, DP, BIAS>), dim3((unsigned)(qblocks * a.batch * a.heads), a.q_parts),
+    hipLaunchKernelGGL((attn_backward_q_kernel<T, DP, BIAS, WIN>), dim3((unsigned)(qblocks * a.batch * a.heads), a.q_parts),
                        dim3(kBlock), 5 * tab, s, a);
   const int64_t key_wgs = kblocks * a.batch * a.k_heads, all_wgs = key_wgs + (BIAS ? (a.buckets * a.heads + 3) / 4 : 0);
   if (all_wgs > 0)
-    hipLaunchKernelGGL((attn_backward_kv_kernel<T, DP, BIAS>), dim3((unsigned)all_wgs, a.kv_parts), dim3(kBlock), tab, s, a,
+    hipLaunchKernelGGL((attn_backward_kv_kernel<T, DP, BIAS, WIN>), dim3((unsigned)all_wgs, a.kv_parts), dim3(kBlock), tab, s, a,
                        (int)key_wgs);
   auto join = [&](const float* part, int parts, int64_t n, int sums, float scale, void* out0, void* out1) {
     const dim3 grid((unsigned)((n / 8 + kBlock - 1) / kBlock), sums);
@@ -673,7 +955,21 @@ hipError_t launch_width(const AttnArgs& a, hipStream_t s) {
   };
   if (a.q_parts > 1) join(a.part_q, a.q_parts, (int64_t)a.batch * a.lq * a.heads * a.d, 1, a.scale, a.dq, nullptr);
   if (a.kv_parts > 1) join(a.part_kv, a.kv_parts, (int64_t)a.batch * a.lk * a.k_heads * a.d, 2, a.scale, a.dk, a.dv);
+  if constexpr (WIN) {
+    if (a.sinks > 0) {  // (after the joins, which write the first keys' places too)
+      const int64_t plane = (int64_t)a.batch * a.sinks * a.k_heads * a.d;
+      hipLaunchKernelGGL((attn_backward_sinks_kernel<T, DP, BIAS>), dim3((unsigned)((a.sinks + 31) / 32 * a.batch * a.k_heads), a.sink_parts),
+                         dim3(kBlock), 0, s, a);
+      if (a.sink_parts > 1)
+        hipLaunchKernelGGL(attn_join_sinks_kernel<T>, dim3((unsigned)((plane / 8 + kBlock - 1) / kBlock), 2), dim3(kBlock), 0, s, a);
+    }
+  }
   return hipGetLastError();
+}
+
+template <class T, int DP, bool BIAS>
+hipError_t launch_width(const AttnArgs& a, hipStream_t s) {
+  return a.windowed ? launch_window<T, DP, BIAS, true>(a, s) : launch_window<T, DP, BIAS, false>(a, s);
 }
 
 template <class T, bool BIAS>
@@ -698,12 +994,24 @@ hipError_t backward(const AttnArgs& a, hipStream_t s) {
 // of 64 81 and 85; but causal 8192 rows, 8 heads on 1 of 128 932 for two workgroups a CU and 874 for four.)
 int attn_q_parts(const AttnArgs& a, int cus) {
   const int64_t wgs = (a.lq + kAttnRows - 1) / kAttnRows * (int64_t)a.batch * a.heads;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / wgs, a.lk / 512, (int64_t)64}));
+  if (window_narrow(a)) return 1;
+  int64_t keys = a.lk;  // that a workgroup walks
+  if (a.windowed) keys = std::min(keys, (int64_t)a.sinks + a.before + a.after + std::min(a.lq, kAttnRows));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / wgs, keys / 512, (int64_t)64}));
 }
 int attn_kv_parts(const AttnArgs& a, int cus) {
   const int64_t wgs = (a.lk + kAttnRows - 1) / kAttnRows * (int64_t)a.batch * a.k_heads;
-  const int64_t tiles = (a.lq + 63) / 64 * (int64_t)(a.heads / a.k_heads);
+  int64_t rows = a.lq;  // that a workgroup walks of each head
+  if (a.windowed) rows = std::min(rows, (int64_t)a.before + a.after + kAttnRows);
+  const int64_t tiles = (rows + 63) / 64 * (int64_t)(a.heads / a.k_heads);
   return (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / wgs, tiles / 8, (int64_t)16}));
+}
+
+// Parts of the rows for the first keys' dk and dv: enough workgroups for one of a CU, of at least 4 tiles a wave.
+int attn_sink_parts(const AttnArgs& a, int cus) {
+  const int64_t wgs = (a.sinks + 31) / 32 * (int64_t)a.batch * a.k_heads;
+  const int64_t tiles = (a.lq + 31) / 32 * (int64_t)(a.heads / a.k_heads);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({cus / std::max<int64_t>(wgs, 1), tiles / 16, (int64_t)64}));
 }
 
 hipError_t launch_attn_backward(const AttnArgs& a, hipStream_t s) {

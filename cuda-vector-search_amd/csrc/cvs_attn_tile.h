@@ -48,6 +48,67 @@ struct TileLoad {
     for (int i = 0; i < N; ++i)
       load_lds((unsigned)(first - low + row[i]) < (unsigned)(rows - low) ? at[i] : kOutside, base + first * stride_bytes, to + i * (WAVES * 1024));
   }
+  // The same of rows low .. rows - 1 and of the first `head`.
+  __device__ __forceinline__ void load_window(const unsigned char* base, int64_t stride_bytes, int first, int rows,
+                                              const unsigned char* lds, int low, int head) const {
+    const uint32_t to = lds_address(lds) + (WAVES > 1 ? threadIdx.x >> 6 : 0) * 1024;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const bool in = (unsigned)(first - low + row[i]) < (unsigned)(rows - low) || first + row[i] < head;
+      load_lds(in ? at[i] : kOutside, base + first * stride_bytes, to + i * (WAVES * 1024));
+    }
+  }
+};
+
+// What a window leaves of the keys for rows at positions p0 .. p1: the first `head` and low .. end - 1, in tiles of
+// ROWS.  Tile u of these is the keys' tile u below `heads`, and u + gap from there.
+template <int ROWS>
+struct WindowTiles {
+  int head, low, end, heads, gap, count;
+
+  __device__ __forceinline__ WindowTiles() {}
+  __device__ __forceinline__ WindowTiles(const AttnArgs& a, int nk, int p0, int p1) {
+    const int last = a.causal ? min(nk, max(p1 + 1, 0)) : nk;
+    head = p0 <= p1 ? min(a.sinks, last) : 0;
+    low = min(max(p0 - a.before, 0), last);
+    end = p0 <= p1 ? max(min(last, p1 + a.after + 1), low) : low;
+    heads = (head + ROWS - 1) / ROWS;
+    const int t0 = max(low / ROWS, heads), t1 = end > low ? (end + ROWS - 1) / ROWS : t0;
+    gap = t0 - heads;
+    count = heads + max(t1 - t0, 0);
+  }
+  __device__ __forceinline__ int tile(int u) const { return u < heads ? u : u + gap; }
+};
+
+// Whether rows at positions p0 .. p1 see a key of the `rows` ones from j0 on (were there that many).
+__device__ __forceinline__ bool window_meets(const AttnArgs& a, int j0, int rows, int p0, int p1) {
+  return (j0 < a.sinks || (j0 + rows > p0 - a.before && j0 <= p1 + a.after)) && (!a.causal || j0 <= p1);
+}
+
+// The keys that the row at position p sees, counted from `from` on: (unsigned)(key - low) <= span, or key < head.
+struct WindowMask {
+  int low, head;
+  unsigned span;
+
+  __device__ __forceinline__ WindowMask(const AttnArgs& a, int nk, int p, int from) {
+    const int lo = p - a.before, hi = min(nk - 1, p + a.after);
+    low = hi < lo ? 1 << 30 : lo - from;
+    span = hi < lo ? 0 : hi - lo;
+    head = min(nk, a.causal ? min(a.sinks, p + 1) : a.sinks) - from;
+  }
+  // Puts `out` in the places of a block (keys of 32 from `key` on, 8 (lane / 32) of them in `from`) that are not seen.
+  __device__ __forceinline__ void apply(f32x16& x, int key, bool heads, float out) const {
+    if (heads) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int k = key + elem_row(e, 0);
+        x[e] = (unsigned)(k - low) <= span || k < head ? x[e] : out;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] = (unsigned)(key + elem_row(e, 0) - low) <= span ? x[e] : out;
+    }
+  }
 };
 
 // This wave's loads into LDS have landed and its LDS operations are done; then every wave's.
@@ -170,6 +231,16 @@ __device__ __forceinline__ int query_count(const AttnArgs& a, int b) {
 }
 __device__ __forceinline__ int query_offset(const AttnArgs& a, int b) {
   return a.query_start == nullptr ? a.lk - a.lq : min(max(a.query_start[b], -(1 << 29)), 1 << 29);
+}
+// Whether no row sees more than a few keys.  Their gradients ds are then differences of few terms (of one key,
+// zero), and delta is taken from those terms themselves, in a pass of its own.
+__host__ __device__ inline bool window_narrow(const AttnArgs& a) { return a.windowed && a.before + a.after + a.sinks < 64; }
+
+// The rows that see a key of a window: first .. end - 1.
+__device__ __forceinline__ void window_rows(const AttnArgs& a, int nk, int nq, int off, int& first, int& end) {
+  first = a.causal ? max(-off, 0) : a.sinks > 0 ? 0 : max(-off - a.after, 0);
+  end = nk == 0 ? 0 : a.sinks > 0 ? nq : min(nq, nk + a.before - off);
+  first = min(first, max(end, 0));
 }
 // The first row that sees a key, were there any, and the end of the keys that some row sees.
 __device__ __forceinline__ int first_row(const AttnArgs& a, int off) { return a.causal ? max(-off, 0) : 0; }

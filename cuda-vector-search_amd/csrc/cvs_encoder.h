@@ -180,10 +180,15 @@ struct AttnArgs {
   int table_parts;
   int kv_parts;                   // parts of the queries that dk and dv are summed over
   float* part_kv;                 // [kv_parts, 2, batch, lk, k_heads, d] when kv_parts > 1
+  // sliding window: a row at position p sees keys p - before .. p + after (causal: after is 0) and the first `sinks`
+  int windowed, before, after, sinks;  // sinks <= lk
+  int sink_parts;                 // parts of the queries that dk and dv of the first keys are summed over
+  float* part_sinks;              // [sink_parts, 2, batch, sinks, k_heads, d] when sink_parts > 1
 };
 constexpr int kAttnRows = 128;    // query (or key) rows of a workgroup
 int attn_q_parts(const AttnArgs& a, int cus);
 int attn_kv_parts(const AttnArgs& a, int cus);
+int attn_sink_parts(const AttnArgs& a, int cus);
 int attn_splits(const AttnArgs& a, int cus);
 hipError_t launch_attn_forward(const AttnArgs& a, hipStream_t s);
 hipError_t launch_attn_backward(const AttnArgs& a, hipStream_t s);

@@ -208,7 +208,16 @@ int check_heads(const void* p, const int64_t* stride, const char* what) {
   return CVS_OK;
 }
 
-AttnArgs attn_args(const cvs_attention* p) {
+// (positions are below 2^28 + 2^29, query_start being brought to +-2^29: every sum of the kernels' fits an int)
+int check_window(const cvs_attention* p, const cvs_attention_window* w) {
+  if (w == nullptr) return CVS_OK;
+  if (w->before < 0 || w->after < 0 || w->sinks < 0) return fail(CVS_ERR_INVALID, "attention: a window's sizes must not be negative");
+  if (p->q_len >= (1 << 28) || p->k_len >= (1 << 28)) return fail(CVS_ERR_INVALID, "attention: windows take lengths below 2^28");
+  if ((std::min(w->sinks, p->k_len) + 31) / 32 * p->batch * p->heads >= (1 << 23)) return fail(CVS_ERR_INVALID, "attention: too many first keys");
+  return CVS_OK;
+}
+
+AttnArgs attn_args(const cvs_attention* p, const cvs_attention_window* w) {
   AttnArgs a = {};
   a.type = p->type;
   a.batch = (int)p->batch, a.lq = (int)p->q_len, a.lk = (int)p->k_len;
@@ -221,6 +230,13 @@ AttnArgs attn_args(const cvs_attention* p) {
   a.table = p->bias_table;
   a.buckets = (int)p->buckets, a.max_distance = (int)p->max_distance;
   a.splits = 1;
+  if (w != nullptr) {
+    constexpr int64_t kAll = (int64_t)3 << 28;  // no position is further from a key
+    a.windowed = 1;
+    a.before = (int)std::min(w->before, kAll);
+    a.after = a.causal ? 0 : (int)std::min(w->after, kAll);
+    a.sinks = (int)std::min(w->sinks, p->k_len);
+  }
   if (a.table != nullptr) {
     a.one_way = a.causal ? a.buckets : a.buckets / 2;
     const int exact = a.one_way / 2, wide = a.one_way - exact;
@@ -239,8 +255,8 @@ AttnArgs attn_args(const cvs_attention* p) {
 }
 
 struct AttnPlan {
-  int splits = 1, table_parts = 0, kv_parts = 1, q_parts = 1;
-  int64_t part_kv = 0, part_q = 0, part_out = 0, part_ml = 0, delta = 0, part_peak = 0, part_table = 0, bytes = 0;
+  int splits = 1, table_parts = 0, kv_parts = 1, q_parts = 1, sink_parts = 1;
+  int64_t part_sinks = 0, part_kv = 0, part_q = 0, part_out = 0, part_ml = 0, delta = 0, part_peak = 0, part_table = 0, bytes = 0;
 };
 
 AttnPlan plan_attention(const AttnArgs& a, bool backward, int cus) {
@@ -258,6 +274,8 @@ AttnPlan plan_attention(const AttnArgs& a, bool backward, int cus) {
       p.part_table = at, at += up256((int64_t)a.heads * p.table_parts * a.buckets * 4);
     }
     p.kv_parts = rows == 0 || a.lk == 0 ? 1 : attn_kv_parts(a, cus);
+    if (rows > 0 && a.sinks > 0) p.sink_parts = attn_sink_parts(a, cus);
+    if (p.sink_parts > 1) p.part_sinks = at, at += up256((int64_t)p.sink_parts * 2 * a.batch * a.sinks * a.k_heads * a.d * 4);
     if (p.kv_parts > 1) p.part_kv = at, at += up256((int64_t)p.kv_parts * 2 * a.batch * a.lk * a.k_heads * a.d * 4);
   } else {
     p.splits = rows == 0 ? 1 : attn_splits(a, cus);
@@ -268,6 +286,86 @@ AttnPlan plan_attention(const AttnArgs& a, bool backward, int cus) {
   }
   p.bytes = at;
   return p;
+}
+
+int attention_plan(const cvs_attention* p, const cvs_attention_window* w, int backward, int device, int64_t* workspace_bytes) {
+  DevInfo di;
+  int rc = dev_info(device, &di);
+  if (rc == CVS_OK) rc = check_attention(p);
+  if (rc == CVS_OK) rc = check_window(p, w);
+  if (rc == CVS_OK && workspace_bytes != nullptr) *workspace_bytes = plan_attention(attn_args(p, w), backward != 0, di.cus).bytes;
+  return rc;
+}
+
+int attention_forward(const cvs_attention* p, const cvs_attention_window* w, void* out, float* lse, void* workspace,
+                      int64_t workspace_bytes, int device, void* stream) {
+  DevInfo di;
+  int rc = gfx950(device, &di);
+  if (rc == CVS_OK) rc = check_attention(p);
+  if (rc == CVS_OK) rc = check_window(p, w);
+  if (rc != CVS_OK || p->batch == 0 || p->q_len == 0) return rc;
+  if (p->q == nullptr || (p->k_len > 0 && (p->k == nullptr || p->v == nullptr)) || out == nullptr)
+    return fail(CVS_ERR_INVALID, "attention: null pointer");
+  rc = check_heads(p->q, p->q_stride, "q");
+  if (rc == CVS_OK) rc = check_heads(p->k, p->k_stride, "k");
+  if (rc == CVS_OK) rc = check_heads(p->v, p->v_stride, "v");
+  if (rc == CVS_OK && !aligned16(out)) rc = fail(CVS_ERR_INVALID, "out must be 16-byte aligned");
+  if (rc != CVS_OK) return rc;
+  AttnArgs a = attn_args(p, w);
+  const AttnPlan plan = plan_attention(a, false, di.cus);
+  rc = check_workspace(workspace, workspace_bytes, plan.bytes);
+  if (rc != CVS_OK) return rc;
+  DeviceGuard guard(device);
+  if (guard.err != hipSuccess) return hip_fail(guard.err, "hipSetDevice");
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
+  a.out = out, a.lse = lse;
+  a.splits = plan.splits;
+  a.part_out = reinterpret_cast<float*>(ws + plan.part_out);
+  a.part_ml = reinterpret_cast<float*>(ws + plan.part_ml);
+  return done(launch_attn_forward(a, s), "attention launch");
+}
+
+int attention_backward(const cvs_attention* p, const cvs_attention_window* w, const void* dout, const int64_t* dout_stride,
+                       const void* out, const float* lse, void* dq, void* dk, void* dv, void* dbias_table, void* workspace,
+                       int64_t workspace_bytes, int device, void* stream) {
+  DevInfo di;
+  int rc = gfx950(device, &di);
+  if (rc == CVS_OK) rc = check_attention(p);
+  if (rc == CVS_OK) rc = check_window(p, w);
+  if (rc != CVS_OK || p->batch == 0 || (p->q_len == 0 && p->k_len == 0)) return rc;
+  const bool rows = p->q_len > 0, keys = p->k_len > 0;
+  if (dout_stride == nullptr || (rows && (p->q == nullptr || dout == nullptr || out == nullptr || lse == nullptr || dq == nullptr)) ||
+      (keys && (p->k == nullptr || p->v == nullptr || dk == nullptr || dv == nullptr)) ||
+      (p->bias_table != nullptr && dbias_table == nullptr))
+    return fail(CVS_ERR_INVALID, "attention: null pointer");
+  rc = check_heads(p->q, p->q_stride, "q");
+  if (rc == CVS_OK) rc = check_heads(p->k, p->k_stride, "k");
+  if (rc == CVS_OK) rc = check_heads(p->v, p->v_stride, "v");
+  if (rc == CVS_OK) rc = check_heads(dout, dout_stride, "dout");
+  if (rc == CVS_OK && !(aligned16(out) && aligned16(dq) && aligned16(dk) && aligned16(dv)))
+    rc = fail(CVS_ERR_INVALID, "attention: pointers must be 16-byte aligned");
+  if (rc != CVS_OK) return rc;
+  AttnArgs a = attn_args(p, w);
+  const AttnPlan plan = plan_attention(a, true, di.cus);
+  rc = check_workspace(workspace, workspace_bytes, plan.bytes);
+  if (rc != CVS_OK) return rc;
+  DeviceGuard guard(device);
+  if (guard.err != hipSuccess) return hip_fail(guard.err, "hipSetDevice");
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
+  a.out = const_cast<void*>(out), a.lse = const_cast<float*>(lse), a.dout = dout;
+  for (int i = 0; i < 3; ++i) a.dos[i] = dout_stride[i];
+  a.dq = dq, a.dk = dk, a.dv = dv, a.dtable = dbias_table;
+  a.delta = reinterpret_cast<float*>(ws + plan.delta);
+  a.part_peak = reinterpret_cast<float*>(ws + plan.part_peak);
+  a.part_table = reinterpret_cast<float*>(ws + plan.part_table);
+  a.table_parts = plan.table_parts;
+  a.kv_parts = plan.kv_parts, a.q_parts = plan.q_parts, a.sink_parts = plan.sink_parts;
+  a.part_sinks = reinterpret_cast<float*>(ws + plan.part_sinks);
+  a.part_q = reinterpret_cast<float*>(ws + plan.part_q);
+  a.part_kv = reinterpret_cast<float*>(ws + plan.part_kv);
+  return done(launch_attn_backward(a, s), "attention backward launch");
 }
 
 }  // namespace
@@ -598,79 +696,38 @@ int cvs_linear_int8(const void* x, const void* w, const float* w_scales, const v
 }
 
 int cvs_attention_plan(const cvs_attention* p, int backward, int device, int64_t* workspace_bytes) {
-  DevInfo di;
-  int rc = dev_info(device, &di);
-  if (rc == CVS_OK) rc = check_attention(p);
-  if (rc == CVS_OK && workspace_bytes != nullptr) *workspace_bytes = plan_attention(attn_args(p), backward != 0, di.cus).bytes;
-  return rc;
+  return attention_plan(p, nullptr, backward, device, workspace_bytes);
 }
 
 int cvs_attention_forward(const cvs_attention* p, void* out, float* lse, void* workspace, int64_t workspace_bytes,
                           int device, void* stream) {
-  DevInfo di;
-  int rc = gfx950(device, &di);
-  if (rc == CVS_OK) rc = check_attention(p);
-  if (rc != CVS_OK || p->batch == 0 || p->q_len == 0) return rc;
-  if (p->q == nullptr || (p->k_len > 0 && (p->k == nullptr || p->v == nullptr)) || out == nullptr)
-    return fail(CVS_ERR_INVALID, "attention: null pointer");
-  rc = check_heads(p->q, p->q_stride, "q");
-  if (rc == CVS_OK) rc = check_heads(p->k, p->k_stride, "k");
-  if (rc == CVS_OK) rc = check_heads(p->v, p->v_stride, "v");
-  if (rc == CVS_OK && !aligned16(out)) rc = fail(CVS_ERR_INVALID, "out must be 16-byte aligned");
-  if (rc != CVS_OK) return rc;
-  AttnArgs a = attn_args(p);
-  const AttnPlan plan = plan_attention(a, false, di.cus);
-  rc = check_workspace(workspace, workspace_bytes, plan.bytes);
-  if (rc != CVS_OK) return rc;
-  DeviceGuard guard(device);
-  if (guard.err != hipSuccess) return hip_fail(guard.err, "hipSetDevice");
-  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
-  a.out = out, a.lse = lse;
-  a.splits = plan.splits;
-  a.part_out = reinterpret_cast<float*>(ws + plan.part_out);
-  a.part_ml = reinterpret_cast<float*>(ws + plan.part_ml);
-  return done(launch_attn_forward(a, s), "attention launch");
+  return attention_forward(p, nullptr, out, lse, workspace, workspace_bytes, device, stream);
 }
 
 int cvs_attention_backward(const cvs_attention* p, const void* dout, const int64_t* dout_stride, const void* out,
                            const float* lse, void* dq, void* dk, void* dv, void* dbias_table, void* workspace,
                            int64_t workspace_bytes, int device, void* stream) {
-  DevInfo di;
-  int rc = gfx950(device, &di);
-  if (rc == CVS_OK) rc = check_attention(p);
-  if (rc != CVS_OK || p->batch == 0 || (p->q_len == 0 && p->k_len == 0)) return rc;
-  const bool rows = p->q_len > 0, keys = p->k_len > 0;
-  if (dout_stride == nullptr || (rows && (p->q == nullptr || dout == nullptr || out == nullptr || lse == nullptr || dq == nullptr)) ||
-      (keys && (p->k == nullptr || p->v == nullptr || dk == nullptr || dv == nullptr)) ||
-      (p->bias_table != nullptr && dbias_table == nullptr))
-    return fail(CVS_ERR_INVALID, "attention: null pointer");
-  rc = check_heads(p->q, p->q_stride, "q");
-  if (rc == CVS_OK) rc = check_heads(p->k, p->k_stride, "k");
-  if (rc == CVS_OK) rc = check_heads(p->v, p->v_stride, "v");
-  if (rc == CVS_OK) rc = check_heads(dout, dout_stride, "dout");
-  if (rc == CVS_OK && !(aligned16(out) && aligned16(dq) && aligned16(dk) && aligned16(dv)))
-    rc = fail(CVS_ERR_INVALID, "attention: pointers must be 16-byte aligned");
-  if (rc != CVS_OK) return rc;
-  AttnArgs a = attn_args(p);
-  const AttnPlan plan = plan_attention(a, true, di.cus);
-  rc = check_workspace(workspace, workspace_bytes, plan.bytes);
-  if (rc != CVS_OK) return rc;
-  DeviceGuard guard(device);
-  if (guard.err != hipSuccess) return hip_fail(guard.err, "hipSetDevice");
-  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
-  a.out = const_cast<void*>(out), a.lse = const_cast<float*>(lse), a.dout = dout;
-  for (int i = 0; i < 3; ++i) a.dos[i] = dout_stride[i];
-  a.dq = dq, a.dk = dk, a.dv = dv, a.dtable = dbias_table;
-  a.delta = reinterpret_cast<float*>(ws + plan.delta);
-  a.part_peak = reinterpret_cast<float*>(ws + plan.part_peak);
-  a.part_table = reinterpret_cast<float*>(ws + plan.part_table);
-  a.table_parts = plan.table_parts;
-  a.kv_parts = plan.kv_parts, a.q_parts = plan.q_parts;
-  a.part_q = reinterpret_cast<float*>(ws + plan.part_q);
-  a.part_kv = reinterpret_cast<float*>(ws + plan.part_kv);
-  return done(launch_attn_backward(a, s), "attention backward launch");
+  return attention_backward(p, nullptr, dout, dout_stride, out, lse, dq, dk, dv, dbias_table, workspace, workspace_bytes, device,
+                            stream);
+}
+
+int cvs_attention_window_plan(const cvs_attention* p, const cvs_attention_window* w, int backward, int device,
+                              int64_t* workspace_bytes) {
+  if (w == nullptr) return fail(CVS_ERR_INVALID, "attention: null window");
+  return attention_plan(p, w, backward, device, workspace_bytes);
+}
+
+int cvs_attention_window_forward(const cvs_attention* p, const cvs_attention_window* w, void* out, float* lse, void* workspace,
+                                 int64_t workspace_bytes, int device, void* stream) {
+  if (w == nullptr) return fail(CVS_ERR_INVALID, "attention: null window");
+  return attention_forward(p, w, out, lse, workspace, workspace_bytes, device, stream);
+}
+
+int cvs_attention_window_backward(const cvs_attention* p, const cvs_attention_window* w, const void* dout,
+                                  const int64_t* dout_stride, const void* out, const float* lse, void* dq, void* dk, void* dv,
+                                  void* dbias_table, void* workspace, int64_t workspace_bytes, int device, void* stream) {
+  if (w == nullptr) return fail(CVS_ERR_INVALID, "attention: null window");
+  return attention_backward(p, w, dout, dout_stride, out, lse, dq, dk, dv, dbias_table, workspace, workspace_bytes, device, stream);
 }
 
 }  // extern "C"

@@ -181,11 +181,17 @@ class AttentionArgs(ctypes.Structure):
         ("buckets", ctypes.c_int64), ("max_distance", ctypes.c_int64)]
 
 
+class AttentionWindow(ctypes.Structure):
+    """cvs_attention_window (include/cvs.h)."""
+
+    _fields_ = [(n, ctypes.c_int64) for n in ("before", "after", "sinks")]
+
+
 def _bind_encoder(lib: ctypes.CDLL) -> None:
     """Signatures of the text-encoder operators."""
     i64, i32, vp, f64 = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_double
     out = ctypes.POINTER(i64)
-    att = ctypes.POINTER(AttentionArgs)
+    att, win = ctypes.POINTER(AttentionArgs), ctypes.POINTER(AttentionWindow)
     for name, args in {
         "cvs_layer_norm": [vp, vp, vp, i64, i64, i64, f64, i32, vp, vp, vp, i32, vp],
         "cvs_layer_norm_backward_plan": [i64, i64, i32, i32, out],
@@ -204,6 +210,9 @@ def _bind_encoder(lib: ctypes.CDLL) -> None:
         "cvs_attention_plan": [att, i32, i32, out],
         "cvs_attention_forward": [att, vp, vp, vp, i64, i32, vp],
         "cvs_attention_backward": [att, vp, out, vp, vp, vp, vp, vp, vp, vp, i64, i32, vp],
+        "cvs_attention_window_plan": [att, win, i32, i32, out],
+        "cvs_attention_window_forward": [att, win, vp, vp, vp, i64, i32, vp],
+        "cvs_attention_window_backward": [att, win, vp, out, vp, vp, vp, vp, vp, vp, vp, i64, i32, vp],
     }.items():
         fn = getattr(lib, name)
         fn.restype = i32

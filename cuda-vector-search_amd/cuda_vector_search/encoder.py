@@ -9,7 +9,8 @@ these operators.  Each runs hand-written gfx950 kernels (``libcvs_hip.so`` throu
 * ``gated_linear(x, gate, up, ...)``, the gated feed-forward block's two products, activation
   and product;
 * ``attention(q, k, v, ...)``, softmax attention over sequences of differing lengths,
-  causal or not, with shared key heads and a learned bias by relative position;
+  causal or not, with shared key heads, a learned bias by relative position, a sliding window
+  and first keys that stay visible;
 * ``linear_int8(x, values, scales, ...)``, for serving: ``linear`` of a weight that
   ``quantize_rows`` laid out, in products of 8-bit whole numbers.
 
@@ -588,15 +589,34 @@ def _attention_check(q, k, v, bias_table, scale) -> None:
             raise RuntimeError("bias_table must be [buckets, heads]")
 
 
-def _attention_args(q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance):
-    """(AttentionArgs, its _AttentionCall or None, tensors it points into) after the checks."""
+def _window(window, sinks):
+    """The window as _ext.AttentionWindow, or None."""
+    sinks = operator.index(sinks)
+    if window is None:
+        if sinks:
+            raise RuntimeError("sinks need a window (without one every key is visible)")
+        return None
+    try:
+        before, after = window
+    except TypeError:
+        before = after = window
+    before, after = operator.index(before), operator.index(after)
+    if before < 0 or after < 0 or sinks < 0:
+        raise RuntimeError("window and sinks must not be negative")
+    most = 1 << 30  # (a longer one is no different)
+    return _ext.AttentionWindow(min(before, most), min(after, most), min(sinks, most))
+
+
+def _attention_args(q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance, win):
+    """(AttentionArgs, its _AttentionCall or None, tensors it points into) after the checks; win: an
+    _ext.AttentionWindow or None."""
     # values, not tensors that hold them: those are found by identity and may have changed since
     scale = None if scale is None else float(scale)
     causal = bool(causal)
     max_distance = 0 if bias_table is None else operator.index(max_distance)
     try:
         key = (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype, q.device, k.device,
-               v.device, causal, scale, max_distance,
+               v.device, causal, scale, max_distance, None if win is None else bytes(win),
                None if bias_table is None else (bias_table.shape, bias_table.dtype, bias_table.device))
         call = _calls.get(key)
     except (AttributeError, TypeError):  # no tensors: the checks say which
@@ -634,11 +654,14 @@ def _attention_args(q, k, v, bias_table, key_lengths, query_lengths, query_start
     return a, call, hold
 
 
-def _attention_workspace(lib, a, call, backward: bool, q):
+def _attention_workspace(lib, a, win, call, backward: bool, q):
     size = None if call is None else call.bytes[backward]
     if size is None:
         out = _I64(0)
-        _check(lib.cvs_attention_plan(ctypes.byref(a), backward, q.device.index, ctypes.byref(out)))
+        if win is None:
+            _check(lib.cvs_attention_plan(ctypes.byref(a), backward, q.device.index, ctypes.byref(out)))
+        else:
+            _check(lib.cvs_attention_window_plan(ctypes.byref(a), ctypes.byref(win), backward, q.device.index, ctypes.byref(out)))
         size = int(out.value)
         if call is not None:
             call.bytes[backward] = size
@@ -647,7 +670,7 @@ def _attention_workspace(lib, a, call, backward: bool, q):
 
 @_bare
 def attention_forward(q, k, v, bias_table=None, key_lengths=None, query_lengths=None, query_start=None,
-                      causal: bool = False, scale=None, max_distance: int = 128, lse: bool = True):
+                      causal: bool = False, scale=None, max_distance: int = 128, lse: bool = True, window=None, sinks: int = 0):
     """(out, lse) of softmax attention: ``q`` [batch, q_len, heads, width], ``k`` and ``v``
     [batch, k_len, k_heads, width] (any strides whose rows of ``width`` are contiguous), out like q,
     lse float32 [batch, heads, q_len] (natural logarithm; None when not asked for).
@@ -663,24 +686,32 @@ def attention_forward(q, k, v, bias_table=None, key_lengths=None, query_lengths=
     Buckets: half of a direction's for one distance each, the others evenly in the
     logarithm up to ``max_distance`` (the last one also holds what is further); causal: all
     buckets for the past, else the first half for keys at or before the row.
+
+    ``window``, a number or (before, after): of the keys above, a row at position p sees only those from p - before to
+    p + after (one number: both; causal: to p) and the first ``sinks`` of the sequence.
     """
-    a, call, hold = _attention_args(q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance)
+    win = _window(window, sinks)
+    a, call, hold = _attention_args(q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance, win)
     lib = _library()
     out = _new(q)
     sums = q.new_empty((a.batch, a.heads, a.q_len), dtype=torch.float32) if lse else None
     dev = q.device.index
-    ws = _attention_workspace(lib, a, call, False, q)
-    _check(lib.cvs_attention_forward(ctypes.byref(a), out.data_ptr(), _ptr(sums), _ptr(ws), 0 if ws is None else ws.numel(),
-                                     dev, _ext.raw_stream(dev)))
+    ws = _attention_workspace(lib, a, win, call, False, q)
+    rest = (out.data_ptr(), _ptr(sums), _ptr(ws), 0 if ws is None else ws.numel(), dev, _ext.raw_stream(dev))
+    if win is None:
+        _check(lib.cvs_attention_forward(ctypes.byref(a), *rest))
+    else:
+        _check(lib.cvs_attention_window_forward(ctypes.byref(a), ctypes.byref(win), *rest))
     return out, sums
 
 
 @_bare
 def attention_backward(dout, q, k, v, out, lse, bias_table=None, key_lengths=None, query_lengths=None, query_start=None,
-                       causal: bool = False, scale=None, max_distance: int = 128):
+                       causal: bool = False, scale=None, max_distance: int = 128, window=None, sinks: int = 0):
     """(dq, dk, dv, dbias_table) of ``attention_forward`` for ``dout``, from its ``out`` and ``lse``;
     dbias_table is None without a table."""
-    a, call, hold = _attention_args(q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance)
+    win = _window(window, sinks)
+    a, call, hold = _attention_args(q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance, win)
     _tensor(dout, "dout", q, q.shape)
     _tensor(out, "out", q, q.shape)
     lse = _stats(lse, "lse", q, (a.batch, a.heads, a.q_len))
@@ -692,32 +723,39 @@ def attention_backward(dout, q, k, v, out, lse, bias_table=None, key_lengths=Non
     if a.batch == 0 or (a.q_len == 0 and a.k_len == 0):
         return dq, dk, dv, None if dtable is None else dtable.zero_()
     dev = q.device.index
-    ws = _attention_workspace(lib, a, call, True, q)
-    _check(lib.cvs_attention_backward(ctypes.byref(a), dout.data_ptr(), dout_stride, out.data_ptr(), lse.data_ptr(),
-                                      dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dtable), _ptr(ws),
-                                      0 if ws is None else ws.numel(), dev, _ext.raw_stream(dev)))
+    ws = _attention_workspace(lib, a, win, call, True, q)
+    rest = (dout.data_ptr(), dout_stride, out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+            _ptr(dtable), _ptr(ws), 0 if ws is None else ws.numel(), dev, _ext.raw_stream(dev))
+    if win is None:
+        _check(lib.cvs_attention_backward(ctypes.byref(a), *rest))
+    else:
+        _check(lib.cvs_attention_window_backward(ctypes.byref(a), ctypes.byref(win), *rest))
     return dq, dk, dv, dtable
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance):
-        out, lse = attention_forward.inner(q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance)
+    def forward(ctx, q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance, window, sinks):
+        if window is not None:  # (as it is now, for the backward pass too)
+            win = _window(window, sinks)
+            window, sinks = (win.before, win.after), win.sinks
+        out, lse = attention_forward.inner(q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance,
+                                           True, window, sinks)
         ctx.save_for_backward(q, k, v, out, lse, bias_table, key_lengths, query_lengths, query_start)
-        ctx.more = (causal, scale, max_distance)
+        ctx.more = (causal, scale, max_distance, window, sinks)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, *masks = ctx.saved_tensors
-        return (*attention_backward.inner(dout, q, k, v, out, lse, *masks, *ctx.more), None, None, None, None, None, None)
+        return (*attention_backward.inner(dout, q, k, v, out, lse, *masks, *ctx.more), None, None, None, None, None, None, None, None)
 
 
 def attention(q, k, v, bias_table=None, key_lengths=None, query_lengths=None, query_start=None, causal: bool = False,
-              scale=None, max_distance: int = 128):
+              scale=None, max_distance: int = 128, window=None, sinks: int = 0):
     """Softmax attention, [batch, q_len, heads, width]; arguments as ``attention_forward``'s."""
     args = (q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance)
     if _through_autograd(q, k, v, bias_table):
-        return _Attention.apply(*args)
-    return attention_forward.inner(*args, lse=False)[0]
+        return _Attention.apply(*args, window, sinks)
+    return attention_forward.inner(*args, lse=False, window=window, sinks=sinks)[0]

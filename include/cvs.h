@@ -399,6 +399,24 @@ int cvs_attention_backward(const cvs_attention* p, const void* dout, const int64
                            const float* lse, void* dq, void* dk, void* dv, void* dbias_table, void* workspace,
                            int64_t workspace_bytes, int device, void* stream);
 
+/*
+ * Attention with a sliding window: of the keys that cvs_attention leaves, a row at position p sees those
+ * from p - before to p + after (`after` is nothing where causal) and the first `sinks` of the sequence.  A
+ * row that the window leaves nothing has output 0 and log sum -inf; keys that no row sees reach no
+ * result.  q_len and k_len are below 2^28.  Everything else is as in the calls above.
+ */
+typedef struct cvs_attention_window {
+  int64_t before, after, sinks;
+} cvs_attention_window;
+
+int cvs_attention_window_plan(const cvs_attention* p, const cvs_attention_window* w, int backward, int device,
+                              int64_t* workspace_bytes);
+int cvs_attention_window_forward(const cvs_attention* p, const cvs_attention_window* w, void* out, float* lse, void* workspace,
+                                 int64_t workspace_bytes, int device, void* stream);
+int cvs_attention_window_backward(const cvs_attention* p, const cvs_attention_window* w, const void* dout,
+                                  const int64_t* dout_stride, const void* out, const float* lse, void* dq, void* dk, void* dv,
+                                  void* dbias_table, void* workspace, int64_t workspace_bytes, int device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

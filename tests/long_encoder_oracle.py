@@ -108,3 +108,72 @@ def linear_int8_bounds(x, values, scales, b, act, res, dtype):
     bias = torch.zeros(()).double() if b is None else b
     slip = 6 * o.F32 * ((z - bias).abs() + bias.abs())
     return (o.U[dtype] * y.abs() + o.TINY[dtype] + 1.13 * slip + 1e-6 * (1 + o.activate(z, act).abs() if act else 0) + 2 * o.F32 * y.abs())
+
+
+# ---- attention with a window ------------------------------------------------------------
+
+
+def window_seen(b, lq, lk, before, after, sinks, causal=False, key_lengths=None, query_lengths=None, query_start=None):
+    """(positions key - row [b, lq, lk], which pairs are seen)."""
+    start = torch.full((b,), lk - lq) if query_start is None else query_start.long().cpu()
+    j = torch.arange(lk)
+    rel = j[None, None, :] - torch.arange(lq)[None, :, None] - start[:, None, None]
+    seen = ((rel >= -before) & (rel <= after)) | (j < sinks)
+    if causal:
+        seen = seen & (rel <= 0)
+    if key_lengths is not None:
+        seen = seen & (j[None, :] < key_lengths.long().cpu()[:, None])[:, None, :]
+    if query_lengths is not None:
+        seen = seen & (torch.arange(lq)[None, :] < query_lengths.long().cpu()[:, None])[:, :, None]
+    return rel, seen
+
+
+def window_attention(q, k, v, do, scale, dtype, before, after, sinks, table=None, max_distance=128, causal=False, own_delta=False,
+                     **masks):
+    """{"out", "lse", "dq", "dk", "dv", "dtable"}: (value, bound) of each, by the definition and its formulas.
+
+    Bounds as encoder_oracle's: delta is off by the rounding of ``out``, or (``own_delta``) by its own fp32 sums only."""
+    (b, lq, h, _), lk, hk = q.shape, k.shape[1], k.shape[2]
+    rel, seen = window_seen(b, lq, lk, before, after, sinks, causal, **masks)
+    keys, rows = seen.any(1)[:, :, None, None], seen.any(2)[:, :, None, None]
+    zero = torch.zeros((), dtype=torch.float64)
+    k, v = (torch.where(keys, t, zero).repeat_interleave(h // hk, 2).transpose(1, 2) for t in (k, v))
+    q, g = (torch.where(rows, t, zero).transpose(1, 2) for t in (q, do))
+    s = torch.matmul(q, k.transpose(2, 3).contiguous()) * scale
+    found = None
+    if table is not None:
+        found = o.bucket(rel, table.shape[0], causal, max_distance)
+        s = s + table[found].permute(0, 3, 1, 2)
+    s = s.masked_fill(~seen[:, None], -math.inf)
+    lse = torch.logsumexp(s, 3)
+    none = torch.isinf(lse)
+    p = torch.exp(s - torch.where(none, zero, lse)[..., None])
+    u, tiny = o.U[dtype], o.TINY[dtype]
+    out = torch.matmul(p, v)
+    bound = u * out.abs() + tiny + (u + o.SCORE) * torch.matmul(p, v.abs()) + tiny * v.abs().sum(2, keepdim=True)
+    res = {"out": (out.transpose(1, 2), bound.transpose(1, 2)),
+           "lse": (lse, 2.0**-17 + 2.0**-20 * torch.where(none, zero, lse).abs())}
+    dp = torch.matmul(g, v.transpose(2, 3).contiguous())
+    ds = p * (dp - (p * dp).sum(3, keepdim=True))
+    size = torch.matmul(g.abs(), v.abs().transpose(2, 3).contiguous())
+    if own_delta:
+        slip = 2.0**-20 * (p * size).sum(3, keepdim=True)
+    else:
+        slip = u * (g * out).abs().sum(3, keepdim=True) + tiny * g.abs().sum(3, keepdim=True)
+    off = o.SCORE * ds.abs() + p * (slip + 2.0**-20 * size)  # of ds, before it is rounded
+    inner, round_p = off + u * ds.abs() + tiny, o.SCORE * p + u * p + tiny
+
+    def share(t):
+        return t.transpose(1, 2).reshape(b, lk, hk, h // hk, -1).sum(3)
+
+    def t23(t):
+        return t.transpose(2, 3).contiguous()
+
+    for name, value, more in (("dq", (torch.matmul(ds, k) * scale).transpose(1, 2), scale * torch.matmul(inner, k.abs()).transpose(1, 2)),
+                              ("dk", share(torch.matmul(t23(ds), q)) * scale, scale * share(torch.matmul(t23(inner), q.abs()))),
+                              ("dv", share(torch.matmul(t23(p), g)), share(torch.matmul(t23(round_p), g.abs())))):
+        res[name] = value, u * value.abs() + tiny + more
+    if table is not None:
+        dt = o._by_bucket(ds, found, table)
+        res["dtable"] = dt, u * dt.abs() + tiny + o._by_bucket(off, found, table)
+    return res
