@@ -19,7 +19,8 @@ namespace {
 template <class T, int WM, int WN, int BM, int BN, int RING, int WGS, bool NS, int KIND>
 __global__ __launch_bounds__(64 * WM * WN, WGS) void gemm_kind_kernel(GemmKindArgs a) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[gemm_lds<WM, WN, BM, BN, RING>()];
-  gemm_tile<T, WM, WN, BM, BN, RING, false, NS, KIND>(a, blockIdx.x, smem);
+  __shared__ __attribute__((aligned(16))) float vectors[gemm_vectors<KIND, WM * BM * 32, WN * BN * 16>()];
+  gemm_tile<T, WM, WN, BM, BN, RING, false, NS, KIND>(a, blockIdx.x, smem, vectors);
 }
 
 // Adds the parts of a split reduction, in order, and finishes: 8 columns a thread.
@@ -31,7 +32,7 @@ __global__ __launch_bounds__(kBlock) void gated_join_kernel(GemmKindArgs a) {
   if (i >= a.m) return;
   const int j = (int)(at - i * pieces) * 8;
   const int64_t plane = (int64_t)a.m * a.n * 2;
-  float z[2][8], h[8];
+  float z[2][8], h[8], bias[2][8];
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -45,7 +46,14 @@ __global__ __launch_bounds__(kBlock) void gated_join_kernel(GemmKindArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) z[u][e] += lo[e], z[u][4 + e] += hi[e];
     }
-  finish_gated8<T>(a, j, z[0], z[1], h);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const T* from = (const T*)(u == 0 ? a.bias : a.bias2);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bias[u][e] = 0.f;
+    if (from != nullptr) load8(from + j, bias[u]);
+  }
+  finish_gated8(a.act, bias[0], bias[1], z[0], z[1], h);
   if (a.pre != nullptr) {
     store8((T*)a.pre + i * 2 * a.n + j, z[0]);
     store8((T*)a.pre + i * 2 * a.n + a.n + j, z[1]);

@@ -186,38 +186,35 @@ __device__ __forceinline__ void gate8(float* z, int act) {
   }
 }
 
-// 8 neighbouring sums of both factors, at column j, in place: biases added (what pre receives); h: the output.
-template <class T>
-__device__ __forceinline__ void finish_gated8(const GemmKindArgs& a, int j, float* gate, float* up, float* h) {
-  float b[8];
-  if (a.bias != nullptr) {
-    load8((const T*)a.bias + j, b);
+// 8 neighbouring sums of both factors in place, with their biases (what pre receives); h: the output.
+__device__ __forceinline__ void finish_gated8(int act, const float* bias, const float* bias2, float* gate, float* up, float* h) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) gate[e] += b[e];
-  }
-  if (a.bias2 != nullptr) {
-    load8((const T*)a.bias2 + j, b);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) up[e] += b[e];
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) h[e] = gate[e];
-  gate8(h, a.act);
+  for (int e = 0; e < 8; ++e) gate[e] += bias[e], up[e] += bias2[e], h[e] = gate[e];
+  gate8(h, act);
 #pragma unroll
   for (int e = 0; e < 8; ++e) h[e] *= up[e];
 }
 
-// 8 neighbouring whole sums of row i, columns j .. j + 7, in units of both scales (one after the other: their
-// product alone could leave fp32's range).
-__device__ __forceinline__ void unscale8(const GemmKindArgs& a, int i, int j, float* z) {
-  const float r = a.row_scale[i];
-  const f32x4 lo = *reinterpret_cast<const f32x4*>(a.col_scale + j), hi = *reinterpret_cast<const f32x4*>(a.col_scale + j + 4);
+// 8 neighbouring whole sums in units of both scales (one after the other: their product alone could leave fp32's
+// range), with the bias, through the activation.
+__device__ __forceinline__ void finish_int8(int act, float row, const float* col, const float* bias, float* z) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    z[e] = z[e] * r * lo[e];
-    z[4 + e] = z[4 + e] * r * hi[e];
-  }
+  for (int e = 0; e < 8; ++e) z[e] = fmaf(z[e] * col[e], row, bias[e]);
+  activate8(z, act);
 }
+
+// 8 floats of LDS or memory, 16-byte aligned.
+__device__ __forceinline__ void take8(const float* p, float* f) {
+  const f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] = lo[e], f[4 + e] = hi[e];
+}
+
+// What a tile's epilogue takes of its rows and columns, in LDS: gated, both biases; int8, the columns' bias and
+// scales, the rows' scales.  Loaded before the products, whose time hides it (block by block in the epilogue, each
+// waited for, int8's 32768 x 4096, k = 1024 took 205 us instead of 177).
+template <int KIND, int TM, int TN>
+constexpr int gemm_vectors() { return KIND == kGated ? 2 * TN : KIND == kInt8 ? 2 * TN + TM : 4; }
 
 // Workgroups of a product: tiles rounded up to a multiple of 8, times the parts of the reduction.
 __host__ __device__ inline int gemm_grid(const GemmArgs& a, int tm, int tn) {
@@ -228,8 +225,9 @@ template <int WM, int WN, int BM, int BN, int RING>
 constexpr int gemm_lds() { return RING * (WM * BM + WN * BN) * 32 * kDepth * 2; }
 
 // Workgroup `id` of a product: WM x WN waves of BM x BN blocks of 32 x 32, RING stages in LDS (smem).
+// (vectors: gemm_vectors floats of LDS of the gated and int8 kinds.)
 template <class T, int WM, int WN, int BM, int BN, int RING, bool MS, bool NS, int KIND = kPlain>
-__device__ __forceinline__ void gemm_tile(const typename Operand<T, KIND>::Args& a, int id, unsigned char* smem) {
+__device__ __forceinline__ void gemm_tile(const typename Operand<T, KIND>::Args& a, int id, unsigned char* smem, float* vectors = nullptr) {
   static_assert((KIND != kGated || (BN % 2 == 0 && !MS && !NS)) && (KIND != kInt8 || (!MS && !NS)), "kinds' operands");
   constexpr int FN = KIND == kGated ? BN / 2 : BN;  // blocks of output columns of a wave
   constexpr int W = WM * WN, TM = WM * BM * 32, TN = WN * FN * 32, NROWS = WN * BN * 32;
@@ -259,6 +257,20 @@ __device__ __forceinline__ void gemm_tile(const typename Operand<T, KIND>::Args&
   const int rows = min(kRows, tiles_m - strip * kRows);
   const int m0 = (strip * kRows + in_strip % rows) * TM, n0 = in_strip / rows * TN;
 
+  // what the epilogue takes (a column, and a row, a thread): under way during the products, then to LDS
+  static_assert(TN <= 64 * W && TM <= 64 * W, "a column and a row a thread");
+  float of_col[2] = {0.f, 0.f}, of_row = 0.f;
+  if constexpr (KIND == kGated || KIND == kInt8) {
+    const int j = min(n0 + min(tid, TN - 1), a.n - 1);
+    if (a.bias != nullptr) of_col[0] = (float)((const T*)a.bias)[j];
+    if constexpr (KIND == kGated) {
+      if (a.bias2 != nullptr) of_col[1] = (float)((const T*)a.bias2)[j];
+    } else {
+      of_col[1] = a.col_scale[j];
+      of_row = a.row_scale[min(m0 + min(tid, TM - 1), a.m - 1)];
+    }
+  }
+
   const int part_stages = (a.k + kDepth - 1) / kDepth, stages = KIND == kTwoParts ? 2 * part_stages : part_stages;
   const int s_begin = (int)((int64_t)stages * split / a.splits);
   const int s_end = (int)((int64_t)stages * (split + 1) / a.splits);
@@ -284,7 +296,7 @@ __device__ __forceinline__ void gemm_tile(const typename Operand<T, KIND>::Args&
   for (int j = 0; j < LM; ++j) place(j, MS, a.ldm, m0, a.m, &vm[j], &km[j]);
 #pragma unroll
   for (int j = 0; j < LN; ++j) {
-    if constexpr (KIND == kGated) {  // line 32 u + r: row r of the wave's block u / BN, of N's FN blocks or N2's
+    if constexpr (KIND == kGated) {  // line 32 u + r: row r of wave column u / BN's block u % BN, of FN of N's, then of N2's
       const int line = (wave + W * j) * 8 + (lane >> 3), u = line >> 5;
       const int row = (u / BN * FN + u % BN % FN) * 32 + (line & 31);
       kn[j] = ((lane & 7) ^ piece_swizzle(line)) * 8;
@@ -439,7 +451,53 @@ __device__ __forceinline__ void gemm_tile(const typename Operand<T, KIND>::Args&
     }
   }
 
+  if constexpr (KIND == kGated || KIND == kInt8) {
+    if (a.splits == 1) {
+      if (tid < TN) vectors[tid] = of_col[0], vectors[TN + tid] = of_col[1];
+      if (KIND == kInt8 && tid < TM) vectors[2 * TN + tid] = of_row;
+      __syncthreads();
+    }
+  }
+
   // Lane: a row of the output, two times 8 neighbouring columns of each block.
+  if (KIND == kInt8 && a.splits == 1) {
+    typename Frag<T>::V res[BM][FN][2];  // all of them under way together
+    if (a.residual != nullptr) {
+#pragma unroll
+      for (int i = 0; i < BM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            res[i][j][h] = *reinterpret_cast<const typename Frag<T>::V*>(
+                (const T*)a.residual + (int64_t)min(m0 + (wm * BM + i) * 32 + l32, a.m - 1) * a.ld_res + min(n0 + (wn * FN + j) * 32 + 16 * h + 8 * g, a.n - 8));
+    }
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      float col[16], bias[16];
+      const int at = (wn * FN + j) * 32 + 8 * g;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        take8(vectors + at + 16 * h, bias + 8 * h);
+        take8(vectors + TN + at + 16 * h, col + 8 * h);
+      }
+#pragma unroll
+      for (int i = 0; i < BM; ++i) {
+        const float row = vectors[2 * TN + (wm * BM + i) * 32 + l32];
+        float z[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z[e] = (float)acc[i][j][e];
+        finish_int8(a.act, row, col, bias, z);
+        finish_int8(a.act, row, col + 8, bias + 8, z + 8);
+        if (a.residual != nullptr) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) z[e] += (float)res[i][j][e >> 3][e & 7];
+        }
+        store_block((T*)a.out, a.n, a.m, a.n, m0 + (wm * BM + i) * 32, n0 + (wn * FN + j) * 32, z, z + 8);
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < BM; ++i) {
     const int row0 = m0 + (wm * BM + i) * 32, row = row0 + l32;
@@ -469,8 +527,14 @@ __device__ __forceinline__ void gemm_tile(const typename Operand<T, KIND>::Args&
         float gate[16], up[16], h[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) gate[e] = acc[i][j][e], up[e] = acc[i][j + FN][e];
-        finish_gated8<T>(a, min(col, a.n - 8), gate, up, h);
-        finish_gated8<T>(a, min(col + 16, a.n - 8), gate + 8, up + 8, h + 8);
+        float bias[16], bias2[16];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          take8(vectors + (wn * FN + j) * 32 + 8 * g + 16 * u, bias + 8 * u);
+          take8(vectors + TN + (wn * FN + j) * 32 + 8 * g + 16 * u, bias2 + 8 * u);
+        }
+        finish_gated8(a.act, bias, bias2, gate, up, h);
+        finish_gated8(a.act, bias + 8, bias2 + 8, gate + 8, up + 8, h + 8);
         if (a.pre != nullptr) {
           store_block((T*)a.pre, 2 * (int64_t)a.n, a.m, a.n, row0, col0, gate, gate + 8);
           store_block((T*)a.pre + a.n, 2 * (int64_t)a.n, a.m, a.n, row0, col0, up, up + 8);
@@ -482,10 +546,6 @@ __device__ __forceinline__ void gemm_tile(const typename Operand<T, KIND>::Args&
         for (int e = 0; e < 16; ++e) z[e] = (float)acc[i][j][e];
         // rows and columns past the edge: those of the last ones again, not stored
         const int r = min(row, a.m - 1);
-        if constexpr (KIND == kInt8) {
-          unscale8(a, r, min(col, a.n - 8), z);
-          unscale8(a, r, min(col + 16, a.n - 8), z + 8);
-        }
         finish8<T>(a, r, min(col, a.n - 8), z, pre);
         finish8<T>(a, r, min(col + 16, a.n - 8), z + 8, pre + 8);
         if (a.pre != nullptr) store_block((T*)a.pre, a.n, a.m, a.n, row0, col0, pre, pre + 8);

@@ -146,7 +146,8 @@ void quantize(const QuantArgs& a, hipStream_t s) {
 template <class T, int WM, int WN, int BM, int BN, int RING, int WGS>
 __global__ __launch_bounds__(64 * WM * WN, WGS) void gemm_int8_kernel(GemmKindArgs a) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[gemm_lds<WM, WN, BM, BN, RING>()];
-  gemm_tile<T, WM, WN, BM, BN, RING, false, false, kInt8>(a, blockIdx.x, smem);
+  __shared__ __attribute__((aligned(16))) float vectors[gemm_vectors<kInt8, WM * BM * 32, WN * BN * 32>()];
+  gemm_tile<T, WM, WN, BM, BN, RING, false, false, kInt8>(a, blockIdx.x, smem, vectors);
 }
 
 // Adds the parts of a split reduction and finishes: 8 columns a thread.
@@ -164,11 +165,17 @@ __global__ __launch_bounds__(kBlock) void int8_join_kernel(GemmKindArgs a) {
     lo += *reinterpret_cast<const i32x4*>(p);
     hi += *reinterpret_cast<const i32x4*>(p + 4);
   }
-  float z[8], pre[8];
+  float z[8], col[8], more[8];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) z[e] = (float)lo[e], z[4 + e] = (float)hi[e];
-  unscale8(a, (int)i, j, z);
-  finish8<T>(a, (int)i, j, z, pre);
+  for (int e = 0; e < 4; ++e) z[e] = (float)lo[e], z[4 + e] = (float)hi[e], more[e] = more[4 + e] = 0.f;
+  take8(a.col_scale + j, col);
+  if (a.bias != nullptr) load8((const T*)a.bias + j, more);
+  finish_int8(a.act, a.row_scale[i], col, more, z);
+  if (a.residual != nullptr) {
+    load8((const T*)a.residual + i * a.ld_res + j, more);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] += more[e];
+  }
   store8((T*)a.out + i * a.n + j, z);
 }
 
