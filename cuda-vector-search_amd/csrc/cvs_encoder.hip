@@ -161,8 +161,9 @@ struct Int8Plan {
 };
 
 Int8Plan plan_linear_int8(int64_t m, int64_t k, int64_t n, int cus) {
-  Int8Plan p;
+  Int8Plan p = {};
   p.product = plan_int8(m, n, k, cus);
+  if (int8_few_rows(m, k)) return p;
   int64_t at = 0;
   p.values = at, at += up256(m * k);
   p.scales = at, at += up256(m * 4);
@@ -681,17 +682,18 @@ int cvs_linear_int8(const void* x, const void* w, const float* w_scales, const v
   if (guard.err != hipSuccess) return hip_fail(guard.err, "hipSetDevice");
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
+  GemmKindArgs a = {};
+  a.type = type, a.m = (int)m, a.n = (int)n, a.N = w, a.col_scale = w_scales;
+  a.bias = bias, a.residual = residual, a.ld_res = residual_stride, a.act = act, a.out = y;
+  if (int8_few_rows(m, k)) return done(launch_int8_rows(a, x, x_stride, (int)k, s), "linear int8 launch");
   QuantArgs q = {};
   q.type = type, q.n = m, q.d = (int)k, q.x = x, q.x_stride = x_stride;
   q.values = reinterpret_cast<signed char*>(ws + p.values), q.scales = reinterpret_cast<float*>(ws + p.scales);
   hipError_t e = launch_quantize(q, s);
   if (e != hipSuccess) return hip_fail(e, "linear int8 launch");
-  GemmKindArgs a = {};
-  a.type = type, a.m = (int)m, a.n = (int)n, a.k = (int)(k / 2);
-  a.M = q.values, a.ldm = k / 2, a.N = w, a.ldn = k / 2;
-  a.row_scale = q.scales, a.col_scale = w_scales;
-  a.bias = bias, a.residual = residual, a.ld_res = residual_stride, a.act = act;
-  a.out = y, a.partial = reinterpret_cast<float*>(ws + p.gemm), a.splits = p.product.splits;
+  a.k = (int)(k / 2), a.M = q.values, a.ldm = k / 2, a.ldn = k / 2;
+  a.row_scale = q.scales;
+  a.partial = reinterpret_cast<float*>(ws + p.gemm), a.splits = p.product.splits;
   return done(launch_int8(a, p.product, s), "linear int8 launch");
 }
 

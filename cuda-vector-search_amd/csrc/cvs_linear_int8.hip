@@ -143,6 +143,121 @@ void quantize(const QuantArgs& a, hipStream_t s) {
     hipLaunchKernelGGL(quantize_long_kernel<T>, dim3((unsigned)a.n), block, 0, s, a);
 }
 
+// Few rows (single tokens, a query), one launch: a workgroup has 32 columns of the weight, its waves a quarter of
+// their depth each, straight from memory to the matrix cores, and takes all rows in whole numbers itself, while the
+// weight is on its way.  Bound by latency: a launch, the rows, the weight (loaded together), and the waves' join.
+constexpr int kFewRows = 32;         // columns of a block
+constexpr int kFewBytes = 60 << 10;  // of LDS for the rows: rows times depth
+
+// Bytes of LDS between rows: depth padded to whole blocks of 128 (four waves' 32), and 16 so that rows start in other banks.
+__host__ __device__ inline int few_stride(int d) { return (d + 127) / 128 * 128 + 16; }
+
+template <class T>
+__global__ __launch_bounds__(kBlock) void int8_rows_kernel(GemmKindArgs a, const void* x, int64_t x_stride, int d) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char rows[];  // [m][few_stride]; then the waves' sums
+  __shared__ float scale[kFewRows];
+  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int stride = few_stride(d), n0 = blockIdx.x * 32;
+  const int steps = (d + 127) / 128;  // blocks of 32 values of each wave
+  constexpr int AHEAD = 8;            // the weight's first loads, under way before the rows are looked at
+  const unsigned char* w = (const unsigned char*)a.N + (int64_t)min(n0 + tile_row(l32), a.n - 1) * d;
+  auto weight = [&](int s) -> i32x4 {
+    const int c = (s * 4 + wave) * 32 + 16 * g;
+    i32x4 v = {0, 0, 0, 0};
+    if (c < d) v = *reinterpret_cast<const i32x4*>(w + c);
+    return v;
+  };
+  i32x4 first[AHEAD];
+#pragma unroll
+  for (int s = 0; s < AHEAD; ++s) first[s] = s < steps ? weight(s) : i32x4{0, 0, 0, 0};
+
+  // this wave's rows, every fourth: their loads go together (and again where a row is longer than a wave)
+  constexpr int R = kFewRows / 4;
+  u32x4 lo[R], hi[R];
+  auto load = [&](int c) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      lo[r] = hi[r] = u32x4{0, 0, 0, 0};
+      if (wave + 4 * r < a.m && c < d) {
+        const T* row = (const T*)x + (wave + 4 * r) * x_stride + c;
+        lo[r] = *reinterpret_cast<const u32x4*>(row);
+        hi[r] = *reinterpret_cast<const u32x4*>(row + 8);
+      }
+    }
+  };
+  u16x2 top[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) top[r] = u16x2{0, 0};
+  for (int c = lane * 16; c < d + lane * 16; c += 1024) {
+    load(c);
+#pragma unroll
+    for (int r = 0; r < R; ++r) top[r] = top_of(hi[r], top_of(lo[r], top[r]));
+  }
+  RowUnit unit[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    uint32_t bits = max((uint32_t)top[r][0], (uint32_t)top[r][1]);
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) bits = max(bits, (uint32_t)__shfl_xor((int)bits, s));
+    unit[r] = RowUnit::of<T>(bits);
+    if (lane == 0 && wave + 4 * r < a.m) scale[wave + 4 * r] = unit[r].scale;
+  }
+  for (int c = lane * 16; c < stride - 16 + lane * 16; c += 1024) {
+    if (d > 1024) load(c);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (wave + 4 * r < a.m && c < stride - 16)
+        *reinterpret_cast<u32x4*>(rows + (wave + 4 * r) * stride + c) = unit[r].whole16<T>(lo[r], hi[r]);
+  }
+  __syncthreads();
+
+  i32x16 sum;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) sum[e] = 0;
+  const unsigned char* from = rows + min(l32, a.m - 1) * stride + wave * 32 + 16 * g;
+  auto multiply = [&](int s, i32x4 v) {
+    sum = __builtin_amdgcn_mfma_i32_32x32x32_i8(v, *reinterpret_cast<const i32x4*>(from + s * 128), sum, 0, 0, 0);
+  };
+#pragma unroll
+  for (int s = 0; s < AHEAD; ++s)
+    if (s < steps) multiply(s, first[s]);
+  for (int s = AHEAD; s < steps; s += AHEAD) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) first[u] = s + u < steps ? weight(s + u) : i32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (s + u < steps) multiply(s + u, first[u]);
+  }
+  __syncthreads();  // the rows have been read
+  // lane: row l32's columns 8 g .. 8 g + 7 and 16 + those
+  i32x4* sums = reinterpret_cast<i32x4*>(rows);  // [wave][16-byte piece][lane]
+#pragma unroll
+  for (int q = 0; q < 4; ++q) sums[(wave * 4 + q) * 64 + lane] = i32x4{sum[4 * q], sum[4 * q + 1], sum[4 * q + 2], sum[4 * q + 3]};
+  __syncthreads();
+  // 8 columns a thread: 128 threads
+  const int half = threadIdx.x >> 6 & 1, i = l32, j = n0 + 16 * half + 8 * g;
+  if (threadIdx.x >= 128 || i >= a.m || j >= a.n) return;
+  float z[8], col[8], more[8];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    i32x4 t = sums[(2 * half + q) * 64 + lane];
+#pragma unroll
+    for (int v = 1; v < 4; ++v) t += sums[(v * 4 + 2 * half + q) * 64 + lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[4 * q + e] = (float)t[e], more[4 * q + e] = 0.f;
+  }
+  take8(a.col_scale + j, col);
+  if (a.bias != nullptr) load8((const T*)a.bias + j, more);
+  finish_int8(a.act, scale[i], col, more, z);
+  if (a.residual != nullptr) {
+    load8((const T*)a.residual + (int64_t)i * a.ld_res + j, more);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] += more[e];
+  }
+  store8((T*)a.out + (int64_t)i * a.n + j, z);
+}
+
 template <class T, int WM, int WN, int BM, int BN, int RING, int WGS>
 __global__ __launch_bounds__(64 * WM * WN, WGS) void gemm_int8_kernel(GemmKindArgs a) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[gemm_lds<WM, WN, BM, BN, RING>()];
@@ -215,6 +330,18 @@ hipError_t launch_quantize(const QuantArgs& a, hipStream_t s) {
 GemmPlan plan_int8(int64_t m, int64_t n, int64_t k, int cus) {
   static constexpr TileChoice kTiles[] = {{256, 256, 1, 512, 1.8}, {256, 192, 1, 512, 1.7}, {128, 128, 2, 256, 1.2}, {64, 64, 3, 256, 0.9}};
   return plan_tiles(kTiles, 4, m, n, (k / 2 + kDepth - 1) / kDepth, 1, cus);
+}
+
+bool int8_few_rows(int64_t m, int64_t k) { return m <= kFewRows && m * few_stride((int)k) <= kFewBytes; }
+
+hipError_t launch_int8_rows(const GemmKindArgs& a, const void* x, int64_t x_stride, int d, hipStream_t s) {
+  const dim3 grid((unsigned)((a.n + 31) / 32)), block(kBlock);
+  const size_t lds = std::max(a.m * few_stride(d), 4 * 4096);
+  if (a.type == kF16)
+    hipLaunchKernelGGL(int8_rows_kernel<_Float16>, grid, block, lds, s, a, x, x_stride, d);
+  else
+    hipLaunchKernelGGL(int8_rows_kernel<__bf16>, grid, block, lds, s, a, x, x_stride, d);
+  return hipGetLastError();
 }
 
 hipError_t launch_int8(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s) {

@@ -83,6 +83,15 @@ def _bare(passes):
     return call
 
 
+def _wanted(values) -> bool:
+    """Whether torch would differentiate some of the values."""
+    if torch.is_grad_enabled():
+        for t in values:
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                return True
+    return forward_ad._current_level >= 0 and _has_tangent(values)
+
+
 def _serving(call_):
     """A call without a gradient: refused where torch would want one, or records a trace."""
 
@@ -90,7 +99,7 @@ def _serving(call_):
     def call(*args, **kwargs):
         if _tracing() is not None:
             raise RuntimeError(f"{call_.__name__} cannot be traced")
-        if _through_autograd(*args, *kwargs.values()):
+        if _wanted(args) or _wanted(kwargs.values()):
             raise RuntimeError(f"{call_.__name__} has no derivative: call it under torch.no_grad()")
         return call_(*args, **kwargs)
 
@@ -166,6 +175,30 @@ def _new(t: torch.Tensor) -> torch.Tensor:
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def _form(t):
+    """What a call's checks look at of a tensor, but for where it lies; None for None."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+_known: dict = {}  # calls whose tensors' forms passed the checks and needed no copies: what these decided
+
+
+def _know(key, value) -> None:
+    if key is not None:
+        if len(_known) >= 4096:
+            _known.clear()
+        _known[key] = value
+
+
+def _on16(*tensors) -> bool:
+    """Whether tensors (or None) start on 16 bytes."""
+    at = 0
+    for t in tensors:
+        if t is not None:
+            at |= t.data_ptr()
+    return at % 16 == 0
 
 
 # ---- layer norm -----------------------------------------------------------------
@@ -386,26 +419,41 @@ def gated_linear_forward(x, gate, up, gate_bias=None, up_bias=None, activation="
     and ``up`` [n, k] (halves of one weight, say).  ``activation``: "silu" (z sigmoid(z)),
     "gelu" (by the error function), "sigmoid", "relu", "tanh" or None.  pre [..., 2 n] is both products,
     the gate's first, for the backward pass, None without ``keep_pre``."""
-    n, k = _gated_args(x, gate, up, activation)
-    biases = []
-    for name, bias in (("gate_bias", gate_bias), ("up_bias", up_bias)):
-        if bias is not None:
-            _tensor(bias, name, x, (n,))
-            bias = _packed(bias)
-        biases.append(bias)
+    given = (x, gate, up, gate_bias, up_bias)
+    try:
+        key = ("gated", activation, *map(_form, given))
+        call = _known.get(key)
+    except (AttributeError, TypeError):  # no tensors: the checks say which
+        key = call = None
     lib = _library()
-    r = _rows(x, k, True)
-    m = r.shape[0]
-    y = x.new_empty((*x.shape[:-1], n))
-    pre = x.new_empty((*x.shape[:-1], 2 * n)) if keep_pre else None
+    if call is None or not _on16(*given):
+        n, k = _gated_args(x, gate, up, activation)
+        for name, bias in (("gate_bias", gate_bias), ("up_bias", up_bias)):
+            if bias is not None:
+                _tensor(bias, name, x, (n,))
+        r = _rows(x, k, True)
+        m, dev = r.shape[0], x.device.index
+        gate, up, gate_bias, up_bias = (None if t is None else _packed(t) for t in (gate, up, gate_bias, up_bias))
+        size = 0
+        if m:
+            out = _I64(0)
+            _check(lib.cvs_gated_linear_plan(m, k, n, dev, ctypes.byref(out)))
+            size = out.value
+        call = (m, k, n, _row_stride(r), GATES[activation], TYPES[x.dtype], size, dev)
+        if r.data_ptr() == x.data_ptr() and all(a is b for a, b in zip((gate, up, gate_bias, up_bias), given[1:])):
+            _know(key, call)
+        x, like = r, x
+    else:
+        like = x
+    m, k, n, stride, act, kind, size, dev = call
+    shape = like.shape[:-1]
+    y = like.new_empty((*shape, n))
+    pre = like.new_empty((*shape, 2 * n)) if keep_pre else None
     if m == 0:
         return y, pre
-    gate, up = _packed(gate), _packed(up)
-    dev = x.device.index
-    ws = _workspace(("gated", m, k, n, dev), x, lambda out: lib.cvs_gated_linear_plan(m, k, n, dev, out))
-    _check(lib.cvs_gated_linear(r.data_ptr(), gate.data_ptr(), up.data_ptr(), _ptr(biases[0]), _ptr(biases[1]), m, k, n,
-                                _row_stride(r), GATES[activation], TYPES[x.dtype], y.data_ptr(), _ptr(pre), _ptr(ws),
-                                0 if ws is None else ws.numel(), dev, _ext.raw_stream(dev)))
+    ws = like.new_empty(size, dtype=torch.uint8) if size else None
+    _check(lib.cvs_gated_linear(x.data_ptr(), gate.data_ptr(), up.data_ptr(), _ptr(gate_bias), _ptr(up_bias), m, k, n, stride,
+                                act, kind, y.data_ptr(), _ptr(pre), _ptr(ws), size, dev, _ext.raw_stream(dev)))
     return y, pre
 
 
@@ -492,12 +540,7 @@ def quantize_rows(x):
     return values, scales
 
 
-@_serving
-def linear_int8(x, values, scales, bias=None, activation=None, residual=None):
-    """activation(x weight^T + bias) + residual for ``x`` [..., k] and a weight [n, k] in 8-bit whole numbers, ``values``
-    (int8 [n, k]) times ``scales`` (float32 [n], its channels'), as ``quantize_rows`` lays them out once.  x's rows
-    (its tokens) are taken in 8-bit whole numbers too, by the same rule, inside; sums are whole and exact.
-    k is a multiple of 16, n of 8.  No derivative."""
+def _int8_args(x, values, scales, bias, activation, residual):
     _tensor(x, "x")
     if x.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError("linear_int8 takes float16 or bfloat16")
@@ -512,26 +555,51 @@ def linear_int8(x, values, scales, bias=None, activation=None, residual=None):
     _int8_width(k)
     if n < 8 or n % 8:
         raise RuntimeError("linear_int8 takes a multiple of 8 output features (zero-pad them)")
-    scales = _packed(_stats(scales, "scales", x, (n,)))
-    shape = (*x.shape[:-1], n)
+    _stats(scales, "scales", x, (n,))
     if bias is not None:
         _tensor(bias, "bias", x, (n,))
     if residual is not None:
-        _tensor(residual, "residual", x, shape)
+        _tensor(residual, "residual", x, (*x.shape[:-1], n))
+    return n, k
+
+
+@_serving
+def linear_int8(x, values, scales, bias=None, activation=None, residual=None):
+    """activation(x weight^T + bias) + residual for ``x`` [..., k] and a weight [n, k] in 8-bit whole numbers, ``values``
+    (int8 [n, k]) times ``scales`` (float32 [n], its channels'), as ``quantize_rows`` lays them out once.  x's rows
+    (its tokens) are taken in 8-bit whole numbers too, by the same rule, inside; sums are whole and exact.
+    k is a multiple of 16, n of 8.  No derivative."""
+    given = (x, values, scales, bias, residual)
+    try:
+        key = ("int8", activation, *map(_form, given))
+        call = _known.get(key)
+    except (AttributeError, TypeError):  # no tensors: the checks say which
+        key = call = None
     lib = _library()
-    r = _rows(x, k, True)
-    m = r.shape[0]
+    if call is None or not _on16(*given):
+        n, k = _int8_args(x, values, scales, bias, activation, residual)
+        r = _rows(x, k, True)
+        m, dev = r.shape[0], x.device.index
+        values, scales, bias = (None if t is None else _packed(t) for t in (values, scales, bias))
+        residual = None if residual is None else _rows(residual, n, True)
+        size = 0
+        if m:
+            out = _I64(0)
+            _check(lib.cvs_linear_int8_plan(m, k, n, dev, ctypes.byref(out)))
+            size = out.value
+        call = ((*x.shape[:-1], n), m, k, n, _row_stride(r), 0 if residual is None else _row_stride(residual),
+                ACTIVATIONS[activation], TYPES[x.dtype], size, dev)
+        if (r.data_ptr() == x.data_ptr() and all(a is b for a, b in zip((values, scales, bias), given[1:4]))
+                and (residual is None or residual.data_ptr() == given[4].data_ptr())):
+            _know(key, call)
+        x = r
+    shape, m, k, n, stride, res_stride, act, kind, size, dev = call
     y = x.new_empty(shape)
     if m == 0:
         return y
-    values = _packed(values)
-    bias = None if bias is None else _packed(bias)
-    res = None if residual is None else _rows(residual, n, True)
-    dev = x.device.index
-    ws = _workspace(("int8", m, k, n, dev), x, lambda out: lib.cvs_linear_int8_plan(m, k, n, dev, out))
-    _check(lib.cvs_linear_int8(r.data_ptr(), values.data_ptr(), scales.data_ptr(), _ptr(bias), _ptr(res), m, k, n,
-                               _row_stride(r), 0 if res is None else _row_stride(res), ACTIVATIONS[activation], TYPES[x.dtype],
-                               y.data_ptr(), _ptr(ws), 0 if ws is None else ws.numel(), dev, _ext.raw_stream(dev)))
+    ws = x.new_empty(size, dtype=torch.uint8) if size else None
+    _check(lib.cvs_linear_int8(x.data_ptr(), values.data_ptr(), scales.data_ptr(), _ptr(bias), _ptr(residual), m, k, n, stride,
+                               res_stride, act, kind, y.data_ptr(), _ptr(ws), size, dev, _ext.raw_stream(dev)))
     return y
 
 
@@ -590,7 +658,7 @@ def _attention_check(q, k, v, bias_table, scale) -> None:
 
 
 def _window(window, sinks):
-    """The window as _ext.AttentionWindow, or None."""
+    """(before, after, sinks), or None."""
     sinks = operator.index(sinks)
     if window is None:
         if sinks:
@@ -604,19 +672,18 @@ def _window(window, sinks):
     if before < 0 or after < 0 or sinks < 0:
         raise RuntimeError("window and sinks must not be negative")
     most = 1 << 30  # (a longer one is no different)
-    return _ext.AttentionWindow(min(before, most), min(after, most), min(sinks, most))
+    return min(before, most), min(after, most), min(sinks, most)
 
 
 def _attention_args(q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance, win):
-    """(AttentionArgs, its _AttentionCall or None, tensors it points into) after the checks; win: an
-    _ext.AttentionWindow or None."""
+    """(AttentionArgs, its _AttentionCall or None, tensors it points into) after the checks; win: of _window."""
     # values, not tensors that hold them: those are found by identity and may have changed since
     scale = None if scale is None else float(scale)
     causal = bool(causal)
     max_distance = 0 if bias_table is None else operator.index(max_distance)
     try:
         key = (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype, q.device, k.device,
-               v.device, causal, scale, max_distance, None if win is None else bytes(win),
+               v.device, causal, scale, max_distance, win,
                None if bias_table is None else (bias_table.shape, bias_table.dtype, bias_table.device))
         call = _calls.get(key)
     except (AttributeError, TypeError):  # no tensors: the checks say which
@@ -654,6 +721,10 @@ def _attention_args(q, k, v, bias_table, key_lengths, query_lengths, query_start
     return a, call, hold
 
 
+def _attention_window(win):
+    return None if win is None else ctypes.byref(_ext.AttentionWindow(*win))
+
+
 def _attention_workspace(lib, a, win, call, backward: bool, q):
     size = None if call is None else call.bytes[backward]
     if size is None:
@@ -661,7 +732,7 @@ def _attention_workspace(lib, a, win, call, backward: bool, q):
         if win is None:
             _check(lib.cvs_attention_plan(ctypes.byref(a), backward, q.device.index, ctypes.byref(out)))
         else:
-            _check(lib.cvs_attention_window_plan(ctypes.byref(a), ctypes.byref(win), backward, q.device.index, ctypes.byref(out)))
+            _check(lib.cvs_attention_window_plan(ctypes.byref(a), win, backward, q.device.index, ctypes.byref(out)))
         size = int(out.value)
         if call is not None:
             call.bytes[backward] = size
@@ -696,12 +767,13 @@ def attention_forward(q, k, v, bias_table=None, key_lengths=None, query_lengths=
     out = _new(q)
     sums = q.new_empty((a.batch, a.heads, a.q_len), dtype=torch.float32) if lse else None
     dev = q.device.index
+    win = _attention_window(win)
     ws = _attention_workspace(lib, a, win, call, False, q)
     rest = (out.data_ptr(), _ptr(sums), _ptr(ws), 0 if ws is None else ws.numel(), dev, _ext.raw_stream(dev))
     if win is None:
         _check(lib.cvs_attention_forward(ctypes.byref(a), *rest))
     else:
-        _check(lib.cvs_attention_window_forward(ctypes.byref(a), ctypes.byref(win), *rest))
+        _check(lib.cvs_attention_window_forward(ctypes.byref(a), win, *rest))
     return out, sums
 
 
@@ -723,13 +795,14 @@ def attention_backward(dout, q, k, v, out, lse, bias_table=None, key_lengths=Non
     if a.batch == 0 or (a.q_len == 0 and a.k_len == 0):
         return dq, dk, dv, None if dtable is None else dtable.zero_()
     dev = q.device.index
+    win = _attention_window(win)
     ws = _attention_workspace(lib, a, win, call, True, q)
     rest = (dout.data_ptr(), dout_stride, out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
             _ptr(dtable), _ptr(ws), 0 if ws is None else ws.numel(), dev, _ext.raw_stream(dev))
     if win is None:
         _check(lib.cvs_attention_backward(ctypes.byref(a), *rest))
     else:
-        _check(lib.cvs_attention_window_backward(ctypes.byref(a), ctypes.byref(win), *rest))
+        _check(lib.cvs_attention_window_backward(ctypes.byref(a), win, *rest))
     return dq, dk, dv, dtable
 
 
@@ -737,8 +810,7 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance, window, sinks):
         if window is not None:  # (as it is now, for the backward pass too)
-            win = _window(window, sinks)
-            window, sinks = (win.before, win.after), win.sinks
+            *window, sinks = _window(window, sinks)
         out, lse = attention_forward.inner(q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance,
                                            True, window, sinks)
         ctx.save_for_backward(q, k, v, out, lse, bias_table, key_lengths, query_lengths, query_start)
