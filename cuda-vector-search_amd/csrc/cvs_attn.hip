@@ -135,12 +135,14 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 3) void attn_forward_kernel(A
       scores();
     }
     V cols[2][2][DB];
+    if constexpr (!WIN) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+      for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int d = 0; d < DB; ++d) cols[kb][s][d] = col_frag<T, DP>(sv[buf], kb * 32 + 16 * s, d * 32);
+          for (int d = 0; d < DB; ++d) cols[kb][s][d] = col_frag<T, DP>(sv[buf], kb * 32 + 16 * s, d * 32);
+    }
     keep_order();
     if constexpr (WIN) {
       if (j0 + kKeys > nk || near + kKeys - 1 > a.after || near < 31 - a.before) {
@@ -148,6 +150,13 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 3) void attn_forward_kernel(A
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) mask.apply(x[kb], kb * 32, j0 < a.sinks, -__builtin_inff());
       }
+      // (before the mask, under the products, there are not the registers)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int d = 0; d < DB; ++d) cols[kb][s][d] = col_frag<T, DP>(sv[buf], kb * 32 + 16 * s, d * 32);
     } else if (j0 + kKeys > nk || (a.causal && near + kKeys - 1 > 0)) {
       const int seen = min(nk - 1, a.causal ? i + off : nk) - j0 - 8 * g;  // last key of the tile that the row sees
 #pragma unroll

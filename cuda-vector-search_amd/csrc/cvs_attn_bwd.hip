@@ -518,6 +518,181 @@ __device__ __forceinline__ void add_table(const AttnArgs& a, int at) {
   if (lane == 0) ((T*)a.dtable)[(int64_t)bucket * a.heads + h] = (T)s;
 }
 
+// dk and dv of the first keys, which rows see from anywhere: 32 keys as columns, each wave walking row tiles of
+// its own (32 rows, of all heads that share the key head, one after the other) through a buffer of its own, with
+// no barrier; a tile's operands are in registers before the next one's loads go into its place, under the
+// products.  The waves' sums are joined at the end; parts of the rows by attn_join_sinks_kernel.  Workgroup
+// `id` of these is one of the kv kernel's launch, whose others hide its waits: its kernel of its own took 20 us of
+// 8 sequences of up to 2048, 12 heads of 64, and as many of 8192 rows, 16 heads on 4 of 128.
+// tq, tg: four tiles of 32 rows of q and of dout; slse, sdelta: of 32 values.
+template <class T, int DP, bool BIAS>
+__device__ __forceinline__ void sink_gradients(const AttnArgs& a, int id, unsigned char* tq, unsigned char* tg, float* slse, float* sdelta) {
+  typedef typename Frag<T>::V V;
+  constexpr int KS = DP / 16, DB = DP / 32, TILE = 32 * DP * 2;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kheads = a.batch * a.k_heads, group = a.heads / a.k_heads;
+  const int bk = id % kheads, part = id / kheads % a.sink_parts, j0 = id / kheads / a.sink_parts * 32;
+  const int b = bk / a.k_heads, hk = bk % a.k_heads;
+  const int nk = key_count(a, b), nq = query_count(a, b), off = query_offset(a, b);
+  const int j = j0 + l32;
+  int row0, row1;
+  window_rows(a, nk, nq, off, row0, row1);
+  const int heads_seen = min(a.sinks, a.causal ? min(nk, max(row1 + off, 0)) : nk);  // keys of these that some row sees
+  const bool seen = row0 < row1 && j < heads_seen;
+  const unsigned char* krow = (const unsigned char*)a.k + 2 * (b * a.ks[0] + j * a.ks[1] + hk * a.ks[2]);
+  const unsigned char* vrow = (const unsigned char*)a.v + 2 * (b * a.vs[0] + j * a.vs[1] + hk * a.vs[2]);
+  unsigned char *sq = tq + wave * TILE, *sg = tg + wave * TILE;
+  slse += wave * 32, sdelta += wave * 32;
+
+  // row tiles of all heads in a row (fewer than 2^25); this part's, of which each wave takes every fourth
+  const int t0 = (a.causal ? max(row0, j0 - off) : row0) / 32;
+  const unsigned nt = row0 < row1 && j0 < heads_seen ? max((row1 + 31) / 32 - t0, 0) : 0;
+  const unsigned all = nt * group, f0 = all * part / a.sink_parts, f1 = all * (part + 1) / a.sink_parts;
+  const TileLoad<DP, 32, 1> lq(2 * a.qs[1], a.d), lg(2 * a.dos[1], a.d);
+  float stat = 0.f;  // lanes 0 .. 31: -log2 sum of a row, the others: -delta
+  auto load = [&](unsigned f) {
+    const int h = hk * group + f / nt, t = t0 + f % nt;
+    lq.load((const unsigned char*)a.q + 2 * (b * a.qs[0] + h * a.qs[2]), 2 * a.qs[1], t * 32, row1, sq, row0);
+    lg.load((const unsigned char*)a.dout + 2 * (b * a.dos[0] + h * a.dos[2]), 2 * a.dos[1], t * 32, row1, sg, row0);
+    const int i = t * 32 + l32;
+    const int64_t at = ((int64_t)b * a.heads + h) * a.lq + i;
+    const bool in = i >= row0 && i < row1;
+    if (g == 0) {
+      stat = in ? -a.lse[at] * kLog2e : -kNever;
+      if (stat == __builtin_inff()) stat = -kNever;  // a row that sees nothing
+    } else {
+      stat = in ? -a.delta[at] : 0.f;
+    }
+  };
+  unsigned f = f0 + wave;
+  if (f < f1) load(f);
+  V kf[KS], vf[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    kf[s] = global_frag<T>(krow, s, a.d, seen);
+    vf[s] = global_frag<T>(vrow, s, a.d, seen);
+  }
+  f32x16 dk[DB], dv[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) dk[d] = dv[d] = zero16();
+  const float c = a.scale * kLog2e;
+  float shrink = 1.f;  // of ds, where they would not fit (as the other keys')
+  if constexpr (kLift<T> != 0) {
+    const int64_t count = (int64_t)group * a.q_parts * ((a.lq + kAttnRows - 1) / kAttnRows);
+    const float* from = a.part_peak + bk * count;
+    float peak = 0.f;
+    for (int64_t t = lane; t < count; t += 64) peak = fmaxf(peak, from[t]);
+    shrink = ldexpf(1.f, -max(__builtin_amdgcn_readfirstlane(kLift<T> - room(wave_max(peak))), 0));
+  }
+  for (; f < f1; f += 4) {
+    wait_vmcnt_lgkm0<0>();
+    asm volatile("" ::: "memory");
+    (g == 0 ? slse : sdelta)[l32] = g == 0 ? stat + kLift<T> : stat;
+    const int h = hk * group + f / nt, i0 = (t0 + f % nt) * 32;
+    const int near = j0 - i0 - off;
+    V qrows[KS], grows[KS], qcols[2][DB], gcols[2][DB];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qrows[s] = row_frag<T, DP>(sq, 0, s), grows[s] = row_frag<T, DP>(sg, 0, s);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) qcols[s][d] = col_frag<T, DP>(sq, 16 * s, d * 32), gcols[s][d] = col_frag<T, DP>(sg, 16 * s, d * 32);
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    f32x16 lse, delta;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) lse[e] = slse[elem_row(e, g)], delta[e] = sdelta[elem_row(e, g)];
+    wait_vmcnt_lgkm0<63>();  // every read of the buffers
+    asm volatile("" ::: "memory");
+    keep_order();
+    if (f + 4 < f1) load(f + 4);
+    f32x16 p = zero16(), ds = zero16();  // (delta may be made of dout . v's own sums: subtracted as they stand)
+    float shift = 0.f;
+    if (BIAS) {
+      const float unit = 1.f / a.scale;
+      const T* table = (const T*)a.table + h;
+      auto bias = [&](int rel) {
+        int u = a.bucket_of[min(abs(rel), a.far)];
+        if (rel > 0) u = a.causal ? 0 : u + a.one_way;
+        return (float)table[(int64_t)u * a.heads] * unit;
+      };
+      if (near - 31 >= a.far || near + 31 <= -a.far) {
+        shift = bias(near) * c;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[e] = bias(near + l32 - elem_row(e, g));
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) p = Frag<T>::mfma(qrows[s], kf[s], p);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) ds = Frag<T>::mfma(grows[s], vf[s], ds);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], c, lse[e] + shift));
+    if (a.causal && near + 31 > 0) {
+      const int first = j - off - i0 - 8 * g;  // first row of the block that sees the key
+#pragma unroll
+      for (int e = 0; e < 16; ++e) p[e] = elem_row(e, 0) < first ? 0.f : p[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) ds[e] = (ds[e] + delta[e]) * p[e];
+    if (kLift<T> != 0 && shrink != 1.f) times<1>(&ds, shrink);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const V pf = pack8<T>(p, s), df = pack8<T>(ds, s);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        dv[d] = Frag<T>::mfma(gcols[s][d], pf, dv[d]);
+        dk[d] = Frag<T>::mfma(qcols[s][d], df, dk[d]);
+      }
+    }
+  }
+  // join the waves: dk, then dv, each wave's [32 columns][DP] in the place of two tiles, the pieces of 4 in an order by column
+  wait_vmcnt_lgkm0<0>();
+  auto sums_of = [&](int w) { return reinterpret_cast<float*>((w < 2 ? tq : tg) + (w & 1) * 2 * TILE); };
+  const int64_t plane = (int64_t)a.batch * a.sinks * a.k_heads * a.d;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    float* sums = sums_of(wave);
+    __syncthreads();
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x16& acc = u == 0 ? dk[d] : dv[d];
+        const int piece = (d * 32 + 16 * (q >> 1) + 8 * g + 4 * (q & 1)) / 4;
+        *reinterpret_cast<f32x4*>(sums + l32 * DP + ((piece ^ (l32 & 7)) * 4)) =
+            f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+      }
+    __syncthreads();
+    const float undo = u == 0 ? kUnlift<T> / shrink : kUnlift<T>;
+    for (int t = threadIdx.x; t < 32 * (DP / 8); t += kBlock) {
+      const int col = t / (DP / 8), c8 = t % (DP / 8) * 8;
+      if (c8 >= a.d || j0 + col >= a.sinks) continue;
+      float z[8];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          s += *reinterpret_cast<const f32x4*>(sums_of(w) + col * DP + (((c8 / 4 + half) ^ (col & 7)) * 4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[4 * half + e] = j0 + col < heads_seen ? s[e] * undo : 0.f;
+      }
+      if (a.sink_parts > 1) {
+        float* o = a.part_sinks + (2 * part + u) * plane + (((int64_t)b * a.sinks + j0 + col) * a.k_heads + hk) * a.d + c8;
+        *reinterpret_cast<f32x4*>(o) = f32x4{z[0], z[1], z[2], z[3]};
+        *reinterpret_cast<f32x4*>(o + 4) = f32x4{z[4], z[5], z[6], z[7]};
+      } else {
+        V v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (T)(u == 0 ? z[e] * a.scale : z[e]);
+        *reinterpret_cast<V*>((T*)(u == 0 ? a.dk : a.dv) + (((int64_t)b * a.lk + j0 + col) * a.k_heads + hk) * a.d + c8) = v;
+      }
+    }
+  }
+}
+
 // dk and dv of 128 keys (wave w: 32 of them as columns), over a part of the queries that see
 // them.  Where there is a bias, the workgroups from `key_wgs` on add up its table's gradient.
 // The keys' rows of both operands and both sums stay in registers, at width 128 some 420 of them:
@@ -525,7 +700,7 @@ __device__ __forceinline__ void add_table(const AttnArgs& a, int at) {
 // another.  2 x 4096, 16 heads on 4 of 128, causal: 329 us, 0.84 PFLOP/s of its four products;
 // 64 x 512, 12 heads of 64, two workgroups a CU: 148 us, with a bias 156.
 template <class T, int DP, bool BIAS, bool WIN>
-__global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kernel(AttnArgs a, int key_wgs) {
+__global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kernel(AttnArgs a, int key_wgs, int sink_wgs) {
   typedef typename Frag<T>::V V;
   constexpr int KS = DP / 16, DB = DP / 32, ROWS = 64, QB = ROWS / 32, TILE = ROWS * DP * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char sq[2][TILE], sg[2][TILE];
@@ -534,8 +709,14 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
 
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if constexpr (WIN) {  // (after the others, whose CUs are free at different times)
+    if ((int)blockIdx.x >= key_wgs && (int)blockIdx.x < key_wgs + sink_wgs) {
+      if (blockIdx.y == 0) sink_gradients<T, DP, BIAS>(a, (int)blockIdx.x - key_wgs, sq[0], sg[0], slse[0], sdelta[0]);
+      return;
+    }
+  }
   if (BIAS && (int)blockIdx.x >= key_wgs) {
-    if (blockIdx.y == 0) add_table<T>(a, ((int)blockIdx.x - key_wgs) * 4 + wave);
+    if (blockIdx.y == 0) add_table<T>(a, ((int)blockIdx.x - key_wgs - (WIN ? sink_wgs : 0)) * 4 + wave);
     return;
   }
   const int kheads = a.batch * a.k_heads, group = a.heads / a.k_heads;
@@ -573,7 +754,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
   // tiles of queries that see a key of this workgroup, those of all heads in a row; this part's
   int t0 = (a.causal ? max(block * kAttnRows - off, 0) : 0) / ROWS;
   int nt = block * kAttnRows < seen_keys ? max((nq + ROWS - 1) / ROWS - t0, 0) : 0;
-  if constexpr (WIN) {  // (the first keys' gradients are attn_backward_sinks_kernel's)
+  if constexpr (WIN) {  // (the first keys' gradients are sink_gradients')
     const int lo = max(row0, block * kAttnRows - off - a.after), hi = min(row1, block * kAttnRows + kAttnRows - off + a.before);
     t0 = lo / ROWS;
     nt = block * kAttnRows < seen_keys && block * kAttnRows + kAttnRows > a.sinks && lo < hi ? (hi + ROWS - 1) / ROWS - t0 : 0;
@@ -733,187 +914,30 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
   store_head_row<T, DP>((T*)a.dv + at, dv, kUnlift<T>, a.d);
 }
 
-// dk and dv of the first keys, which rows see from anywhere: 32 keys as columns, each wave walking row tiles of
-// its own (32 rows, of all heads that share the key head, one after the other) through buffers of its own, with
-// no barrier, its next tile's loads under way; the waves' sums are joined at the end.  A part of
-// the rows (blockIdx.y) each; parts are added by attn_join_sinks_kernel.
-template <class T, int DP, bool BIAS>
-__global__ __launch_bounds__(kBlock, 1) void attn_backward_sinks_kernel(AttnArgs a) {
-  typedef typename Frag<T>::V V;
-  constexpr int KS = DP / 16, DB = DP / 32, TILE = 32 * DP * 2, LOADS = TILE / 1024;
-  // per wave: two tiles of q and of dout; at the end its sums
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[4][2][2][TILE];
-  __shared__ __attribute__((aligned(16))) float stats[4][2][32];  // kLift - log2 sums, -deltas
-
-  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kheads = a.batch * a.k_heads, group = a.heads / a.k_heads;
-  const int bk = blockIdx.x % kheads, block = blockIdx.x / kheads;
-  const int b = bk / a.k_heads, hk = bk % a.k_heads;
-  const int nk = key_count(a, b), nq = query_count(a, b), off = query_offset(a, b);
-  const int j0 = block * 32, j = j0 + l32;
-  int row0, row1;
-  window_rows(a, nk, nq, off, row0, row1);
-  const int heads_seen = min(a.sinks, a.causal ? min(nk, max(row1 + off, 0)) : nk);  // keys of these that some row sees
-  const bool seen = row0 < row1 && j < heads_seen;
-  const unsigned char* krow = (const unsigned char*)a.k + 2 * (b * a.ks[0] + j * a.ks[1] + hk * a.ks[2]);
-  const unsigned char* vrow = (const unsigned char*)a.v + 2 * (b * a.vs[0] + j * a.vs[1] + hk * a.vs[2]);
-  V kf[KS], vf[KS];
-#pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    kf[s] = global_frag<T>(krow, s, a.d, seen);
-    vf[s] = global_frag<T>(vrow, s, a.d, seen);
-  }
-  f32x16 dk[DB], dv[DB];
-#pragma unroll
-  for (int d = 0; d < DB; ++d) dk[d] = dv[d] = zero16();
-  const float c = a.scale * kLog2e;
-  float shrink = 1.f;  // of ds, where they would not fit (as the kv kernel's)
-  if constexpr (kLift<T> != 0) {
-    const int64_t count = (int64_t)group * a.q_parts * ((a.lq + kAttnRows - 1) / kAttnRows);
-    const float* from = a.part_peak + bk * count;
-    float peak = 0.f;
-    for (int64_t t = lane; t < count; t += 64) peak = fmaxf(peak, from[t]);
-    shrink = ldexpf(1.f, -max(__builtin_amdgcn_readfirstlane(kLift<T> - room(wave_max(peak))), 0));
-  }
-
-  // row tiles of all heads in a row; this part's, of which each wave takes every fourth
-  const int t0 = (a.causal ? max(row0, j0 - off) : row0) / 32;
-  const int nt = row0 < row1 && j0 < heads_seen ? max((row1 + 31) / 32 - t0, 0) : 0;
-  const int64_t all = (int64_t)nt * group;
-  const int64_t f0 = all * blockIdx.y / a.sink_parts, f1 = all * (blockIdx.y + 1) / a.sink_parts;
-  const TileLoad<DP, 32, 1> lq(2 * a.qs[1], a.d), lg(2 * a.dos[1], a.d);
-  float stat = 0.f;  // lanes 0 .. 31: -log2 sum of a row, the others: -delta
-  auto load = [&](int64_t f, int buf) {
-    const int h = hk * group + (int)(f / nt), t = t0 + (int)(f % nt);
-    lq.load((const unsigned char*)a.q + 2 * (b * a.qs[0] + h * a.qs[2]), 2 * a.qs[1], t * 32, row1, smem[wave][buf][0], row0);
-    lg.load((const unsigned char*)a.dout + 2 * (b * a.dos[0] + h * a.dos[2]), 2 * a.dos[1], t * 32, row1, smem[wave][buf][1], row0);
-    const int i = t * 32 + l32;
-    const int64_t at = ((int64_t)b * a.heads + h) * a.lq + i;
-    const bool in = i >= row0 && i < row1;
-    if (g == 0) {
-      stat = in ? -a.lse[at] * kLog2e : -kNever;
-      if (stat == __builtin_inff()) stat = -kNever;  // a row that sees nothing
-    } else {
-      stat = in ? -a.delta[at] : 0.f;
-    }
-  };
-  int64_t f = f0 + wave;
-  int buf = 0;
-  if (f < f1) load(f, 0);
-  for (; f < f1; f += 4, buf ^= 1) {
-    wait_vmcnt_lgkm0<0>();  // this tile's loads, and the reads of the buffers to be loaded next
-    asm volatile("" ::: "memory");
-    stats[wave][g][l32] = g == 0 ? stat + kLift<T> : stat;
-    if (f + 4 < f1) load(f + 4, buf ^ 1);
-    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-    const unsigned char* sq = smem[wave][buf][0];
-    const unsigned char* sg = smem[wave][buf][1];
-    const int h = hk * group + (int)(f / nt), i0 = (t0 + (int)(f % nt)) * 32;
-    const int near = j0 - i0 - off;
-    f32x16 p = zero16(), ds;
-    float shift = 0.f;
-    if (BIAS) {
-      const float unit = 1.f / a.scale;
-      const T* table = (const T*)a.table + h;
-      auto bias = [&](int rel) {
-        int u = a.bucket_of[min(abs(rel), a.far)];
-        if (rel > 0) u = a.causal ? 0 : u + a.one_way;
-        return (float)table[(int64_t)u * a.heads] * unit;
-      };
-      if (near - 31 >= a.far || near + 31 <= -a.far) {
-        shift = bias(near) * c;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) p[e] = bias(near + l32 - elem_row(e, g));
-      }
-    }
-#pragma unroll
-    for (int s = 0; s < KS; ++s) p = Frag<T>::mfma(row_frag<T, DP>(sq, 0, s), kf[s], p);
-    ds = zero16();  // (delta may be made of dout . v's own sums: subtracted as they stand)
-#pragma unroll
-    for (int s = 0; s < KS; ++s) ds = Frag<T>::mfma(row_frag<T, DP>(sg, 0, s), vf[s], ds);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) ds[e] += stats[wave][1][elem_row(e, g)];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], c, stats[wave][0][elem_row(e, g)] + shift));
-    if (a.causal && near + 31 > 0) {
-      const int first = j - off - i0 - 8 * g;  // first row of the block that sees the key
-#pragma unroll
-      for (int e = 0; e < 16; ++e) p[e] = elem_row(e, 0) < first ? 0.f : p[e];
-    }
-#pragma unroll
-    for (int e = 0; e < 16; ++e) ds[e] *= p[e];
-    if (kLift<T> != 0 && shrink != 1.f) times<1>(&ds, shrink);
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const V pf = pack8<T>(p, s), df = pack8<T>(ds, s);
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        dv[d] = Frag<T>::mfma(col_frag<T, DP>(sg, 16 * s, d * 32), pf, dv[d]);
-        dk[d] = Frag<T>::mfma(col_frag<T, DP>(sq, 16 * s, d * 32), df, dk[d]);
-      }
-    }
-  }
-  // join the waves: [2][32 columns][DP] each, the pieces of 4 in an order by column
-  wait_vmcnt_lgkm0<0>();
-  float* sums = reinterpret_cast<float*>(smem[wave]);
-#pragma unroll
-  for (int u = 0; u < 2; ++u)
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x16& acc = u == 0 ? dk[d] : dv[d];
-        const int piece = (d * 32 + 16 * (q >> 1) + 8 * g + 4 * (q & 1)) / 4;
-        *reinterpret_cast<f32x4*>(sums + (u * 32 + l32) * DP + ((piece ^ (l32 & 7)) * 4)) =
-            f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
-      }
-  __syncthreads();
-  const float undo_k = kUnlift<T> / shrink, undo_v = kUnlift<T>;
-  const int64_t plane = (int64_t)a.batch * a.sinks * a.k_heads * a.d;
-  for (int t = threadIdx.x; t < 2 * 32 * (DP / 8); t += kBlock) {
-    const int u = t / (32 * (DP / 8)), col = t / (DP / 8) % 32, c8 = t % (DP / 8) * 8;
-    if (c8 >= a.d || j0 + col >= a.sinks) continue;
-    float z[8];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      f32x4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-        s += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(smem[w]) + (u * 32 + col) * DP + (((c8 / 4 + half) ^ (col & 7)) * 4));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) z[4 * half + e] = j0 + col < heads_seen ? s[e] * (u == 0 ? undo_k : undo_v) : 0.f;
-    }
-    if (a.sink_parts > 1) {
-      float* o = a.part_sinks + (2 * blockIdx.y + u) * plane + (((int64_t)b * a.sinks + j0 + col) * a.k_heads + hk) * a.d + c8;
-      *reinterpret_cast<f32x4*>(o) = f32x4{z[0], z[1], z[2], z[3]};
-      *reinterpret_cast<f32x4*>(o + 4) = f32x4{z[4], z[5], z[6], z[7]};
-    } else {
-      V v;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = (T)(u == 0 ? z[e] * a.scale : z[e]);
-      *reinterpret_cast<V*>((T*)(u == 0 ? a.dk : a.dv) + (((int64_t)b * a.lk + j0 + col) * a.k_heads + hk) * a.d + c8) = v;
-    }
-  }
-}
-
-// Adds the parts of the first keys' dk and dv, in order: 8 values a thread.
+// Adds the parts of the first keys' dk and dv: 8 values to 16 lanes, which take every 16th part and add their
+// sums in a fixed order (a thread alone waited for 64 parts' loads in turn, 21 us).
 template <class T>
 __global__ __launch_bounds__(kBlock) void attn_join_sinks_kernel(AttnArgs a) {
   const int64_t row = (int64_t)a.sinks * a.k_heads * a.d, plane = a.batch * row;
-  const int64_t at = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * 8;
+  const int64_t at = ((int64_t)blockIdx.x * (kBlock / 16) + threadIdx.x / 16) * 8;
   if (at >= plane) return;
-  f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
-  for (int p = 0; p < a.sink_parts; ++p) {
+  const int lane = threadIdx.x % 16;
+  float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int p = lane; p < a.sink_parts; p += 16) {
     const f32x4* from = reinterpret_cast<const f32x4*>(a.part_sinks + (2 * p + blockIdx.y) * plane + at);
-    lo += from[0];
-    hi += from[1];
+    const f32x4 lo = from[0], hi = from[1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[e] += lo[e], z[4 + e] += hi[e];
   }
+#pragma unroll
+  for (int s = 8; s > 0; s >>= 1)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] += __shfl_xor(z[e], s);
+  if (lane != 0) return;
   const float scale = blockIdx.y == 0 ? a.scale : 1.f;
   typename Frag<T>::V v;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = (T)(lo[e] * scale), v[4 + e] = (T)(hi[e] * scale);
+  for (int e = 0; e < 8; ++e) v[e] = (T)(z[e] * scale);
   *reinterpret_cast<typename Frag<T>::V*>((T*)(blockIdx.y == 0 ? a.dk : a.dv) + at / row * a.lk * a.k_heads * a.d + at % row) = v;
 }
 
@@ -945,24 +969,20 @@ hipError_t launch_window(const AttnArgs& a, hipStream_t s) {
   if (qblocks > 0)
     hipLaunchKernelGGL((attn_backward_q_kernel<T, DP, BIAS, WIN>), dim3((unsigned)(qblocks * a.batch * a.heads), a.q_parts),
                        dim3(kBlock), 5 * tab, s, a);
-  const int64_t key_wgs = kblocks * a.batch * a.k_heads, all_wgs = key_wgs + (BIAS ? (a.buckets * a.heads + 3) / 4 : 0);
+  const int64_t sink_wgs = WIN ? (int64_t)(a.sinks + 31) / 32 * a.batch * a.k_heads * a.sink_parts : 0;
+  const int64_t key_wgs = kblocks * a.batch * a.k_heads, all_wgs = sink_wgs + key_wgs + (BIAS ? (a.buckets * a.heads + 3) / 4 : 0);
   if (all_wgs > 0)
     hipLaunchKernelGGL((attn_backward_kv_kernel<T, DP, BIAS, WIN>), dim3((unsigned)all_wgs, a.kv_parts), dim3(kBlock), tab, s, a,
-                       (int)key_wgs);
+                       (int)key_wgs, (int)sink_wgs);
   auto join = [&](const float* part, int parts, int64_t n, int sums, float scale, void* out0, void* out1) {
     const dim3 grid((unsigned)((n / 8 + kBlock - 1) / kBlock), sums);
     hipLaunchKernelGGL(attn_join_grads_kernel<T>, grid, dim3(kBlock), 0, s, part, parts, sums * n, n, scale, (T*)out0, (T*)out1);
   };
   if (a.q_parts > 1) join(a.part_q, a.q_parts, (int64_t)a.batch * a.lq * a.heads * a.d, 1, a.scale, a.dq, nullptr);
   if (a.kv_parts > 1) join(a.part_kv, a.kv_parts, (int64_t)a.batch * a.lk * a.k_heads * a.d, 2, a.scale, a.dk, a.dv);
-  if constexpr (WIN) {
-    if (a.sinks > 0) {  // (after the joins, which write the first keys' places too)
-      const int64_t plane = (int64_t)a.batch * a.sinks * a.k_heads * a.d;
-      hipLaunchKernelGGL((attn_backward_sinks_kernel<T, DP, BIAS>), dim3((unsigned)((a.sinks + 31) / 32 * a.batch * a.k_heads), a.sink_parts),
-                         dim3(kBlock), 0, s, a);
-      if (a.sink_parts > 1)
-        hipLaunchKernelGGL(attn_join_sinks_kernel<T>, dim3((unsigned)((plane / 8 + kBlock - 1) / kBlock), 2), dim3(kBlock), 0, s, a);
-    }
+  if (WIN && a.sink_parts > 1) {  // (after the join, which writes the first keys' places too)
+    const int64_t plane = (int64_t)a.batch * a.sinks * a.k_heads * a.d;
+    hipLaunchKernelGGL(attn_join_sinks_kernel<T>, dim3((unsigned)((plane / 8 + 15) / 16), 2), dim3(kBlock), 0, s, a);
   }
   return hipGetLastError();
 }
@@ -1004,14 +1024,17 @@ int attn_kv_parts(const AttnArgs& a, int cus) {
   int64_t rows = a.lq;  // that a workgroup walks of each head
   if (a.windowed) rows = std::min(rows, (int64_t)a.before + a.after + kAttnRows);
   const int64_t tiles = (rows + 63) / 64 * (int64_t)(a.heads / a.k_heads);
+  if (a.windowed && a.d > 64) cus /= 2;  // (one workgroup a CU, and all of them walk as many rows)
   return (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / wgs, tiles / 8, (int64_t)16}));
 }
 
-// Parts of the rows for the first keys' dk and dv: enough workgroups for one of a CU, of at least 4 tiles a wave.
-int attn_sink_parts(const AttnArgs& a, int cus) {
+// Parts of the rows for the first keys' dk and dv, of at least 16 tiles of 32 rows, 4 a wave, so that these workgroups
+// take no longer than the other keys'.  (Where there are parts of the others' rows too, their join
+// overwrites what a single part writes: two at least.)
+int attn_sink_parts(const AttnArgs& a, int kv_parts, int cus) {
   const int64_t wgs = (a.sinks + 31) / 32 * (int64_t)a.batch * a.k_heads;
   const int64_t tiles = (a.lq + 31) / 32 * (int64_t)(a.heads / a.k_heads);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({cus / std::max<int64_t>(wgs, 1), tiles / 16, (int64_t)64}));
+  return (int)std::max<int64_t>(kv_parts > 1 ? 2 : 1, std::min<int64_t>({tiles / 16, 8 * cus / wgs, (int64_t)64}));
 }
 
 hipError_t launch_attn_backward(const AttnArgs& a, hipStream_t s) {

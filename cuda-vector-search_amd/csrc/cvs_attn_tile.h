@@ -54,7 +54,7 @@ struct TileLoad {
     const uint32_t to = lds_address(lds) + (WAVES > 1 ? threadIdx.x >> 6 : 0) * 1024;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const bool in = (unsigned)(first - low + row[i]) < (unsigned)(rows - low) || first + row[i] < head;
+      const bool in = ((unsigned)(first - low + row[i]) < (unsigned)(rows - low)) | (first + row[i] < head);
       load_lds(in ? at[i] : kOutside, base + first * stride_bytes, to + i * (WAVES * 1024));
     }
   }
@@ -102,7 +102,7 @@ struct WindowMask {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int k = key + elem_row(e, 0);
-        x[e] = (unsigned)(k - low) <= span || k < head ? x[e] : out;
+        x[e] = ((unsigned)(k - low) <= span) | (k < head) ? x[e] : out;  // (|: no branch an element)
       }
     } else {
 #pragma unroll

@@ -191,7 +191,7 @@ struct AttnArgs {
 constexpr int kAttnRows = 128;    // query (or key) rows of a workgroup
 int attn_q_parts(const AttnArgs& a, int cus);
 int attn_kv_parts(const AttnArgs& a, int cus);
-int attn_sink_parts(const AttnArgs& a, int cus);
+int attn_sink_parts(const AttnArgs& a, int kv_parts, int cus);
 int attn_splits(const AttnArgs& a, int cus);
 hipError_t launch_attn_forward(const AttnArgs& a, hipStream_t s);
 hipError_t launch_attn_backward(const AttnArgs& a, hipStream_t s);

@@ -214,7 +214,7 @@ int check_window(const cvs_attention* p, const cvs_attention_window* w) {
   if (w == nullptr) return CVS_OK;
   if (w->before < 0 || w->after < 0 || w->sinks < 0) return fail(CVS_ERR_INVALID, "attention: a window's sizes must not be negative");
   if (p->q_len >= (1 << 28) || p->k_len >= (1 << 28)) return fail(CVS_ERR_INVALID, "attention: windows take lengths below 2^28");
-  if ((std::min(w->sinks, p->k_len) + 31) / 32 * p->batch * p->heads >= (1 << 23)) return fail(CVS_ERR_INVALID, "attention: too many first keys");
+  if ((std::min(w->sinks, p->k_len) + 31) / 32 * p->batch * p->heads >= (1 << 21)) return fail(CVS_ERR_INVALID, "attention: too many first keys");
   return CVS_OK;
 }
 
@@ -275,9 +275,9 @@ AttnPlan plan_attention(const AttnArgs& a, bool backward, int cus) {
       p.part_table = at, at += up256((int64_t)a.heads * p.table_parts * a.buckets * 4);
     }
     p.kv_parts = rows == 0 || a.lk == 0 ? 1 : attn_kv_parts(a, cus);
-    if (rows > 0 && a.sinks > 0) p.sink_parts = attn_sink_parts(a, cus);
-    if (p.sink_parts > 1) p.part_sinks = at, at += up256((int64_t)p.sink_parts * 2 * a.batch * a.sinks * a.k_heads * a.d * 4);
     if (p.kv_parts > 1) p.part_kv = at, at += up256((int64_t)p.kv_parts * 2 * a.batch * a.lk * a.k_heads * a.d * 4);
+    if (rows > 0 && a.sinks > 0) p.sink_parts = attn_sink_parts(a, p.kv_parts, cus);
+    if (p.sink_parts > 1) p.part_sinks = at, at += up256((int64_t)p.sink_parts * 2 * a.batch * a.sinks * a.k_heads * a.d * 4);
   } else {
     p.splits = rows == 0 ? 1 : attn_splits(a, cus);
     if (p.splits > 1) {

@@ -168,6 +168,17 @@ __global__ __launch_bounds__(kBlock) void int8_rows_kernel(GemmKindArgs a, const
     if (c < d) v = *reinterpret_cast<const i32x4*>(w + c);
     return v;
   };
+  // the epilogue's: 8 columns a thread of the first 128
+  const int half = threadIdx.x >> 6 & 1, i = l32, j = n0 + 16 * half + 8 * g;
+  const bool mine = threadIdx.x < 128 && i < a.m && j < a.n;
+  typename Frag<T>::V bias = {}, res = {};
+  f32x4 col[2] = {};
+  if (mine) {
+    col[0] = *reinterpret_cast<const f32x4*>(a.col_scale + j);
+    col[1] = *reinterpret_cast<const f32x4*>(a.col_scale + j + 4);
+    if (a.bias != nullptr) bias = *reinterpret_cast<const typename Frag<T>::V*>((const T*)a.bias + j);
+    if (a.residual != nullptr) res = *reinterpret_cast<const typename Frag<T>::V*>((const T*)a.residual + (int64_t)i * a.ld_res + j);
+  }
   i32x4 first[AHEAD];
 #pragma unroll
   for (int s = 0; s < AHEAD; ++s) first[s] = s < steps ? weight(s) : i32x4{0, 0, 0, 0};
@@ -235,25 +246,20 @@ __global__ __launch_bounds__(kBlock) void int8_rows_kernel(GemmKindArgs a, const
 #pragma unroll
   for (int q = 0; q < 4; ++q) sums[(wave * 4 + q) * 64 + lane] = i32x4{sum[4 * q], sum[4 * q + 1], sum[4 * q + 2], sum[4 * q + 3]};
   __syncthreads();
-  // 8 columns a thread: 128 threads
-  const int half = threadIdx.x >> 6 & 1, i = l32, j = n0 + 16 * half + 8 * g;
-  if (threadIdx.x >= 128 || i >= a.m || j >= a.n) return;
-  float z[8], col[8], more[8];
+  if (!mine) return;
+  float z[8], scales[8], add[8];
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     i32x4 t = sums[(2 * half + q) * 64 + lane];
 #pragma unroll
     for (int v = 1; v < 4; ++v) t += sums[(v * 4 + 2 * half + q) * 64 + lane];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) z[4 * q + e] = (float)t[e], more[4 * q + e] = 0.f;
+    for (int e = 0; e < 4; ++e) z[4 * q + e] = (float)t[e], scales[4 * q + e] = col[q][e], add[4 * q + e] = (float)bias[4 * q + e];
   }
-  take8(a.col_scale + j, col);
-  if (a.bias != nullptr) load8((const T*)a.bias + j, more);
-  finish_int8(a.act, scale[i], col, more, z);
+  finish_int8(a.act, scale[i], scales, add, z);
   if (a.residual != nullptr) {
-    load8((const T*)a.residual + (int64_t)i * a.ld_res + j, more);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) z[e] += more[e];
+    for (int e = 0; e < 8; ++e) z[e] += (float)res[e];
   }
   store8((T*)a.out + (int64_t)i * a.n + j, z);
 }
