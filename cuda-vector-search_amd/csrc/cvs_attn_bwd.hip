@@ -278,6 +278,8 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
     if (t0 < tiles) load(t0);
   }
 
+  constexpr bool kPlaces = WIN && DP == 128;
+  const uint32_t places_of[2] = {kPlaces ? wide_row_place() : 0, kPlaces ? wide_col_place() : 0};
   // the tiles that a row of this wave sees a key of; through the others it only loads its share
   int mine = r0 < nq ? tiles : t0;
   if (!WIN && a.causal) mine = max(t0, min(mine, (r0 + 32 + off + ROWS - 1) / ROWS));
@@ -291,10 +293,16 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
     float base[KB];
     const int near0 = tile0 - r0 - off;  // position of the tile's first key and the wave's first row
     V krows[KB][KS], vrows[KB][KS], kcols[KB][2][DB];
+    uint32_t row_place = 0, v_place = 0, col_place = 0;
+    if constexpr (kPlaces) {
+      row_place = lds_address(sk[buf]) + places_of[0], v_place = lds_address(sv[buf]) + places_of[0];
+      col_place = lds_address(sk[buf]) + places_of[1];
+      asm volatile("" : "+v"(row_place), "+v"(v_place), "+v"(col_place));
+    }
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) krows[kb][s] = row_frag<T, DP>(sk[buf], kb * 32, s);
+      for (int kb = 0; kb < KB; ++kb) krows[kb][s] = kPlaces ? wide_row_frag<T>(row_place, s) : row_frag<T, DP>(sk[buf], kb * 32, s);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       const int near = near0 + kb * 32;
@@ -316,7 +324,7 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) vrows[kb][s] = row_frag<T, DP>(sv[buf], kb * 32, s);
+        for (int kb = 0; kb < KB; ++kb) vrows[kb][s] = kPlaces ? wide_row_frag<T>(v_place, s) : row_frag<T, DP>(sv[buf], kb * 32, s);
     };
     auto read_kcols = [&]() {
 #pragma unroll
@@ -324,7 +332,8 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-          for (int d = 0; d < DB; ++d) kcols[kb][s][d] = col_frag<T, DP>(sk[buf], kb * 32 + 16 * s, d * 32);
+          for (int d = 0; d < DB; ++d)
+            kcols[kb][s][d] = kPlaces ? wide_col_frag<T>(col_place, 16 * s, d * 32) : col_frag<T, DP>(sk[buf], kb * 32 + 16 * s, d * 32);
     };
     if (DP <= 64) {
       keep_order();

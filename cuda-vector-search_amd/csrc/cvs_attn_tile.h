@@ -137,6 +137,29 @@ __device__ __forceinline__ typename Frag<T>::V col_frag(const unsigned char* lds
   return join_tr<T>(read_tr(at + row_offset<DP>(row, col >> 3)), read_tr(at + row_offset<DP>(row + 4, col >> 3)));
 }
 
+// The same operands of a tile of 32 rows of 128 columns, from this lane's place in it (kept in one register, and the
+// pieces' offsets, which the swizzle makes exclusive ors, taken from it anew: where all the offsets of a loop's
+// operands do not fit the registers).
+__device__ __forceinline__ uint32_t wide_row_place() {
+  const int lane = threadIdx.x & 63, row = tile_row(lane & 31);
+  return row * 256 + (((lane >> 5) ^ wide_swizzle(row)) << 4);
+}
+__device__ __forceinline__ uint32_t wide_col_place() {
+  const int lane = threadIdx.x & 63, p = lane >> 4, s = lane & 15;
+  const int c = ((s & 1) << 1) | ((s >> 1) & 1), row = 8 * (p >> 1) + (s >> 2);
+  return row * 256 + (((2 * (p & 1) + (c >> 1)) ^ wide_swizzle(row)) << 4) + (c & 1) * 8;
+}
+template <class T>
+__device__ __forceinline__ typename Frag<T>::V wide_row_frag(uint32_t at, int ks) {
+  return *(const __attribute__((address_space(3))) typename Frag<T>::V*)(uintptr_t)(at ^ (ks << 5));
+}
+template <class T>
+__device__ __forceinline__ typename Frag<T>::V wide_col_frag(uint32_t at, int r0, int c0) {
+  typedef __attribute__((address_space(3))) s16x4* P;
+  return join_tr<T>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(uintptr_t)((at ^ (c0 << 1)) + r0 * 256)),
+                    __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(uintptr_t)((at ^ (c0 << 1) ^ 16) + r0 * 256 + 1024)));
+}
+
 // B operand: column = row `row` of a head in memory (zeros when !in or past d), depth 16 ks + 8 (lane / 32) + 0 .. 7.
 template <class T>
 __device__ __forceinline__ typename Frag<T>::V global_frag(const unsigned char* row, int ks, int d, bool in) {
