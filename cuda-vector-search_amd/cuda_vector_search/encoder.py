@@ -421,16 +421,18 @@ def gated_linear_forward(x, gate, up, gate_bias=None, up_bias=None, activation="
     the gate's first, for the backward pass, None without ``keep_pre``."""
     given = (x, gate, up, gate_bias, up_bias)
     try:
-        key = ("gated", activation, *map(_form, given))
+        key = ("gated", activation, *map(_form, given)) if _tracing() is None else None  # (a trace's sizes are tensors)
         call = _known.get(key)
     except (AttributeError, TypeError):  # no tensors: the checks say which
         key = call = None
-    lib = _library()
-    if call is None or not _on16(*given):
+    if call is None:
         n, k = _gated_args(x, gate, up, activation)
         for name, bias in (("gate_bias", gate_bias), ("up_bias", up_bias)):
             if bias is not None:
                 _tensor(bias, name, x, (n,))
+    lib = _library()
+    if call is None or not _on16(*given):
+        n, k = gate.shape
         r = _rows(x, k, True)
         m, dev = r.shape[0], x.device.index
         gate, up, gate_bias, up_bias = (None if t is None else _packed(t) for t in (gate, up, gate_bias, up_bias))
@@ -560,7 +562,6 @@ def _int8_args(x, values, scales, bias, activation, residual):
         _tensor(bias, "bias", x, (n,))
     if residual is not None:
         _tensor(residual, "residual", x, (*x.shape[:-1], n))
-    return n, k
 
 
 @_serving
@@ -575,9 +576,11 @@ def linear_int8(x, values, scales, bias=None, activation=None, residual=None):
         call = _known.get(key)
     except (AttributeError, TypeError):  # no tensors: the checks say which
         key = call = None
+    if call is None:
+        _int8_args(x, values, scales, bias, activation, residual)
     lib = _library()
     if call is None or not _on16(*given):
-        n, k = _int8_args(x, values, scales, bias, activation, residual)
+        n, k = values.shape
         r = _rows(x, k, True)
         m, dev = r.shape[0], x.device.index
         values, scales, bias = (None if t is None else _packed(t) for t in (values, scales, bias))

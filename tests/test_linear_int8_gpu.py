@@ -85,7 +85,9 @@ def test_quantize_rows_not_finite_zero_and_views(eng):
 SIZES = [(1, 16, 8, None, F16), (1, 768, 2048, "gelu", F16), (3, 4096, 72, "tanh", BF16), (23, 384, 1536, "gelu", F16), (32, 2048, 200, "relu", F16),
          (33, 2048, 200, "relu", F16), (16, 8192, 640, None, BF16), (65, 144, 136, "tanh", F16), (300, 768, 104, "gelu", BF16),
          (404, 3728, 1240, None, F16), (2049, 272, 1000, "gelu", F16), (6478, 64, 1752, "gelu", BF16), (8486, 64, 912, "tanh", F16),
-         (1000, 4112, 64, None, BF16), (2, 131072, 16, None, F16)]
+         (1000, 4112, 64, None, BF16), (2, 131072, 16, None, F16),
+         # the most rows and depth of one launch, and past them
+         (32, 1792, 200, "gelu", BF16), (31, 1040, 72, None, F16), (14, 4112, 40, "relu", F16), (29, 2048, 64, None, BF16), (32, 16, 8, "tanh", F16)]
 
 
 @pytest.mark.parametrize("m,k,n,act,dtype", SIZES)

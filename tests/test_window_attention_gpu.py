@@ -72,6 +72,19 @@ def test_window_attention(eng, b, lq, lk, h, hk, d, dtype, buckets, causal, ragg
     hold(tensors, doubles, 1 / math.sqrt(d), dtype, before, after, sinks, lengths, causal=causal, max_distance=128)
 
 
+# sizes whose keys are walked in parts (forward, dq) and whose rows are (dk and dv, the first keys')
+PARTS = [(1, 130, 2000, 2, 2, 64, F16, 0, False, 1500, 300, 4), (1, 130, 2000, 2, 1, 128, BF16, 32, True, 1400, 0, 2),
+         (1, 3000, 3000, 1, 1, 64, F16, 0, False, 1000, 500, 5), (1, 2500, 2500, 2, 1, 128, BF16, 0, True, 1100, 0, 40),
+         (2, 7, 2600, 2, 2, 32, BF16, 32, False, 2000, 200, 70), (1, 1500, 1500, 2, 2, 96, F16, 16, False, 0, 20, 9)]
+
+
+@pytest.mark.parametrize("b,lq,lk,h,hk,d,dtype,buckets,causal,before,after,sinks", PARTS)
+def test_window_in_parts(eng, b, lq, lk, h, hk, d, dtype, buckets, causal, before, after, sinks):
+    say("window in parts", b, lq, lk, h, hk, d, dtype, buckets, causal, before, after, sinks)
+    tensors, doubles, lengths = attention_inputs(b, lq, lk, h, hk, d, dtype, buckets, False, seed=131)
+    hold(tensors, doubles, 1 / math.sqrt(d), dtype, before, after, sinks, lengths, causal=causal, max_distance=128)
+
+
 @pytest.mark.parametrize("lq,start", [(1, [0, 57, 199]), (4, [3, 100, 150]), (70, [-80, 0, 129]), (40, [-20, -39, 500]), (200, [-100, 150, 0])])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("before,after,sinks", [(30, 5, 0), (2, 80, 3), (0, 0, 0), (150, 0, 40)])
