@@ -98,6 +98,15 @@ __device__ __forceinline__ float wave_max(float v) {
 template <int DP>
 constexpr int kTile = DP > 64 ? 32 : 64;
 
+// A window's gradients round what the products take to 16 bits; dk's and dv's sums over many rows average those
+// roundings.  Of few rows they do not: there the products take what was rounded off too.
+__host__ __device__ __forceinline__ bool few_rows(const AttnArgs& a) { return (int64_t)a.lq * (a.heads / a.k_heads) < kAttnRows; }
+// Whether a window's delta is attn_delta_kernel's: that of a sequence whose keys fill no more than a tile the q kernel
+// makes from its own sums.
+__host__ __device__ __forceinline__ bool exact_delta(const AttnArgs& a, bool bias, int nk, int rows) {
+  return window_narrow(a) || ((bias || few_rows(a)) && nk > rows);
+}
+
 // dtable's sums.  A block of ds, laid out by position (row j - i + 31, pitch 36 words: column
 // writes and row reads without bank conflicts; places that no pair of the block has stay
 // zero), is added along the rows, a position a lane, in a fixed order.  (LDS atomics
@@ -119,6 +128,126 @@ __device__ __forceinline__ void take_positions(const float* skew, float* sums) {
   for (int q = 1; q < 8; ++q) s += from[q];
   sums[lane] += (s[0] + s[1]) + (s[2] + s[3]);
   __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+}
+
+// delta of a window's rows: sum p dp / sum p of the sums that the gradients themselves are made of; in a narrow
+// window peak + sum p (dp - peak) / sum p with the largest dp as peak: of one key it is dp itself, and ds is 0.
+// dout . out has out's rounding in it, some 2^-9 of |dout| |out|, which is all that is left in sums of ds that cancel:
+// the table's gradients, whose sum over a row's keys is 0 (of 2 heads, 166 keys back, an error of 3.1e-4 for 1.6e-4
+// in fp16), and those of few rows.  128 rows of a workgroup, 32 of a wave as columns; two products, so that four
+// workgroups' registers and LDS fit a CU and cover each other's waits for the tiles, which a pass within the
+// q kernel, two a CU, did not.
+template <class T, int DP, bool BIAS>
+__global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 4) void attn_delta_kernel(AttnArgs a) {
+  typedef typename Frag<T>::V V;
+  constexpr int KS = DP / 16, ROWS = kTile<DP>, KB = ROWS / 32, TILE = ROWS * DP * 2;
+  __shared__ __attribute__((aligned(1024))) unsigned char sk[2][TILE], sv[2][TILE];
+  extern __shared__ float tab[];  // bias by position
+
+  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int heads = a.batch * a.heads;
+  const int block = (a.lq + kAttnRows - 1) / kAttnRows - 1 - blockIdx.x / heads;  // (as the q kernel's)
+  const int bh = blockIdx.x % heads;
+  const int b = bh / a.heads, h = bh % a.heads, hk = h / (a.heads / a.k_heads);
+  const int nk = key_count(a, b), nq = query_count(a, b), off = query_offset(a, b);
+  if (!exact_delta(a, BIAS, nk, ROWS)) return;
+  const int r0 = block * kAttnRows + wave * 32, i = r0 + l32;
+  const unsigned char* qrow = (const unsigned char*)a.q + 2 * (b * a.qs[0] + i * a.qs[1] + h * a.qs[2]);
+  const unsigned char* grow = (const unsigned char*)a.dout + 2 * (b * a.dos[0] + i * a.dos[1] + h * a.dos[2]);
+  const unsigned char* kbase = (const unsigned char*)a.k + 2 * (b * a.ks[0] + hk * a.ks[2]);
+  const unsigned char* vbase = (const unsigned char*)a.v + 2 * (b * a.vs[0] + hk * a.vs[2]);
+  const int last_row = min(block * kAttnRows + kAttnRows, nq) - 1;
+  const WindowTiles<ROWS> win(a, nk, block * kAttnRows + off, last_row + off);
+  int row_first, row_end;  // the rows that see a key of a window
+  window_rows(a, nk, nq, off, row_first, row_end);
+  const TileLoad<DP, ROWS> lk(2 * a.ks[1], a.d), lv(2 * a.vs[1], a.d);
+  auto load = [&](int t) {
+    const int first = win.tile(t) * ROWS;
+    lk.load_window(kbase, 2 * a.ks[1], first, win.end, sk[t & 1], win.low, win.head);
+    lv.load_window(vbase, 2 * a.vs[1], first, win.end, sv[t & 1], win.low, win.head);
+  };
+  BiasLoad<T> bias;
+  if (BIAS) bias.buckets(a);
+  if (win.count > 0) load(0);
+  V qf[KS], gf[KS];
+  const bool in = i >= row_first && i < row_end;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    qf[s] = global_frag<T>(qrow, s, a.d, in);
+    gf[s] = global_frag<T>(grow, s, a.d, in);
+  }
+  const int64_t row_at = (int64_t)bh * a.lq + i;
+  float lse = in ? a.lse[row_at] * kLog2e : kNever;
+  if (BIAS) {
+    bias.values(a, h);
+    bias.store(a, tab);
+  }
+  const int reach = a.far + kReach;
+  const bool blind = !in || lse == -__builtin_inff();  // a row that sees nothing
+  if (blind) lse = kNever;
+  const float c = a.scale * kLog2e;
+  const bool narrow = window_narrow(a);
+  float sp = 0.f, spd = 0.f, peak = narrow ? -kNever : 0.f;
+  for (int t = 0; t < win.count; ++t) {
+    tile_barrier();
+    if (t + 1 < win.count) load(t + 1);
+    const int tile0 = win.tile(t) * ROWS;
+    if (r0 >= nq) continue;
+#pragma unroll 1
+    for (int kb = 0; kb < KB; ++kb) {
+      const int j0 = tile0 + kb * 32, near = j0 - r0 - off;
+        if (!window_meets(a, j0, 32, r0 + off, min(r0 + 31, nq - 1) + off)) continue;
+      V krows[KS], vrows[KS];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) krows[s] = row_frag<T, DP>(sk[t & 1], kb * 32, s);
+      f32x16 p = zero16(), dp = zero16();
+      float base = -lse;
+      if (BIAS) {
+        if (near - 31 >= a.far || near + 31 <= -a.far) {
+          base += tab[near > 0 ? 2 * reach : 0] * c;
+        } else {
+          const float* at = tab + (near - l32 + 8 * g + reach);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) p[e] = at[elem_row(e, 0)];
+        }
+      }
+      keep_order();
+#pragma unroll
+      for (int s = 0; s < KS; ++s) vrows[s] = row_frag<T, DP>(sv[t & 1], kb * 32, s);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) p = Frag<T>::mfma(krows[s], qf[s], p);
+      keep_order();
+#pragma unroll
+      for (int s = 0; s < KS; ++s) dp = Frag<T>::mfma(vrows[s], gf[s], dp);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], c, base));
+      if (j0 + 32 > nk || near + 31 > a.after || near < 31 - a.before) {
+        WindowMask(a, nk, i + off, j0 + 8 * g).apply(p, 0, j0 < a.sinks, 0.f);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dp[e] = p[e] > 0.f ? dp[e] : peak;
+      }
+      if (narrow) {
+        float top = -kNever;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = p[e] > 0.f ? fmaxf(top, dp[e]) : top;
+        top = fmaxf(peak, halves_max(top));
+        if (top > peak) {
+          spd = peak == -kNever ? 0.f : fmaf(sp, peak - top, spd);
+          peak = top;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dp[e] = p[e] > 0.f ? dp[e] - peak : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        sp += p[e];
+        spd = fmaf(p[e], dp[e], spd);
+      }
+    }
+  }
+  sp = halves_sum(sp), spd = halves_sum(spd);
+  if (i < a.lq && g == 0) a.delta[row_at] = !blind && sp > 0.f ? (narrow ? peak + spd / sp : spd / sp) : 0.f;
 }
 
 // delta, dq of 128 queries (wave w: 32 of them as columns), and their sums for dtable.  The queries'
@@ -160,13 +289,14 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
   WindowTiles<ROWS> win;
   int row_first, row_end;  // the rows that see a key of a window
   const bool narrow = WIN && window_narrow(a);
+  const bool exact = WIN && exact_delta(a, BIAS, nk, ROWS);  // attn_delta_kernel's
   // this wave's rows see keys of the first tile only
   bool one = (a.causal ? min(nk, r0 + 32 + off) : nk) <= ROWS;
   if constexpr (WIN) {
     win = WindowTiles<ROWS>(a, nk, block * kAttnRows + off, last_row + off);
     all = win.count;
     window_rows(a, nk, nq, off, row_first, row_end);
-    one = !narrow && (one || (!a.causal && min(nk, max(r0 + 32 + off + a.after, a.sinks)) <= ROWS));
+    one = !exact && (one || (!a.causal && min(nk, max(r0 + 32 + off + a.after, a.sinks)) <= ROWS));
   }
   // this workgroup's part of the tiles (fewer than 2^24, at most 64 parts); the first part writes
   // delta, or, where the wave's rows take it from the first tile, the part that has it
@@ -175,7 +305,7 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
     t0 = (int)((unsigned)all * blockIdx.y / (unsigned)a.q_parts);
     tiles = (int)((unsigned)all * (blockIdx.y + 1) / (unsigned)a.q_parts);
   }
-  const bool writes_delta = one && all > 0 ? t0 == 0 && tiles > 0 : blockIdx.y == 0;
+  const bool writes_delta = exact ? false : one && all > 0 ? t0 == 0 && tiles > 0 : blockIdx.y == 0;
   BiasLoad<T> bias;
   if (BIAS) bias.buckets(a);
   const TileLoad<DP, ROWS> lk(2 * a.ks[1], a.d), lv(2 * a.vs[1], a.d);
@@ -218,6 +348,7 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
 #pragma unroll
     for (int j = 0; j < 8; ++j) delta = fmaf((float)gf[s][j], (float)of[s][j], delta);
   delta = one ? 0.f : halves_sum(delta);
+  if (WIN && exact) delta = in ? a.delta[row_at] : 0.f;
   const bool blind = !in || lse == -__builtin_inff();  // a row that sees nothing
   if (blind) lse = kNever;
 
@@ -226,57 +357,7 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
   for (int d = 0; d < DB; ++d) dq[d] = zero16();
   const float c = a.scale * kLog2e;
   Lifted col = {kLift<T>};  // of this column's probabilities and ds
-
-  if (WIN && narrow) {
-    // delta = peak + sum p (dp - peak) / sum p with the largest dp as peak: of one key it is dp itself
-    float sp = 0.f, spd = 0.f, peak = -kNever;
-    for (int t = 0; t < all; ++t) {  // (one part)
-      tile_barrier();
-      if (t + 1 < all) load(t + 1);
-      const int tile0 = win.tile(t) * ROWS;
-      if (r0 >= nq || !window_meets(a, tile0, ROWS, r0 + off, min(r0 + 31, nq - 1) + off)) continue;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        const int j0 = tile0 + kb * 32, near = j0 - r0 - off;
-        f32x16 p = zero16(), dp = zero16();
-        float base = -lse;
-        if (BIAS) {
-          if (near - 31 >= a.far || near + 31 <= -a.far) {
-            base += tab[near > 0 ? 2 * reach : 0] * c;
-          } else {
-            const float* at = tab + (near - l32 + 8 * g + reach);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) p[e] = at[elem_row(e, 0)];
-          }
-        }
-#pragma unroll
-        for (int s = 0; s < KS; ++s) p = Frag<T>::mfma(row_frag<T, DP>(sk[t & 1], kb * 32, s), qf[s], p);
-#pragma unroll
-        for (int s = 0; s < KS; ++s) dp = Frag<T>::mfma(row_frag<T, DP>(sv[t & 1], kb * 32, s), gf[s], dp);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], c, base));
-        const WindowMask mask(a, nk, i + off, j0 + 8 * g);
-        mask.apply(p, 0, j0 < a.sinks, 0.f);
-        float top = -kNever;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) top = p[e] > 0.f ? fmaxf(top, dp[e]) : top;
-        top = fmaxf(peak, halves_max(top));
-        if (top > peak) {
-          spd = peak == -kNever ? 0.f : fmaf(sp, peak - top, spd);
-          peak = top;
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          sp += p[e];
-          spd = fmaf(p[e], p[e] > 0.f ? dp[e] - peak : 0.f, spd);
-        }
-      }
-    }
-    sp = halves_sum(sp), spd = halves_sum(spd);
-    delta = sp > 0.f ? peak + spd / sp : 0.f;
-    tile_barrier();
-    if (t0 < tiles) load(t0);
-  }
+  float left = 0.f;         // sum of ds so far, of which delta's own rounding would leave nothing
 
   constexpr bool kPlaces = WIN && DP == 128;
   const uint32_t places_of[2] = {kPlaces ? wide_row_place() : 0, kPlaces ? wide_col_place() : 0};
@@ -401,6 +482,10 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
 #pragma unroll
         for (int e = 0; e < 16; ++e) ds[kb][e] -= delta;
     }
+    if constexpr (WIN) {  // past both branches: the compiler leaves an 8-pass product 11 wait states, which takes 12
+      asm volatile("s_nop 0");
+      keep_order();
+    }
     if constexpr (kLift<T> != 0) {
       float top = 0.f;
 #pragma unroll
@@ -418,6 +503,12 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
       if constexpr (kLift<T> == 0) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) ds[kb][e] *= p[kb][e];
+      }
+      if constexpr (WIN && !BIAS) {
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s += ds[kb][e];
+        left = kLift<T> == 0 ? left + s : fmaf(s, col.unit, left);
       }
       if (BIAS) {
         if (in_range) {
@@ -445,6 +536,11 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
         const V df = pack8<T>(ds[kb], s);
 #pragma unroll
         for (int d = 0; d < DB; ++d) dq[d] = Frag<T>::mfma(kcols[kb][s][d], df, dq[d]);
+        if constexpr (WIN) {
+          const V rest = pack8_rest<T>(ds[kb], s, df);
+#pragma unroll
+          for (int d = 0; d < DB; ++d) dq[d] = Frag<T>::mfma(kcols[kb][s][d], rest, dq[d]);
+        }
       }
       if (BIAS) {
         keep_order();
@@ -455,6 +551,12 @@ __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) 
   for (int t = mine; t < tiles; ++t) {
     tile_barrier();
     if (t + 1 < tiles) load(t + 1);
+  }
+  // ds sums to 0 over a row's keys: what is left is delta's error, from the rounded `out`, times the probabilities'
+  // sum of 1, and dk and dv are made without it (unless a NaN that other rows see is in it)
+  if (WIN && !BIAS && !exact && !one && a.q_parts == 1) {
+    left = halves_sum(left) * kUnlift<T>;
+    delta += fabsf(left) < kNever ? left : 0.f;
   }
   if (blind) {  // (the sums may be NaN: 0 times a value that other rows see)
     delta = 0.f;
@@ -534,7 +636,7 @@ __device__ __forceinline__ void add_table(const AttnArgs& a, int at) {
 // `id` of these is one of the kv kernel's launch, whose others hide its waits: its kernel of its own took 20 us of
 // 8 sequences of up to 2048, 12 heads of 64, and as many of 8192 rows, 16 heads on 4 of 128.
 // tq, tg: four tiles of 32 rows of q and of dout; slse, sdelta: of 32 values.
-template <class T, int DP, bool BIAS>
+template <class T, int DP, bool BIAS, bool REST>
 __device__ __forceinline__ void sink_gradients(const AttnArgs& a, int id, unsigned char* tq, unsigned char* tg, float* slse, float* sdelta) {
   typedef typename Frag<T>::V V;
   constexpr int KS = DP / 16, DB = DP / 32, TILE = 32 * DP * 2;
@@ -654,6 +756,14 @@ __device__ __forceinline__ void sink_gradients(const AttnArgs& a, int id, unsign
         dv[d] = Frag<T>::mfma(gcols[s][d], pf, dv[d]);
         dk[d] = Frag<T>::mfma(qcols[s][d], df, dk[d]);
       }
+      if constexpr (REST) {
+        const V pr = pack8_rest<T>(p, s, pf), dr = pack8_rest<T>(ds, s, df);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          dv[d] = Frag<T>::mfma(gcols[s][d], pr, dv[d]);
+          dk[d] = Frag<T>::mfma(qcols[s][d], dr, dk[d]);
+        }
+      }
     }
   }
   // join the waves: dk, then dv, each wave's [32 columns][DP] in the place of two tiles, the pieces of 4 in an order by column
@@ -708,7 +818,7 @@ __device__ __forceinline__ void sink_gradients(const AttnArgs& a, int id, unsign
 // one wave a SIMD then, whose products (37% of the time), exponentials and packing follow one
 // another.  2 x 4096, 16 heads on 4 of 128, causal: 329 us, 0.84 PFLOP/s of its four products;
 // 64 x 512, 12 heads of 64, two workgroups a CU: 148 us, with a bias 156.
-template <class T, int DP, bool BIAS, bool WIN>
+template <class T, int DP, bool BIAS, bool WIN, bool REST>
 __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kernel(AttnArgs a, int key_wgs, int sink_wgs) {
   typedef typename Frag<T>::V V;
   constexpr int KS = DP / 16, DB = DP / 32, ROWS = 64, QB = ROWS / 32, TILE = ROWS * DP * 2;
@@ -720,7 +830,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if constexpr (WIN) {  // (after the others, whose CUs are free at different times)
     if ((int)blockIdx.x >= key_wgs && (int)blockIdx.x < key_wgs + sink_wgs) {
-      if (blockIdx.y == 0) sink_gradients<T, DP, BIAS>(a, (int)blockIdx.x - key_wgs, sq[0], sg[0], slse[0], sdelta[0]);
+      if (blockIdx.y == 0) sink_gradients<T, DP, BIAS, REST>(a, (int)blockIdx.x - key_wgs, sq[0], sg[0], slse[0], sdelta[0]);
       return;
     }
   }
@@ -824,11 +934,11 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
     for (int t = mine; t < last; ++t) {
       const int buf = t & 1;
       turn(t);
-      if (WIN && (t * ROWS > j0 + 31 - off + a.before || t * ROWS + ROWS <= j0 - off - a.after)) continue;
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
         const int i0 = t * ROWS + qb * 32;
         const int near = j0 - i0 - off;
+        if (WIN && (near + 31 < -a.before || near - 31 > a.after)) continue;
         V qrows[KS], grows[KS], qcols[2][DB], gcols[2][DB];
         f32x16 p, ds, base;
         float shift = 0.f;
@@ -899,6 +1009,14 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kern
           for (int d = 0; d < DB; ++d) {
             dv[d] = Frag<T>::mfma(gcols[s][d], pf, dv[d]);
             dk[d] = Frag<T>::mfma(qcols[s][d], df, dk[d]);
+          }
+          if constexpr (REST) {
+            const V pr = pack8_rest<T>(p, s, pf), dr = pack8_rest<T>(ds, s, df);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+              dv[d] = Frag<T>::mfma(gcols[s][d], pr, dv[d]);
+              dk[d] = Frag<T>::mfma(qcols[s][d], dr, dk[d]);
+            }
           }
         }
       }
@@ -975,14 +1093,25 @@ template <class T, int DP, bool BIAS, bool WIN>
 hipError_t launch_window(const AttnArgs& a, hipStream_t s) {
   const int64_t qblocks = (a.lq + kAttnRows - 1) / kAttnRows, kblocks = (a.lk + kAttnRows - 1) / kAttnRows;
   const size_t tab = BIAS ? (2 * (a.far + kReach) + 1) * sizeof(float) : 0;
-  if (qblocks > 0)
-    hipLaunchKernelGGL((attn_backward_q_kernel<T, DP, BIAS, WIN>), dim3((unsigned)(qblocks * a.batch * a.heads), a.q_parts),
-                       dim3(kBlock), 5 * tab, s, a);
+  // (also where delta keeps out's rounding: dq's parts do not sum up a row's ds)
+  const bool rests = WIN && (few_rows(a) || a.q_parts > 1);
+  if (qblocks > 0) {
+    const dim3 grid((unsigned)(qblocks * a.batch * a.heads), a.q_parts);
+    if constexpr (WIN) {
+      if (exact_delta(a, BIAS, a.lk, kTile<DP>))
+        hipLaunchKernelGGL((attn_delta_kernel<T, DP, BIAS>), dim3(grid.x), dim3(kBlock), tab, s, a);
+    }
+    hipLaunchKernelGGL((attn_backward_q_kernel<T, DP, BIAS, WIN>), grid, dim3(kBlock), 5 * tab, s, a);
+  }
   const int64_t sink_wgs = WIN ? (int64_t)(a.sinks + 31) / 32 * a.batch * a.k_heads * a.sink_parts : 0;
   const int64_t key_wgs = kblocks * a.batch * a.k_heads, all_wgs = sink_wgs + key_wgs + (BIAS ? (a.buckets * a.heads + 3) / 4 : 0);
-  if (all_wgs > 0)
-    hipLaunchKernelGGL((attn_backward_kv_kernel<T, DP, BIAS, WIN>), dim3((unsigned)all_wgs, a.kv_parts), dim3(kBlock), tab, s, a,
-                       (int)key_wgs, (int)sink_wgs);
+  if (all_wgs > 0) {
+    const dim3 grid((unsigned)all_wgs, a.kv_parts);
+    if (rests)
+      hipLaunchKernelGGL((attn_backward_kv_kernel<T, DP, BIAS, WIN, WIN>), grid, dim3(kBlock), tab, s, a, (int)key_wgs, (int)sink_wgs);
+    else
+      hipLaunchKernelGGL((attn_backward_kv_kernel<T, DP, BIAS, WIN, false>), grid, dim3(kBlock), tab, s, a, (int)key_wgs, (int)sink_wgs);
+  }
   auto join = [&](const float* part, int parts, int64_t n, int sums, float scale, void* out0, void* out1) {
     const dim3 grid((unsigned)((n / 8 + kBlock - 1) / kBlock), sums);
     hipLaunchKernelGGL(attn_join_grads_kernel<T>, grid, dim3(kBlock), 0, s, part, parts, sums * n, n, scale, (T*)out0, (T*)out1);

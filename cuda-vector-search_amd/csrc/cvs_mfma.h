@@ -116,6 +116,15 @@ __device__ __forceinline__ typename Frag<T>::V pack8(const f32x16& v, int s) {
   return r;
 }
 
+// What pack8 rounded off, as a second operand.
+template <class T>
+__device__ __forceinline__ typename Frag<T>::V pack8_rest(const f32x16& v, int s, const typename Frag<T>::V& packed) {
+  typename Frag<T>::V r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = (T)(v[8 * s + j] - (float)packed[j]);
+  return r;
+}
+
 // Maximum and sum of lane l's value and lane l ^ 32's.
 __device__ __forceinline__ float halves_max(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
