@@ -366,6 +366,11 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_rows_kernel(Attn
       const V p = pack8<T>(x, s);
 #pragma unroll
       for (int d = 0; d < DB; ++d) acc[d] = Frag<T>::mfma(cols[s][d], p, acc[d]);
+      if constexpr (WIN) {  // (of one row, p's rounding does not average out; hidden behind the keys' loads)
+        const V rest = pack8_rest<T>(x, s, p);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[d] = Frag<T>::mfma(cols[s][d], rest, acc[d]);
+      }
     }
   }
   // join the waves: sums relative to the largest of their m, column by column

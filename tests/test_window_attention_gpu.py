@@ -85,6 +85,31 @@ def test_window_in_parts(eng, b, lq, lk, h, hk, d, dtype, buckets, causal, befor
     hold(tensors, doubles, 1 / math.sqrt(d), dtype, before, after, sinks, lengths, causal=causal, max_distance=128)
 
 
+# A value rounded once is off by at most U relative to it, evenly: a tensor so rounded by at most U / sqrt(3) of its norm.
+# Where the products take p and ds in 16 bits, those roundings are as large and independent: sqrt(2) times that.  The
+# second sum of squares is of few values, or falls on few p: 5 standard deviations of a mean of 1000 evenly spread
+# squares (sqrt(0.8 / 1000) each) give 1.07, and fp32 sums add less than a thousandth.
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("b,lq,lk,h,hk,d,buckets,causal,before,after,sinks", [
+    (8, 1, 700, 2, 2, 64, 0, False, 20, 200, 0), (16, 1, 500, 2, 1, 64, 32, True, 245, 0, 4), (4, 3, 300, 4, 4, 128, 0, True, 260, 0, 0),
+    (3, 600, 900, 16, 8, 32, 64, True, 166, 0, 0), (2, 500, 500, 16, 16, 64, 32, False, 90, 90, 1), (1, 700, 700, 4, 2, 128, 0, True, 300, 0, 4)])
+def test_window_errors_are_the_roundings(eng, dtype, b, lq, lk, h, hk, d, buckets, causal, before, after, sinks):
+    say("window errors", dtype, b, lq, lk, h, hk, d, buckets, causal, before, after, sinks)
+    (q, k, v, do, table), (qd, kd, vd, dod, td), _ = attention_inputs(b, lq, lk, h, hk, d, dtype, buckets, False, seed=136)
+    args = dict(causal=causal, max_distance=128)
+    want = lo.window_attention(qd, kd, vd, dod, d**-0.5, dtype, before, after, sinks, td, **args)
+    out, lse = encoder.attention_forward(q, k, v, table, window=(before, after), sinks=sinks, scale=d**-0.5, **args)
+    got = encoder.attention_backward(do, q, k, v, out, lse, table, window=(before, after), sinks=sinks, scale=d**-0.5, **args)
+    few = lq * (h // hk) < 128
+    for name, a in zip(("out", *GRADS), (out, *got)):
+        if a is None:
+            continue
+        exact = want[name][0].double()
+        roundings = 1 if few or name in ("dq", "dtable") else 2
+        off = float((a.double().cpu() - exact).norm() / exact.norm())
+        assert off <= 1.07 * o.U[dtype] * math.sqrt(roundings / 3), (name, off / o.U[dtype])
+
+
 @pytest.mark.parametrize("lq,start", [(1, [0, 57, 199]), (4, [3, 100, 150]), (70, [-80, 0, 129]), (40, [-20, -39, 500]), (200, [-100, 150, 0])])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("before,after,sinks", [(30, 5, 0), (2, 80, 3), (0, 0, 0), (150, 0, 40)])
