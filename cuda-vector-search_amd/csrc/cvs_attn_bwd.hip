@@ -656,10 +656,10 @@ __device__ __forceinline__ void sink_gradients(const AttnArgs& a, int id, unsign
   unsigned char *sq = tq + wave * TILE, *sg = tg + wave * TILE;
   slse += wave * 32, sdelta += wave * 32;
 
-  // row tiles of all heads in a row (fewer than 2^25); this part's, of which each wave takes every fourth
+  // row tiles of all heads in a row (fewer than 2^31: their results lie in memory); this part's, of which each wave takes every fourth
   const int t0 = (a.causal ? max(row0, j0 - off) : row0) / 32;
   const unsigned nt = row0 < row1 && j0 < heads_seen ? max((row1 + 31) / 32 - t0, 0) : 0;
-  const unsigned all = nt * group, f0 = all * part / a.sink_parts, f1 = all * (part + 1) / a.sink_parts;
+  const unsigned all = nt * group, f0 = (uint64_t)all * part / a.sink_parts, f1 = (uint64_t)all * (part + 1) / a.sink_parts;
   const TileLoad<DP, 32, 1> lq(2 * a.qs[1], a.d), lg(2 * a.dos[1], a.d);
   float stat = 0.f;  // lanes 0 .. 31: -log2 sum of a row, the others: -delta
   auto load = [&](unsigned f) {
