@@ -84,8 +84,8 @@ hipError_t launch_gemm_pair(const GemmArgs& a, const GemmPlan& pa, const GemmArg
 // dz [m, 2 n] times both weights.
 GemmPlan plan_gated(int64_t m, int64_t n, int64_t k, int cus);
 hipError_t launch_gated(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s);
-GemmPlan plan_two_parts(int64_t m, int64_t n, int64_t k, int cus);
-hipError_t launch_two_parts(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s);
+GemmPlan plan_two_parts(int64_t m, int64_t n, int64_t k, bool rests, int cus);
+hipError_t launch_two_parts(const GemmKindArgs& a, const GemmPlan& p, bool rests, hipStream_t s);
 
 // dz = [dy up act'(gate), dy act(gate)] ([m, 2 n], contiguous) of pre = [gate, up], and dz's column sums.
 struct GatedGradArgs {
@@ -100,7 +100,14 @@ struct GatedGradArgs {
   void* dup_bias;
   float* partial;         // [parts, 2, n] when either is not null
   int parts;
+  bool rests;             // dz is [2 m, 2 n]: what rounding took off its rows behind them
+  const void* x;          // and x is copied to twice [2 m, k], to go with them, or null
+  int64_t x_stride;
+  int k;
+  void* twice;
 };
+// Of so few rows what dz loses to 16 bits is kept (cvs_gated.hip).
+inline bool gated_few_rows(int64_t m) { return m <= 32; }
 int gated_grad_parts(int64_t m, int64_t n, int cus);
 hipError_t launch_gated_grad(const GatedGradArgs& a, hipStream_t s);
 

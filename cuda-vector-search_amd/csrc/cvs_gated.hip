@@ -61,15 +61,16 @@ __global__ __launch_bounds__(kBlock) void gated_join_kernel(GemmKindArgs a) {
   store8((T*)a.out + i * a.n + j, h);
 }
 
+// (halves: the second half of the rows is what rounding took off the first)
 template <class T>
-__global__ __launch_bounds__(kBlock) void two_parts_join_kernel(GemmKindArgs a) {
-  const int64_t at = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * 8, plane = (int64_t)a.m * a.n;
+__global__ __launch_bounds__(kBlock) void two_parts_join_kernel(GemmKindArgs a, int halves) {
+  const int64_t at = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * 8, plane = (int64_t)a.m / halves * a.n;
   if (at >= plane) return;
   float z[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) z[e] = 0.f;
   const float* p = a.partial + at;
-  for (int s = 0; s < a.splits; ++s, p += plane) {
+  for (int s = 0; s < a.splits * halves; ++s, p += plane) {
     const f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 4);
 #pragma unroll
     for (int e = 0; e < 4; ++e) z[e] += lo[e], z[4 + e] += hi[e];
@@ -100,7 +101,7 @@ hipError_t gated(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s) {
 }
 
 template <class T>
-hipError_t two_parts(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s) {
+hipError_t two_parts(const GemmKindArgs& a, const GemmPlan& p, bool rests, hipStream_t s) {
   if (p.tile == 256 && p.tile_n == 256)
     launch_tiles<T, 4, 2, 2, 4, 2, 1, true, kTwoParts>(a, s);
   else if (p.tile == 256)
@@ -111,7 +112,7 @@ hipError_t two_parts(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s) {
     launch_tiles<T, 2, 2, 1, 1, 3, 2, true, kTwoParts>(a, s);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
-  hipLaunchKernelGGL(two_parts_join_kernel<T>, join_grid(a), dim3(kBlock), 0, s, a);
+  hipLaunchKernelGGL(two_parts_join_kernel<T>, join_grid(a), dim3(kBlock), 0, s, a, rests ? 2 : 1);
   return hipGetLastError();
 }
 
@@ -145,8 +146,22 @@ __device__ __forceinline__ void gate_grads8(const float* dy, const float* g, con
 // Pieces of 8 columns of a workgroup, as act_grad_kernel's: few for few rows.
 __host__ __device__ inline int gated_grad_width(int64_t m, int n) { return m <= 256 ? 16 : min(n / 8, kBlock); }
 
-// dz and its column sums, bound by memory: three values in, two out.  A workgroup has up to 256
-// pieces of 8 columns (blockIdx.x) and as many of its part's rows at a time as its threads cover.
+// What rounding to T took off 8 values; nothing of those that it made infinite.
+template <class T>
+__device__ __forceinline__ void rest8(float* v) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float left = v[e] - (float)(T)v[e];
+    v[e] = fabsf(left) < __builtin_inff() ? left : 0.f;
+  }
+}
+
+// dz and its column sums, bound by memory: three values in, two out (16384 rows of 2 x 2048 61 us, 5.5 TB/s).  A
+// workgroup has up to 256 pieces of 8 columns (blockIdx.x) and as many of its part's rows at a time as its
+// threads cover.  The products take dz in 16 bits, and sums over many rows and columns average what that loses: dx and the
+// weights' gradients are sqrt(2) times as far off as rounding them alone makes them.  Of few rows they may
+// be further off (one row of 384 features 1.66 times), so there dz's rounding errors are 16-bit rows of their own, behind
+// its rows: up to 32 rows the products' tiles and stages of 64 hold both without another one.
 template <class T>
 __global__ __launch_bounds__(kBlock) void gated_grad_kernel(GatedGradArgs a) {
   __shared__ float red[kBlock * 8];
@@ -181,8 +196,21 @@ __global__ __launch_bounds__(kBlock) void gated_grad_kernel(GatedGradArgs a) {
           store8((T*)a.dz + row * 2 * a.n + a.n + c, du);
 #pragma unroll
           for (int e = 0; e < 8; ++e) sum[0][e] += dg[e], sum[1][e] += du[e];
+          if (a.rests) {
+            rest8<T>(dg), rest8<T>(du);
+            store8((T*)a.dz + (a.m + row) * 2 * a.n + c, dg);
+            store8((T*)a.dz + (a.m + row) * 2 * a.n + a.n + c, du);
+          }
         }
       }
+    }
+  }
+  if (a.rests && a.x != nullptr) {
+    const int64_t pieces_x = a.k / 8, all = a.m * pieces_x, step = (int64_t)gridDim.x * kBlock;
+    for (int64_t t = (int64_t)blockIdx.x * kBlock + threadIdx.x; t < all; t += step) {
+      const u32x4 v = *reinterpret_cast<const u32x4*>((const T*)a.x + t / pieces_x * a.x_stride + t % pieces_x * 8);
+      reinterpret_cast<u32x4*>(a.twice)[t] = v;
+      reinterpret_cast<u32x4*>(a.twice)[all + t] = v;
     }
   }
   if (a.dgate_bias == nullptr && a.dup_bias == nullptr) return;
@@ -218,13 +246,15 @@ hipError_t launch_gated(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s)
   return a.type == kF16 ? gated<_Float16>(a, p, s) : gated<__bf16>(a, p, s);
 }
 
-GemmPlan plan_two_parts(int64_t m, int64_t n, int64_t k, int cus) {
+GemmPlan plan_two_parts(int64_t m, int64_t n, int64_t k, bool rests, int cus) {
   static constexpr TileChoice kTiles[] = {{256, 256, 1, 512, 1.8}, {256, 192, 1, 512, 1.7}, {128, 128, 2, 256, 1.2}, {64, 64, 3, 256, 0.9}};
-  return plan_tiles(kTiles, 4, m, n, 2 * ((k + kDepth - 1) / kDepth), 1, cus);
+  GemmPlan p = plan_tiles(kTiles, 4, m, n, 2 * ((k + kDepth - 1) / kDepth), 1, cus);
+  if (rests && p.splits == 1) p.splits = 2, p.ws_bytes = 2 * m * n * 4;  // (the join adds the halves; there are two stages at least)
+  return p;
 }
 
-hipError_t launch_two_parts(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s) {
-  return a.type == kF16 ? two_parts<_Float16>(a, p, s) : two_parts<__bf16>(a, p, s);
+hipError_t launch_two_parts(const GemmKindArgs& a, const GemmPlan& p, bool rests, hipStream_t s) {
+  return a.type == kF16 ? two_parts<_Float16>(a, p, rests, s) : two_parts<__bf16>(a, p, rests, s);
 }
 
 int gated_grad_parts(int64_t m, int64_t n, int cus) {

@@ -60,6 +60,34 @@ def test_gated_linear(eng, m, k, n, act, dtype):
                 assert a is None
 
 
+# A value rounded once is off by at most U relative to it, evenly: a tensor so rounded by at most U / sqrt(3) of its norm (5
+# standard deviations of a mean of 1000 squares, sqrt(0.8 / 1000) each, give 1.07).  Up to 32 rows nothing else is
+# rounded to 16 bits (fp16's subnormals and fp32 sums are below a hundredth of it here); of more rows dz is.
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("m,k,n,act", [(1, 1024, 384, "silu"), (2, 1000, 64, "sigmoid"), (6, 1536, 8, "relu"), (8, 1000, 4096, "tanh"),
+                                       (32, 384, 200, "gelu"), (33, 384, 200, None), (3, 8192, 16, "silu")])
+def test_gated_gradients_errors_are_the_roundings(eng, dtype, m, k, n, act):
+    say("gated errors", m, k, n, act, dtype)
+    (x, xd), (wg, wgd), (wu, wud), (bg, _), (bu, _), (dy, dyd) = inputs(m, k, n, dtype, seed=67)
+    _, pre = encoder.gated_linear_forward(x, wg, wu, bg, bu, act, keep_pre=True)
+    want = lo.gated_grads(dyd, xd, wgd, wud, pre.double().cpu(), act)
+    for name, a, r in list(zip(NAMES, encoder.gated_linear_backward(dy, x, wg, wu, pre, act), want))[:3]:
+        off = float((a.double().cpu() - r).norm() / r.norm())
+        assert off <= 1.08 * o.U[dtype] * math.sqrt((1 if m <= 32 else 2) / 3), (name, off / o.U[dtype])
+
+
+def test_gated_gradients_past_the_type(eng):
+    """Of few rows too, what rounding makes infinite stays so, and NaN reaches its own rows' results only."""
+    x, g, u = (torch.ones(s, dtype=F16, device="cuda") for s in ((2, 16), (8, 16), (8, 16)))
+    pre = torch.full((2, 16), 300.0, dtype=F16, device="cuda")
+    dy = torch.full((2, 8), 300.0, dtype=F16, device="cuda")
+    dx = encoder.gated_linear_backward(dy, x, g, u, pre, None)[0]
+    assert torch.isposinf(dx).all()
+    dy[1] = math.nan
+    dx, dg, du = encoder.gated_linear_backward(dy, x, g, u, pre, None)[:3]
+    assert torch.isposinf(dx[0]).all() and dx[1].isnan().all() and dg.isnan().all() and du.isnan().all()
+
+
 def test_gated_linear_halves_of_one_weight_and_shapes(eng):
     """Weights that are halves of one, or stored the other way; rows that are views."""
     big, bigd = rand((6, 40, 600), 16, F16)
