@@ -335,3 +335,54 @@ def test_layer_on_other_streams_and_graph_replays(eng):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, want))
         assert all(torch.equal(a, b) for a, b in zip(step(), want))
+
+
+def test_few_rows_on_two_streams_and_in_graphs(eng):
+    """Calls of few rows, narrow windows and split key axes, at once on two streams and as two graphs whose replays alternate:
+    each has its own scratch, and changed inputs are read anew."""
+    torch.manual_seed(11)
+
+    def make(lq, h, d, dtype, buckets, before, sinks):
+        q, do = (torch.randn(2, lq, h, d, device="cuda").to(dtype) for _ in range(2))
+        k, v = (torch.randn(2, 1300, h, d, device="cuda").to(dtype) for _ in range(2))
+        table = torch.randn(buckets, h, device="cuda").to(dtype) if buckets else None
+        x, dy = torch.randn(lq, 64, device="cuda").to(dtype), torch.randn(lq, 40, device="cuda").to(dtype)
+        gate, up = (torch.randn(40, 64, device="cuda").to(dtype) for _ in range(2))
+        more = dict(causal=True, window=(before, 0), sinks=sinks, max_distance=100)
+
+        def step():
+            out, lse = encoder.attention_forward(q, k, v, table, **more)
+            grads = encoder.attention_backward(do, q, k, v, out, lse, table, **more)
+            _, pre = encoder.gated_linear_forward(x, gate, up, keep_pre=True)
+            return [t for t in (out, lse, *grads, *encoder.gated_linear_backward(dy, x, gate, up, pre)) if t is not None]
+
+        return step, (q, do, x, dy)
+
+    forms = [(1, 4, 64, BF16, 32, 900, 0), (5, 2, 128, F16, 0, 30, 2), (32, 1, 32, BF16, 16, 1200, 4), (130, 1, 64, F16, 0, 1299, 0)]
+    made = [make(*form) for form in forms]
+    want = [[t.clone() for t in step()] for step, _ in made]
+    torch.cuda.synchronize()
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    for turn in range(3):
+        got = []
+        for n, (step, _) in enumerate(made):
+            with torch.cuda.stream(sides[n % 2]):
+                got.append(step())
+        for side in sides:
+            side.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+    graphs, held = [], []
+    for step, _ in made:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            held.append(step())
+    for turn in range(3):
+        for _, inputs in made:
+            for t in inputs:
+                t.mul_(0.75)
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for (step, _), results in zip(made, held):
+            assert all(torch.equal(a, b) for a, b in zip(results, step()))
