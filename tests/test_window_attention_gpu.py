@@ -386,3 +386,18 @@ def test_few_rows_on_two_streams_and_in_graphs(eng):
         torch.cuda.synchronize()
         for (step, _), results in zip(made, held):
             assert all(torch.equal(a, b) for a, b in zip(results, step()))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("b,lq,lk,h,d,buckets,causal,before,after,sinks", [
+    (2, 200, 200, 2, 64, 32, False, 40, 40, 1), (1, 300, 300, 1, 128, 16, True, 200, 0, 0), (2, 3, 150, 2, 32, 8, False, 3, 3, 0),
+    (1, 130, 130, 2, 64, 32, False, 10, 10, 0)])
+def test_window_with_infinite_bias(eng, dtype, b, lq, lk, h, d, buckets, causal, before, after, sinks):
+    """Buckets of minus infinity hide keys as the mask does: some of a row's, or all."""
+    tensors, doubles, _ = attention_inputs(b, lq, lk, h, h, d, dtype, buckets, False, seed=77)
+    for hidden in ([0], [1, 2, 3], list(range(buckets // 2)), list(range(buckets))):
+        say("infinite bias", dtype, b, lq, lk, h, d, buckets, causal, before, after, sinks, hidden)
+        table, exact = tensors[4].clone(), doubles[4].clone()
+        table[hidden, 0] = exact[hidden, 0] = -math.inf
+        hold((*tensors[:4], table), (*doubles[:4], exact), 1 / math.sqrt(d), dtype, before, after, sinks, {}, causal=causal,
+             max_distance=128, poison=False)
