@@ -135,10 +135,9 @@ __device__ __forceinline__ void take_positions(const float* skew, float* sums) {
 // window peak + sum p (dp - peak) / sum p with the largest dp as peak: of one key it is dp itself, and ds is 0.
 // dout . out has out's rounding in it, some 2^-9 of |dout| |out|, which is all that is left in sums of ds that cancel:
 // the table's gradients, whose sum over a row's keys is 0 (of 2 heads, 166 keys back, an error of 3.1e-4 for 1.6e-4
-// in fp16), and those of few rows.  128 rows of a workgroup, 32 of a wave as columns; two products, so that four
-// workgroups' registers and LDS fit a CU and cover each other's waits for the tiles, which a pass within the
-// q kernel, two a CU, did not.  Bound by vector instructions, and by start and end: 8 x up to 2048, 12 heads of 64,
-// window 128, bias: 30 us.
+// in fp16), and those of few rows.  128 rows of a workgroup, 32 of a wave as columns; a kernel of its own, so that the
+// parts of dq do not each repeat it, with four workgroups' registers and LDS a CU.  Bound by vector instructions, and by start
+// and end: 8 x up to 2048, 12 heads of 64, window 128, bias: 30 us (31 as a pass of the q kernel).
 template <class T, int DP, bool BIAS>
 __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 4) void attn_delta_kernel(AttnArgs a) {
   typedef typename Frag<T>::V V;
@@ -1101,7 +1100,7 @@ template <class T, int DP, bool BIAS, bool WIN>
 hipError_t launch_window(const AttnArgs& a, hipStream_t s) {
   const int64_t qblocks = (a.lq + kAttnRows - 1) / kAttnRows, kblocks = (a.lk + kAttnRows - 1) / kAttnRows;
   const size_t tab = BIAS ? (2 * (a.far + kReach) + 1) * sizeof(float) : 0;
-  // (also where delta keeps out's rounding: dq's parts do not sum up a row's ds)
+  // few rows, or dq in parts, none of which has a row's whole sum of ds to correct delta with
   const bool rests = WIN && (few_rows(a) || a.q_parts > 1);
   if (qblocks > 0) {
     const dim3 grid((unsigned)(qblocks * a.batch * a.heads), a.q_parts);
