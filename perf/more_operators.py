@@ -357,20 +357,13 @@ _PLAIN = {("window", "forward"): _window_forward, ("window", "backward"): _windo
 # ---- the framework's calls ------------------------------------------------------
 
 
-_encoder = None
-
-
 def _package():
-    """The framework's module, imported once, as a program does."""
-    global _encoder
-    if _encoder is None:
-        root = str(Path(__file__).resolve().parents[1] / "cuda-vector-search_amd")
-        if root not in sys.path:
-            sys.path.insert(0, root)
-        from cuda_vector_search import encoder
+    root = str(Path(__file__).resolve().parents[1] / "cuda-vector-search_amd")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    from cuda_vector_search import encoder
 
-        _encoder = encoder
-    return _encoder
+    return encoder
 
 
 def run(s):
