@@ -64,6 +64,7 @@ struct GemmKindArgs : GemmArgs {
   const void* N2;         // gated: the second factor's weight; two parts: N of the second part
   const void* bias2;      // gated: [n] or null
   int64_t m_second;       // two parts: elements from M's first part to its second
+  const float* unit;      // two parts, weights: what the sums are in units of, or null
   const float* row_scale; // int8: [m]
   const float* col_scale; // int8: [n]
 };
@@ -86,6 +87,8 @@ GemmPlan plan_gated(int64_t m, int64_t n, int64_t k, int cus);
 hipError_t launch_gated(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s);
 GemmPlan plan_two_parts(int64_t m, int64_t n, int64_t k, bool rests, int cus);
 hipError_t launch_two_parts(const GemmKindArgs& a, const GemmPlan& p, bool rests, hipStream_t s);
+// The weights' gradients, dz^T x: plan_gemm's tiles, both operands strided.
+hipError_t launch_weights(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s);
 
 // dz = [dy up act'(gate), dy act(gate)] ([m, 2 n], contiguous) of pre = [gate, up], and dz's column sums.
 struct GatedGradArgs {
@@ -101,6 +104,8 @@ struct GatedGradArgs {
   float* partial;         // [parts, 2, n] when either is not null
   int parts;
   bool rests;             // dz is [2 m, 2 n]: what rounding took off its rows behind them
+  float* peaks;           // float16: [gated_grad_workgroups] largest finite |dz|
+  float* unit;            // float16: dz is held times 1 / unit
   const void* x;          // and x is copied to twice [2 m, k], to go with them, or null
   int64_t x_stride;
   int k;
@@ -109,6 +114,7 @@ struct GatedGradArgs {
 // Of so few rows what dz loses to 16 bits is kept (cvs_gated.hip).
 inline bool gated_few_rows(int64_t m) { return m <= 32; }
 int gated_grad_parts(int64_t m, int64_t n, int cus);
+int64_t gated_grad_workgroups(int64_t m, int64_t n, int parts);
 hipError_t launch_gated_grad(const GatedGradArgs& a, hipStream_t s);
 
 // Rows in 8-bit whole numbers with a scale each, and the product of such operands (ldm, ldn and k in

@@ -115,7 +115,7 @@ struct GatedBackwardPlan {
   int parts;
   bool rests;     // dz's rows twice: rounded, and what that took off
   int64_t rows;   // of dz
-  int64_t dz, twice, partial, gemm, bytes;  // offsets, then all
+  int64_t dz, twice, partial, peaks, unit, gemm, bytes;  // offsets, then all
 };
 
 GatedBackwardPlan plan_gated_backward(int64_t m, int64_t k, int64_t n, int cus) {
@@ -130,6 +130,8 @@ GatedBackwardPlan plan_gated_backward(int64_t m, int64_t k, int64_t n, int cus) 
   p.dz = at, at += up256(2 * p.rows * n * 2);
   p.twice = at, at += p.rests ? up256(p.rows * k * 2) : 0;
   p.partial = at, at += up256((int64_t)p.parts * 2 * n * 4);
+  p.peaks = at, at += up256(gated_grad_workgroups(m, n, p.parts) * 4);
+  p.unit = at, at += up256(4);
   p.gemm = at, at += up256(std::max({p.dx.ws_bytes, p.dw.ws_bytes, p.one.ws_bytes}));  // (one product after the other)
   p.bytes = at;
   return p;
@@ -611,24 +613,26 @@ int cvs_gated_linear_backward(const void* dy, const void* x, const void* gate, c
   g.type = type, g.act = act, g.m = m, g.n = (int)n, g.dy = dy, g.dy_stride = dy_stride, g.pre = pre;
   g.dz = ws + p.dz, g.dgate_bias = dgate_bias, g.dup_bias = dup_bias;
   g.partial = reinterpret_cast<float*>(ws + p.partial), g.parts = p.parts, g.rests = p.rests;
+  g.peaks = reinterpret_cast<float*>(ws + p.peaks), g.unit = reinterpret_cast<float*>(ws + p.unit);
   if (p.rests && (dgate != nullptr || dup != nullptr)) g.x = x, g.x_stride = x_stride, g.k = (int)k, g.twice = ws + p.twice;
   hipError_t e = launch_gated_grad(g, s);
   float* sums = reinterpret_cast<float*>(ws + p.gemm);
+  const float* unit = type == CVS_TYPE_F16 ? g.unit : nullptr;
   if (e == hipSuccess && dx != nullptr) {  // dx = dg [m, n] gate [n, k] + du up
     GemmKindArgs a = {};
     a.type = type, a.m = (int)p.rows, a.n = (int)k, a.k = (int)n;
     a.M = g.dz, a.ldm = 2 * n, a.m_second = n, a.N = gate, a.N2 = up, a.ldn = k, a.n_strided = true;
-    a.out = dx, a.partial = sums, a.splits = p.dx.splits;
+    a.out = dx, a.partial = sums, a.splits = p.dx.splits, a.unit = unit;
     e = launch_two_parts(a, p.dx, p.rests, s);
   }
   // dgate = dg^T x, dup = du^T x: one product of 2 n rows where they lie one behind the other
   auto weight = [&](int64_t first, int64_t rows, const GemmPlan& plan, void* out) {
-    GemmArgs a = {};
+    GemmKindArgs a = {};
     a.type = type, a.m = (int)rows, a.n = (int)k, a.k = (int)p.rows;
     a.M = static_cast<unsigned char*>(g.dz) + 2 * first, a.ldm = 2 * n, a.m_strided = true;
     a.N = p.rests ? g.twice : x, a.ldn = p.rests ? k : x_stride, a.n_strided = true;
-    a.out = out, a.partial = sums, a.splits = plan.splits;
-    return launch_gemm(a, plan, s);
+    a.out = out, a.partial = sums, a.splits = plan.splits, a.unit = unit;
+    return launch_weights(a, plan, s);
   };
   if (e == hipSuccess && dgate != nullptr && dup == static_cast<unsigned char*>(dgate) + 2 * n * k) {
     e = weight(0, 2 * n, p.dw, dgate);

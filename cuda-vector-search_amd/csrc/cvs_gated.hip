@@ -7,7 +7,7 @@
 //
 // Forward, a tile of the product has as many columns of g as of u, the same ones, so that g and
 // u meet in a wave's registers.  Backward, dx is one sum over two reductions and both weights'
-// gradients are one product whose rows are dz's 2 n columns (cvs_linear.hip's).
+// gradients are one product whose rows are dz's 2 n columns.
 #include <algorithm>
 
 #include "cvs_gemm_tile.h"
@@ -16,11 +16,11 @@ namespace cvs {
 
 namespace {
 
-template <class T, int WM, int WN, int BM, int BN, int RING, int WGS, bool NS, int KIND>
+template <class T, int WM, int WN, int BM, int BN, int RING, int WGS, int KIND>
 __global__ __launch_bounds__(64 * WM * WN, WGS) void gemm_kind_kernel(GemmKindArgs a) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[gemm_lds<WM, WN, BM, BN, RING>()];
   __shared__ __attribute__((aligned(16))) float vectors[gemm_vectors<KIND, WM * BM * 32, WN * BN * 16>()];
-  gemm_tile<T, WM, WN, BM, BN, RING, false, NS, KIND>(a, blockIdx.x, smem, vectors);
+  gemm_tile<T, WM, WN, BM, BN, RING, KIND == kWeights, KIND != kGated, KIND>(a, blockIdx.x, smem, vectors);
 }
 
 // Adds the parts of a split reduction, in order, and finishes: 8 columns a thread.
@@ -61,9 +61,9 @@ __global__ __launch_bounds__(kBlock) void gated_join_kernel(GemmKindArgs a) {
   store8((T*)a.out + i * a.n + j, h);
 }
 
-// (halves: the second half of the rows is what rounding took off the first)
+// The same of two parts and of weights (halves: the second half of the rows is what rounding took off the first).
 template <class T>
-__global__ __launch_bounds__(kBlock) void two_parts_join_kernel(GemmKindArgs a, int halves) {
+__global__ __launch_bounds__(kBlock) void sums_join_kernel(GemmKindArgs a, int halves) {
   const int64_t at = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * 8, plane = (int64_t)a.m / halves * a.n;
   if (at >= plane) return;
   float z[8];
@@ -75,13 +75,18 @@ __global__ __launch_bounds__(kBlock) void two_parts_join_kernel(GemmKindArgs a, 
 #pragma unroll
     for (int e = 0; e < 4; ++e) z[e] += lo[e], z[4 + e] += hi[e];
   }
+  if (a.unit != nullptr) {
+    const float unit = *a.unit;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] *= unit;
+  }
   store8((T*)a.out + at, z);
 }
 
-template <class T, int WM, int WN, int BM, int BN, int RING, int WGS, bool NS, int KIND>
+template <class T, int WM, int WN, int BM, int BN, int RING, int WGS, int KIND>
 void launch_tiles(const GemmKindArgs& a, hipStream_t s) {
   const dim3 grid(gemm_grid(a, WM * BM * 32, WN * BN * (KIND == kGated ? 16 : 32))), block(64 * WM * WN);
-  hipLaunchKernelGGL((gemm_kind_kernel<T, WM, WN, BM, BN, RING, WGS, NS, KIND>), grid, block, 0, s, a);
+  hipLaunchKernelGGL((gemm_kind_kernel<T, WM, WN, BM, BN, RING, WGS, KIND>), grid, block, 0, s, a);
 }
 
 dim3 join_grid(const GemmKindArgs& a) { return dim3((unsigned)(((int64_t)a.m * (a.n / 8) + kBlock - 1) / kBlock)); }
@@ -89,30 +94,30 @@ dim3 join_grid(const GemmKindArgs& a) { return dim3((unsigned)(((int64_t)a.m * (
 template <class T>
 hipError_t gated(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s) {
   if (p.tile == 256)
-    launch_tiles<T, 4, 2, 2, 4, 2, 1, false, kGated>(a, s);
+    launch_tiles<T, 4, 2, 2, 4, 2, 1, kGated>(a, s);
   else if (p.tile == 128)
-    launch_tiles<T, 2, 2, 2, 2, 2, 2, false, kGated>(a, s);
+    launch_tiles<T, 2, 2, 2, 2, 2, 2, kGated>(a, s);
   else
-    launch_tiles<T, 2, 2, 1, 2, 3, 2, false, kGated>(a, s);
+    launch_tiles<T, 2, 2, 1, 2, 3, 2, kGated>(a, s);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
   hipLaunchKernelGGL(gated_join_kernel<T>, join_grid(a), dim3(kBlock), 0, s, a);
   return hipGetLastError();
 }
 
-template <class T>
-hipError_t two_parts(const GemmKindArgs& a, const GemmPlan& p, bool rests, hipStream_t s) {
+template <class T, int KIND>
+hipError_t sums(const GemmKindArgs& a, const GemmPlan& p, int halves, hipStream_t s) {
   if (p.tile == 256 && p.tile_n == 256)
-    launch_tiles<T, 4, 2, 2, 4, 2, 1, true, kTwoParts>(a, s);
+    launch_tiles<T, 4, 2, 2, 4, 2, 1, KIND>(a, s);
   else if (p.tile == 256)
-    launch_tiles<T, 4, 2, 2, 3, 2, 1, true, kTwoParts>(a, s);
+    launch_tiles<T, 4, 2, 2, 3, 2, 1, KIND>(a, s);
   else if (p.tile == 128)
-    launch_tiles<T, 2, 2, 2, 2, 2, 2, true, kTwoParts>(a, s);
+    launch_tiles<T, 2, 2, 2, 2, 2, 2, KIND>(a, s);
   else
-    launch_tiles<T, 2, 2, 1, 1, 3, 2, true, kTwoParts>(a, s);
+    launch_tiles<T, 2, 2, 1, 1, 3, 2, KIND>(a, s);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
-  hipLaunchKernelGGL(two_parts_join_kernel<T>, join_grid(a), dim3(kBlock), 0, s, a, rests ? 2 : 1);
+  hipLaunchKernelGGL(sums_join_kernel<T>, join_grid(a), dim3(kBlock), 0, s, a, halves);
   return hipGetLastError();
 }
 
@@ -146,6 +151,40 @@ __device__ __forceinline__ void gate_grads8(const float* dy, const float* g, con
 // Pieces of 8 columns of a workgroup, as act_grad_kernel's: few for few rows.
 __host__ __device__ inline int gated_grad_width(int64_t m, int n) { return m <= 256 ? 16 : min(n / 8, kBlock); }
 
+// float16 holds small gradients as subnormals, of few digits, which sums over many rows are not (of 4096 rows and dy of
+// 2^-18 dgate was off by 0.7%), and none past 65504, which products with small weights are not.  So dz is held there times 2^4,
+// or, where that brings its largest value past 2^15 or leaves it below 2^-2, times what brings it to 2^14 to 2^15, and
+// the products' sums are taken back: a dz loses 2^-23 of the largest at most beside its own rounding.  The largest is known
+// once all are made: gated_grad_kernel makes them times 2^4 and leaves each workgroup's largest, and a launch after it,
+// REFIT, looks at these and makes dz again where they do not fit (the pass of 16384 rows of 2 x 2048, k = 768: 297 us,
+// 359 where dz is made again, 295 without any of this; of 23 rows, k = 384 48, bound by the host, for 46).
+template <class T>
+constexpr bool kFits = true;
+template <>
+constexpr bool kFits<_Float16> = false;
+constexpr int kDzLift = 4;
+
+// The largest of a workgroup's values, in every thread (red: 4 floats of LDS).
+__device__ __forceinline__ float workgroup_max(float v, float* red) {
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) v = fmaxf(v, __shfl_xor(v, s));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+// The largest magnitude of 16 values, of those that are finite.
+__device__ __forceinline__ float finite_max8(const float* v, const float* w) {
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float x = fabsf(v[e]), y = fabsf(w[e]);
+    top = fmaxf(top, fmaxf(x < __builtin_inff() ? x : 0.f, y < __builtin_inff() ? y : 0.f));
+  }
+  return top;
+}
+
 // What rounding to T took off 8 values; nothing of those that it made infinite.
 template <class T>
 __device__ __forceinline__ void rest8(float* v) {
@@ -163,9 +202,21 @@ __device__ __forceinline__ void rest8(float* v) {
 // be further off (one row of 384 features 1.66 times), so there dz's rounding errors are 16-bit rows of their own, behind
 // its rows: up to 32 rows the products' tiles and stages of 64 hold both without another one (23 x 2 x 1536, k = 384: 26 us
 // both ways; 32 x 2 x 4096, k = 1024: 32 for 27).
-template <class T>
+template <class T, bool REFIT>
 __global__ __launch_bounds__(kBlock) void gated_grad_kernel(GatedGradArgs a) {
   __shared__ float red[kBlock * 8];
+  const int64_t wg = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  float lift = kFits<T> ? 1.f : (float)(1 << kDzLift), peak = 0.f;
+  if constexpr (REFIT) {
+    const int64_t all = (int64_t)gridDim.x * gridDim.y;
+    float top = 0.f;
+    for (int64_t t = threadIdx.x; t < all; t += kBlock) top = fmaxf(top, a.peaks[t]);
+    top = workgroup_max(top, red);
+    const bool fits = top == 0.f || (top * lift < 32768.f && top * lift >= 0.25f);
+    if (!fits) lift = ldexpf(1.f, min(15 - __builtin_amdgcn_frexp_expf(top), 60));
+    if (wg == 0 && threadIdx.x == 0) *a.unit = 1.f / lift;
+    if (fits) return;
+  }
   const int width = gated_grad_width(a.m, a.n);
   const int pieces = min(a.n / 8 - (int)blockIdx.x * width, width), lanes = kBlock / pieces;
   const int p = threadIdx.x % pieces, rl = threadIdx.x / pieces;
@@ -193,10 +244,15 @@ __global__ __launch_bounds__(kBlock) void gated_grad_kernel(GatedGradArgs a) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) df[e] = (float)d[u][e], gf[e] = (float)g[u][e], uf[e] = (float)z[u][e];
           gate_grads8(df, gf, uf, a.act, dg, du);
-          store8((T*)a.dz + row * 2 * a.n + c, dg);
-          store8((T*)a.dz + row * 2 * a.n + a.n + c, du);
 #pragma unroll
           for (int e = 0; e < 8; ++e) sum[0][e] += dg[e], sum[1][e] += du[e];
+          if constexpr (!kFits<T>) {
+            if constexpr (!REFIT) peak = fmaxf(peak, finite_max8(dg, du));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dg[e] *= lift, du[e] *= lift;
+          }
+          store8((T*)a.dz + row * 2 * a.n + c, dg);
+          store8((T*)a.dz + row * 2 * a.n + a.n + c, du);
           if (a.rests) {
             rest8<T>(dg), rest8<T>(du);
             store8((T*)a.dz + (a.m + row) * 2 * a.n + c, dg);
@@ -205,6 +261,11 @@ __global__ __launch_bounds__(kBlock) void gated_grad_kernel(GatedGradArgs a) {
         }
       }
     }
+  }
+  if constexpr (REFIT) return;
+  if constexpr (!kFits<T>) {
+    peak = workgroup_max(peak, red);
+    if (threadIdx.x == 0) a.peaks[wg] = peak;
   }
   if (a.rests && a.x != nullptr) {
     const int64_t pieces_x = a.k / 8, all = a.m * pieces_x, step = (int64_t)gridDim.x * kBlock;
@@ -257,7 +318,17 @@ GemmPlan plan_two_parts(int64_t m, int64_t n, int64_t k, bool rests, int cus) {
 }
 
 hipError_t launch_two_parts(const GemmKindArgs& a, const GemmPlan& p, bool rests, hipStream_t s) {
-  return a.type == kF16 ? two_parts<_Float16>(a, p, rests, s) : two_parts<__bf16>(a, p, rests, s);
+  const int halves = rests ? 2 : 1;
+  return a.type == kF16 ? sums<_Float16, kTwoParts>(a, p, halves, s) : sums<__bf16, kTwoParts>(a, p, halves, s);
+}
+
+hipError_t launch_weights(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s) {
+  return a.type == kF16 ? sums<_Float16, kWeights>(a, p, 1, s) : sums<__bf16, kWeights>(a, p, 1, s);
+}
+
+int64_t gated_grad_workgroups(int64_t m, int64_t n, int parts) {
+  const int64_t width = gated_grad_width(m, (int)n);
+  return (n / 8 + width - 1) / width * parts;
 }
 
 int gated_grad_parts(int64_t m, int64_t n, int cus) {
@@ -270,10 +341,12 @@ int gated_grad_parts(int64_t m, int64_t n, int cus) {
 hipError_t launch_gated_grad(const GatedGradArgs& a, hipStream_t s) {
   const int width = gated_grad_width(a.m, a.n);
   const dim3 grid((a.n / 8 + width - 1) / width, a.parts), block(kBlock);
-  if (a.type == kF16)
-    hipLaunchKernelGGL(gated_grad_kernel<_Float16>, grid, block, 0, s, a);
-  else
-    hipLaunchKernelGGL(gated_grad_kernel<__bf16>, grid, block, 0, s, a);
+  if (a.type == kF16) {
+    hipLaunchKernelGGL((gated_grad_kernel<_Float16, false>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((gated_grad_kernel<_Float16, true>), grid, block, 0, s, a);
+  } else {
+    hipLaunchKernelGGL((gated_grad_kernel<__bf16, false>), grid, block, 0, s, a);
+  }
   hipError_t e = hipGetLastError();
   const int first = a.dgate_bias != nullptr ? a.n : 0, second = a.dup_bias != nullptr ? a.n : 0;
   if (e == hipSuccess && a.parts > 1 && first + second > 0)

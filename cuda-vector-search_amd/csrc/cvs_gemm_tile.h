@@ -12,7 +12,8 @@
 // Kinds of product beside that one:
 //   gated      act(M N^T + bias) * (M N2^T + bias2): a tile's rows of N are half N's, half N2's of the same
 //              columns, so that a wave holds both factors of an output and nothing but it is written;
-//   two parts  sum over both of two reductions, M N^T + M' N2^T, M' at M + m_second;
+//   two parts  sum over both of two reductions, M N^T + M' N2^T, M' at M + m_second, times *unit;
+//   weights    both operands strided, times *unit;
 //   int8       8-bit whole numbers, two to a 16-bit unit of k and of the strides (a depth step's 16
 //              bytes of a lane are 16 values, and a product takes as many cycles as one of 8 16-bit
 //              values), 32-bit sums, times row_scale[i] col_scale[j].
@@ -149,7 +150,7 @@ __device__ __forceinline__ void store_block(T* out, int64_t ld, int m, int n, in
   }
 }
 
-enum GemmKind : int { kPlain, kGated, kTwoParts, kInt8 };
+enum GemmKind : int { kPlain, kGated, kTwoParts, kWeights, kInt8 };
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
@@ -270,6 +271,10 @@ __device__ __forceinline__ void gemm_tile(const typename Operand<T, KIND>::Args&
       of_row = a.row_scale[min(m0 + min(tid, TM - 1), a.m - 1)];
     }
   }
+
+  float unit = 1.f;
+  if constexpr (KIND == kTwoParts || KIND == kWeights)
+    if (a.unit != nullptr) unit = *a.unit;
 
   const int part_stages = (a.k + kDepth - 1) / kDepth, stages = KIND == kTwoParts ? 2 * part_stages : part_stages;
   const int s_begin = (int)((int64_t)stages * split / a.splits);
@@ -540,6 +545,11 @@ __device__ __forceinline__ void gemm_tile(const typename Operand<T, KIND>::Args&
           store_block((T*)a.pre + a.n, 2 * (int64_t)a.n, a.m, a.n, row0, col0, up, up + 8);
         }
         store_block((T*)a.out, a.n, a.m, a.n, row0, col0, h, h + 8);
+      } else if constexpr (KIND == kTwoParts || KIND == kWeights) {
+        float z[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z[e] = acc[i][j][e] * unit;
+        store_block((T*)a.out, a.n, a.m, a.n, row0, col0, z, z + 8);
       } else {
         float z[16], pre[16];
 #pragma unroll
