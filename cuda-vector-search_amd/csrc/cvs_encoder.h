@@ -65,6 +65,8 @@ struct GemmKindArgs : GemmArgs {
   const void* bias2;      // gated: [n] or null
   int64_t m_second;       // two parts: elements from M's first part to its second
   const float* unit;      // two parts, weights: what the sums are in units of, or null
+  int m_first;            // weights: rows of out, those after them are out2's
+  void* out2;
   const float* row_scale; // int8: [m]
   const float* col_scale; // int8: [n]
 };
@@ -87,7 +89,7 @@ GemmPlan plan_gated(int64_t m, int64_t n, int64_t k, int cus);
 hipError_t launch_gated(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s);
 GemmPlan plan_two_parts(int64_t m, int64_t n, int64_t k, bool rests, int cus);
 hipError_t launch_two_parts(const GemmKindArgs& a, const GemmPlan& p, bool rests, hipStream_t s);
-// The weights' gradients, dz^T x: plan_gemm's tiles, both operands strided.
+// The weights' gradients, dz^T x, one behind the other's rows: plan_gemm's tiles, both operands strided.
 hipError_t launch_weights(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s);
 
 // dz = [dy up act'(gate), dy act(gate)] ([m, 2 n], contiguous) of pre = [gate, up], and dz's column sums.

@@ -622,24 +622,24 @@ int cvs_gated_linear_backward(const void* dy, const void* x, const void* gate, c
     GemmKindArgs a = {};
     a.type = type, a.m = (int)p.rows, a.n = (int)k, a.k = (int)n;
     a.M = g.dz, a.ldm = 2 * n, a.m_second = n, a.N = gate, a.N2 = up, a.ldn = k, a.n_strided = true;
-    a.out = dx, a.partial = sums, a.splits = p.dx.splits, a.unit = unit;
+    a.out = dx, a.m_first = a.m, a.partial = sums, a.splits = p.dx.splits, a.unit = unit;
     e = launch_two_parts(a, p.dx, p.rests, s);
   }
-  // dgate = dg^T x, dup = du^T x: one product of 2 n rows where they lie one behind the other
-  auto weight = [&](int64_t first, int64_t rows, const GemmPlan& plan, void* out) {
+  // dgate = dg^T x, dup = du^T x: one product of 2 n rows
+  auto weights = [&](int64_t first, int64_t rows, const GemmPlan& plan, void* out, void* out2) {
     GemmKindArgs a = {};
     a.type = type, a.m = (int)rows, a.n = (int)k, a.k = (int)p.rows;
     a.M = static_cast<unsigned char*>(g.dz) + 2 * first, a.ldm = 2 * n, a.m_strided = true;
     a.N = p.rests ? g.twice : x, a.ldn = p.rests ? k : x_stride, a.n_strided = true;
-    a.out = out, a.partial = sums, a.splits = plan.splits, a.unit = unit;
+    a.out = out, a.out2 = out2, a.m_first = (int)n, a.partial = sums, a.splits = plan.splits, a.unit = unit;
     return launch_weights(a, plan, s);
   };
-  if (e == hipSuccess && dgate != nullptr && dup == static_cast<unsigned char*>(dgate) + 2 * n * k) {
-    e = weight(0, 2 * n, p.dw, dgate);
-  } else {
-    if (e == hipSuccess && dgate != nullptr) e = weight(0, n, p.one, dgate);
-    if (e == hipSuccess && dup != nullptr) e = weight(n, n, p.one, dup);
-  }
+  if (e == hipSuccess && dgate != nullptr && dup != nullptr)
+    e = weights(0, 2 * n, p.dw, dgate, dup);
+  else if (e == hipSuccess && dgate != nullptr)
+    e = weights(0, n, p.one, dgate, nullptr);
+  else if (e == hipSuccess && dup != nullptr)
+    e = weights(n, n, p.one, dup, nullptr);
   return done(e, "gated linear backward launch");
 }
 

@@ -80,7 +80,8 @@ __global__ __launch_bounds__(kBlock) void sums_join_kernel(GemmKindArgs a, int h
 #pragma unroll
     for (int e = 0; e < 8; ++e) z[e] *= unit;
   }
-  store8((T*)a.out + at, z);
+  const int64_t first = (int64_t)a.m_first * a.n;
+  store8(at < first ? (T*)a.out + at : (T*)a.out2 + (at - first), z);
 }
 
 template <class T, int WM, int WN, int BM, int BN, int RING, int WGS, int KIND>

@@ -13,7 +13,7 @@
 //   gated      act(M N^T + bias) * (M N2^T + bias2): a tile's rows of N are half N's, half N2's of the same
 //              columns, so that a wave holds both factors of an output and nothing but it is written;
 //   two parts  sum over both of two reductions, M N^T + M' N2^T, M' at M + m_second, times *unit;
-//   weights    both operands strided, times *unit;
+//   weights    both operands strided, times *unit, rows from m_first on to out2;
 //   int8       8-bit whole numbers, two to a 16-bit unit of k and of the strides (a depth step's 16
 //              bytes of a lane are 16 values, and a product takes as many cycles as one of 8 16-bit
 //              values), 32-bit sums, times row_scale[i] col_scale[j].
@@ -127,26 +127,46 @@ __device__ __forceinline__ void finish8(const GemmArgs& a, int i, int j, float* 
   }
 }
 
-// Stores a 32 x 32 block of which lane l holds, of row l % 32, columns 8 g .. and 16 + 8 g ..
-// (g = l / 32): 16 lanes exchange their pieces with the next 16 so that four lanes write
-// 64 contiguous bytes of a row.
+// A 32 x 32 block of which lane l holds, of row l % 32, columns 8 g .. and 16 + 8 g .. (g = l / 32), packed
+// for a store: 16 lanes exchange their pieces with the next 16 so that four lanes write 64 contiguous
+// bytes of a row.
 template <class T>
-__device__ __forceinline__ void store_block(T* out, int64_t ld, int m, int n, int row0, int col0, const float* z0, const float* z1) {
+__device__ __forceinline__ void pack_block(const float* z0, const float* z1, u32x4& x, u32x4& y) {
   typename Frag<T>::V v0, v1;
 #pragma unroll
   for (int e = 0; e < 8; ++e) v0[e] = (T)z0[e], v1[e] = (T)z1[e];
-  u32x4 x = __builtin_bit_cast(u32x4, v0), y = __builtin_bit_cast(u32x4, v1);
+  x = __builtin_bit_cast(u32x4, v0), y = __builtin_bit_cast(u32x4, v1);
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const auto s = __builtin_amdgcn_permlane16_swap(x[r], y[r], false, false);
     x[r] = s[0], y[r] = s[1];
   }
+}
+template <class T>
+__device__ __forceinline__ void store_block(T* out, int64_t ld, int m, int n, int row0, int col0, const float* z0, const float* z1) {
+  u32x4 x, y;
+  pack_block<T>(z0, z1, x, y);
   const int lane = threadIdx.x & 63;
   const int row = row0 + (lane & 15), col = col0 + 16 * ((lane >> 4) & 1) + 8 * (lane >> 5);
   if (col < n) {
     T* to = out + (int64_t)row * ld + col;
     if (row < m) *reinterpret_cast<u32x4*>(to) = x;
     if (row + 16 < m) *reinterpret_cast<u32x4*>(to + 16 * ld) = y;
+  }
+}
+
+// The same of rows of which those from `border` on are another matrix's.
+template <class T>
+__device__ __forceinline__ void store_block_of_two(T* out, T* out2, int border, int64_t ld, int m, int n, int row0, int col0,
+                                                   const float* z0, const float* z1) {
+  u32x4 x, y;
+  pack_block<T>(z0, z1, x, y);
+  const int lane = threadIdx.x & 63;
+  const int row = row0 + (lane & 15), col = col0 + 16 * ((lane >> 4) & 1) + 8 * (lane >> 5);
+  auto at = [&](int r) { return (r < border ? out + r * ld : out2 + (r - border) * ld) + col; };
+  if (col < n) {
+    if (row < m) *reinterpret_cast<u32x4*>(at(row)) = x;
+    if (row + 16 < m) *reinterpret_cast<u32x4*>(at(row + 16)) = y;
   }
 }
 
@@ -549,7 +569,10 @@ __device__ __forceinline__ void gemm_tile(const typename Operand<T, KIND>::Args&
         float z[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) z[e] = acc[i][j][e] * unit;
-        store_block((T*)a.out, a.n, a.m, a.n, row0, col0, z, z + 8);
+        if constexpr (KIND == kWeights)
+          store_block_of_two((T*)a.out, (T*)a.out2, a.m_first, a.n, a.m, a.n, row0, col0, z, z + 8);
+        else
+          store_block((T*)a.out, a.n, a.m, a.n, row0, col0, z, z + 8);
       } else {
         float z[16], pre[16];
 #pragma unroll

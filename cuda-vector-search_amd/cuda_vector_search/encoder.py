@@ -471,11 +471,7 @@ def gated_linear_backward(dy, x, gate, up, pre, activation="silu", needs=(True, 
     m = r.shape[0]
     dx = _new(x) if needs[0] else None
     new = x.new_zeros if m == 0 else x.new_empty
-    if needs[1] and needs[2]:
-        both = new((2, n, k))  # (one behind the other: one product)
-        dgate, dup = both[0], both[1]
-    else:
-        dgate, dup = (new((n, k)) if need else None for need in needs[1:3])
+    dgate, dup = (new((n, k)) if need else None for need in needs[1:3])
     dgate_bias, dup_bias = (new((n,)) if need else None for need in needs[3:5])
     grads = dx, dgate, dup, dgate_bias, dup_bias
     if m == 0 or all(t is None for t in grads):

@@ -331,8 +331,7 @@ int cvs_gated_linear(const void* x, const void* gate, const void* up, const void
 
 /*
  * Gradients of cvs_gated_linear for dy [m, n] (rows dy_stride elements apart): dx [m, k], dgate and dup
- * [n, k], dgate_bias and dup_bias [n], each of which may be NULL.  Both weights' are one product where
- * dup lies right behind dgate.
+ * [n, k], dgate_bias and dup_bias [n], each of which may be NULL.
  */
 int cvs_gated_linear_backward_plan(int64_t m, int64_t k, int64_t n, int device, int64_t* workspace_bytes);
 int cvs_gated_linear_backward(const void* dy, const void* x, const void* gate, const void* up, const void* pre, int64_t m,
