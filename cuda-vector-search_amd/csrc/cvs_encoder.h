@@ -132,7 +132,7 @@ struct QuantArgs {
 };
 hipError_t launch_quantize(const QuantArgs& a, hipStream_t s);
 // Few rows: one launch, of rows x (m of d values), whole numbers and product.
-bool int8_few_rows(int64_t m, int64_t k);
+bool int8_few_rows(int64_t m, int64_t n, int64_t k, const GemmPlan& tiles, int cus);
 hipError_t launch_int8_rows(const GemmKindArgs& a, const void* x, int64_t x_stride, int d, hipStream_t s);
 GemmPlan plan_int8(int64_t m, int64_t n, int64_t k, int cus);
 hipError_t launch_int8(const GemmKindArgs& a, const GemmPlan& p, hipStream_t s);

@@ -164,13 +164,15 @@ int check_int8(int64_t m, int64_t k, int64_t n, int act, int type) {
 
 struct Int8Plan {
   GemmPlan product;
+  bool few;  // one launch, without a workspace
   int64_t values, scales, gemm, bytes;  // offsets, then all
 };
 
 Int8Plan plan_linear_int8(int64_t m, int64_t k, int64_t n, int cus) {
   Int8Plan p = {};
   p.product = plan_int8(m, n, k, cus);
-  if (int8_few_rows(m, k)) return p;
+  p.few = int8_few_rows(m, n, k, p.product, cus);
+  if (p.few) return p;
   int64_t at = 0;
   p.values = at, at += up256(m * k);
   p.scales = at, at += up256(m * 4);
@@ -695,7 +697,7 @@ int cvs_linear_int8(const void* x, const void* w, const float* w_scales, const v
   GemmKindArgs a = {};
   a.type = type, a.m = (int)m, a.n = (int)n, a.N = w, a.col_scale = w_scales;
   a.bias = bias, a.residual = residual, a.ld_res = residual_stride, a.act = act, a.out = y;
-  if (int8_few_rows(m, k)) return done(launch_int8_rows(a, x, x_stride, (int)k, s), "linear int8 launch");
+  if (p.few) return done(launch_int8_rows(a, x, x_stride, (int)k, s), "linear int8 launch");
   QuantArgs q = {};
   q.type = type, q.n = m, q.d = (int)k, q.x = x, q.x_stride = x_stride;
   q.values = reinterpret_cast<signed char*>(ws + p.values), q.scales = reinterpret_cast<float*>(ws + p.scales);

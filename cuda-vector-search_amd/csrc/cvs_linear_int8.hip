@@ -147,13 +147,20 @@ void quantize(const QuantArgs& a, hipStream_t s) {
 // Few rows (single tokens, a query), one launch: a workgroup has 32 columns of the weight, its waves a quarter of
 // their depth each, straight from memory to the matrix cores, and takes all rows in whole numbers itself, while the
 // weight is on its way.  Bound by latency: a launch, the rows, the weight (loaded together), and the waves' join; 7.2 us
-// of 1 x 2048, k = 768, 8.2 of 23 x 1536, k = 384.  A call of it against the quantising launch and the tiles: 1 x 2048,
-// k = 768 9.4 and 13.1 us, 32 x 4096, k = 1024 9.5 and 13.4, 16 x 2048, k = 2048 11.3 and 15.7, 28 x 512, k = 2048 13.5
-// and 16.0; the other way round 32 x 4096, k = 1792 14.4 and 13.2, 8 x 4096, k = 4096 16.6 and 16.0, 4 x 2048, k = 8192 23.2
-// and 16.0.
-constexpr int kFewRows = 32;         // columns of a block
-constexpr int kFewDepth = 2048;      // the weight past the first 1024 values of a row comes after the rows
-constexpr int kFewBytes = 60 << 10;  // of LDS for the rows: rows times depth
+// of 1 x 2048, k = 768, 8.2 of 23 x 1536, k = 384.
+//
+// Calls of it (one after the other, bound by the host or the GPU) against the quantising launch and the tiles, us:
+//   up to 1024 values a row   32 x 256, k = 768 9.1, 13.0; 32 x 8192, k = 1024 9.5, 13.0; 16 x 16384, k = 1024 10.1, 13.1;
+//                             32 x 16384, k = 1024 12.4, 12.9; 1 x 24576, k = 1024 12.4, 12.6; 8 x 32768, k = 768 14.2, 12.4;
+//                             1 x 131072, k = 768 44.3, 23.8: every workgroup takes all the rows, so the columns may
+//                             fill the CUs once, or twice of half as many rows;
+//   up to 2048, read twice    18 x 768, k = 1040 12.7, 12.9; 18 x 8192, k = 1920 12.1, 13.0; 20 x 768, k = 1040 14.6, 12.8;
+//                             24 x 512, k = 1280 13.3, 13.0; 32 x 4096, k = 1792 14.4, 12.9; 8 x 16384, k = 2048 13.0, 12.6;
+//   and tiles in parts        28 x 8192, k = 2048 14.9, 15.7 (a third launch joins them);
+//   deeper                    8 x 4096, k = 4096 16.6, 16.0; 4 x 2048, k = 8192 23.2, 16.0.
+// (In a captured graph, where launches cost the host nothing, the tiles are ahead from some 16 rows: 32 x 4096, k = 1024 8.9, 7.6.)
+constexpr int kFewRows = 32;     // columns of a block
+constexpr int kFewDepth = 2048;  // the weight past the first 1024 values of a row comes after the rows
 
 // Bytes of LDS between rows: depth padded to whole blocks of 128 (four waves' 32), and 16 so that rows start in other banks.
 __host__ __device__ inline int few_stride(int d) { return (d + 127) / 128 * 128 + 16; }
@@ -345,7 +352,11 @@ GemmPlan plan_int8(int64_t m, int64_t n, int64_t k, int cus) {
   return plan_tiles(kTiles, 4, m, n, (k / 2 + kDepth - 1) / kDepth, 1, cus);
 }
 
-bool int8_few_rows(int64_t m, int64_t k) { return m <= kFewRows && k <= kFewDepth && m * few_stride((int)k) <= kFewBytes; }
+bool int8_few_rows(int64_t m, int64_t n, int64_t k, const GemmPlan& tiles, int cus) {
+  const int64_t rounds = ((n + 31) / 32 + cus - 1) / cus;
+  if (k <= 1024) return rounds <= 2 && m * rounds <= kFewRows;
+  return k <= kFewDepth && rounds == 1 && m <= (tiles.splits > 1 ? 28 : 18);  // (57 KiB of rows at most)
+}
 
 hipError_t launch_int8_rows(const GemmKindArgs& a, const void* x, int64_t x_stride, int d, hipStream_t s) {
   const dim3 grid((unsigned)((a.n + 31) / 32)), block(kBlock);

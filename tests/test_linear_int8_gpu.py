@@ -192,3 +192,32 @@ def test_int8_refusals(eng):
         encoder.linear_int8(t(4, 32), v, s, activation="silu")
     with torch.no_grad():
         assert encoder.linear_int8(x, v, s).shape == (4, 24)
+
+
+def workspace(m, k, n):
+    import ctypes
+
+    from cuda_vector_search import _ext
+
+    out = ctypes.c_int64(-1)
+    assert _ext.load().lib.cvs_linear_int8_plan(m, k, n, 0, ctypes.byref(out)) == 0
+    return out.value
+
+
+def test_linear_int8_few_rows_take_one_launch_where_it_is_the_faster(eng):
+    """Every workgroup of the one launch takes all rows: not for outputs of more columns than the CUs take at once, nor for
+    more rows than it was found faster for.  (Only the tiles have a workspace.)"""
+    for m, k, n in ((1, 768, 2048), (23, 384, 1536), (32, 1024, 8192), (16, 1024, 16384), (16, 1920, 8192), (28, 2048, 8192)):
+        assert workspace(m, k, n) == 0, (m, k, n)
+    for m, k, n in ((1, 768, 131072), (8, 768, 32768), (32, 1792, 4096), (24, 1280, 512), (8, 2048, 16384), (29, 2048, 512), (1, 2064, 64), (33, 64, 64)):
+        assert workspace(m, k, n) > 0, (m, k, n)
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 64, 131072), (16, 1024, 16384), (17, 1024, 16384), (28, 2048, 264), (29, 2048, 264), (16, 1040, 8192),
+                                   (16, 1040, 8200), (2, 48, 1 << 20)])
+def test_linear_int8_on_both_sides_of_the_rule(eng, m, k, n):
+    say("int8 rule", m, k, n)
+    x, xd = rand((m, k), 91, F16)
+    values, scales = encoder.quantize_rows(rand((n, k), 92, F16, 1 / math.sqrt(k))[0])
+    args = (xd, values.double().cpu(), scales.double().cpu(), None, "tanh", None)
+    o.within(encoder.linear_int8(x, values, scales, activation="tanh"), lo.linear_int8(*args)[0], lo.linear_int8_bounds(*args, F16), "y")
