@@ -1096,9 +1096,13 @@ __global__ __launch_bounds__(kBlock) void attn_join_grads_kernel(const float* pa
   *reinterpret_cast<typename Frag<T>::V*>((blockIdx.y == 0 ? out0 : out1) + at) = v;
 }
 
+// Workgroups of dk's and dv's launch: of the keys, of the first keys, and of the table's sums after them.
+int64_t key_workgroups(const AttnArgs& a) { return (a.lk + kAttnRows - 1) / kAttnRows * (int64_t)a.batch * a.k_heads; }
+int64_t sink_workgroups(const AttnArgs& a) { return ((int64_t)a.sinks + 31) / 32 * a.batch * a.k_heads * a.sink_parts; }
+
 template <class T, int DP, bool BIAS, bool WIN>
 hipError_t launch_window(const AttnArgs& a, hipStream_t s) {
-  const int64_t qblocks = (a.lq + kAttnRows - 1) / kAttnRows, kblocks = (a.lk + kAttnRows - 1) / kAttnRows;
+  const int64_t qblocks = (a.lq + kAttnRows - 1) / kAttnRows;
   const size_t tab = BIAS ? (2 * (a.far + kReach) + 1) * sizeof(float) : 0;
   // few rows, or dq in parts, none of which has a row's whole sum of ds to correct delta with
   const bool rests = WIN && (few_rows(a) || a.q_parts > 1);
@@ -1110,8 +1114,7 @@ hipError_t launch_window(const AttnArgs& a, hipStream_t s) {
     }
     hipLaunchKernelGGL((attn_backward_q_kernel<T, DP, BIAS, WIN>), grid, dim3(kBlock), 5 * tab, s, a);
   }
-  const int64_t sink_wgs = WIN ? (int64_t)(a.sinks + 31) / 32 * a.batch * a.k_heads * a.sink_parts : 0;
-  const int64_t key_wgs = kblocks * a.batch * a.k_heads, all_wgs = sink_wgs + key_wgs + (BIAS ? (a.buckets * a.heads + 3) / 4 : 0);
+  const int64_t sink_wgs = WIN ? sink_workgroups(a) : 0, key_wgs = key_workgroups(a), all_wgs = attn_key_workgroups(a);
   if (all_wgs > 0) {
     const dim3 grid((unsigned)all_wgs, a.kv_parts);
     if (rests)
@@ -1182,6 +1185,10 @@ int attn_sink_parts(const AttnArgs& a, int kv_parts, int cus) {
   const int64_t wgs = (a.sinks + 31) / 32 * (int64_t)a.batch * a.k_heads;
   const int64_t tiles = (a.lq + 31) / 32 * (int64_t)(a.heads / a.k_heads);
   return (int)std::max<int64_t>(kv_parts > 1 ? 2 : 1, std::min<int64_t>({tiles / 16, 8 * cus / wgs, (int64_t)64}));
+}
+
+int64_t attn_key_workgroups(const AttnArgs& a) {
+  return key_workgroups(a) + sink_workgroups(a) + (a.table != nullptr ? (a.buckets * a.heads + 3) / 4 : 0);
 }
 
 hipError_t launch_attn_backward(const AttnArgs& a, hipStream_t s) {

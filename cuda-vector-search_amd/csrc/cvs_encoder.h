@@ -208,6 +208,7 @@ int attn_q_parts(const AttnArgs& a, int cus);
 int attn_kv_parts(const AttnArgs& a, int cus);
 int attn_sink_parts(const AttnArgs& a, int kv_parts, int cus);
 int attn_splits(const AttnArgs& a, int cus);
+int64_t attn_key_workgroups(const AttnArgs& a);  // of dk's and dv's launch, a part of its rows
 hipError_t launch_attn_forward(const AttnArgs& a, hipStream_t s);
 hipError_t launch_attn_backward(const AttnArgs& a, hipStream_t s);
 

@@ -223,7 +223,6 @@ int check_window(const cvs_attention* p, const cvs_attention_window* w) {
   if (w == nullptr) return CVS_OK;
   if (w->before < 0 || w->after < 0 || w->sinks < 0) return fail(CVS_ERR_INVALID, "attention: a window's sizes must not be negative");
   if (p->q_len >= (1 << 28) || p->k_len >= (1 << 28)) return fail(CVS_ERR_INVALID, "attention: windows take lengths below 2^28");
-  if ((std::min(w->sinks, p->k_len) + 31) / 32 * p->batch * p->heads >= (1 << 21)) return fail(CVS_ERR_INVALID, "attention: too many first keys");
   return CVS_OK;
 }
 
@@ -298,12 +297,23 @@ AttnPlan plan_attention(const AttnArgs& a, bool backward, int cus) {
   return p;
 }
 
+// (dk's and dv's launch has workgroups for the first keys, and fewer than 2^32 threads)
+int check_first_keys(const AttnArgs& a, const AttnPlan& plan) {
+  AttnArgs b = a;
+  b.sink_parts = plan.sink_parts;
+  return attn_key_workgroups(b) < (1 << 24) ? CVS_OK : fail(CVS_ERR_INVALID, "attention: too many first keys for a backward pass");
+}
+
 int attention_plan(const cvs_attention* p, const cvs_attention_window* w, int backward, int device, int64_t* workspace_bytes) {
   DevInfo di;
   int rc = dev_info(device, &di);
   if (rc == CVS_OK) rc = check_attention(p);
   if (rc == CVS_OK) rc = check_window(p, w);
-  if (rc == CVS_OK && workspace_bytes != nullptr) *workspace_bytes = plan_attention(attn_args(p, w), backward != 0, di.cus).bytes;
+  if (rc != CVS_OK) return rc;
+  const AttnArgs a = attn_args(p, w);
+  const AttnPlan plan = plan_attention(a, backward != 0, di.cus);
+  if (backward != 0) rc = check_first_keys(a, plan);
+  if (rc == CVS_OK && workspace_bytes != nullptr) *workspace_bytes = plan.bytes;
   return rc;
 }
 
@@ -358,7 +368,8 @@ int attention_backward(const cvs_attention* p, const cvs_attention_window* w, co
   if (rc != CVS_OK) return rc;
   AttnArgs a = attn_args(p, w);
   const AttnPlan plan = plan_attention(a, true, di.cus);
-  rc = check_workspace(workspace, workspace_bytes, plan.bytes);
+  rc = check_first_keys(a, plan);
+  if (rc == CVS_OK) rc = check_workspace(workspace, workspace_bytes, plan.bytes);
   if (rc != CVS_OK) return rc;
   DeviceGuard guard(device);
   if (guard.err != hipSuccess) return hip_fail(guard.err, "hipSetDevice");

@@ -758,7 +758,8 @@ def attention_forward(q, k, v, bias_table=None, key_lengths=None, query_lengths=
     buckets for the past, else the first half for keys at or before the row.
 
     ``window``, a number or (before, after): of the keys above, a row at position p sees only those from p - before to
-    p + after (one number: both; causal: to p) and the first ``sinks`` of the sequence.
+    p + after (one number: both; causal: to p) and the first ``sinks`` of the sequence.  Lengths are
+    below 2^28 then, and starts past 2^29 either way count as that.
     """
     win = _window(window, sinks)
     a, call, hold = _attention_args(q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance, win)

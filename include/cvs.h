@@ -402,7 +402,9 @@ int cvs_attention_backward(const cvs_attention* p, const void* dout, const int64
  * Attention with a sliding window: of the keys that cvs_attention leaves, a row at position p sees those
  * from p - before to p + after (`after` is nothing where causal) and the first `sinks` of the sequence.  A
  * row that the window leaves nothing has output 0 and log sum -inf; keys that no row sees reach no
- * result.  q_len and k_len are below 2^28.  Everything else is as in the calls above.
+ * result.  q_len and k_len are below 2^28, query_start counts as the nearest of -2^29 .. 2^29 (of a window of at most
+ * 2^28 keys to either side that is no difference), and a backward pass takes fewer than 2^24 workgroups for dk and dv: one for each 128
+ * keys and each 32 first keys of a sequence's key head, or a few.  Everything else is as in the calls above.
  */
 typedef struct cvs_attention_window {
   int64_t before, after, sinks;
