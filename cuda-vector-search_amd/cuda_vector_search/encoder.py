@@ -809,8 +809,11 @@ def attention_backward(dout, q, k, v, out, lse, bias_table=None, key_lengths=Non
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance, window, sinks):
-        if window is not None:  # (as it is now, for the backward pass too)
-            *window, sinks = _window(window, sinks)
+        # as they are now, for the backward pass too
+        win = _window(window, sinks)
+        window, sinks = (None, 0) if win is None else (win[:2], win[2])
+        causal, scale = bool(causal), None if scale is None else float(scale)
+        max_distance = 0 if bias_table is None else operator.index(max_distance)
         out, lse = attention_forward.inner(q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance,
                                            True, window, sinks)
         ctx.save_for_backward(q, k, v, out, lse, bias_table, key_lengths, query_lengths, query_start)

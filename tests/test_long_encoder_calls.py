@@ -21,3 +21,21 @@ def test_weights_gradients_have_memory_of_their_own():
     encoder.gated_linear(x, gate, up).float().sum().backward()
     for t in (gate.grad, up.grad):
         assert t.untyped_storage().nbytes() == t.numel() * t.element_size()
+
+
+def test_a_backward_pass_takes_the_forward_passes_scale_and_flag(monkeypatch):
+    """Values held in tensors or other objects may have changed by then."""
+    seen = []
+    args = encoder._attention_args
+
+    def record(q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance, win):
+        seen.append((bool(causal), float(scale), int(max_distance), win))
+        return args(q, k, v, bias_table, key_lengths, query_lengths, query_start, causal, scale, max_distance, win)
+
+    monkeypatch.setattr(encoder, "_attention_args", record)
+    x = half(N, WIDTH).view(1, N, 1, WIDTH).requires_grad_()
+    scale, causal, window, distance = torch.tensor(0.25), torch.tensor(True), torch.tensor([2, 1]), torch.tensor(20)
+    y = encoder.attention(x, x, x, half(4, 1), causal=causal, scale=scale, max_distance=distance, window=window, sinks=1)
+    scale.fill_(0.5), causal.fill_(False), window.fill_(3), distance.fill_(30)
+    y.float().sum().backward()
+    assert len(seen) == 2 and seen[0] == seen[1] == (True, 0.25, 20, (2, 1, 1))
