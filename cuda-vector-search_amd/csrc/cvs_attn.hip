@@ -10,9 +10,9 @@
 // cores take them); scores, maxima, sums and the output's sum are fp32.
 //
 // A row that sees no key gets zeros, and -inf as its log sum.  Keys past the last one that a
-// workgroup's rows see are not read (a cache's places not yet written); a value that is not
-// finite, of a key that a later row of the same workgroup sees, does reach the earlier rows,
-// as 0 times it.
+// workgroup's rows see are not read (a cache's places not yet written), nor, with a window, those before the first
+// one and after the first keys; a value that is not finite, of a key that some row of the workgroup sees, does
+// reach its other rows, the earlier ones and those whose window has moved past the key, as 0 times it.
 #include <algorithm>
 
 #include "cvs_attn_tile.h"
@@ -28,7 +28,8 @@ constexpr int kKeys = 64;  // keys of a tile
 // instructions between the products: 2 x 8192, 12 heads of 64, 469 us, 0.88 PFLOP/s; 2 x 4096, 16 heads
 // of 128, 270 us, 1.02; at short sequences by a workgroup's start and end (64 x up to 512, 12 heads
 // of 64, bias: 57 us).  With a window a workgroup walks the first keys' tiles and its rows' own: 8192 rows, 12 heads of 64,
-// window 128, 4 first keys 23 us, five to seven tiles a workgroup, most of it start and end.
+// window 128, 4 first keys 23 us, five to seven tiles a workgroup: some 9 of start and end (windows of 0 to 1024 keys to either
+// side, 13.5 to 86 us, are a line of 2.05 us a tile), under which nothing of another workgroup runs, all 768 having started at once.
 template <class T, int DP, bool BIAS, bool WIN>
 __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 3) void attn_forward_kernel(AttnArgs a) {
   typedef typename Frag<T>::V V;

@@ -198,7 +198,7 @@ __global__ __launch_bounds__(kBlock, DP > 64 ? 2 : 4) void attn_delta_kernel(Att
 #pragma unroll 1
     for (int kb = 0; kb < KB; ++kb) {
       const int j0 = tile0 + kb * 32, near = j0 - r0 - off;
-        if (!window_meets(a, j0, 32, r0 + off, min(r0 + 31, nq - 1) + off)) continue;
+      if (!window_meets(a, j0, 32, r0 + off, min(r0 + 31, nq - 1) + off)) continue;
       V krows[KS], vrows[KS];
 #pragma unroll
       for (int s = 0; s < KS; ++s) krows[s] = row_frag<T, DP>(sk[t & 1], kb * 32, s);

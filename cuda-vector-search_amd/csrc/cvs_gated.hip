@@ -158,7 +158,7 @@ __host__ __device__ inline int gated_grad_width(int64_t m, int n) { return m <= 
 // the products' sums are taken back: a dz loses 2^-23 of the largest at most beside its own rounding.  The largest is known
 // once all are made: gated_grad_kernel makes them times 2^4 and leaves each workgroup's largest, and a launch after it,
 // REFIT, looks at these and makes dz again where they do not fit (the pass of 16384 rows of 2 x 2048, k = 768: 297 us,
-// 359 where dz is made again, 295 without any of this; of 23 rows, k = 384 48, bound by the host, for 46).
+// 359 where dz is made again, 295 without any of this; 23 rows of 2 x 1536, k = 384 30.5 and 30.6, in bfloat16 28).
 template <class T>
 constexpr bool kFits = true;
 template <>
@@ -299,9 +299,11 @@ __global__ __launch_bounds__(kBlock) void gated_grad_kernel(GatedGradArgs a) {
 }  // namespace
 
 // Tiles of 256 x (128 + 128) (8 waves, one workgroup a CU), 128 x (64 + 64) (two) and 64 x (64 + 64) (two),
-// with the costs of plan_gemm's products of as many blocks.  16384 x 2 x 2048, k = 768, three results: 126 us, 0.82 PFLOP/s;
-// 10007 x 2 x 2664, k = 1000: 143 us, 0.75; 23 x 2 x 1536, k = 384: 6.6 us, a launch's latency.  Bound by the products at
-// the clock that power leaves (1.6 to 1.9 of 2.4 GHz); dx of two sums 16384 x 768, k = 2 x 2048 122 us, 0.85.
+// with the costs of plan_gemm's products of as many blocks.  16384 x 2 x 2048, k = 768, three results: 127 us, 0.81 PFLOP/s,
+// of the first passes, 144 to 159 of those after them; 10007 x 2 x 2664, k = 1000: 143 us, 0.75; 23 x 2 x 1536, k = 384: 6.6 us,
+// a launch's latency; dx of two sums 16384 x 768, k = 2 x 2048 115 us, 0.89.  The clock falls under load, to 2.1 to 2.2 of
+// 2.4 GHz, and the matrix cores are busy in 30 to 35% of its cycles: a wave waits 37% of its time at barriers and for loads, and
+// 38% for an instruction's turn (a stage is 64 steps of a short reduction, and no other workgroup's work is on the CU).
 GemmPlan plan_gated(int64_t m, int64_t n, int64_t k, int cus) {
   static constexpr TileChoice kTiles[] = {{256, 128, 1, 512, 1.8}, {128, 64, 2, 256, 1.2}, {64, 64, 2, 256, 0.9}};
   return plan_tiles(kTiles, 3, m, n, (k + kDepth - 1) / kDepth, 2, cus);

@@ -17,7 +17,9 @@ these operators.  Each runs hand-written gfx950 kernels (``libcvs_hip.so`` throu
 All but the last are differentiable.  ``*_forward`` and ``*_backward`` are the passes
 themselves, for programs that keep the saved tensors on their own.  Tensors are float16
 or bfloat16 (``layer_norm``: float32 too), all of one type; results have it too, with
-fp32 sums inside.  A refused argument raises ``RuntimeError`` with the reason; there
+fp32 sums inside.  What a kernel multiplies with of its own making, attention's probabilities, their
+gradients, and the products' gradients behind an activation or gate, is rounded to that type first, as the
+matrix cores take it (of few rows windows and gates keep what that takes off).  A refused argument raises ``RuntimeError`` with the reason; there
 is no torch fallback.  Forward-mode derivatives and proxy tracing are refused too;
 ``torch.jit.trace`` records the differentiable ones as Python calls.
 """
